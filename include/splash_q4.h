@@ -414,6 +414,142 @@ int sq_moe_expert_load(void *graph, sq_buffer staging, sq_buffer arena, sq_buffe
  * params). */
 uint32_t sq_moe_expert_load_groups(const sq_moe_expert_load_params *params);
 
+/* ---- rotary positions, a paged key/value cache, and attention over it ---- */
+
+/* What lies between a layer's q|k|v projection and its output projection. A batch of new rows (one token, a verify
+ * lane, a chunk of a prompt; of up to SQ_KV_MAX_SEQUENCES sequences at once) is rotated, its keys and values are
+ * written into the cache's pages, and its queries attend to every key of their sequence. Every entry point validates
+ * what the host can see, launches on the stream's own device, allocates nothing, and may be captured into a graph.
+ * What only the device can see (row starts, lengths, page ids) is bounds-checked in the kernels: nothing outside the
+ * views is read or written whatever they hold. */
+
+/* bf16 rows of attention heads: row r's head h is the head_dim values from element r * row_stride + h * head_dim on. A
+ * fused projection's query, key and value columns are three of these over one tensor. row_stride is at least heads *
+ * head_dim and a multiple of 8; the buffer is 16-byte aligned and holds the last row's heads. */
+typedef struct sq_head_rows {
+  sq_buffer buffer;
+  uint32_t heads, row_stride;
+} sq_head_rows;
+
+/* Rotary positions. The first rotary_dim values of a head are pairs, (i, i + rotary_dim / 2) in the HALF layout and
+ * (2i, 2i + 1) in the INTERLEAVED one, i < rotary_dim / 2; a row at position p turns pair i by the angle p *
+ * frequencies[i] and scales it by magnitude; the values from rotary_dim on are copied. frequencies: doubles, radians a
+ * position, on the device, 8-byte aligned. Angles are reduced in 64 bits, so far positions keep their phase. */
+#define SQ_ROPE_HALF 0u
+#define SQ_ROPE_INTERLEAVED 1u
+typedef struct sq_rope {
+  uint32_t rotary_dim, layout;
+  float magnitude;
+  sq_buffer frequencies;
+} sq_rope;
+/* The frequencies f_i = base^(-2 i / rotary_dim), scaled for contexts past original_positions:
+ *  LINEAR      f_i / factor.
+ *  NTK         base * factor^(rotary_dim / (rotary_dim - 2)) in the place of base (rotary_dim > 2).
+ *  YARN        f_i (1 - r) + (f_i / factor) r, r the ramp 0..1 from the pair that turns `high` times over
+ *              original_positions to the one that turns `low` times (rounded outwards); magnitude 0.1 ln(factor) + 1.
+ *              high 0 takes 32 and low 0 takes 1.
+ *  WAVELENGTH  with w_i = 2 pi / f_i: f_i below original_positions / high, f_i / factor above original_positions /
+ *              low, and between them (1 - t) f_i / factor + t f_i, t = (original_positions / w_i - low) / (high - low).
+ *              high 0 takes 4 and low 0 takes 1.
+ * magnitude is 1 but for YARN. */
+#define SQ_ROPE_SCALING_NONE 0u
+#define SQ_ROPE_SCALING_LINEAR 1u
+#define SQ_ROPE_SCALING_NTK 2u
+#define SQ_ROPE_SCALING_YARN 3u
+#define SQ_ROPE_SCALING_WAVELENGTH 4u
+typedef struct sq_rope_config {
+  uint32_t rotary_dim, layout, scaling, original_positions;
+  double base, factor, low, high;
+} sq_rope_config;
+/* Host only: fills frequencies[0 .. rotary_dim / 2) (host memory; the caller uploads them once) and *magnitude. */
+int sq_rope_frequencies(const sq_rope_config *config, double *frequencies, float *magnitude);
+/* output = input rotated, row r at positions[r] (uint32 [rows], on the device). input and output have the same heads;
+ * output may be input itself (same pointer and stride), and otherwise shares no element with it. head_dim is a multiple
+ * of 16 up to 256; rotary_dim is even and at most head_dim. rows may be 0. */
+int sq_rope_add(void *graph, const sq_rope *rope, sq_buffer positions, uint32_t rows, uint32_t head_dim,
+                const sq_head_rows *input, const sq_head_rows *output);
+
+/* The cache: `pages` pages of page_rows tokens (a power of two, 16..1024), keys and values each [pages][kv_heads]
+ * [page_rows][head_dim] (head_dim a multiple of 16 up to 256), 16-byte aligned. The 8-bit formats hold a code a value
+ * and one fp32 scale a token and head ([pages][kv_heads][page_rows], keys and values apart); a code stands for code *
+ * scale. INT8: scale = m / 127, code = x 127 / m rounded to the nearest even, m the head row's largest magnitude. E4M3:
+ * scale = m / 448, code = x 448 / m rounded to the nearest value of that type. A head row of zeros has scale 0; one with
+ * an infinity or NaN has a NaN scale and zero codes, so all of it reads back as NaN. BF16 pages hold the rows as they
+ * are, and have no scales. */
+#define SQ_KV_BF16 0u
+#define SQ_KV_INT8 1u
+#define SQ_KV_E4M3 2u
+#define SQ_KV_MAX_SEQUENCES 1024u
+typedef struct sq_kv_shape {
+  uint32_t kv_heads, head_dim, page_rows, format;
+} sq_kv_shape;
+typedef struct sq_kv_cache {
+  sq_kv_shape shape;
+  uint32_t pages;
+  sq_buffer keys, values, key_scales, value_scales;
+} sq_kv_cache;
+typedef struct sq_kv_size {
+  uint64_t keys, values, key_scales, value_scales; /* bytes of each buffer; the scales' are 0 for BF16 */
+} sq_kv_size;
+int sq_kv_cache_size(const sq_kv_shape *shape, uint32_t pages, sq_kv_size *out);
+/* The new rows of a batch, packed one sequence after the other: sequence s has rows row_starts[s] .. row_starts[s + 1] -
+ * 1 (uint32 [sequences + 1], not decreasing), and lengths[s] keys (uint32) with them, so that its row i of n sits at
+ * position lengths[s] - n + i; token t of it is row t % page_rows of page page_table[s * pages_per_sequence + t /
+ * page_rows] (uint32). rows is the rows that the head rows hold: rows from row_starts[sequences] on belong to no
+ * sequence and are left as they were. A length past pages_per_sequence * page_rows counts as that many. A table entry
+ * that names no page of the cache is a hole: nothing is written there, it reads back as zeros, and attention does not
+ * see its keys. Rows before position 0 (more rows than keys) are not written and read back as zeros. */
+typedef struct sq_kv_batch {
+  uint32_t sequences, rows, pages_per_sequence;
+  sq_buffer row_starts, lengths, page_table;
+} sq_kv_batch;
+/* Writes the batch's key and value rows into their pages. With a rope the keys are rotated at their positions (and
+ * rounded to bf16, as sq_rope_add rounds them) before they are stored; with queries and rotated as well (both NULL
+ * otherwise), the query rows are rotated into `rotated`, which may be the queries themselves, in the same launch. keys,
+ * values and queries are left as they are. Two rows of one call must not name one token's place: pages that sequences
+ * share are written by neither. */
+int sq_kv_add_write(void *graph, const sq_kv_cache *cache, const sq_kv_batch *batch, const sq_head_rows *keys,
+                    const sq_head_rows *values, const sq_rope *rope, const sq_head_rows *queries,
+                    const sq_head_rows *rotated);
+/* The way back: the batch's rows out of their pages as bf16 (code * scale rounded once). keys or values may be NULL. */
+int sq_kv_add_read(void *graph, const sq_kv_cache *cache, const sq_kv_batch *batch, const sq_head_rows *keys,
+                   const sq_head_rows *values);
+
+/* Attention: for each row of the batch at position p and query head h, over the keys j of its sequence that it sees,
+ *   output = sum_j e^(scale q.k_j - max) v_j / sum_j e^(scale q.k_j - max)
+ * with key/value head h / (heads / kv_heads). causal: a row sees the keys up to its own position, and with a window
+ * (0: none) only the last `window` of them, its own among them; not causal: every key of its sequence. A row that sees
+ * no key gets zeros. Keys that a row does not see do not touch its output, whatever they hold. heads is a multiple of
+ * kv_heads, at most 64 times as many. Scores, maxima, sums and the output's accumulators are fp32; the weights e^...
+ * are rounded to bf16 for the matrix units, 8-bit codes enter them exactly. */
+typedef struct sq_attention_shape {
+  uint32_t heads;
+  sq_kv_shape kv;
+  uint32_t causal, window;
+  float scale;
+} sq_attention_shape;
+/* A plan for batches of at most `sequences` sequences and `rows` rows; chunk_rows, the most new rows that one sequence
+ * usually has, picks the tile (any batch is computed right whatever it is). tile_rows: the rows times query heads of one
+ * key head that a tile holds (16, 32, 64 or 128). partials and counters: the bytes of workspace; the counters are zero
+ * at allocation and every call returns them to zero, and one workspace serves one stream at a time. */
+typedef struct sq_attention_plan {
+  sq_attention_shape shape;
+  uint32_t sequences, rows, chunk_rows, tile_rows, workgroups;
+  uint64_t partials, counters;
+} sq_attention_plan;
+typedef struct sq_attention_buffers {
+  sq_head_rows query, output; /* output may be the query itself, and otherwise shares no element with it */
+  sq_buffer partials, counters;
+} sq_attention_buffers;
+int sq_attention_plan_for(const sq_device *device, const sq_attention_shape *shape, uint32_t sequences, uint32_t rows,
+                          uint32_t chunk_rows, sq_attention_plan *out);
+/* The work (tiles of 64 keys over every sequence, key head and tile of rows) is split evenly over the workgroups
+ * whatever the lengths are; a tile of rows whose keys several workgroups share is joined by the last of them, in key
+ * order, so a batch repeats its bits from run to run. How the work falls depends on the whole batch, so a row's output
+ * bits may differ between batches. */
+int sq_attention_add(void *graph, const sq_attention_buffers *buffers, const sq_kv_cache *cache,
+                     const sq_kv_batch *batch, const sq_attention_plan *plan);
+
 #ifdef __cplusplus
 }
 #endif

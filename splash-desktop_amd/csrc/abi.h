@@ -211,3 +211,16 @@ struct SqMoeExpertLoadParams {
 static_assert(sizeof(SqMoeExpertLoadParams) == 192, "MoeExpertLoadParams is 192 bytes");
 // The threads of a moe_expert_load workgroup, each of which repacks one (row, 32-wide K group) pair (MoE.h:170-172).
 #define SQ_MOE_EXPERT_LOAD_THREADS 256u
+
+// ---------------------------------------------------------------- attention and its cache (no counterpart restated)
+#define SQ_ROPE_HALF 0u
+#define SQ_ROPE_INTERLEAVED 1u
+#define SQ_ROPE_SCALING_NONE 0u
+#define SQ_ROPE_SCALING_LINEAR 1u
+#define SQ_ROPE_SCALING_NTK 2u
+#define SQ_ROPE_SCALING_YARN 3u
+#define SQ_ROPE_SCALING_WAVELENGTH 4u
+#define SQ_KV_BF16 0u
+#define SQ_KV_INT8 1u
+#define SQ_KV_E4M3 2u
+#define SQ_KV_MAX_SEQUENCES 1024u

@@ -8,6 +8,7 @@
 #include <string>
 
 #include "../kernels/kernels.hpp"
+#include "attention.hpp"
 #include "moe.hpp"
 #include "ops.hpp"
 
@@ -612,6 +613,125 @@ int sq_moe_expert_load(void *graph, sq_buffer staging, sq_buffer arena, sq_buffe
     SqMoeExpertLoadParams p;
     std::memcpy(&p, &need(params, "params"), sizeof p);
     MoE::addExpertLoad(stream(graph), buf(staging), buf(arena), buf(slots), buf(sources), p, jobs, buf(grid));
+  });
+}
+
+}  // extern "C"
+
+// ---- rotary positions, paged cache, attention
+
+namespace {
+HeadRowsView headRows(const sq_head_rows &r) { return {buf(r.buffer), r.heads, r.row_stride}; }
+Rope rope(const sq_rope &r) { return {r.rotary_dim, RopeLayout(r.layout), r.magnitude, buf(r.frequencies)}; }
+KvShape kvShape(const sq_kv_shape &s) { return {s.kv_heads, s.head_dim, s.page_rows, KvFormat(s.format)}; }
+KvCache kvCache(const sq_kv_cache &c) {
+  return {kvShape(c.shape), c.pages, buf(c.keys), buf(c.values), buf(c.key_scales), buf(c.value_scales)};
+}
+KvBatch kvBatch(const sq_kv_batch &b) {
+  return {b.sequences, b.rows, b.pages_per_sequence, buf(b.row_starts), buf(b.lengths), buf(b.page_table)};
+}
+AttentionShape attentionShape(const sq_attention_shape &s) {
+  if (s.causal > 1) throw std::invalid_argument("attention is causal (1) or not (0)");
+  return {s.heads, kvShape(s.kv), s.causal != 0, s.window, s.scale};
+}
+sq_attention_plan cattention(const AttentionPlan &p) {
+  sq_attention_plan out{};
+  const AttentionShape &s = p.shape;
+  out.shape = {s.heads,
+               {s.kv.kvHeads, s.kv.headDim, s.kv.pageRows, uint32_t(s.kv.format)},
+               uint32_t(s.causal),
+               s.window,
+               s.scale};
+  out.sequences = p.sequences;
+  out.rows = p.rows;
+  out.chunk_rows = p.chunkRows;
+  out.tile_rows = p.tileRows;
+  out.workgroups = p.workgroups;
+  out.partials = p.partials;
+  out.counters = p.counters;
+  return out;
+}
+// The plan a caller holds, rebuilt for the compute units its workgroups say and checked.
+AttentionPlan attentionPlan(const sq_attention_plan &p) {
+  const AttentionPlan out = Attention::plan(DeviceCapabilities{p.workgroups / 2}, attentionShape(p.shape), p.sequences,
+                                            p.rows, p.chunk_rows);
+  const sq_attention_plan same = cattention(out);
+  if (same.tile_rows != p.tile_rows || same.workgroups != p.workgroups || same.partials != p.partials ||
+      same.counters != p.counters)
+    throw std::invalid_argument("the attention plan's fields are not a plan's");
+  return out;
+}
+}  // namespace
+
+extern "C" {
+
+int sq_rope_frequencies(const sq_rope_config *config, double *frequencies, float *magnitude) {
+  return guarded([&] {
+    const sq_rope_config &c = need(config, "rope config");
+    *need(magnitude, "magnitude") =
+        Rope::frequenciesOf({c.rotary_dim, RopeLayout(c.layout), RopeScaling(c.scaling), c.original_positions, c.base,
+                             c.factor, c.low, c.high},
+                            need(frequencies, "frequencies"));
+  });
+}
+
+int sq_rope_add(void *graph, const sq_rope *r, sq_buffer positions, uint32_t rows, uint32_t head_dim,
+                const sq_head_rows *input, const sq_head_rows *output) {
+  return guarded([&] {
+    Rope::add(stream(graph), rope(need(r, "rope")), buf(positions), rows, head_dim, headRows(need(input, "rope input")),
+              headRows(need(output, "rope output")));
+  });
+}
+
+int sq_kv_cache_size(const sq_kv_shape *shape, uint32_t pages, sq_kv_size *out) {
+  return guarded([&] {
+    const KvSize s = kvShape(need(shape, "cache shape")).bytes(pages);
+    *need(out, "cache size") = {s.keys, s.values, s.keyScales, s.valueScales};
+  });
+}
+
+int sq_kv_add_write(void *graph, const sq_kv_cache *cache, const sq_kv_batch *batch, const sq_head_rows *keys,
+                    const sq_head_rows *values, const sq_rope *r, const sq_head_rows *queries,
+                    const sq_head_rows *rotated) {
+  return guarded([&] {
+    Rope turn;
+    HeadRowsView q, out;
+    if (r) turn = rope(*r);
+    if (queries) q = headRows(*queries);
+    if (rotated) out = headRows(*rotated);
+    KvCache::addWrite(stream(graph), kvCache(need(cache, "cache")), kvBatch(need(batch, "batch")),
+                      headRows(need(keys, "key rows")), headRows(need(values, "value rows")), r ? &turn : nullptr,
+                      queries ? &q : nullptr, rotated ? &out : nullptr);
+  });
+}
+
+int sq_kv_add_read(void *graph, const sq_kv_cache *cache, const sq_kv_batch *batch, const sq_head_rows *keys,
+                   const sq_head_rows *values) {
+  return guarded([&] {
+    HeadRowsView k, v;
+    if (keys) k = headRows(*keys);
+    if (values) v = headRows(*values);
+    KvCache::addRead(stream(graph), kvCache(need(cache, "cache")), kvBatch(need(batch, "batch")), keys ? &k : nullptr,
+                     values ? &v : nullptr);
+  });
+}
+
+int sq_attention_plan_for(const sq_device *device, const sq_attention_shape *shape, uint32_t sequences, uint32_t rows,
+                          uint32_t chunk_rows, sq_attention_plan *out) {
+  return guarded([&] {
+    *need(out, "attention plan") = cattention(Attention::plan(DeviceCapabilities{device ? device->compute_units : 0},
+                                                              attentionShape(need(shape, "attention shape")), sequences,
+                                                              rows, chunk_rows));
+  });
+}
+
+int sq_attention_add(void *graph, const sq_attention_buffers *b, const sq_kv_cache *cache, const sq_kv_batch *batch,
+                     const sq_attention_plan *plan) {
+  return guarded([&] {
+    const sq_attention_buffers &buffers = need(b, "attention buffers");
+    Attention::add(stream(graph), headRows(buffers.query), headRows(buffers.output), buf(buffers.partials),
+                   buf(buffers.counters), kvCache(need(cache, "cache")), kvBatch(need(batch, "batch")),
+                   attentionPlan(need(plan, "attention plan")));
   });
 }
 

@@ -211,4 +211,51 @@ hipError_t launch_moe_combine(const uint16_t *expert_output, const uint32_t *rou
                               const float *routing_weights, const uint16_t *residual, uint16_t *output,
                               const SqMoeCombineParams &params, hipStream_t stream);
 
+// Rows of attention heads (bf16): row r's head h from element r * stride + h * head_dim on.
+struct HeadRows {
+  uint16_t *rows;
+  uint32_t heads, stride;
+};
+// Rotary positions: pair i < pairs turns by position * frequencies[i] radians, its cosine and sine times magnitude.
+struct RopeArgs {
+  const double *frequencies;
+  uint32_t pairs, interleaved;
+  float magnitude;
+};
+hipError_t launch_rope(const RopeArgs &rope, const uint32_t *positions, uint32_t rows, uint32_t head_dim,
+                       const HeadRows &input, const HeadRows &output, hipStream_t stream);
+
+// A paged cache and a batch of rows over it (include/splash_q4.h states both). The host has checked the views' sizes;
+// the kernels check what the row starts, lengths and page table hold.
+struct KvArgs {
+  uint8_t *keys, *values;
+  float *key_scales, *value_scales;
+  const uint32_t *row_starts, *lengths, *page_table;
+  uint32_t sequences, rows, pages_per_sequence, pages, page_shift, kv_heads, head_dim, format;
+};
+// rope.pairs 0: keys are written as they are; queries.rows null: no queries.
+hipError_t launch_kv_write(const KvArgs &kv, const HeadRows &keys, const HeadRows &values, const RopeArgs &rope,
+                           const HeadRows &queries, const HeadRows &rotated, hipStream_t stream);
+// A null view is not read.
+hipError_t launch_kv_read(const KvArgs &kv, const HeadRows &keys, const HeadRows &values, hipStream_t stream);
+
+// Attention of the batch's rows over the cache, on tiles of tile_rows packed rows (a row's group query heads of one
+// key head side by side), the work split over `workgroups` workgroups.
+struct AttendArgs {
+  KvArgs kv;
+  const uint16_t *query;
+  uint16_t *output;
+  uint32_t query_stride, output_stride, group;
+  uint32_t causal, window;
+  float scale;
+  float *partials;
+  uint32_t *counters;
+  uint32_t workgroups;
+};
+constexpr uint32_t kAttendMaxGroup = 64;
+// The floats of partials and the counters that `workgroups` workgroups on tiles of tile_rows rows use.
+uint64_t attend_partials(uint32_t tile_rows, uint32_t head_dim, uint32_t workgroups);
+uint64_t attend_counters(uint32_t workgroups);
+hipError_t launch_attend_rows(uint32_t tile_rows, const AttendArgs &args, hipStream_t stream);
+
 }  // namespace sq::kern

@@ -9,7 +9,7 @@ from __future__ import annotations
 import ctypes
 import os
 import pathlib
-from ctypes import POINTER, Structure, byref, c_char_p, c_int, c_uint32, c_uint64, c_void_p
+from ctypes import POINTER, Structure, byref, c_char_p, c_double, c_float, c_int, c_uint32, c_uint64, c_void_p
 
 PACKAGE_ROOT = pathlib.Path(__file__).resolve().parent.parent
 LIBRARY = PACKAGE_ROOT / "lib" / "libsplash_q4.so"
@@ -146,6 +146,59 @@ class MoeBuffers(Structure):
                 ("verify_rows", Buffer)]
 
 
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1
+ROPE_SCALING_NONE, ROPE_SCALING_LINEAR, ROPE_SCALING_NTK, ROPE_SCALING_YARN, ROPE_SCALING_WAVELENGTH = range(5)
+KV_BF16, KV_INT8, KV_E4M3 = 0, 1, 2
+KV_MAX_SEQUENCES = 1024
+
+
+class HeadRows(Structure):
+    _fields_ = [("buffer", Buffer), ("heads", c_uint32), ("row_stride", c_uint32)]
+
+
+class Rope(Structure):
+    _fields_ = [("rotary_dim", c_uint32), ("layout", c_uint32), ("magnitude", c_float), ("frequencies", Buffer)]
+
+
+class RopeConfig(Structure):
+    _fields_ = [(n, c_uint32) for n in ("rotary_dim", "layout", "scaling", "original_positions")] + \
+               [(n, c_double) for n in ("base", "factor", "low", "high")]
+
+
+class KvShape(Structure):
+    _fields_ = [(n, c_uint32) for n in ("kv_heads", "head_dim", "page_rows", "format")]
+
+
+_KV_BUFFERS = ("keys", "values", "key_scales", "value_scales")
+
+
+class KvCache(Structure):
+    _fields_ = [("shape", KvShape), ("pages", c_uint32)] + [(n, Buffer) for n in _KV_BUFFERS]
+
+
+class KvSize(Structure):
+    _fields_ = [(n, c_uint64) for n in _KV_BUFFERS]
+
+
+class KvBatch(Structure):
+    _fields_ = [("sequences", c_uint32), ("rows", c_uint32), ("pages_per_sequence", c_uint32),
+                ("row_starts", Buffer), ("lengths", Buffer), ("page_table", Buffer)]
+
+
+class AttentionShape(Structure):
+    _fields_ = [("heads", c_uint32), ("kv", KvShape), ("causal", c_uint32), ("window", c_uint32), ("scale", c_float)]
+
+
+class AttentionPlan(Structure):
+    _fields_ = [("shape", AttentionShape)] + \
+               [(n, c_uint32) for n in ("sequences", "rows", "chunk_rows", "tile_rows", "workgroups")] + \
+               [("partials", c_uint64), ("counters", c_uint64)]
+
+
+class AttentionBuffers(Structure):
+    _fields_ = [("query", HeadRows), ("output", HeadRows), ("partials", Buffer), ("counters", Buffer)]
+
+
 class SqError(RuntimeError):
     def __init__(self, code: int, message: str):
         super().__init__(message)
@@ -209,6 +262,16 @@ _SIGNATURES = {
                           POINTER(MoeShape), c_uint32],
     "sq_moe_expert_load": [c_void_p, Buffer, Buffer, Buffer, Buffer, POINTER(ExpertLoadParams), c_uint32, Buffer],
     "sq_moe_expert_load_groups": [POINTER(ExpertLoadParams)],
+    "sq_rope_frequencies": [POINTER(RopeConfig), POINTER(c_double), POINTER(c_float)],
+    "sq_rope_add": [c_void_p, POINTER(Rope), Buffer, c_uint32, c_uint32, POINTER(HeadRows), POINTER(HeadRows)],
+    "sq_kv_cache_size": [POINTER(KvShape), c_uint32, POINTER(KvSize)],
+    "sq_kv_add_write": [c_void_p, POINTER(KvCache), POINTER(KvBatch), POINTER(HeadRows), POINTER(HeadRows),
+                        POINTER(Rope), POINTER(HeadRows), POINTER(HeadRows)],
+    "sq_kv_add_read": [c_void_p, POINTER(KvCache), POINTER(KvBatch), POINTER(HeadRows), POINTER(HeadRows)],
+    "sq_attention_plan_for": [POINTER(Device), POINTER(AttentionShape), c_uint32, c_uint32, c_uint32,
+                              POINTER(AttentionPlan)],
+    "sq_attention_add": [c_void_p, POINTER(AttentionBuffers), POINTER(KvCache), POINTER(KvBatch),
+                         POINTER(AttentionPlan)],
 }
 
 
@@ -354,3 +417,94 @@ def stream_read(src, sink, workgroups: int, threads: int, nbytes: int | None = N
     """The read-only streaming kernel over `nbytes` of src (measurement aid, sq_diag_stream_read)."""
     call("sq_diag_stream_read", stream if stream is not None else stream_handle(), view(src, nbytes), view(sink),
          workgroups, threads)
+
+
+# ---------------------------------------------------------------- rotary positions, paged cache, attention
+
+def head_rows(tensor, head_dim: int) -> HeadRows:
+    """A bf16 tensor's rows of heads: [rows, heads * head_dim] (a column slice of a fused projection's output too)."""
+    width = tensor.shape[-1]
+    if tensor.dim() != 2 or width % head_dim or (tensor.numel() and tensor.stride(1) != 1) or \
+            tensor.element_size() != 2:
+        raise ValueError("head rows are a 2-byte [rows, heads * head_dim] tensor with adjacent columns")
+    rows, stride = tensor.shape[0], tensor.stride(0) if tensor.shape[0] > 1 else max(width, tensor.stride(0))
+    nbytes = 2 * ((rows - 1) * stride + width) if rows else 0
+    return HeadRows(Buffer(tensor.data_ptr(), nbytes), width // head_dim, stride)
+
+
+def rope_frequencies(config: RopeConfig) -> tuple[list[float], float]:
+    """The pairs' radians a position, and the magnitude."""
+    values, magnitude = (c_double * max(config.rotary_dim // 2, 1))(), c_float()
+    call("sq_rope_frequencies", byref(config), values, byref(magnitude))
+    return list(values), magnitude.value
+
+
+class RotaryPositions:
+    """A rope with its frequencies on the device."""
+
+    def __init__(self, config: RopeConfig, device_name: str = "cuda"):
+        import torch
+        values, magnitude = rope_frequencies(config)
+        self.frequencies = torch.tensor(values, dtype=torch.float64, device=device_name)
+        self.struct = Rope(config.rotary_dim, config.layout, magnitude, view(self.frequencies))
+
+
+def rope_add(rope: RotaryPositions, positions, input, output, head_dim: int, stream=None) -> None:
+    x, y = head_rows(input, head_dim), head_rows(output, head_dim)
+    call("sq_rope_add", stream if stream is not None else stream_handle(), byref(rope.struct), view(positions),
+         input.shape[0], head_dim, byref(x), byref(y))
+
+
+def kv_cache_size(shape: KvShape, pages: int) -> KvSize:
+    out = KvSize()
+    call("sq_kv_cache_size", byref(shape), pages, byref(out))
+    return out
+
+
+def kv_cache(shape: KvShape, pages: int, keys, values, key_scales=None, value_scales=None) -> KvCache:
+    return KvCache(shape, pages, view(keys), view(values), view(key_scales), view(value_scales))
+
+
+def kv_batch(row_starts, lengths, page_table, rows: int) -> KvBatch:
+    """row_starts [sequences + 1], lengths [sequences] and page_table [sequences, pages] are 32-bit tensors."""
+    return KvBatch(lengths.shape[0], rows, page_table.shape[1], view(row_starts), view(lengths), view(page_table))
+
+
+def kv_write(cache: KvCache, batch: KvBatch, keys, values, rope: RotaryPositions | None = None, queries=None,
+             rotated=None, stream=None) -> None:
+    d = cache.shape.head_dim
+    k, v = head_rows(keys, d), head_rows(values, d)
+    q, r = (byref(head_rows(t, d)) if t is not None else None for t in (queries, rotated))
+    call("sq_kv_add_write", stream if stream is not None else stream_handle(), byref(cache), byref(batch), byref(k),
+         byref(v), byref(rope.struct) if rope is not None else None, q, r)
+
+
+def kv_read(cache: KvCache, batch: KvBatch, keys=None, values=None, stream=None) -> None:
+    d = cache.shape.head_dim
+    k, v = (byref(head_rows(t, d)) if t is not None else None for t in (keys, values))
+    call("sq_kv_add_read", stream if stream is not None else stream_handle(), byref(cache), byref(batch), k, v)
+
+
+def attention_plan(shape: AttentionShape, sequences: int, rows: int, chunk_rows: int,
+                   dev: Device | None = None) -> AttentionPlan:
+    out = AttentionPlan()
+    call("sq_attention_plan_for", byref(dev or Device(0)), byref(shape), sequences, rows, chunk_rows, byref(out))
+    return out
+
+
+class AttentionScratch:
+    """Device workspace for an attention plan (the counters zeroed at allocation, as they must be)."""
+
+    def __init__(self, plan: AttentionPlan, device_name: str = "cuda"):
+        import torch
+        self.partials = torch.empty(max(plan.partials, 16), dtype=torch.uint8, device=device_name)
+        self.counters = torch.zeros(max(plan.counters, 16) // 4, dtype=torch.int32, device=device_name)
+
+
+def attention_add(plan: AttentionPlan, cache: KvCache, batch: KvBatch, query, output, scratch: AttentionScratch,
+                  stream=None) -> None:
+    d = cache.shape.head_dim
+    buffers = AttentionBuffers(head_rows(query, d), head_rows(output, d), view(scratch.partials),
+                               view(scratch.counters))
+    call("sq_attention_add", stream if stream is not None else stream_handle(), byref(buffers), byref(cache),
+         byref(batch), byref(plan))
