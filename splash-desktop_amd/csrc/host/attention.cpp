@@ -256,14 +256,11 @@ AttentionPlan Attention::plan(const DeviceCapabilities &device, const AttentionS
   if (!rows || rows > kMaxRows) throw std::invalid_argument("an attention plan takes 1 to 2^20 rows");
   if (!chunkRows || chunkRows > rows) throw std::invalid_argument("a sequence's new rows are 1 to the plan's rows");
   AttentionPlan out{shape, sequences, rows, chunkRows};
-  // The smallest tile that holds a sequence's rows with their query heads, or the largest: a tile of more rows than that
-  // reads no key less.
+  // The smallest tile of few rows that holds a sequence's new rows with their query heads, so that their keys are read
+  // once; past the largest of those, the wide tile.
   const uint64_t packed = uint64_t{chunkRows} * shape.group();
-  const uint32_t largest = shape.kv.headDim <= 128 ? 64 : 32;
-  out.tileRows = 16;
-  while (out.tileRows < largest && (out.tileRows < packed || out.tileRows < shape.group())) out.tileRows *= 2;
-  if (out.tileRows < shape.group())
-    throw std::invalid_argument("attention heads of more than 128 values have at most 32 query heads a key head");
+  out.tileRows = kern::kAttendWideRows;
+  for (uint32_t few = kern::attend_few_rows(shape.kv.headDim); few >= 16 && few >= packed; few /= 2) out.tileRows = few;
   const uint32_t units = device.computeUnits ? device.computeUnits : 256;
   out.workgroups = (2 * units + 7) / 8 * 8;
   out.partials = kern::attend_partials(out.tileRows, shape.kv.headDim, out.workgroups) * 4;
@@ -293,7 +290,9 @@ void Attention::add(hipStream_t graph, const HeadRowsView &query, const HeadRows
                               float(double(shape.scale) * std::numbers::log2e), partials.as<float>(),
                               counters.as<uint32_t>(), plan.workgroups};
   const OnStreamDevice on(graph);
-  launched(kern::launch_attend_rows(plan.tileRows, args, graph), "attention");
+  launched(plan.tileRows == kern::kAttendWideRows ? kern::launch_attend_tile(args, graph)
+                                                  : kern::launch_attend_rows(plan.tileRows, args, graph),
+           "attention");
 }
 
 }  // namespace sq::ops

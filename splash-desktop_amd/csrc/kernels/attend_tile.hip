@@ -1,0 +1,461 @@
+// Attention of many rows a key head (tiles of 128 rows times query heads): chunks of prompts, bound by the matrix units
+// and by the softmax between the two products.
+//
+// Four waves of 32 rows share tiles of 64 keys in LDS, two tiles deep: while one is multiplied the next arrives. Both
+// products run transposed on 32x32x16 MFMAs: S^T = K Q^T leaves 16 of each 32 keys of one row in a lane (lane (h, r), l =
+// 32 h + r, holds keys 8 j + 4 h + i of row r), so a row's maximum and sum are the lane's own but for one exchange with
+// the lane 32 away, and the eight weights of 16 keys that the second product O^T = V^T P^T wants of a lane are eight that
+// it already holds: the contraction takes its keys in that order, 4 h .. + 3 and 8 + 4 h .. + 3 of 16. V^T in that order
+// comes from ds_read_b64_tr_b16, which reads four keys' rows and gives each lane one value of them.
+//
+// LDS holds both tiles as bf16, a key a row, its 16-byte chunks exchanged by the row (chunk c of row k at c ^ swap(k)) so
+// that 16 rows of one chunk (K's reads) and four rows of four chunks (V's) fall on all 64 banks. bf16 pages are copied
+// straight into LDS (the exchange is in the addresses that the lanes read from); codes pass through registers and become
+// bf16 once for all four waves, exactly. Scales multiply the scores, and the weights before they are rounded.
+//
+// Keys past the sequence's end and holes read as zeros (buffer resources end there). Only tiles that some row does not
+// see whole compare positions.
+#include "attend.hpp"
+#include "device.hpp"
+
+namespace sq::kern {
+namespace {
+
+constexpr int kWaves = 4, kThreads = 64 * kWaves, kRows = 32 * kWaves;
+constexpr float kRaise = 8.0f;               // as in the tiles of few rows: the running maximum moves past this
+constexpr uint32_t kNowhere = 0x7FFFFFF0u;   // past every resource's range: reads zero
+
+typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16;
+typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf16x2;
+
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
+                                                 0);
+}
+__device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
+  return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});
+}
+__device__ __forceinline__ uint32_t high_halves(uint32_t k0, uint32_t k1) {
+  return __builtin_amdgcn_perm(k1, k0, 0x07060302u);
+}
+template <uint32_t FMT>
+__device__ __forceinline__ u32x2 code_pairs4(uint32_t w) {
+  if constexpr (FMT == SQ_KV_E4M3) {
+    return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true))};
+  } else {
+    uint32_t f[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = __float_as_uint((float)(int8_t)(w >> (8 * e)));
+    return u32x2{high_halves(f[0], f[1]), high_halves(f[2], f[3])};
+  }
+}
+// op over the two lanes that hold a row's keys.
+__device__ __forceinline__ float other_max(float v) {
+  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+__device__ __forceinline__ float other_sum(float v) {
+  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+// A vector a lane from a buffer straight into LDS: lane l's lands at lds + 16 l.
+__device__ __forceinline__ void copy_to_lds(__amdgpu_buffer_rsrc_t from, uint8_t *lds, uint32_t at) {
+  const auto to = (__attribute__((address_space(3))) void *)lds;
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(from, to, 16, at, 0, 0, 0);
+}
+// Four keys' values, transposed (lane i of 16 gives the address of key i / 4's values 4 (i % 4) .. + 3 and gets value i
+// of the four keys).
+__device__ __forceinline__ u32x2 read_transposed(const uint8_t *lds) {
+  typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)lds));
+}
+// Every wave's stores to LDS and copies into it have landed.
+__device__ __forceinline__ void tile_barrier() {
+  __builtin_amdgcn_s_waitcnt(0);
+  __syncthreads();
+}
+
+// A head row in LDS: DIM bf16 values, CHUNKS 16-byte chunks. Where chunk c of key k lies.
+template <int DIM>
+struct Tile {
+  static constexpr int kRowBytes = 2 * DIM, kChunks = DIM / 8, kBytes = kKeyTile * kRowBytes;
+  // 128-byte rows (DIM 64) lie two to a round of the banks, so the pair's number takes the row's place.
+  static __device__ __forceinline__ uint32_t key_swap(uint32_t k) { return DIM == 64 ? (k >> 1) & 7u : k & 15u; }
+  static __device__ __forceinline__ uint32_t value_swap(uint32_t k) {
+    return DIM == 64 ? 4u * ((k >> 1) & 1u) : 4u * (k & 3u);
+  }
+};
+
+template <uint32_t FMT, int DIM>
+__global__ __launch_bounds__(kThreads, DIM == 256 ? 1 : 2) void attend_tile_kernel(AttendArgs a) {
+  using T = Tile<DIM>;
+  constexpr bool kCodes = FMT != SQ_KV_BF16;
+  constexpr int kSteps = DIM / 16, kBlocks = DIM / 32, kBytes = kCodes ? 1 : 2;
+  constexpr int kPartFloats = kRows * (DIM + 2);
+  // A wave fetches 16 keys of the tile, kLoads vectors a lane of K and of V.
+  constexpr int kLoads = 16 * DIM * kBytes / 1024, kRowLanes = DIM * kBytes / 16, kLoadRows = 64 / kRowLanes;
+  __shared__ __attribute__((aligned(1024))) uint8_t tiles[2][2][T::kBytes];   // [stage][K, V]
+  __shared__ f32x4 scales[kCodes ? 2 : 1][2][kKeyTile / 4];
+  __shared__ int64_t prefix[kMaxSequences + 1], scan[kWaves];
+  __shared__ uint32_t arrival;
+  const uint32_t lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
+  const uint32_t wave = uniform(threadIdx.x >> 6);
+  const int fit = kRows / (int)a.group;
+  const uint32_t dim = a.kv.head_dim, row_bytes = dim * kBytes;
+  const Line line = make_line<kThreads>(a, fit, 4 * kKeyTile, prefix, scan);
+  const uint32_t piece = piece_of(line, blockIdx.x);
+  if (blockIdx.x / 8 >= (line.active + 7) / 8 || piece >= line.active) return;
+  int64_t x = line.share * piece;
+  const int64_t end = x + line.share < line.total ? x + line.share : line.total;
+
+  // Where this lane's vectors lie in 16 keys of a page, and (codes) in the LDS tile.
+  uint32_t key_from[kLoads], value_from[kLoads], code_to[kLoads];
+#pragma unroll
+  for (int j = 0; j < kLoads; ++j) {
+    const uint32_t k = kLoadRows * j + lane / kRowLanes, c = lane % kRowLanes;
+    if constexpr (kCodes) {
+      // A vector of 16 codes is two chunks of LDS, 2 c and 2 c + 1.
+      key_from[j] = value_from[j] = 16 * c < dim ? k * row_bytes + 16 * c : kNowhere;
+      code_to[j] = (16 * wave + k) * T::kRowBytes;
+    } else {
+      // LDS takes the lanes' vectors in lane order, so the lane reads the chunk that its place holds.
+      const uint32_t kc = c ^ T::key_swap(k), vc = c ^ T::value_swap(k);
+      key_from[j] = 8 * kc < dim ? k * row_bytes + 16 * kc : kNowhere;
+      value_from[j] = 8 * vc < dim ? k * row_bytes + 16 * vc : kNowhere;
+      code_to[j] = 0;
+    }
+  }
+  // The K operand's row (key r of a block of 32) and the V operand's (keys 4 h + i / 4 of 16, i = lane % 16), chunk 0.
+  const uint32_t key_at = r * T::kRowBytes + 16 * (h ^ T::key_swap(r));
+  const uint32_t vi = lane & 15, vk = 4 * h + vi / 4;
+  const uint32_t value_at = vk * T::kRowBytes + 8 * (vi % 2) + 16 * ((2 * (lane / 16 % 2) + vi % 4 / 2) ^ T::value_swap(vk));
+
+  while (x < end) {
+    const Part part = next_part(a, line, fit, x, end, piece);
+    if (part.t1 <= part.t0) continue;
+    const Units &u = part.units;
+    const int row0 = fit * part.m, rows = min(fit, u.rows - row0), live = rows * (int)a.group;
+    const int unit_end = u.causal ? min(u.keys, u.base + row0 + rows) : u.keys;   // keys that any row sees
+    const int tile0 = u.first_tile(part.m);
+    const int k_begin = kKeyTile * (tile0 + part.t0), k_end = min(unit_end, kKeyTile * (tile0 + part.t1));
+    const int clear_begin = u.window ? u.base + row0 + rows - u.window : 0;
+    const int clear_end = u.causal ? u.base + row0 + 1 : u.keys;
+
+    // This lane's row.
+    const int p = 32 * (int)wave + (int)r, pi = p / (int)a.group, pg = p - pi * (int)a.group;
+    const bool on = p < live;
+    const int at = u.base + row0 + pi;
+    const int low = u.window ? at - u.window + 1 : 0;
+    const int high = u.causal ? min(at + 1, u.keys) : u.keys;
+    const bool busy = 32 * (int)wave < live;   // waves past the unit's rows only fetch
+    u32x4 q[kSteps];
+    {
+      const uint16_t *row = a.query + (size_t)(part.first_row + row0 + (on ? pi : 0)) * a.query_stride +
+                            (part.head * a.group + (on ? pg : 0)) * dim;
+#pragma unroll
+      for (int s = 0; s < kSteps; ++s) {
+        const uint32_t d = 16 * s + 8 * h;
+        q[s] = on && d < dim ? *(const u32x4 *)(row + d) : u32x4{0u, 0u, 0u, 0u};
+      }
+    }
+    float m = -INFINITY, l = 0.0f;
+    f32x16 o[kBlocks];
+#pragma unroll
+    for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) o[b][i] = 0.0f;
+
+    // The tile at k: the page of this wave's 16 keys (~0u for none), and which of the four 16 keys have none. A page of 64
+    // rows or more holds the whole tile.
+    struct Pages {
+      uint32_t own, holes;
+    };
+    const auto pages_at = [&](int k) __attribute__((always_inline)) {
+      Pages out{~0u, 0u};
+      if (k >= k_end) return out;
+      if (a.kv.page_shift >= 6) {
+        const uint32_t page = uniform(page_of(a.kv, part.sequence, k));
+        out = {k + 16 * (int)wave < k_end ? page : ~0u, page == ~0u ? 15u : 0u};
+      } else {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const uint32_t page = k + 16 * g < k_end ? uniform(page_of(a.kv, part.sequence, k + 16 * g)) : ~0u;
+          if (page == ~0u) out.holes |= 1u << g;
+          if (g == (int)wave) out.own = page;
+        }
+      }
+      return out;
+    };
+    u32x4 code_k[kCodes ? kLoads : 1], code_v[kCodes ? kLoads : 1];
+    float code_scale = 0.0f;
+    const auto fetch = [&](int k, uint32_t page, int stage) __attribute__((always_inline)) {
+      const int from = k + 16 * (int)wave, n = page == ~0u ? 0 : min(16, k_end - from);
+      const size_t base = ((((size_t)(page == ~0u ? 0 : page) * a.kv.kv_heads + part.head) << a.kv.page_shift) +
+                           ((uint32_t)from & ((1u << a.kv.page_shift) - 1)));
+      const __amdgpu_buffer_rsrc_t keys = buffer_rsrc(a.kv.keys + base * row_bytes, (uint32_t)n * row_bytes),
+                                   values = buffer_rsrc(a.kv.values + base * row_bytes, (uint32_t)n * row_bytes);
+      if constexpr (kCodes) {
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+          code_k[j] = buffer_b128<0>(keys, key_from[j], 0);
+          code_v[j] = buffer_b128<0>(values, value_from[j], 0);
+        }
+        // Lanes 0..15 the keys' scales, 16..31 the values'.
+        const float *from_scales = lane < 16 ? a.kv.key_scales : a.kv.value_scales;
+        code_scale = lane < 32 && (int)(lane & 15) < n ? from_scales[base + (lane & 15)] : 0.0f;
+      } else {
+        uint8_t *to_k = &tiles[stage][0][16 * wave * T::kRowBytes], *to_v = &tiles[stage][1][16 * wave * T::kRowBytes];
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+          copy_to_lds(keys, to_k + 1024 * j, key_from[j]);
+          copy_to_lds(values, to_v + 1024 * j, value_from[j]);
+        }
+      }
+    };
+    // The fetched codes into LDS as bf16.
+    const auto place = [&](int stage) __attribute__((always_inline)) {
+      if constexpr (kCodes) {
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+          const uint32_t k = kLoadRows * j + lane / kRowLanes, c = 2 * (lane % kRowLanes);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const u32x2 k0 = code_pairs4<FMT>(code_k[j][2 * i]), k1 = code_pairs4<FMT>(code_k[j][2 * i + 1]);
+            const u32x2 v0 = code_pairs4<FMT>(code_v[j][2 * i]), v1 = code_pairs4<FMT>(code_v[j][2 * i + 1]);
+            *(u32x4 *)&tiles[stage][0][code_to[j] + 16 * ((c + i) ^ T::key_swap(k))] = u32x4{k0[0], k0[1], k1[0], k1[1]};
+            *(u32x4 *)&tiles[stage][1][code_to[j] + 16 * ((c + i) ^ T::value_swap(k))] =
+                u32x4{v0[0], v0[1], v1[0], v1[1]};
+          }
+        }
+        if (lane < 32) ((float *)&scales[stage][lane / 16][4 * wave])[lane & 15] = code_scale;
+      }
+    };
+
+    __syncthreads();   // the last part's tiles have been read
+    Pages pages = pages_at(k_begin);
+    fetch(k_begin, pages.own, 0);
+    uint32_t holes = pages.holes;
+    pages = pages_at(k_begin + kKeyTile);   // a tile ahead of the fetch that wants it
+    place(0);
+    tile_barrier();
+    int stage = 0;
+    for (int k = k_begin; k < k_end; k += kKeyTile, stage ^= 1) {
+      const bool more = k + kKeyTile < k_end;
+      if (more) fetch(k + kKeyTile, pages.own, stage ^ 1);
+      const uint32_t next_holes = pages.holes;
+      pages = pages_at(k + 2 * kKeyTile);
+      const uint8_t *kt = tiles[stage][0], *vt = tiles[stage][1];
+      const bool clear = k >= clear_begin && k + kKeyTile <= clear_end && k + kKeyTile <= k_end && !holes;
+      u32x4 w[4];   // the weights of 16 keys each, as the second product's operand
+      if (busy) {
+        f32x16 s[2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[b][i] = 0.0f;
+#pragma unroll
+          for (int c = 0; c < kSteps; ++c)
+            s[b] = mfma32(*(const u32x4 *)&kt[32 * b * T::kRowBytes + (key_at ^ (32 * c))], q[c], s[b]);
+        }
+        float top = -INFINITY;
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            f32x4 by{a.scale, a.scale, a.scale, a.scale};
+            if constexpr (kCodes) by *= scales[stage][0][8 * b + 2 * j + h];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              float t = s[b][4 * j + i] * by[i];
+              if (!clear) {
+                const int key = k + 32 * b + 8 * j + 4 * (int)h + i;
+                t = key >= low && key < high && !(holes >> (2 * b + j / 2) & 1) ? t : -INFINITY;
+              }
+              s[b][4 * j + i] = t;
+              top = fmaxf(top, t);
+            }
+          }
+        if (__any(top > m + kRaise)) {
+          const float next = fmaxf(m, other_max(top));
+          const float shrink = exp2_fast(m - finite_max(next));
+          m = next;
+          l *= shrink;
+#pragma unroll
+          for (int b = 0; b < kBlocks; ++b) o[b] *= shrink;
+        }
+        const float from = finite_max(m);
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            s[b][i] = exp2_fast(s[b][i] - from);
+            l += s[b][i];
+          }
+        if constexpr (kCodes) {
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const f32x4 by = scales[stage][1][8 * b + 2 * j + h];
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const int key = k + 32 * b + 8 * j + 4 * (int)h + i;
+                // The scale of a key that the row does not see may be a NaN.
+                const bool sees = clear || (key >= low && key < high && !(holes >> (2 * b + j / 2) & 1));
+                s[b][4 * j + i] = sees ? s[b][4 * j + i] * by[i] : 0.0f;
+              }
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          const int b = t / 2, i = 8 * (t % 2);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[t][e] = bf16_pair(s[b][i + 2 * e], s[b][i + 2 * e + 1]);
+        }
+      }
+      if constexpr (!kCodes) {
+        if (!clear) {
+          // Infinities and NaNs among the tile's values must not reach rows that do not see them through 0 * inf: the
+          // rows that do see them add their products one by one, and they leave the tile.
+          constexpr int kMine = T::kBytes / 16 / kThreads;
+          uint32_t any = 0;
+#pragma unroll
+          for (int i = 0; i < kMine; ++i) {
+            const u32x4 v = *(const u32x4 *)&vt[16 * (threadIdx.x + kThreads * i)];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              any |= (uint32_t)((v[e] & 0x7F80u) == 0x7F80u) | (uint32_t)((v[e] & 0x7F800000u) == 0x7F800000u);
+          }
+          if (__syncthreads_or((int)any)) {
+            if (busy) {
+#pragma unroll
+              for (int t = 0; t < 4; ++t)
+#pragma unroll 1
+                for (uint32_t key = 0; key < 16; ++key) {
+                  // Key `key` of 16 is weight 4 (key / 8) + key % 4 of the lanes with h = key / 4 % 2.
+                  const uint32_t first = key & 8 ? w[t][2] : w[t][0], second = key & 8 ? w[t][3] : w[t][1];
+                  const uint32_t word = (uint32_t)__shfl((int)(key & 2 ? second : first), (int)(r + 32 * (key / 4 % 2)));
+                  const float weight = __uint_as_float(key & 1 ? word & 0xFFFF0000u : word << 16);
+                  const int j = k + 16 * t + (int)key;
+                  const bool sees = on && j >= low && j < high && !(holes >> t & 1);
+                  const uint32_t row = 16 * t + key;
+#pragma unroll
+                  for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                      const uint32_t chunk = (4 * b + i) ^ T::value_swap(row);
+                      const u32x2 v = *(const u32x2 *)&vt[row * T::kRowBytes + 16 * chunk + 8 * h];
+#pragma unroll
+                      for (int e = 0; e < 4; ++e) {
+                        const uint32_t bits = e & 1 ? v[e / 2] >> 16 : v[e / 2] & 0xFFFFu;
+                        if (sees && (bits & 0x7F80u) == 0x7F80u) o[b][4 * i + e] += weight * bf16_to_f32(bits);
+                      }
+                    }
+                }
+            }
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) {
+              u32x4 *v = (u32x4 *)&tiles[stage][1][16 * (threadIdx.x + kThreads * i)];
+              u32x4 clean = *v;
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                if ((clean[e] & 0x7F80u) == 0x7F80u) clean[e] &= 0xFFFF0000u;
+                if ((clean[e] & 0x7F800000u) == 0x7F800000u) clean[e] &= 0x0000FFFFu;
+              }
+              *v = clean;
+            }
+            __syncthreads();
+          }
+        }
+      }
+      if (busy) {
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int b = 0; b < kBlocks; ++b) {
+            const uint8_t *from = &vt[16 * t * T::kRowBytes + (value_at ^ (64 * b))];
+            const u32x2 v0 = read_transposed(from), v1 = read_transposed(from + 8 * T::kRowBytes);
+            o[b] = mfma32(u32x4{v0[0], v0[1], v1[0], v1[1]}, w[t], o[b]);
+          }
+      }
+      if (more) place(stage ^ 1);
+      tile_barrier();
+      holes = next_holes;
+    }
+    l = other_sum(l);
+
+    if (part.parts > 1) {
+      float *mine = a.partials + (size_t)part_slot(part.first_piece, part.part) * kPartFloats + wave * (32 * (DIM + 2));
+      if (busy) {
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) store_pair(mine + (8 * b + i) * 128 + 2 * lane, o[b][2 * i], o[b][2 * i + 1]);
+        if (h == 0) store_pair(mine + 32 * DIM + 2 * lane, m, l);
+      }
+      if (!last_part(a.counters + part.first_piece, part.parts, &arrival)) continue;
+      if (busy) {
+        m = -INFINITY;
+        l = 0.0f;
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[b][i] = 0.0f;
+        for (uint32_t j = 0; j < part.parts; ++j) {
+          const float *from = a.partials + (size_t)part_slot(part.first_piece, j) * kPartFloats + wave * (32 * (DIM + 2));
+          float pm, pl;
+          load_pair(from + 32 * DIM + 2 * r, pm, pl);
+          if (pl == 0.0f) pm = -INFINITY;
+          const float next = fmaxf(m, pm);
+          const float keep = l != 0.0f ? exp2_fast(m - finite_max(next)) : 0.0f;
+          const float take = pl != 0.0f ? exp2_fast(pm - finite_max(next)) : 0.0f;
+          m = next;
+          l = l * keep + pl * take;
+#pragma unroll
+          for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              float v0, v1;
+              load_pair(from + (8 * b + i) * 128 + 2 * lane, v0, v1);
+              o[b][2 * i] = o[b][2 * i] * keep + v0 * take;
+              o[b][2 * i + 1] = o[b][2 * i + 1] * keep + v1 * take;
+            }
+        }
+      }
+    }
+    if (on) {
+      const float by = l == 0.0f ? 0.0f : 1.0f / l;
+      uint16_t *out = a.output + (size_t)(part.first_row + row0 + pi) * a.output_stride + (part.head * a.group + pg) * dim;
+#pragma unroll
+      for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const uint32_t d = 32 * b + 8 * j + 4 * h;
+          if (d < dim)
+            *(u32x2 *)(out + d) = u32x2{bf16_pair(o[b][4 * j] * by, o[b][4 * j + 1] * by),
+                                        bf16_pair(o[b][4 * j + 2] * by, o[b][4 * j + 3] * by)};
+        }
+    }
+  }
+}
+
+template <uint32_t FMT>
+hipError_t launch_dim(const AttendArgs &a, hipStream_t stream) {
+  const dim3 grid(a.workgroups), block(kThreads);
+  if (a.kv.head_dim <= 64) hipLaunchKernelGGL((attend_tile_kernel<FMT, 64>), grid, block, 0, stream, a);
+  else if (a.kv.head_dim <= 128) hipLaunchKernelGGL((attend_tile_kernel<FMT, 128>), grid, block, 0, stream, a);
+  else hipLaunchKernelGGL((attend_tile_kernel<FMT, 256>), grid, block, 0, stream, a);
+  return hipGetLastError();
+}
+
+}  // namespace
+
+hipError_t launch_attend_tile(const AttendArgs &a, hipStream_t stream) {
+  if (a.kv.format == SQ_KV_BF16) return launch_dim<SQ_KV_BF16>(a, stream);
+  if (a.kv.format == SQ_KV_INT8) return launch_dim<SQ_KV_INT8>(a, stream);
+  return launch_dim<SQ_KV_E4M3>(a, stream);
+}
+
+}  // namespace sq::kern

@@ -256,6 +256,11 @@ constexpr uint32_t kAttendMaxGroup = 64;
 // The floats of partials and the counters that `workgroups` workgroups on tiles of tile_rows rows use.
 uint64_t attend_partials(uint32_t tile_rows, uint32_t head_dim, uint32_t workgroups);
 uint64_t attend_counters(uint32_t workgroups);
+// Tiles of few rows: 16, 32, or (heads of at most 128 values) 64.
+constexpr uint32_t kAttendWideRows = 128;
+inline uint32_t attend_few_rows(uint32_t head_dim) { return head_dim <= 128 ? 64 : 32; }
 hipError_t launch_attend_rows(uint32_t tile_rows, const AttendArgs &args, hipStream_t stream);
+// Tiles of kAttendWideRows rows.
+hipError_t launch_attend_tile(const AttendArgs &args, hipStream_t stream);
 
 }  // namespace sq::kern
