@@ -530,22 +530,22 @@ typedef struct sq_attention_shape {
 } sq_attention_shape;
 /* A plan for batches of at most `sequences` sequences and `rows` rows; chunk_rows, the most new rows that one sequence
  * usually has, picks the tile (any batch is computed right whatever it is). tile_rows: the rows times query heads of one
- * key head that a tile holds (16, 32, 64 or 128). partials and counters: the bytes of workspace; the counters are zero
- * at allocation and every call returns them to zero, and one workspace serves one stream at a time. */
+ * key head that a tile holds (16, 32, 64 or 128); waves: of a workgroup. partials: the bytes of workspace, which may hold anything before a call;
+ * one workspace serves one stream at a time. */
 typedef struct sq_attention_plan {
   sq_attention_shape shape;
-  uint32_t sequences, rows, chunk_rows, tile_rows, workgroups;
-  uint64_t partials, counters;
+  uint32_t sequences, rows, chunk_rows, tile_rows, waves, workgroups;
+  uint64_t partials;
 } sq_attention_plan;
 typedef struct sq_attention_buffers {
   sq_head_rows query, output; /* output may be the query itself, and otherwise shares no element with it */
-  sq_buffer partials, counters;
+  sq_buffer partials;         /* 16-byte aligned */
 } sq_attention_buffers;
 int sq_attention_plan_for(const sq_device *device, const sq_attention_shape *shape, uint32_t sequences, uint32_t rows,
                           uint32_t chunk_rows, sq_attention_plan *out);
 /* The work (tiles of 64 keys over every sequence, key head and tile of rows) is split evenly over the workgroups
- * whatever the lengths are; a tile of rows whose keys several workgroups share is joined by the last of them, in key
- * order, so a batch repeats its bits from run to run. How the work falls depends on the whole batch, so a row's output
+ * whatever the lengths are; a second launch joins the tiles of rows whose keys several workgroups shared, in key order,
+ * so a batch repeats its bits from run to run. How the work falls depends on the whole batch, so a row's output
  * bits may differ between batches. */
 int sq_attention_add(void *graph, const sq_attention_buffers *buffers, const sq_kv_cache *cache,
                      const sq_kv_batch *batch, const sq_attention_plan *plan);

@@ -261,15 +261,20 @@ AttentionPlan Attention::plan(const DeviceCapabilities &device, const AttentionS
   const uint64_t packed = uint64_t{chunkRows} * shape.group();
   out.tileRows = kern::kAttendWideRows;
   for (uint32_t few = kern::attend_few_rows(shape.kv.headDim); few >= 16 && few >= packed; few /= 2) out.tileRows = few;
-  const uint32_t units = device.computeUnits ? device.computeUnits : 256;
-  out.workgroups = (2 * units + 7) / 8 * 8;
-  out.partials = kern::attend_partials(out.tileRows, shape.kv.headDim, out.workgroups) * 4;
-  out.counters = kern::attend_counters(out.workgroups) * 4;
+  const uint32_t format = uint32_t(shape.kv.format);
+  const uint32_t units = ((device.computeUnits ? device.computeUnits : 256) + 7) / 8 * 8;
+  // Few sequences: workgroups of twice the waves, one a compute unit, halve a unit's parts and its waves' turns.
+  const bool few = out.tileRows != kern::kAttendWideRows &&
+                   kern::attend_rows_resident(out.tileRows, shape.kv.headDim, format) > 1 &&
+                   uint64_t{sequences} * shape.kv.kvHeads * 2 <= units;
+  out.waves = few ? 8 : 4;
+  out.workgroups = units * kern::attend_resident(out.tileRows, out.waves, shape.kv.headDim, format);
+  out.partials = kern::attend_partials(out.tileRows, shape.kv.headDim, out.workgroups);
   return out;
 }
 
 void Attention::add(hipStream_t graph, const HeadRowsView &query, const HeadRowsView &output, Buffer partials,
-                    Buffer counters, const KvCache &cache, const KvBatch &batch, const AttentionPlan &plan) {
+                    const KvCache &cache, const KvBatch &batch, const AttentionPlan &plan) {
   const kern::KvArgs kv = kvArgs(cache, batch);
   const AttentionShape &shape = plan.shape;
   if (!(cache.shape == shape.kv)) throw std::invalid_argument("the attention plan is another cache's");
@@ -282,17 +287,28 @@ void Attention::add(hipStream_t graph, const HeadRowsView &query, const HeadRows
                        o = headRows(output, batch.rows, shape.kv.headDim, "output rows");
   requireInPlace(query, output, "attention");
   requireBytes(partials, plan.partials, "attention partials");
-  requireBytes(counters, plan.counters, "attention counters");
-  if (!aligned(partials, 16) || !aligned(counters, 4))
-    throw std::invalid_argument("attention partials are 16-byte aligned, the counters 4-byte");
-  const kern::AttendArgs args{kv,         q.rows,       o.rows,      q.stride,
-                              o.stride,   shape.group(), shape.causal, shape.window,
-                              float(double(shape.scale) * std::numbers::log2e), partials.as<float>(),
-                              counters.as<uint32_t>(), plan.workgroups};
+  if (!aligned(partials, 16)) throw std::invalid_argument("attention partials are 16-byte aligned");
+  const kern::AttendArgs args{kv,
+                              q.rows,
+                              o.rows,
+                              q.stride,
+                              o.stride,
+                              shape.group(),
+                              shape.causal,
+                              shape.window,
+                              float(double(shape.scale) * std::numbers::log2e),
+                              partials.as<float>(),
+                              partials.as<uint8_t>() + plan.partials - (plan.workgroups + 1) * kern::kAttendNoteBytes,
+                              plan.workgroups};
+  // A batch of few units, none longer than a workgroup takes at least, is cut nowhere (attend.hpp), and leaves no parts.
+  const uint64_t units = (batch.rows / (plan.tileRows / shape.group()) + batch.sequences) * uint64_t{shape.kv.kvHeads};
+  const bool whole = plan.tileRows != kern::kAttendWideRows && batch.sequences <= 64 && units * 4 <= plan.workgroups &&
+                     uint64_t{batch.pagesPerSequence} * cache.shape.pageRows + 128 <= kern::kAttendLeast;
   const OnStreamDevice on(graph);
   launched(plan.tileRows == kern::kAttendWideRows ? kern::launch_attend_tile(args, graph)
-                                                  : kern::launch_attend_rows(plan.tileRows, args, graph),
+                                                  : kern::launch_attend_rows(plan.tileRows, plan.waves, args, graph),
            "attention");
+  if (!whole) launched(kern::launch_attend_join(plan.tileRows, args, graph), "attention join");
 }
 
 }  // namespace sq::ops

@@ -76,14 +76,14 @@ struct AttentionShape {
 };
 struct AttentionPlan {
   AttentionShape shape;
-  uint32_t sequences = 0, rows = 0, chunkRows = 0, tileRows = 0, workgroups = 0;
-  uint64_t partials = 0, counters = 0;
+  uint32_t sequences = 0, rows = 0, chunkRows = 0, tileRows = 0, waves = 0, workgroups = 0;
+  uint64_t partials = 0;   // bytes of workspace
 };
 struct Attention {
   static AttentionPlan plan(const DeviceCapabilities &device, const AttentionShape &shape, uint32_t sequences,
                             uint32_t rows, uint32_t chunkRows);
   static void add(hipStream_t graph, const HeadRowsView &query, const HeadRowsView &output, Buffer partials,
-                  Buffer counters, const KvCache &cache, const KvBatch &batch, const AttentionPlan &plan);
+                  const KvCache &cache, const KvBatch &batch, const AttentionPlan &plan);
 };
 
 }  // namespace sq::ops

@@ -646,18 +646,20 @@ sq_attention_plan cattention(const AttentionPlan &p) {
   out.rows = p.rows;
   out.chunk_rows = p.chunkRows;
   out.tile_rows = p.tileRows;
+  out.waves = p.waves;
   out.workgroups = p.workgroups;
   out.partials = p.partials;
-  out.counters = p.counters;
   return out;
 }
 // The plan a caller holds, rebuilt for the compute units its workgroups say and checked.
 AttentionPlan attentionPlan(const sq_attention_plan &p) {
-  const AttentionPlan out = Attention::plan(DeviceCapabilities{p.workgroups / 2}, attentionShape(p.shape), p.sequences,
-                                            p.rows, p.chunk_rows);
+  const AttentionShape shape = attentionShape(p.shape);
+  const uint32_t each =
+      sq::kern::attend_resident(p.tile_rows, p.waves, shape.kv.headDim, uint32_t(shape.kv.format));
+  const AttentionPlan out =
+      Attention::plan({p.workgroups / (each ? each : 1)}, shape, p.sequences, p.rows, p.chunk_rows);
   const sq_attention_plan same = cattention(out);
-  if (same.tile_rows != p.tile_rows || same.workgroups != p.workgroups || same.partials != p.partials ||
-      same.counters != p.counters)
+  if (same.tile_rows != p.tile_rows || same.waves != p.waves || same.workgroups != p.workgroups || same.partials != p.partials)
     throw std::invalid_argument("the attention plan's fields are not a plan's");
   return out;
 }
@@ -730,7 +732,7 @@ int sq_attention_add(void *graph, const sq_attention_buffers *b, const sq_kv_cac
   return guarded([&] {
     const sq_attention_buffers &buffers = need(b, "attention buffers");
     Attention::add(stream(graph), headRows(buffers.query), headRows(buffers.output), buf(buffers.partials),
-                   buf(buffers.counters), kvCache(need(cache, "cache")), kvBatch(need(batch, "batch")),
+                   kvCache(need(cache, "cache")), kvBatch(need(batch, "batch")),
                    attentionPlan(need(plan, "attention plan")));
   });
 }

@@ -2,19 +2,25 @@
 // rows whose keys several workgroups share.
 //
 // A unit is `fit` consecutive rows of one sequence (tile_rows / group of them, with the query heads of one key head)
-// against every key that they see, in tiles of 64 keys. Lengths live on the device and differ by orders of magnitude
-// within a batch, so no grid over (sequence, head, split) is even: instead the units lie end to end on a line, each as
-// long as its keys, and workgroup w takes the w-th of equal pieces of that line. A piece may end inside a unit; the unit
-// then has parts, which the workgroup that finishes last joins.
+// against every key that they see, in tiles of 64 keys. Unit m of a sequence ends at key e_m = position of its last row +
+// 1 (or the sequence's end), starts at key s_m (its first row's window), and is e_m - s_m + 126 long: at least 64 for
+// each of its tiles, ceil(e_m / 64) - floor(s_m / 64) of them, and a little for its fixed cost. Lengths live on the
+// device and differ by orders of magnitude within a batch, so no grid over (sequence, head, split) is even. Two ways of
+// sharing the units out:
 //
-// Unit m of a sequence ends at key e_m = position of its last row + 1 (or the sequence's end), starts at key s_m (its
-// first row's window), and is e_m - s_m + 126 long: at least 64 for each of its tiles, ceil(e_m / 64) - floor(s_m / 64)
-// of them, and a little for its fixed cost. The lengths are linear in m up to the clamps at both ends, so their prefix
-// sums have a closed form, and a workgroup finds its place by a search over the sequences' sums (in LDS) and one over m,
-// in the few hundred instructions that a walk over the units would spend on a handful of them. Offset o of a unit's line
-// lies before tile ceil(o / 64), or past its last tile.
+//  - Few units (a quarter of the workgroups or fewer, all of a sequence's about as long, or short): each is cut into equal parts,
+//    as many as give no part more than the share, and a workgroup takes one part. The share is the work over the
+//    workgroups that cutting leaves whole, so there are enough of them. One token over 700 keys of 8 key heads: 10 us,
+//    where a line (below) cuts units at odd places and gives most workgroups two parts, one after the other: 16 us.
+//  - Otherwise the units lie end to end on a line, and workgroup w takes the w-th of equal pieces of it. A piece may end
+//    inside a unit, which then has parts. The lengths are linear in m up to the clamps at both ends, so their prefix sums
+//    have a closed form, and a workgroup finds its place by a search over the sequences' sums (in LDS) and one over m.
+//    Offset o of a unit lies before its tile ceil(o / 64), or past its last tile.
+//
+// Parts go to the workspace, and a second launch (attend_join.hip) joins them.
 #pragma once
 #include "batch.hpp"
+#include "device.hpp"
 
 namespace sq::kern {
 
@@ -32,9 +38,20 @@ __device__ __forceinline__ int64_t clamped_sum(int lo, int a, int r, int m) {
 // A value that every lane of the wave holds, in scalar registers.
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
 __device__ __forceinline__ uint32_t uniform(uint32_t v) { return (uint32_t)uniform((int)v); }
+__device__ __forceinline__ float uniform(float v) { return __int_as_float(uniform(__float_as_int(v))); }
 __device__ __forceinline__ int64_t uniform(int64_t v) {
   return (int64_t)(((uint64_t)uniform((uint32_t)((uint64_t)v >> 32)) << 32) | uniform((uint32_t)v));
 }
+
+// a / b for a >= 0, b > 0 and a quotient below 2^50: the doubles' quotient is within one of it, and two multiplications
+// settle which (a 64-bit integer division is a hundred instructions in a row).
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  int64_t q = (int64_t)((double)a / (double)b);
+  if (q * b > a) --q;
+  if ((q + 1) * b <= a) ++q;
+  return q;
+}
+__device__ __forceinline__ int64_t quotient_up(int64_t a, int64_t b) { return quotient(a + b - 1, b); }
 
 // One sequence's units.
 struct Units {
@@ -63,134 +80,249 @@ __device__ __forceinline__ Units units_of(const AttendArgs &a, const Sequence &q
   return {(int)q.rows, q.keys, q.keys - (int)q.rows, fit, ((int)q.rows + fit - 1) / fit, window, a.causal != 0};
 }
 
-// The line: prefix[s] is where sequence s starts, prefix[sequences] its end; share is a workgroup's piece of it.
-struct Line {
-  const int64_t *prefix;
-  int64_t total;
-  int64_t share;
-  uint32_t active;   // workgroups with a piece
-};
-
-// Every thread of the workgroup takes part. `prefix` is LDS for sequences + 1 values, `part` for a value a wave. least:
-// the shortest piece worth a workgroup (at least a tile).
-template <int THREADS>
-__device__ __forceinline__ Line make_line(const AttendArgs &a, int fit, int least, int64_t *prefix, int64_t *part) {
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  int64_t carry = 0;
-  for (uint32_t s0 = 0; s0 < a.kv.sequences; s0 += THREADS) {
-    const uint32_t s = s0 + threadIdx.x;
-    int64_t v = s < a.kv.sequences ? units_of(a, sequence_of(a.kv, s), fit).total() * a.kv.kv_heads : 0;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-      const int64_t u = __shfl_up(v, d);
-      if (lane >= (uint32_t)d) v += u;
-    }
-    if (lane == 63) part[wave] = v;
-    __syncthreads();
-    int64_t all = 0;
-#pragma unroll
-    for (int w = 0; w < THREADS / 64; ++w) {
-      if ((uint32_t)w < wave) v += part[w];
-      all += part[w];
-    }
-    if (s < a.kv.sequences) prefix[s + 1] = carry + v;
-    carry += all;
-    __syncthreads();
-  }
-  if (threadIdx.x == 0) prefix[0] = 0;
-  __syncthreads();
-  carry = uniform(carry);
-  const int64_t even = (carry + a.workgroups - 1) / a.workgroups, share = even > least ? even : least;
-  return {prefix, carry, share, (uint32_t)((carry + share - 1) / share)};
-}
-
-// The piece of workgroup `block`. Pieces next to each other on the line share keys (units of one key head), so they go
-// to workgroups of one XCD (consecutive workgroups go round the eight), whose L2 then holds them once. Past the last:
-// a number past line.active.
-__device__ __forceinline__ uint32_t piece_of(const Line &line, uint32_t block) {
-  return block % 8 * ((line.active + 7) / 8) + block / 8;
-}
-
 // A unit's part that one workgroup runs: tiles [t0, t1) of the unit's, `parts` parts in all of which this is `part`.
 struct Part {
   Units units;
   uint32_t sequence, head, first_row;   // first_row: of the sequence, in the batch
   int m, t0, t1;
-  uint32_t part, parts, first_piece;    // first_piece: the workgroup piece that holds part 0
+  uint32_t part, parts, first_piece;    // first_piece: the workgroup's number that holds part 0
 };
-// The part at x < end on the line (wave-uniform), and x moved past it.
-__device__ __forceinline__ Part next_part(const AttendArgs &a, const Line &line, int fit, int64_t &x, int64_t end,
-                                          uint32_t piece) {
-  uint32_t lo = 0, hi = a.kv.sequences;   // the last sequence that starts at or before x
-  while (hi - lo > 1) {
-    const uint32_t mid = (lo + hi) / 2;
-    if (uniform(line.prefix[mid]) <= x) lo = mid;
-    else hi = mid;
-  }
-  Part p;
-  p.sequence = lo;
-  const Sequence q = sequence_of(a.kv, p.sequence);
-  p.units = units_of(a, q, fit);
-  p.first_row = q.first;
-  const int64_t one = p.units.total();
-  int64_t rest = x - uniform(line.prefix[p.sequence]);
-  p.head = (uint32_t)(rest / one);
-  rest -= one * p.head;
-  int mlo = 0, mhi = p.units.count;
-  while (mhi - mlo > 1) {
-    const int mid = (mlo + mhi) / 2;
-    if (p.units.before(mid) <= rest) mlo = mid;
-    else mhi = mid;
-  }
-  p.m = mlo;
-  const int64_t from = rest - p.units.before(mlo), length = p.units.length(mlo);
-  const int64_t to = length < from + (end - x) ? length : from + (end - x);
-  const int tiles = p.units.tiles(mlo);
-  const auto tile_at = [&](int64_t o) {
-    const int64_t t = (o + kKeyTile - 1) / kKeyTile;
-    return t < tiles ? (int)t : tiles;
-  };
-  p.t0 = tile_at(from);
-  p.t1 = tile_at(to);
-  // The parts of a unit are those that start at or before its last tile: a piece is at least a tile long, so each of
-  // them has one.
-  const int64_t unit = x - from;
-  p.first_piece = (uint32_t)(unit / line.share);
-  p.parts = (uint32_t)((unit + (int64_t)kKeyTile * (tiles - 1)) / line.share) - p.first_piece + 1;
-  p.part = piece - p.first_piece;
-  x += to - from;
-  return p;
-}
 
 // A part's place in the workspace. A piece holds at most two parts of shared units: one that an earlier piece began, and
-// one that it begins itself, of which there can be one only, so that the piece's counter counts that unit's parts.
+// one that it begins itself, of which there can be one only. (An even part may be empty, where a unit has fewer tiles
+// than parts: it is stored all the same.) A part is its blocks of 16 rows (32 in the wide tile) one after the other: the
+// accumulators as vectors of four, [vector][lane], then each row's maximum and sum.
 __device__ __forceinline__ uint32_t part_slot(uint32_t first_piece, uint32_t part) {
   return 2 * (first_piece + part) + (part == 0 ? 1 : 0);
 }
+// The first of the four values that a lane's accumulators of vector v are: in a block of 16 rows, where lane (kq, r) holds
+// accumulator t = run j + d as value d of run 4 kq + j; and in one of 32 rows, where lane (h, r) holds 4 j + i of block b
+// as value 32 b + 8 j + 4 h + i.
+__device__ __forceinline__ uint32_t few_value(uint32_t v, uint32_t lane, uint32_t run) {
+  return run * (4 * (lane >> 4) + 4 * v / run) + 4 * v % run;
+}
+__device__ __forceinline__ uint32_t wide_value(uint32_t v, uint32_t lane) {
+  return 32 * (v / 4) + 8 * (v % 4) + 4 * (lane >> 5);
+}
+// What the join wants to know of the shared unit that a piece began: parts below 2 where it began none. Behind the parts
+// in the workspace, and behind the pieces' notes one whose `parts` is the number of pieces.
+struct UnitNote {
+  uint32_t parts, live, row, head;   // live: its rows times query heads; row: its first, in the batch
+};
+__device__ __forceinline__ UnitNote *unit_notes(const AttendArgs &a) { return (UnitNote *)a.notes; }
 
-// Announces this workgroup's part, whose stores (agent-scope, so they lie past the XCD's own L2) come before; true in
-// the workgroup that arrives last, which then sees every part through agent-scope loads. As in split_reduce: each wave
-// waits for its own stores before the barrier, and the counter returns to zero.
-__device__ __forceinline__ bool last_part(uint32_t *counter, uint32_t parts, uint32_t *arrival) {
-  __builtin_amdgcn_s_waitcnt(0);
-  __syncthreads();
-  if (threadIdx.x == 0) {
-    const uint32_t n = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    if (n == parts - 1) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    *arrival = n;
+constexpr uint32_t kNowhere = 0x7FFFFFF0u;   // past every resource's range: loads zeros, and stores nothing
+
+typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf16x2;
+__device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
+  return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});
+}
+
+__device__ __forceinline__ float wave_sum(float v) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
+  return v;
+}
+__device__ __forceinline__ int64_t wave_sum(int64_t v) {
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d);
+  return v;
+}
+__device__ __forceinline__ int from_lane(int v, uint32_t lane) { return __builtin_amdgcn_readlane(v, (int)lane); }
+__device__ __forceinline__ uint32_t from_lane(uint32_t v, uint32_t lane) { return (uint32_t)from_lane((int)v, lane); }
+
+// The workgroup's number among `active` ones with work (`active` or more: none). Numbers next to each other share keys
+// (units of one key head), so they go to workgroups of one XCD (consecutive workgroups go round the eight), whose L2 then
+// holds them once.
+__device__ __forceinline__ uint32_t piece_of(uint32_t active, uint32_t block) {
+  const uint32_t each = (active + 7) / 8;
+  return block / 8 < each ? block % 8 * each + block / 8 : active;
+}
+
+// LDS for the line.
+constexpr uint32_t kCached = 256;   // sequences whose rows and keys stay in LDS
+template <int THREADS>
+struct LineShared {
+  int64_t prefix[kMaxSequences + 1];   // where each sequence starts
+  int64_t waves[THREADS / 64];
+  Sequence sequence[kCached];
+};
+
+// A workgroup's work: one even part (even), or the piece [x, end) of the line.
+struct Work {
+  bool even, pending;
+  uint32_t piece;
+  Part only;
+  const int64_t *prefix;
+  const Sequence *cached;
+  int64_t share, x, end;
+
+  uint32_t active;   // workgroups with work
+
+  // The next part, or false.
+  __device__ __forceinline__ bool next(const AttendArgs &a, int fit, Part &p) {
+    if (even) {
+      p = only;
+      const bool more = pending;
+      pending = false;
+      return more;
+    }
+    do {
+      if (x >= end) return false;
+      step(a, fit, p);
+    } while (p.t1 <= p.t0);
+    return true;
   }
+  // The notes that the join reads, once all of the workgroup's parts are stored: of the unit it began (began.parts 0:
+  // none), and one workgroup's of how many there are.
+  __device__ __forceinline__ void leave(const AttendArgs &a, const UnitNote &began) const {
+    if (threadIdx.x) return;
+    if (piece < active) unit_notes(a)[piece] = began;
+    if (blockIdx.x == 0) unit_notes(a)[a.workgroups].parts = active;
+  }
+  // p in scalar registers, whichever way it came.
+  static __device__ __forceinline__ Part settled(const AttendArgs &a, int fit, const Part &p) {
+    const Sequence q{uniform(p.first_row), (uint32_t)uniform(p.units.rows), uniform(p.units.keys)};
+    return {units_of(a, q, fit),   uniform(p.sequence), uniform(p.head),  q.first, uniform(p.m), uniform(p.t0), uniform(p.t1),
+            uniform(p.part), uniform(p.parts),    uniform(p.first_piece)};
+  }
+  // The part of the line at x, and x moved past it.
+  __device__ __forceinline__ void step(const AttendArgs &a, int fit, Part &p) {
+    uint32_t lo = 0, hi = a.kv.sequences;   // the last sequence that starts at or before x
+    while (hi - lo > 1) {
+      const uint32_t mid = (lo + hi) / 2;
+      if (uniform(prefix[mid]) <= x) lo = mid;
+      else hi = mid;
+    }
+    p.sequence = lo;
+    Sequence q = lo < kCached ? cached[lo] : sequence_of(a.kv, lo);
+    q = {uniform(q.first), uniform(q.rows), uniform(q.keys)};
+    p.units = units_of(a, q, fit);
+    p.first_row = q.first;
+    const int64_t one = p.units.total();
+    int64_t rest = x - uniform(prefix[lo]);
+    p.head = (uint32_t)uniform(quotient(rest, one));
+    rest -= one * p.head;
+    int mlo = 0, mhi = p.units.count;
+    while (mhi - mlo > 1) {
+      const int mid = (mlo + mhi) / 2;
+      if (p.units.before(mid) <= rest) mlo = mid;
+      else mhi = mid;
+    }
+    p.m = mlo;
+    const int64_t from = rest - p.units.before(mlo), length = p.units.length(mlo);
+    const int64_t to = length < from + (end - x) ? length : from + (end - x);
+    const int tiles = p.units.tiles(mlo);
+    const auto tile_at = [&](int64_t o) {
+      const int64_t t = (o + kKeyTile - 1) / kKeyTile;
+      return t < tiles ? (int)t : tiles;
+    };
+    p.t0 = tile_at(from);
+    p.t1 = tile_at(to);
+    // The parts of a unit are those that start at or before its last tile: a piece is at least a tile long, so each of
+    // them has one.
+    const int64_t unit = x - from;
+    p.first_piece = (uint32_t)uniform(quotient(unit, share));
+    p.parts = (uint32_t)uniform(quotient(unit + (int64_t)kKeyTile * (tiles - 1), share)) - p.first_piece + 1;
+    p.part = piece - p.first_piece;
+    x += to - from;
+  }
+};
+
+// Every thread of the workgroup takes part. least: the shortest piece or part worth a workgroup (four tiles at least).
+template <int THREADS>
+__device__ __forceinline__ Work make_work(const AttendArgs &a, int fit, int least, LineShared<THREADS> &shared) {
+  constexpr int kWaves = THREADS / 64;
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, count = a.kv.sequences;
+  Work w{};
+  if (count <= 64) {
+    // Each wave for itself, a sequence a lane, in registers.
+    const Sequence q = lane < count ? sequence_of(a.kv, lane) : Sequence{0u, 0u, 0};
+    const Units u = units_of(a, q, fit);
+    const float heads = (float)a.kv.kv_heads, units = (float)u.count, last = u.count ? (float)u.length(u.count - 1) : 0.0f,
+                first = u.count ? (float)u.length(0) : 0.0f;
+    const float number = uniform(heads * wave_sum(units)), most = uniform(heads * wave_sum(units * last)),
+                work = uniform(heads * wave_sum(units * 0.5f * (first + last)));
+    if (number * 4 <= (float)a.workgroups && (most <= work * 1.25f || most <= number * (float)least)) {
+      // The share that leaves every unit's last part room: units ceil(length / share) <= workgroups. The sums are off by
+      // 2^-18 at most, the share made larger by as much.
+      const int share = max(least, (int)(most * (1 + 0x1p-18f) / ((float)a.workgroups - number)) + 1);
+      const uint32_t parts = u.count ? (uint32_t)(u.length(u.count - 1) + share - 1) / (uint32_t)share : 0u;
+      const uint32_t mine = parts * (uint32_t)u.count * a.kv.kv_heads;
+      uint32_t upto = mine;
+#pragma unroll
+      for (int d = 1; d < 64; d <<= 1) {
+        const uint32_t below = (uint32_t)__shfl_up((int)upto, d);
+        if (lane >= (uint32_t)d) upto += below;
+      }
+      w.even = true;
+      w.active = from_lane(upto, 63);
+      w.piece = piece_of(w.active, blockIdx.x);
+      w.pending = w.piece < w.active;
+      if (!w.pending) return w;
+      // The last sequence that starts at or before the piece: one with units, as the next starts past it.
+      const uint32_t before = upto - mine;
+      const uint32_t s = (uint32_t)__popcll(__ballot(before <= w.piece)) - 1;
+      Part &p = w.only;
+      p.sequence = s;
+      p.units = units_of(a, Sequence{from_lane(q.first, s), from_lane(q.rows, s), from_lane(q.keys, s)}, fit);
+      p.first_row = from_lane(q.first, s);
+      p.parts = from_lane(parts, s);
+      const uint32_t rest = w.piece - from_lane(before, s), unit = rest / p.parts;
+      p.part = rest - unit * p.parts;
+      p.head = unit / (uint32_t)p.units.count;
+      p.m = (int)(unit - p.head * (uint32_t)p.units.count);
+      // The unit's tiles over its parts, the first ones taking what is left over. (A unit much shorter than its
+      // sequence's last may leave parts empty: they count all the same.)
+      const uint32_t tiles = (uint32_t)p.units.tiles(p.m), each = tiles / p.parts, over = tiles - each * p.parts;
+      p.t0 = (int)(each * p.part + min(p.part, over));
+      p.t1 = p.t0 + (int)(each + (p.part < over ? 1 : 0));
+      p.first_piece = w.piece - p.part;
+      return w;
+    }
+  }
+  int64_t carry = 0;
+  for (uint32_t s0 = 0; s0 < count; s0 += THREADS) {
+    const uint32_t s = s0 + threadIdx.x;
+    int64_t v = 0;
+    if (s < count) {
+      const Sequence q = sequence_of(a.kv, s);
+      if (s < kCached) shared.sequence[s] = q;
+      v = units_of(a, q, fit).total() * a.kv.kv_heads;
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int64_t below = __shfl_up(v, d);
+      if (lane >= (uint32_t)d) v += below;
+    }
+    if (s0) __syncthreads();   // the last turn's sums have been read
+    if (lane == 63) shared.waves[wave] = v;
+    __syncthreads();
+    int64_t all = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+      if ((uint32_t)i < wave) v += shared.waves[i];
+      all += shared.waves[i];
+    }
+    if (s < count) shared.prefix[s + 1] = carry + v;
+    carry += all;
+  }
+  if (threadIdx.x == 0) shared.prefix[0] = 0;
   __syncthreads();
-  return *arrival == parts - 1;
+  const int64_t total = uniform(carry), even_share = uniform(quotient_up(total, a.workgroups));
+  w.prefix = shared.prefix;
+  w.cached = shared.sequence;
+  w.share = even_share > least ? even_share : least;
+  w.active = (uint32_t)uniform(quotient_up(total, w.share));
+  w.piece = piece_of(w.active, blockIdx.x);
+  w.x = w.share * w.piece;
+  w.end = w.x + w.share < total ? w.x + w.share : total;
+  return w;
 }
-__device__ __forceinline__ void store_pair(float *at, float a, float b) {
-  const uint64_t v = (uint64_t)__float_as_uint(a) | ((uint64_t)__float_as_uint(b) << 32);
-  __hip_atomic_store((uint64_t *)at, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ void load_pair(const float *at, float &a, float &b) {
-  const uint64_t v = __hip_atomic_load((const uint64_t *)at, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-  a = __uint_as_float((uint32_t)v);
-  b = __uint_as_float((uint32_t)(v >> 32));
-}
+
+// p / group for a packed row p < 128 and a group of at most 64: the fp32 quotient of p + 1/2 is a 128th or more from a
+// whole number, its error far less.
+__device__ __forceinline__ int row_of(int p, float by_group) { return (int)(((float)p + 0.5f) * by_group); }
 
 // 2^x by the hardware instruction (an ulp; results below the normal range flush to zero, far below any weight that
 // counts).

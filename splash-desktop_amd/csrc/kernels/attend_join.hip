@@ -1,0 +1,96 @@
+// The join of units whose keys several workgroups shared: output = sum_j e^(m_j - m) O_j / sum_j e^(m_j - m) l_j over a
+// unit's parts in key order, m their largest maximum. A launch of its own after the attention's: a workgroup of that one
+// would find out that it is the last of its unit's only after its stores and an atomic have gone past the XCDs' caches
+// (3 us a part), and then join all of the unit's rows alone (one token over 131072 int8 keys, 31 parts a unit: 8 us in
+// all), where here every vector of every unit has a wave, and all parts' loads are in flight at once.
+#include "attend.hpp"
+
+namespace sq::kern {
+namespace {
+
+constexpr int kAtOnce = 16, kVectors = 2;   // parts' loads in flight, and the vectors a wave joins
+
+// A wave of blockIdx.x's unit (the one that piece began) joins kVectors of the unit's vectors (attend.hpp: the layout of
+// a part). DIM is the head's values as computed.
+template <bool WIDE>
+__global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, uint32_t dim_computed, uint32_t tile_rows) {
+  const uint32_t rows = WIDE ? 32 : 16, vectors = dim_computed / (WIDE ? 8 : 16);
+  const uint32_t lane = threadIdx.x & 63, item = uniform(blockIdx.y * 4 + (threadIdx.x >> 6));
+  const uint32_t block = item / (vectors / kVectors), first = kVectors * (item % (vectors / kVectors));
+  const UnitNote *notes = unit_notes(a);
+  if (blockIdx.x >= notes[a.workgroups].parts) return;
+  const UnitNote note = notes[blockIdx.x];
+  if (note.parts < 2 || block * rows >= note.live) return;
+  const uint32_t p = block * rows + lane % rows;
+  const bool on = p < note.live;
+  const uint32_t part_floats = tile_rows * (dim_computed + 2), block_floats = rows * (dim_computed + 2);
+  float m = -INFINITY, l = 0.0f;
+  f32x4 sum[kVectors] = {};
+  for (uint32_t j = 0; j < note.parts; j += kAtOnce) {
+    float pm[kAtOnce], pl[kAtOnce];
+    f32x4 got[kAtOnce][kVectors];
+#pragma unroll
+    for (int d = 0; d < kAtOnce; ++d) {
+      // Past the last part the resource is empty: zeros, and nothing read.
+      const bool there = j + d < note.parts;
+      const float *from = a.partials + (size_t)part_slot(blockIdx.x, there ? j + d : 0) * part_floats +
+                          (size_t)block * block_floats;
+      const __amdgpu_buffer_rsrc_t r = buffer_rsrc(from, there ? block_floats * 4 : 0);
+      const u32x2 two = buffer_b64<0>(r, on ? (rows * dim_computed + 2 * (lane % rows)) * 4 : kNowhere, 0);
+      pm[d] = __uint_as_float(two[0]);
+      pl[d] = __uint_as_float(two[1]);
+#pragma unroll
+      for (int v = 0; v < kVectors; ++v)
+        got[d][v] = __builtin_bit_cast(f32x4, buffer_b128<0>(r, on ? ((first + v) * 64 + lane) * 16 : kNowhere, 0));
+    }
+    float next = m;
+#pragma unroll
+    for (int d = 0; d < kAtOnce; ++d) next = pl[d] == 0.0f ? next : fmaxf(next, pm[d]);
+    // A part that saw nothing adds nothing, even to a row whose maximum is infinite.
+    const float keep = l == 0.0f ? 0.0f : exp2_fast(m - finite_max(next));
+    m = next;
+    l *= keep;
+#pragma unroll
+    for (int v = 0; v < kVectors; ++v) sum[v] *= keep;
+#pragma unroll
+    for (int d = 0; d < kAtOnce; ++d) {
+      if (pl[d] == 0.0f) continue;
+      const float by = exp2_fast(pm[d] - finite_max(next));
+      l += pl[d] * by;
+#pragma unroll
+      for (int v = 0; v < kVectors; ++v) sum[v] += got[d][v] * by;
+    }
+  }
+  if (!on) return;
+  const float by = l == 0.0f ? 0.0f : 1.0f / l;
+  const uint32_t i = (uint32_t)row_of((int)p, 1.0f / (float)a.group), g = p - i * a.group;
+  uint16_t *out = a.output + (size_t)(note.row + i) * a.output_stride + (note.head * a.group + g) * a.kv.head_dim;
+#pragma unroll
+  for (int v = 0; v < kVectors; ++v) {
+    const uint32_t value = WIDE ? wide_value(first + v, lane) : few_value(first + v, lane, dim_computed / 16);
+    if (value < a.kv.head_dim)
+      *(u32x2 *)(out + value) = u32x2{bf16_pair(sum[v][0] * by, sum[v][1] * by), bf16_pair(sum[v][2] * by, sum[v][3] * by)};
+  }
+}
+
+uint32_t computed(uint32_t head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
+
+}  // namespace
+
+uint64_t attend_partials(uint32_t tile_rows, uint32_t head_dim, uint32_t workgroups) {
+  // Two parts a workgroup, and a note of the unit it began with one more for how many there are.
+  return (2 * uint64_t{workgroups} * tile_rows * (computed(head_dim) + 2)) * sizeof(float) +
+         (uint64_t{workgroups} + 1) * sizeof(UnitNote);
+}
+
+hipError_t launch_attend_join(uint32_t tile_rows, const AttendArgs &a, hipStream_t stream) {
+  const bool wide = tile_rows == kAttendWideRows;
+  const uint32_t dim = computed(a.kv.head_dim);
+  const uint32_t items = tile_rows / (wide ? 32 : 16) * (dim / (wide ? 8 : 16)) / kVectors;
+  const dim3 grid(a.workgroups, (items + 3) / 4);
+  if (wide) hipLaunchKernelGGL((attend_join_kernel<true>), grid, dim3(256), 0, stream, a, dim, tile_rows);
+  else hipLaunchKernelGGL((attend_join_kernel<false>), grid, dim3(256), 0, stream, a, dim, tile_rows);
+  return hipGetLastError();
+}
+
+}  // namespace sq::kern

@@ -16,16 +16,15 @@
 //
 // Softmax: each wave keeps its own running maximum, lane sums and accumulators, and raises the maximum (which costs
 // lane exchanges and a pass over the accumulators) only when a score exceeds it by 8 (a factor of 256, which fp32 sums
-// and bf16's exponent hold without loss); the four waves of a workgroup join at the end of a part.
+// and bf16's exponent hold without loss); the waves of a workgroup join at the end of a part, through LDS.
 #include "attend.hpp"
 #include "device.hpp"
 
 namespace sq::kern {
 namespace {
 
-constexpr int kWaves = 4, kThreads = 64 * kWaves, kStep = 32;   // keys a wave takes a step
+constexpr int kStep = 32;      // keys a wave takes a step
 constexpr float kRaise = 8.0f;
-constexpr uint32_t kNowhere = 0x7FFFFFF0u;   // past every resource's range: reads zero
 
 // Two of a key's values for each of two keys, regrouped: two keys of each of two values.
 __device__ __forceinline__ uint32_t low_halves(uint32_t k0, uint32_t k1) {
@@ -33,10 +32,6 @@ __device__ __forceinline__ uint32_t low_halves(uint32_t k0, uint32_t k1) {
 }
 __device__ __forceinline__ uint32_t high_halves(uint32_t k0, uint32_t k1) {
   return __builtin_amdgcn_perm(k1, k0, 0x07060302u);
-}
-typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf16x2;
-__device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
-  return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});
 }
 // Four codes as bf16, in their order.
 template <uint32_t FMT>
@@ -66,11 +61,10 @@ __device__ __forceinline__ float row_sum(float v) {
   return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// Sixteen keys of one page: where their values lie, and how many bytes of them there are to read.
+// Sixteen keys of one page: the first one's place in the cache, and how many there are to read (none in a hole).
 struct Keys16 {
-  const uint8_t *keys, *values;
-  const float *key_scales, *value_scales;
-  uint32_t bytes, scale_bytes;
+  size_t at;
+  uint32_t count;
 };
 
 // DIM: the head's values as computed (64, 128 or 256; values past head_dim are zero). MB: blocks of 16 rows.
@@ -104,20 +98,20 @@ struct Rows {
     }
   }
 
-  static __device__ __forceinline__ void load_keys(KeyTile &t, const Keys16 &k, int half, uint32_t row_bytes,
-                                                   uint32_t lane) {
-    const __amdgpu_buffer_rsrc_t r = buffer_rsrc(k.keys, k.bytes);
+  static __device__ __forceinline__ void load_keys(KeyTile &t, const KvArgs &kv, const Keys16 &k, int half,
+                                                   uint32_t row_bytes, uint32_t lane) {
+    const __amdgpu_buffer_rsrc_t r = buffer_rsrc(kv.keys + k.at * row_bytes, k.count * row_bytes);
 #pragma unroll
     for (int j = 0; j < kKeyLoads; ++j) {
       const uint32_t at = 64 * j + 16 * (lane >> 4);
       t.w[half][j] = buffer_b128(r, at < row_bytes ? (lane & 15) * row_bytes + at : kNowhere, 0);
     }
     if constexpr (kCodes)
-      t.scale[half] = __builtin_bit_cast(f32x4, buffer_b128(buffer_rsrc(k.key_scales, k.scale_bytes), 16 * (lane >> 4), 0));
+      t.scale[half] = __builtin_bit_cast(f32x4, buffer_b128(buffer_rsrc(kv.key_scales + k.at, k.count ? 64 : 0), 16 * (lane >> 4), 0));
   }
-  static __device__ __forceinline__ void load_values(ValueTile &t, const Keys16 &k, int half, uint32_t row_bytes,
-                                                     uint32_t lane) {
-    const __amdgpu_buffer_rsrc_t r = buffer_rsrc(k.values, k.bytes);
+  static __device__ __forceinline__ void load_values(ValueTile &t, const KvArgs &kv, const Keys16 &k, int half,
+                                                     uint32_t row_bytes, uint32_t lane) {
+    const __amdgpu_buffer_rsrc_t r = buffer_rsrc(kv.values + k.at * row_bytes, k.count * row_bytes);
     const uint32_t at = (lane & 15) * kRun * kBytes;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
@@ -139,7 +133,7 @@ struct Rows {
     }
     if constexpr (kCodes)
       t.scale[half] =
-          __builtin_bit_cast(f32x4, buffer_b128(buffer_rsrc(k.value_scales, k.scale_bytes), 16 * (lane >> 4), 0));
+          __builtin_bit_cast(f32x4, buffer_b128(buffer_rsrc(kv.value_scales + k.at, k.count ? 64 : 0), 16 * (lane >> 4), 0));
   }
 
   // The rows' values in the K operand's order: bf16 chain j takes values 32 j + 8 kq + e; of codes, whose 16-byte vector
@@ -212,29 +206,34 @@ __device__ __forceinline__ bool unbounded(const uint32_t (&w)[2][4][N]) {
   return any != 0;
 }
 
-template <uint32_t FMT, int DIM, int MB>
-__global__ __launch_bounds__(kThreads, DIM * MB <= (DIM == 256 ? 0 : FMT == SQ_KV_BF16 ? 128 : 256) ? 2 : 1) void attend_rows_kernel(AttendArgs a) {
-  using R = Rows<FMT, DIM, MB>;
-  constexpr bool kCodes = R::kCodes;
-  constexpr int kRun = R::kRun, kRegs = 4 * kRun, kChunk = 8, kChunks = kRegs / kChunk;
-  // A part in the workspace: its accumulators in the waves' register order, then its rows' maxima and sums.
-  constexpr int kPartFloats = MB * (kRegs * 64 + 32);
-  __shared__ int64_t prefix[kMaxSequences + 1], scan[kWaves];
-  __shared__ float joined[kWaves][kChunk][64], maxima[kWaves][MB][16], sums[kWaves][MB][16];
-  __shared__ uint32_t arrival;
-  const uint32_t lane = threadIdx.x & 63, r = lane & 15, kq = lane >> 4;
-  const uint32_t wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
-  const int fit = 16 * MB / (int)a.group;
-  const uint32_t dim = a.kv.head_dim, row_bytes = dim * R::kBytes;
-  const Line line = make_line<kThreads>(a, fit, 2 * kWaves * kStep, prefix, scan);
-  const uint32_t piece = piece_of(line, blockIdx.x);
-  if (blockIdx.x / 8 >= (line.active + 7) / 8 || piece >= line.active) return;
-  int64_t x = line.share * piece;
-  const int64_t end = x + line.share < line.total ? x + line.share : line.total;
+template <int MB, int WAVES>
+struct Shared {
+  LineShared<64 * WAVES> line;
+  f32x4 waves[WAVES][WAVES][64];   // of each wave 4 WAVES accumulators at once, a vector of four for each to sum
+  float maxima[WAVES][MB][16], sums[WAVES][MB][16];
+};
 
-  while (x < end) {
-    const Part part = next_part(a, line, fit, x, end, piece);
-    if (part.t1 <= part.t0) continue;
+template <uint32_t FMT, int DIM, int MB, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, (WAVES == 8 ? 2 : attend_rows_resident(16 * MB, DIM, FMT))) void
+attend_rows_kernel(AttendArgs a) {
+  using R = Rows<FMT, DIM, MB>;
+  constexpr int kWaves = WAVES, kThreads = 64 * WAVES, kJoin = 4 * WAVES;
+  constexpr bool kCodes = R::kCodes;
+  // Accumulator t = kRun j + d of a block is value d of run j.
+  constexpr int kRun = R::kRun, kRegs = 4 * kRun, kChunks = (kRegs + kJoin - 1) / kJoin;
+  constexpr int kVectors = kRegs < kJoin ? kRegs / 4 : kJoin / 4;   // of four accumulators, in a chunk
+  constexpr int kBlockFloats = 16 * (DIM + 2);   // of a part in the workspace
+  __shared__ Shared<MB, WAVES> shared;
+  const uint32_t lane = threadIdx.x & 63, r = lane & 15, kq = lane >> 4;
+  const uint32_t wave = uniform(threadIdx.x >> 6);
+  const int fit = 16 * MB / (int)a.group;
+  const float by_group = 1.0f / (float)a.group;
+  const uint32_t dim = a.kv.head_dim, row_bytes = dim * R::kBytes;
+  Work work = make_work<kThreads>(a, fit, (int)kAttendLeast, shared.line);
+  UnitNote began{};
+  Part next;
+  while (work.next(a, fit, next)) {
+    const Part part = Work::settled(a, fit, next);
     const Units &u = part.units;
     const int row0 = fit * part.m, rows = min(fit, u.rows - row0), live = rows * (int)a.group;
     const int unit_end = u.causal ? min(u.keys, u.base + row0 + rows) : u.keys;   // keys that any row sees
@@ -249,7 +248,7 @@ __global__ __launch_bounds__(kThreads, DIM * MB <= (DIM == 256 ? 0 : FMT == SQ_K
     int low[MB], high[MB];   // the keys this lane's rows see
 #pragma unroll
     for (int b = 0; b < MB; ++b) {
-      const int p = 16 * b + (int)r, i = p / (int)a.group, g = p - i * (int)a.group;
+      const int p = 16 * b + (int)r, i = row_of(p, by_group), g = p - i * (int)a.group;
       const int at = u.base + row0 + i;
       low[b] = u.window ? at - u.window + 1 : 0;
       high[b] = u.causal ? min(at + 1, u.keys) : u.keys;
@@ -263,35 +262,47 @@ __global__ __launch_bounds__(kThreads, DIM * MB <= (DIM == 256 ? 0 : FMT == SQ_K
       }
     }
 
-    // The 16 keys from k on: none if they lie past the unit's keys or in a hole.
-    const auto keys_at = [&](int k) __attribute__((always_inline)) {
-      const int n = min(16, k_end - k);
-      const uint32_t page =
-          n > 0 ? (uint32_t)__builtin_amdgcn_readfirstlane((int)page_of(a.kv, part.sequence, k)) : ~0u;
-      const bool there = page != ~0u;
-      const size_t at = (((size_t)(there ? page : 0) * a.kv.kv_heads + part.head) << a.kv.page_shift) +
-                        ((uint32_t)k & ((1u << a.kv.page_shift) - 1));
-      return Keys16{a.kv.keys + at * row_bytes, a.kv.values + at * row_bytes, a.kv.key_scales + at,
-                    a.kv.value_scales + at, there ? (uint32_t)n * row_bytes : 0u, there ? 64u : 0u};
+    // The page of the 16 keys from k on as the table has it (~0u past the part's keys), and their place: none in a hole.
+    const auto page_at = [&](int k) __attribute__((always_inline)) {
+      return k < k_end ? a.kv.page_table[(size_t)part.sequence * a.kv.pages_per_sequence +
+                                         ((uint32_t)k >> a.kv.page_shift)]
+                       : ~0u;
+    };
+    const auto keys_at = [&](int k, uint32_t entry) __attribute__((always_inline)) {
+      const uint32_t page = uniform(entry);
+      if (page >= a.kv.pages) return Keys16{0, 0u};
+      return Keys16{(((size_t)page * a.kv.kv_heads + part.head) << a.kv.page_shift) +
+                        ((uint32_t)k & ((1u << a.kv.page_shift) - 1)),
+                    (uint32_t)min(16, k_end - k)};
     };
 
     typename R::KeyTile kt;
     typename R::ValueTile vt;
     int k = k_begin + kStep * (int)wave;
     const auto fetch_keys = [&](const Keys16 &ka, const Keys16 &kb) __attribute__((always_inline)) {
-      R::load_keys(kt, ka, 0, row_bytes, lane);
-      R::load_keys(kt, kb, 1, row_bytes, lane);
+      R::load_keys(kt, a.kv, ka, 0, row_bytes, lane);
+      R::load_keys(kt, a.kv, kb, 1, row_bytes, lane);
     };
     const auto fetch_values = [&](const Keys16 &ka, const Keys16 &kb) __attribute__((always_inline)) {
-      R::load_values(vt, ka, 0, row_bytes, lane);
-      R::load_values(vt, kb, 1, row_bytes, lane);
+      R::load_values(vt, a.kv, ka, 0, row_bytes, lane);
+      R::load_values(vt, a.kv, kb, 1, row_bytes, lane);
     };
-    Keys16 ka = keys_at(k), kb = keys_at(k + 16);
-    fetch_keys(ka, kb);
-    fetch_values(ka, kb);
-    for (; k < k_end; k += kStep * kWaves) {
-      const uint32_t hole = (ka.bytes ? 0u : 1u) | (kb.bytes ? 0u : 2u);
-      const Keys16 na = keys_at(k + kStep * kWaves), nb = keys_at(k + kStep * kWaves + 16);
+    // Fetches run a step ahead of the products, and the page table's entries a step ahead of the fetches.
+    constexpr int kStride = kStep * kWaves;
+    uint32_t entry_a = page_at(k), entry_b = page_at(k + 16);
+    Keys16 ka = keys_at(k, entry_a), kb = keys_at(k + 16, entry_b);
+    entry_a = page_at(k + kStride);
+    entry_b = page_at(k + kStride + 16);
+    if (k < k_end) {
+      fetch_keys(ka, kb);
+      fetch_values(ka, kb);
+    }
+    for (; k < k_end; k += kStride) {
+      const bool more = k + kStride < k_end;
+      const uint32_t hole = (ka.count ? 0u : 1u) | (kb.count ? 0u : 2u);
+      const Keys16 na = keys_at(k + kStride, entry_a), nb = keys_at(k + kStride + 16, entry_b);
+      entry_a = page_at(k + 2 * kStride);
+      entry_b = page_at(k + 2 * kStride + 16);
       f32x4 s[MB][2];
       state.scores(kt, s);
       f32x4 key_scale[2], value_scale[2];
@@ -301,7 +312,7 @@ __global__ __launch_bounds__(kThreads, DIM * MB <= (DIM == 256 ? 0 : FMT == SQ_K
         value_scale[0] = vt.scale[0];
         value_scale[1] = vt.scale[1];
       }
-      fetch_keys(na, nb);
+      if (more) fetch_keys(na, nb);
 
       const bool clear = k >= clear_begin && k + kStep <= clear_end && k + kStep <= k_end && !hole;
       uint32_t seen[MB];   // bit 4 h + i: key 16 h + 4 kq + i
@@ -367,16 +378,18 @@ __global__ __launch_bounds__(kThreads, DIM * MB <= (DIM == 256 ? 0 : FMT == SQ_K
               const uint32_t word = i / 2 ? second : first;
               const float weight = __uint_as_float((uint32_t)__shfl((int)(i % 2 ? word & 0xFFFF0000u : word << 16), source));
               const bool sees = (__shfl((int)seen[b], source) >> (4 * h + i)) & 1;
-              const __amdgpu_buffer_rsrc_t values = buffer_rsrc(h ? kb.values : ka.values, h ? kb.bytes : ka.bytes);
+              const Keys16 &from = h ? kb : ka;
+              const __amdgpu_buffer_rsrc_t values =
+                  buffer_rsrc(a.kv.values + from.at * row_bytes, from.count * row_bytes);
 #pragma unroll
-              for (int d = 0; d < kRun; ++d)
+              for (int j = 0; j < 4; ++j)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                for (int d = 0; d < kRun; d += 2) {
                   const uint32_t at = kRun * (4 * kq + j) + d;
-                  const uint32_t bits = at < dim ? __builtin_amdgcn_raw_buffer_load_b16(
-                                                       values, (key % 16) * row_bytes + 2 * at, 0, 0)
-                                                 : 0u;
-                  if (sees && (bits & 0x7F80u) == 0x7F80u) state.o[b][d][j] += weight * bf16_to_f32(bits);
+                  const uint32_t two = at < dim ? buffer_b32(values, (key % 16) * row_bytes + 2 * at, 0) : 0u;
+                  if (sees && (two & 0x7F80u) == 0x7F80u) state.o[b][d][j] += weight * bf16_to_f32(two & 0xFFFFu);
+                  if (sees && (two & 0x7F800000u) == 0x7F800000u)
+                    state.o[b][d + 1][j] += weight * __uint_as_float(two & 0xFFFF0000u);
                 }
             }
 #pragma unroll
@@ -392,145 +405,113 @@ __global__ __launch_bounds__(kThreads, DIM * MB <= (DIM == 256 ? 0 : FMT == SQ_K
         }
       }
       state.accumulate(vt, p);
-      fetch_values(na, nb);
+      if (more) fetch_values(na, nb);
       ka = na;
       kb = nb;
     }
 #pragma unroll
     for (int b = 0; b < MB; ++b) state.l[b] = row_sum(state.l[b]);
 
-    // Joins the waves' states, eight accumulators at a time, into finish(b, chunk, factor, pair): wave w holds sums of
-    // accumulators 8 chunk + 2 w and + 1 (accumulator kRun j + d: value d of run j). total_l and top as the lane's row's.
-    const auto join = [&](auto &&finish, float (&top)[MB], float (&total)[MB]) __attribute__((always_inline)) {
-      __syncthreads();
-      if (lane < 16) {
-#pragma unroll
-        for (int b = 0; b < MB; ++b) {
-          maxima[wave][b][lane] = state.m[b];
-          sums[wave][b][lane] = state.l[b];
-        }
-      }
-      __syncthreads();
-      float mine[MB];
+    // finish(b, c, sum): accumulators kJoin c + 4 wave .. + 3 of block b over every wave, for waves below kVectors.
+    const auto write = [&](int b, int c, f32x4 sum, float total) __attribute__((always_inline)) {
+      const int p = 16 * b + (int)r, i = row_of(p, by_group), g = p - i * (int)a.group;
+      const uint32_t acc = kJoin * c + 4 * wave, value = kRun * (4 * kq + acc / kRun) + acc % kRun;
+      if (p >= live || value >= dim) return;
+      const float by = total == 0.0f ? 0.0f : 1.0f / total;
+      uint16_t *out = a.output + (size_t)(part.first_row + row0 + i) * a.output_stride +
+                      (part.head * a.group + g) * dim + value;
+      *(u32x2 *)out = u32x2{bf16_pair(sum[0] * by, sum[1] * by), bf16_pair(sum[2] * by, sum[3] * by)};
+    };
+    float *mine = a.partials + (size_t)part_slot(part.first_piece, part.part) * (MB * kBlockFloats);
+    if (part.parts > 1 && part.part == 0) began = {part.parts, (uint32_t)live, part.first_row + (uint32_t)row0, part.head};
+    __syncthreads();   // the last join has been read
+    if (lane < 16) {
 #pragma unroll
       for (int b = 0; b < MB; ++b) {
-        top[b] = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) top[b] = fmaxf(top[b], maxima[w][b][r]);
-        total[b] = 0.0f;
-#pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
-          // A wave that saw nothing adds nothing, even to a row whose maximum is infinite.
-          const float s = sums[w][b][r];
-          if (s != 0.0f) total[b] += s * exp2_fast(maxima[w][b][r] - finite_max(top[b]));
-        }
-        mine[b] = state.l[b] != 0.0f ? exp2_fast(state.m[b] - finite_max(top[b])) : 0.0f;
+        shared.maxima[wave][b][lane] = state.m[b];
+        shared.sums[wave][b][lane] = state.l[b];
       }
+    }
 #pragma unroll
-      for (int b = 0; b < MB; ++b)
+    for (int b = 0; b < MB; ++b) {
+      float top = -INFINITY, total = 0.0f, by[kWaves];
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-          if (b || c) __syncthreads();
+      for (int c = 0; c < kChunks; ++c) {
+        if (b || c) __syncthreads();
 #pragma unroll
-          for (int t = 0; t < kChunk; ++t) {
-            const int acc = kChunk * c + t;
-            joined[wave][t][lane] = state.o[b][acc % kRun][acc / kRun] * mine[b];
+        for (int v = 0; v < kVectors; ++v) {
+          f32x4 four;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int acc = kJoin * c + 4 * v + i;
+            four[i] = state.o[b][acc % kRun][acc / kRun];
           }
-          __syncthreads();
-          float sum[2] = {0.0f, 0.0f};
+          shared.waves[wave][v][lane] = four;
+        }
+        __syncthreads();
+        if (c == 0) {
+#pragma unroll
+          for (int w = 0; w < kWaves; ++w) top = fmaxf(top, shared.maxima[w][b][r]);
 #pragma unroll
           for (int w = 0; w < kWaves; ++w) {
-            sum[0] += joined[w][2 * wave][lane];
-            sum[1] += joined[w][2 * wave + 1][lane];
+            // A wave that saw nothing adds nothing, even to a row whose maximum is infinite.
+            const float l = shared.sums[w][b][r];
+            by[w] = l == 0.0f ? 0.0f : exp2_fast(shared.maxima[w][b][r] - finite_max(top));
+            total += l * by[w];
           }
-          finish(b, c, sum);
         }
-    };
-    const auto write = [&](const float (&total)[MB]) __attribute__((always_inline)) {
-      return [&](int b, int c, const float (&sum)[2]) __attribute__((always_inline)) {
-        const int p = 16 * b + (int)r, i = p / (int)a.group, g = p - i * (int)a.group;
-        const uint32_t acc = kChunk * c + 2 * wave, value = kRun * (4 * kq + acc / kRun) + acc % kRun;
-        if (p >= live || value >= dim) return;
-        const float by = total[b] == 0.0f ? 0.0f : 1.0f / total[b];
-        uint16_t *out = a.output + (size_t)(part.first_row + row0 + i) * a.output_stride +
-                        (part.head * a.group + g) * dim + value;
-        *(uint32_t *)out = bf16_pair(sum[0] * by, sum[1] * by);
-      };
-    };
-
-    float top[MB], total[MB];
-    if (part.parts == 1) {
-      join(write(total), top, total);
-      continue;
-    }
-    float *mine = a.partials + (size_t)part_slot(part.first_piece, part.part) * kPartFloats;
-    join([&](int b, int c, const float (&sum)[2])
-             __attribute__((always_inline)) {
-               store_pair(mine + ((b * kChunks + c) * kWaves + wave) * 128 + 2 * lane, sum[0], sum[1]);
-             },
-         top, total);
-    if (wave == 0 && lane < 16) {
+        if ((int)wave >= kVectors) continue;
+        f32x4 sum = shared.waves[0][wave][lane] * by[0];
 #pragma unroll
-      for (int b = 0; b < MB; ++b)
-        store_pair(mine + MB * kRegs * 64 + 32 * b + 2 * lane, top[b], total[b]);
-    }
-    if (!last_part(a.counters + part.first_piece, part.parts, &arrival)) continue;
-    // The last to arrive: each wave joins every fourth part into a state of its own, in key order, and the waves join as
-    // above.
-    state.clear();
-    for (uint32_t j = wave; j < part.parts; j += kWaves) {
-      const float *from = a.partials + (size_t)part_slot(part.first_piece, j) * kPartFloats;
-#pragma unroll
-      for (int b = 0; b < MB; ++b) {
-        float m, l, v[kRegs];
-        load_pair(from + MB * kRegs * 64 + 32 * b + 2 * r, m, l);
-#pragma unroll
-        for (int t = 0; t < kRegs / 2; ++t) load_pair(from + (b * (kRegs / 2) + t) * 128 + 2 * lane, v[2 * t], v[2 * t + 1]);
-        if (l == 0.0f) m = -INFINITY;
-        const float next = fmaxf(state.m[b], m);
-        const float keep = state.l[b] != 0.0f ? exp2_fast(state.m[b] - finite_max(next)) : 0.0f;
-        const float take = l != 0.0f ? exp2_fast(m - finite_max(next)) : 0.0f;
-        state.m[b] = next;
-        state.l[b] = state.l[b] * keep + l * take;
-#pragma unroll
-        for (int t = 0; t < kRegs; ++t) {
-          const float acc = state.o[b][t % kRun][t / kRun];
-          state.o[b][t % kRun][t / kRun] = acc * keep + v[t] * take;
+        for (int w = 1; w < kWaves; ++w) sum += shared.waves[w][wave][lane] * by[w];
+        if (part.parts == 1) {
+          write(b, c, sum, total);
+        } else if (16 * b + (int)r < live) {
+          *(f32x4 *)(mine + b * kBlockFloats + ((c * kVectors + wave) * 64 + lane) * 4) = sum;
         }
       }
+      if (part.parts > 1 && wave == 0 && lane < 16) {
+        float *row = mine + b * kBlockFloats + 16 * DIM + 2 * lane;
+        row[0] = top;
+        row[1] = total;
+      }
     }
-    join(write(total), top, total);
   }
+  work.leave(a, began);
 }
 
-template <uint32_t FMT, int DIM>
-hipError_t launch_blocks(uint32_t tile_rows, const AttendArgs &a, hipStream_t stream) {
-  const dim3 grid(a.workgroups), block(kThreads);
-  if (tile_rows == 16) hipLaunchKernelGGL((attend_rows_kernel<FMT, DIM, 1>), grid, block, 0, stream, a);
-  else if (tile_rows == 32) hipLaunchKernelGGL((attend_rows_kernel<FMT, DIM, 2>), grid, block, 0, stream, a);
-  else if constexpr (DIM <= 128) hipLaunchKernelGGL((attend_rows_kernel<FMT, DIM, 4>), grid, block, 0, stream, a);
+template <uint32_t FMT, int DIM, int MB>
+hipError_t launch_one(uint32_t waves, const AttendArgs &a, hipStream_t stream) {
+  if constexpr (attend_rows_resident(16 * MB, DIM, FMT) > 1) {
+    if (waves == 8) {
+      hipLaunchKernelGGL((attend_rows_kernel<FMT, DIM, MB, 8>), dim3(a.workgroups), dim3(512), 0, stream, a);
+      return hipGetLastError();
+    }
+  }
+  if (waves != 4) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((attend_rows_kernel<FMT, DIM, MB, 4>), dim3(a.workgroups), dim3(256), 0, stream, a);
   return hipGetLastError();
 }
+template <uint32_t FMT, int DIM>
+hipError_t launch_blocks(uint32_t tile_rows, uint32_t waves, const AttendArgs &a, hipStream_t stream) {
+  if (tile_rows == 16) return launch_one<FMT, DIM, 1>(waves, a, stream);
+  if (tile_rows == 32) return launch_one<FMT, DIM, 2>(waves, a, stream);
+  if constexpr (DIM <= 128) return launch_one<FMT, DIM, 4>(waves, a, stream);
+  else return hipErrorInvalidValue;
+}
 template <uint32_t FMT>
-hipError_t launch_dim(uint32_t tile_rows, const AttendArgs &a, hipStream_t stream) {
-  if (a.kv.head_dim <= 64) return launch_blocks<FMT, 64>(tile_rows, a, stream);
-  if (a.kv.head_dim <= 128) return launch_blocks<FMT, 128>(tile_rows, a, stream);
-  return launch_blocks<FMT, 256>(tile_rows, a, stream);
+hipError_t launch_dim(uint32_t tile_rows, uint32_t waves, const AttendArgs &a, hipStream_t stream) {
+  if (a.kv.head_dim <= 64) return launch_blocks<FMT, 64>(tile_rows, waves, a, stream);
+  if (a.kv.head_dim <= 128) return launch_blocks<FMT, 128>(tile_rows, waves, a, stream);
+  return launch_blocks<FMT, 256>(tile_rows, waves, a, stream);
 }
 
 }  // namespace
 
-uint64_t attend_partials(uint32_t tile_rows, uint32_t head_dim, uint32_t workgroups) {
-  // Two parts a workgroup (attend.hpp), each a tile's accumulators and its rows' maxima and sums.
-  const uint64_t dim = head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256;
-  return 2 * uint64_t{workgroups} * tile_rows * (dim + 2);
-}
-uint64_t attend_counters(uint32_t workgroups) { return workgroups; }
-
-hipError_t launch_attend_rows(uint32_t tile_rows, const AttendArgs &a, hipStream_t stream) {
-  if (a.kv.format == SQ_KV_BF16) return launch_dim<SQ_KV_BF16>(tile_rows, a, stream);
-  if (a.kv.format == SQ_KV_INT8) return launch_dim<SQ_KV_INT8>(tile_rows, a, stream);
-  return launch_dim<SQ_KV_E4M3>(tile_rows, a, stream);
+hipError_t launch_attend_rows(uint32_t tile_rows, uint32_t waves, const AttendArgs &a, hipStream_t stream) {
+  if (a.kv.format == SQ_KV_BF16) return launch_dim<SQ_KV_BF16>(tile_rows, waves, a, stream);
+  if (a.kv.format == SQ_KV_INT8) return launch_dim<SQ_KV_INT8>(tile_rows, waves, a, stream);
+  return launch_dim<SQ_KV_E4M3>(tile_rows, waves, a, stream);
 }
 
 }  // namespace sq::kern

@@ -23,17 +23,12 @@ namespace {
 
 constexpr int kWaves = 4, kThreads = 64 * kWaves, kRows = 32 * kWaves;
 constexpr float kRaise = 8.0f;               // as in the tiles of few rows: the running maximum moves past this
-constexpr uint32_t kNowhere = 0x7FFFFFF0u;   // past every resource's range: reads zero
 
 typedef __attribute__((__vector_size__(16 * sizeof(float)))) float f32x16;
-typedef __attribute__((__vector_size__(2 * sizeof(__bf16)))) __bf16 bf16x2;
 
 __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0,
                                                  0);
-}
-__device__ __forceinline__ uint32_t bf16_pair(float a, float b) {
-  return __builtin_bit_cast(uint32_t, bf16x2{(__bf16)a, (__bf16)b});
 }
 __device__ __forceinline__ uint32_t high_halves(uint32_t k0, uint32_t k1) {
   return __builtin_amdgcn_perm(k1, k0, 0x07060302u);
@@ -92,22 +87,19 @@ __global__ __launch_bounds__(kThreads, DIM == 256 ? 1 : 2) void attend_tile_kern
   using T = Tile<DIM>;
   constexpr bool kCodes = FMT != SQ_KV_BF16;
   constexpr int kSteps = DIM / 16, kBlocks = DIM / 32, kBytes = kCodes ? 1 : 2;
-  constexpr int kPartFloats = kRows * (DIM + 2);
+  constexpr int kBlockFloats = 32 * (DIM + 2);   // of a part in the workspace
   // A wave fetches 16 keys of the tile, kLoads vectors a lane of K and of V.
   constexpr int kLoads = 16 * DIM * kBytes / 1024, kRowLanes = DIM * kBytes / 16, kLoadRows = 64 / kRowLanes;
   __shared__ __attribute__((aligned(1024))) uint8_t tiles[2][2][T::kBytes];   // [stage][K, V]
   __shared__ f32x4 scales[kCodes ? 2 : 1][2][kKeyTile / 4];
-  __shared__ int64_t prefix[kMaxSequences + 1], scan[kWaves];
-  __shared__ uint32_t arrival;
+  __shared__ LineShared<kThreads> shared;
   const uint32_t lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
   const uint32_t wave = uniform(threadIdx.x >> 6);
   const int fit = kRows / (int)a.group;
+  const float by_group = 1.0f / (float)a.group;
   const uint32_t dim = a.kv.head_dim, row_bytes = dim * kBytes;
-  const Line line = make_line<kThreads>(a, fit, 4 * kKeyTile, prefix, scan);
-  const uint32_t piece = piece_of(line, blockIdx.x);
-  if (blockIdx.x / 8 >= (line.active + 7) / 8 || piece >= line.active) return;
-  int64_t x = line.share * piece;
-  const int64_t end = x + line.share < line.total ? x + line.share : line.total;
+  Work work = make_work<kThreads>(a, fit, 4 * kKeyTile, shared);
+  UnitNote began{};
 
   // Where this lane's vectors lie in 16 keys of a page, and (codes) in the LDS tile.
   uint32_t key_from[kLoads], value_from[kLoads], code_to[kLoads];
@@ -131,9 +123,9 @@ __global__ __launch_bounds__(kThreads, DIM == 256 ? 1 : 2) void attend_tile_kern
   const uint32_t vi = lane & 15, vk = 4 * h + vi / 4;
   const uint32_t value_at = vk * T::kRowBytes + 8 * (vi % 2) + 16 * ((2 * (lane / 16 % 2) + vi % 4 / 2) ^ T::value_swap(vk));
 
-  while (x < end) {
-    const Part part = next_part(a, line, fit, x, end, piece);
-    if (part.t1 <= part.t0) continue;
+  Part next;
+  while (work.next(a, fit, next)) {
+    const Part part = Work::settled(a, fit, next);
     const Units &u = part.units;
     const int row0 = fit * part.m, rows = min(fit, u.rows - row0), live = rows * (int)a.group;
     const int unit_end = u.causal ? min(u.keys, u.base + row0 + rows) : u.keys;   // keys that any row sees
@@ -143,7 +135,7 @@ __global__ __launch_bounds__(kThreads, DIM == 256 ? 1 : 2) void attend_tile_kern
     const int clear_end = u.causal ? u.base + row0 + 1 : u.keys;
 
     // This lane's row.
-    const int p = 32 * (int)wave + (int)r, pi = p / (int)a.group, pg = p - pi * (int)a.group;
+    const int p = 32 * (int)wave + (int)r, pi = row_of(p, by_group), pg = p - pi * (int)a.group;
     const bool on = p < live;
     const int at = u.base + row0 + pi;
     const int low = u.window ? at - u.window + 1 : 0;
@@ -387,43 +379,23 @@ __global__ __launch_bounds__(kThreads, DIM == 256 ? 1 : 2) void attend_tile_kern
     l = other_sum(l);
 
     if (part.parts > 1) {
-      float *mine = a.partials + (size_t)part_slot(part.first_piece, part.part) * kPartFloats + wave * (32 * (DIM + 2));
+      if (part.part == 0) began = {part.parts, (uint32_t)live, part.first_row + (uint32_t)row0, part.head};
       if (busy) {
-#pragma unroll
-        for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) store_pair(mine + (8 * b + i) * 128 + 2 * lane, o[b][2 * i], o[b][2 * i + 1]);
-        if (h == 0) store_pair(mine + 32 * DIM + 2 * lane, m, l);
-      }
-      if (!last_part(a.counters + part.first_piece, part.parts, &arrival)) continue;
-      if (busy) {
-        m = -INFINITY;
-        l = 0.0f;
-#pragma unroll
-        for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) o[b][i] = 0.0f;
-        for (uint32_t j = 0; j < part.parts; ++j) {
-          const float *from = a.partials + (size_t)part_slot(part.first_piece, j) * kPartFloats + wave * (32 * (DIM + 2));
-          float pm, pl;
-          load_pair(from + 32 * DIM + 2 * r, pm, pl);
-          if (pl == 0.0f) pm = -INFINITY;
-          const float next = fmaxf(m, pm);
-          const float keep = l != 0.0f ? exp2_fast(m - finite_max(next)) : 0.0f;
-          const float take = pl != 0.0f ? exp2_fast(pm - finite_max(next)) : 0.0f;
-          m = next;
-          l = l * keep + pl * take;
+        float *mine = a.partials + ((size_t)part_slot(part.first_piece, part.part) * kWaves + wave) * kBlockFloats;
+        if (on) {
 #pragma unroll
           for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              float v0, v1;
-              load_pair(from + (8 * b + i) * 128 + 2 * lane, v0, v1);
-              o[b][2 * i] = o[b][2 * i] * keep + v0 * take;
-              o[b][2 * i + 1] = o[b][2 * i + 1] * keep + v1 * take;
-            }
+            for (int j = 0; j < 4; ++j)
+              *(f32x4 *)(mine + ((4 * b + j) * 64 + lane) * 4) =
+                  f32x4{o[b][4 * j], o[b][4 * j + 1], o[b][4 * j + 2], o[b][4 * j + 3]};
+        }
+        if (h == 0) {
+          mine[32 * DIM + 2 * lane] = m;
+          mine[32 * DIM + 2 * lane + 1] = l;
         }
       }
+      continue;
     }
     if (on) {
       const float by = l == 0.0f ? 0.0f : 1.0f / l;
@@ -439,6 +411,7 @@ __global__ __launch_bounds__(kThreads, DIM == 256 ? 1 : 2) void attend_tile_kern
         }
     }
   }
+  work.leave(a, began);
 }
 
 template <uint32_t FMT>

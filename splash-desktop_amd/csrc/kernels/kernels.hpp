@@ -248,19 +248,35 @@ struct AttendArgs {
   uint32_t query_stride, output_stride, group;
   uint32_t causal, window;
   float scale;
-  float *partials;
-  uint32_t *counters;
+  float *partials;   // the workspace: parts, then notes
+  void *notes;
   uint32_t workgroups;
 };
 constexpr uint32_t kAttendMaxGroup = 64;
-// The floats of partials and the counters that `workgroups` workgroups on tiles of tile_rows rows use.
+// The bytes of workspace that `workgroups` workgroups on tiles of tile_rows rows use; its notes, kAttendNoteBytes a
+// workgroup and as many once more, are the last of it.
+constexpr uint32_t kAttendNoteBytes = 16;
 uint64_t attend_partials(uint32_t tile_rows, uint32_t head_dim, uint32_t workgroups);
-uint64_t attend_counters(uint32_t workgroups);
-// Tiles of few rows: 16, 32, or (heads of at most 128 values) 64.
+// Tiles of few rows: 16, 32, or (heads of at most 128 values) 64; and the wide tile.
 constexpr uint32_t kAttendWideRows = 128;
 inline uint32_t attend_few_rows(uint32_t head_dim) { return head_dim <= 128 ? 64 : 32; }
-hipError_t launch_attend_rows(uint32_t tile_rows, const AttendArgs &args, hipStream_t stream);
+// The workgroups (of four waves) that a compute unit holds of a tile of few rows at once: by the registers of a wave's
+// keys, values and accumulators.
+constexpr uint32_t attend_rows_resident(uint32_t tile_rows, uint32_t head_dim, uint32_t format) {
+  const uint32_t state = (head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256) * tile_rows / 16;
+  return (state <= 128 ? 2 : state <= 256 ? 1 : 0) + (format != SQ_KV_BF16 && state <= 256 ? 1 : state > 256 ? 1 : 0);
+}
+// The workgroups of a compute unit under a plan of tiles of tile_rows rows and workgroups of `waves` waves.
+inline uint32_t attend_resident(uint32_t tile_rows, uint32_t waves, uint32_t head_dim, uint32_t format) {
+  if (tile_rows == kAttendWideRows) return head_dim <= 128 ? 2 : 1;
+  return waves == 8 ? 1 : attend_rows_resident(tile_rows, head_dim, format);
+}
+hipError_t launch_attend_rows(uint32_t tile_rows, uint32_t waves, const AttendArgs &args, hipStream_t stream);
 // Tiles of kAttendWideRows rows.
 hipError_t launch_attend_tile(const AttendArgs &args, hipStream_t stream);
+// The join of the parts that either left, after it.
+hipError_t launch_attend_join(uint32_t tile_rows, const AttendArgs &args, hipStream_t stream);
+// The length (attend.hpp) up to which a batch of few units is never cut (launch_attend_rows).
+constexpr uint32_t kAttendLeast = 1024;
 
 }  // namespace sq::kern

@@ -191,12 +191,12 @@ class AttentionShape(Structure):
 
 class AttentionPlan(Structure):
     _fields_ = [("shape", AttentionShape)] + \
-               [(n, c_uint32) for n in ("sequences", "rows", "chunk_rows", "tile_rows", "workgroups")] + \
-               [("partials", c_uint64), ("counters", c_uint64)]
+               [(n, c_uint32) for n in ("sequences", "rows", "chunk_rows", "tile_rows", "waves", "workgroups")] + \
+               [("partials", c_uint64)]
 
 
 class AttentionBuffers(Structure):
-    _fields_ = [("query", HeadRows), ("output", HeadRows), ("partials", Buffer), ("counters", Buffer)]
+    _fields_ = [("query", HeadRows), ("output", HeadRows), ("partials", Buffer)]
 
 
 class SqError(RuntimeError):
@@ -493,18 +493,16 @@ def attention_plan(shape: AttentionShape, sequences: int, rows: int, chunk_rows:
 
 
 class AttentionScratch:
-    """Device workspace for an attention plan (the counters zeroed at allocation, as they must be)."""
+    """Device workspace for an attention plan."""
 
     def __init__(self, plan: AttentionPlan, device_name: str = "cuda"):
         import torch
         self.partials = torch.empty(max(plan.partials, 16), dtype=torch.uint8, device=device_name)
-        self.counters = torch.zeros(max(plan.counters, 16) // 4, dtype=torch.int32, device=device_name)
 
 
 def attention_add(plan: AttentionPlan, cache: KvCache, batch: KvBatch, query, output, scratch: AttentionScratch,
                   stream=None) -> None:
     d = cache.shape.head_dim
-    buffers = AttentionBuffers(head_rows(query, d), head_rows(output, d), view(scratch.partials),
-                               view(scratch.counters))
+    buffers = AttentionBuffers(head_rows(query, d), head_rows(output, d), view(scratch.partials))
     call("sq_attention_add", stream if stream is not None else stream_handle(), byref(buffers), byref(cache),
          byref(batch), byref(plan))

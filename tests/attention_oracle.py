@@ -222,7 +222,6 @@ def run_attention(cache, q, scale, causal=True, window=0, chunk=None, scratch=No
     out = out if out is not None else t.full((rows, heads * dim), 123.0, dtype=t.bfloat16, device="cuda")
     sq.attention_add(plan, cache.struct(), cache.batch(), x, out, scratch)
     t.cuda.synchronize()
-    assert not scratch.counters.any().item(), "counters return to zero"
     return from_bf16(out).reshape(rows, heads, dim)
 
 

@@ -172,7 +172,7 @@ def test_cache_and_batch_refusals(message, c, b):
     refused("sq_kv_add_write", message, by(cache(**c)), by(batch(**b)), by(k), by(k), None, None, None)
     refused("sq_kv_add_read", message, by(cache(**c)), by(batch(**b)), by(k), by(k))
     plan = attention_plan(rows=5, sequences=3)
-    buffers = sq.AttentionBuffers(out, out, buffer(plan.partials), buffer(plan.counters))
+    buffers = sq.AttentionBuffers(out, out, buffer(plan.partials))
     refused("sq_attention_add", message, by(buffers), by(cache(**c)), by(batch(**b)), by(plan))
 
 
@@ -214,9 +214,9 @@ def test_attention_plans():
         group = heads // kv_heads
         assert plan.tile_rows >= group
         assert plan.tile_rows == 16 or plan.tile_rows // 2 < chunk * group
-        assert plan.workgroups % 8 == 0 and plan.partials and plan.counters >= 4 * plan.workgroups
+        assert plan.workgroups % 8 == 0 and plan.partials > 16 * plan.workgroups
     small = attention_plan(dev=sq.Device(10))
-    assert small.workgroups == 24
+    assert small.workgroups % 8 == 0 and 10 <= small.workgroups < 32
 
 
 @pytest.mark.parametrize("shape,sizes,message", [
@@ -234,10 +234,10 @@ def test_attention_plan_refusals(shape, sizes, message):
 def test_attention_refusals():
     by = ctypes.byref
     plan, q = attention_plan(), rows_of(5, 4, 64)
-    good = dict(query=q, output=q, partials=buffer(plan.partials), counters=buffer(plan.counters))
+    good = dict(query=q, output=q, partials=buffer(plan.partials))
 
     def no(message, plan=plan, cache=cache(), batch=batch(), **kw):
-        b = sq.AttentionBuffers(*[{**good, **kw}[n] for n in ("query", "output", "partials", "counters")])
+        b = sq.AttentionBuffers(*[{**good, **kw}[n] for n in ("query", "output", "partials")])
         refused("sq_attention_add", message, by(b), by(cache), by(batch), by(plan))
 
     no("another cache", cache=cache(page_rows=64))
@@ -250,13 +250,12 @@ def test_attention_refusals():
     no("output rows", output=rows_of(5, 4, 64, short=1))
     no("in place", output=rows_of(5, 4, 64, 264))
     no("attention partials", partials=buffer(plan.partials - 1))
-    no("attention counters", counters=buffer(plan.counters - 1))
     no("16-byte", partials=buffer(plan.partials, (1 << 20) + 8))
-    for field in ("tile_rows", "workgroups", "partials", "counters"):
+    for field in ("tile_rows", "waves", "workgroups", "partials"):
         wrong = sq.AttentionPlan.from_buffer_copy(plan)
         setattr(wrong, field, getattr(wrong, field) + 8)
         no("fields", plan=wrong)
-    none = sq.AttentionBuffers(*[good[n] for n in ("query", "output", "partials", "counters")])
+    none = sq.AttentionBuffers(*[good[n] for n in ("query", "output", "partials")])
     sq.call("sq_attention_add", None, by(none), by(cache()), by(batch(rows=0)), by(plan))
 
 

@@ -393,7 +393,6 @@ def test_graph_replays_with_other_lengths():
         t.cuda.synchronize()
         for got, want in zip((turned, out, back), e):   # bits: keys that no step has written are NaN
             assert t.equal(got.view(t.int16), want.view(t.int16))
-        assert not scratch.counters.any().item()
 
 
 def test_two_streams_at_once():
