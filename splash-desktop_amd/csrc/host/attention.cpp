@@ -296,7 +296,9 @@ void Attention::add(hipStream_t graph, const HeadRowsView &query, const HeadRows
                               shape.group(),
                               shape.causal,
                               shape.window,
-                              float(double(shape.scale) * std::numbers::log2e),
+                              shape.scale == 0 ? 1.0f : float(std::fabs(double(shape.scale)) * std::numbers::log2e),
+                              shape.scale == 0 ? 0u : ~0u,
+                              shape.scale < 0 ? 0x80008000u : 0u,
                               partials.as<float>(),
                               partials.as<uint8_t>() + plan.partials - (plan.workgroups + 1) * kern::kAttendNoteBytes,
                               plan.workgroups};
@@ -308,7 +310,7 @@ void Attention::add(hipStream_t graph, const HeadRowsView &query, const HeadRows
   launched(plan.tileRows == kern::kAttendWideRows ? kern::launch_attend_tile(args, graph)
                                                   : kern::launch_attend_rows(plan.tileRows, plan.waves, args, graph),
            "attention");
-  if (!whole) launched(kern::launch_attend_join(plan.tileRows, args, graph), "attention join");
+  if (!whole) launched(kern::launch_attend_join(plan.tileRows, uint32_t(std::min<uint64_t>(units, ~0u)), args, graph), "attention join");
 }
 
 }  // namespace sq::ops

@@ -8,29 +8,21 @@
 namespace sq::kern {
 namespace {
 
-constexpr int kAtOnce = 16, kVectors = 2;   // parts' loads in flight, and the vectors a wave joins
-
-// A wave of blockIdx.x's unit (the one that piece began) joins kVectors of the unit's vectors (attend.hpp: the layout of
-// a part). DIM is the head's values as computed.
-template <bool WIDE>
-__global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, uint32_t dim_computed, uint32_t tile_rows) {
-  const uint32_t rows = WIDE ? 32 : 16, vectors = dim_computed / (WIDE ? 8 : 16);
-  const uint32_t lane = threadIdx.x & 63, item = uniform(blockIdx.y * 4 + (threadIdx.x >> 6));
-  const uint32_t block = item / (vectors / kVectors), first = kVectors * (item % (vectors / kVectors));
-  const UnitNote *notes = unit_notes(a);
-  if (blockIdx.x >= notes[a.workgroups].parts) return;
-  const UnitNote note = notes[blockIdx.x];
-  if (note.parts < 2 || block * rows >= note.live) return;
+// VECTORS of a unit's vectors (attend.hpp: the layout of a part) by a wave, AT_ONCE parts' loads in flight.
+template <bool WIDE, int VECTORS, int AT_ONCE>
+__device__ __forceinline__ void join(const AttendArgs &a, const UnitNote &note, uint32_t dim_computed,
+                                     uint32_t tile_rows, uint32_t block, uint32_t first) {
+  const uint32_t rows = WIDE ? 32 : 16, lane = threadIdx.x & 63;
   const uint32_t p = block * rows + lane % rows;
   const bool on = p < note.live;
   const uint32_t part_floats = tile_rows * (dim_computed + 2), block_floats = rows * (dim_computed + 2);
   float m = -INFINITY, l = 0.0f;
-  f32x4 sum[kVectors] = {};
-  for (uint32_t j = 0; j < note.parts; j += kAtOnce) {
-    float pm[kAtOnce], pl[kAtOnce];
-    f32x4 got[kAtOnce][kVectors];
+  f32x4 sum[VECTORS] = {};
+  for (uint32_t j = 0; j < note.parts; j += AT_ONCE) {
+    float pm[AT_ONCE], pl[AT_ONCE];
+    f32x4 got[AT_ONCE][VECTORS];
 #pragma unroll
-    for (int d = 0; d < kAtOnce; ++d) {
+    for (int d = 0; d < AT_ONCE; ++d) {
       // Past the last part the resource is empty: zeros, and nothing read.
       const bool there = j + d < note.parts;
       const float *from = a.partials + (size_t)part_slot(blockIdx.x, there ? j + d : 0) * part_floats +
@@ -40,25 +32,24 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, uint32_t
       pm[d] = __uint_as_float(two[0]);
       pl[d] = __uint_as_float(two[1]);
 #pragma unroll
-      for (int v = 0; v < kVectors; ++v)
+      for (int v = 0; v < VECTORS; ++v)
         got[d][v] = __builtin_bit_cast(f32x4, buffer_b128<0>(r, on ? ((first + v) * 64 + lane) * 16 : kNowhere, 0));
     }
     float next = m;
 #pragma unroll
-    for (int d = 0; d < kAtOnce; ++d) next = pl[d] == 0.0f ? next : fmaxf(next, pm[d]);
+    for (int d = 0; d < AT_ONCE; ++d) next = pl[d] == 0.0f ? next : fmaxf(next, pm[d]);
     // A part that saw nothing adds nothing, even to a row whose maximum is infinite.
     const float keep = l == 0.0f ? 0.0f : exp2_fast(m - finite_max(next));
     m = next;
     l *= keep;
 #pragma unroll
-    for (int v = 0; v < kVectors; ++v) sum[v] *= keep;
+    for (int v = 0; v < VECTORS; ++v) sum[v] *= keep;
 #pragma unroll
-    for (int d = 0; d < kAtOnce; ++d) {
-      if (pl[d] == 0.0f) continue;
-      const float by = exp2_fast(pm[d] - finite_max(next));
+    for (int d = 0; d < AT_ONCE; ++d) {
+      const float by = pl[d] == 0.0f ? 0.0f : exp2_fast(pm[d] - finite_max(next));
       l += pl[d] * by;
 #pragma unroll
-      for (int v = 0; v < kVectors; ++v) sum[v] += got[d][v] * by;
+      for (int v = 0; v < VECTORS; ++v) sum[v] += got[d][v] * by;
     }
   }
   if (!on) return;
@@ -66,11 +57,32 @@ __global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, uint32_t
   const uint32_t i = (uint32_t)row_of((int)p, 1.0f / (float)a.group), g = p - i * a.group;
   uint16_t *out = a.output + (size_t)(note.row + i) * a.output_stride + (note.head * a.group + g) * a.kv.head_dim;
 #pragma unroll
-  for (int v = 0; v < kVectors; ++v) {
+  for (int v = 0; v < VECTORS; ++v) {
     const uint32_t value = WIDE ? wide_value(first + v, lane) : few_value(first + v, lane, dim_computed / 16);
     if (value < a.kv.head_dim)
       *(u32x2 *)(out + value) = u32x2{bf16_pair(sum[v][0] * by, sum[v][1] * by), bf16_pair(sum[v][2] * by, sum[v][3] * by)};
   }
+}
+
+// blockIdx.x's unit (the one that piece began), its vectors over the waves of the blockIdx.y's. Units of two parts, which
+// a line's mostly are, eight vectors at a time; others two. DIM is the head's values as computed.
+template <bool WIDE>
+__global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, uint32_t dim_computed, uint32_t tile_rows) {
+  const UnitNote *notes = unit_notes(a);
+  const uint32_t pieces = notes[a.workgroups].parts;
+  const UnitNote note = notes[blockIdx.x];
+  if (blockIdx.x >= pieces || note.parts < 2) return;
+  const uint32_t rows = WIDE ? 32 : 16, vectors = dim_computed / (WIDE ? 8 : 16);
+  const uint32_t blocks = (note.live + rows - 1) / rows, wave = uniform(blockIdx.y * 4 + (threadIdx.x >> 6));
+  const auto over = [&](auto count, auto at_once) __attribute__((always_inline)) {
+    constexpr int kVectors = decltype(count)::value;
+    const uint32_t each = vectors / kVectors;
+    for (uint32_t item = wave; item < blocks * each; item += 4 * gridDim.y)
+      join<WIDE, kVectors, decltype(at_once)::value>(a, note, dim_computed, tile_rows, item / each,
+                                                     kVectors * (item % each));
+  };
+  if (WIDE && note.parts == 2) over(std::integral_constant<int, 8>{}, std::integral_constant<int, 2>{});
+  else over(std::integral_constant<int, 2>{}, std::integral_constant<int, 16>{});
 }
 
 uint32_t computed(uint32_t head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
@@ -83,11 +95,13 @@ uint64_t attend_partials(uint32_t tile_rows, uint32_t head_dim, uint32_t workgro
          (uint64_t{workgroups} + 1) * sizeof(UnitNote);
 }
 
-hipError_t launch_attend_join(uint32_t tile_rows, const AttendArgs &a, hipStream_t stream) {
+hipError_t launch_attend_join(uint32_t tile_rows, uint32_t units, const AttendArgs &a, hipStream_t stream) {
   const bool wide = tile_rows == kAttendWideRows;
   const uint32_t dim = computed(a.kv.head_dim);
-  const uint32_t items = tile_rows / (wide ? 32 : 16) * (dim / (wide ? 8 : 16)) / kVectors;
-  const dim3 grid(a.workgroups, (items + 3) / 4);
+  // Few units have many parts each, and want more waves on each; of many, launching the workgroups would take longer than
+  // their work (34 us for 4096 of them with 32 MiB of parts).
+  const uint32_t items = tile_rows / (wide ? 32 : 16) * (dim / (wide ? 8 : 16)) / 2;
+  const dim3 grid(a.workgroups, uint64_t{units} * 4 <= a.workgroups ? min((items + 3) / 4, 8u) : 1);
   if (wide) hipLaunchKernelGGL((attend_join_kernel<true>), grid, dim3(256), 0, stream, a, dim, tile_rows);
   else hipLaunchKernelGGL((attend_join_kernel<false>), grid, dim3(256), 0, stream, a, dim, tile_rows);
   return hipGetLastError();

@@ -258,7 +258,7 @@ attend_rows_kernel(AttendArgs a) {
 #pragma unroll
       for (int c = 0; c < R::kChains; ++c) {
         const uint32_t d = R::query_at(c, lane);
-        state.q[b][c] = on && d < dim ? *(const u32x4 *)(row + d) : u32x4{0u, 0u, 0u, 0u};
+        state.q[b][c] = on && d < dim ? (*(const u32x4 *)(row + d) & a.keep) ^ a.flip : u32x4{0u, 0u, 0u, 0u};
       }
     }
 

@@ -65,10 +65,13 @@ __device__ __forceinline__ u32x2 read_transposed(const uint8_t *lds) {
   typedef __attribute__((address_space(3))) i16x4 lds_i16x4;
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_i16x4 *)lds));
 }
-// Every wave's stores to LDS and copies into it have landed.
+// Every wave's stores to LDS have landed, and (unless codes are on their way to registers) its copies into it.
+template <bool CODES>
 __device__ __forceinline__ void tile_barrier() {
-  __builtin_amdgcn_s_waitcnt(0);
-  __syncthreads();
+  __builtin_amdgcn_s_waitcnt(CODES ? 0xC07F : 0);   // lgkmcnt(0), and vmcnt(0)
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 }
 
 // A head row in LDS: DIM bf16 values, CHUNKS 16-byte chunks. Where chunk c of key k lies.
@@ -148,7 +151,7 @@ __global__ __launch_bounds__(kThreads, DIM == 256 ? 1 : 2) void attend_tile_kern
 #pragma unroll
       for (int s = 0; s < kSteps; ++s) {
         const uint32_t d = 16 * s + 8 * h;
-        q[s] = on && d < dim ? *(const u32x4 *)(row + d) : u32x4{0u, 0u, 0u, 0u};
+        q[s] = on && d < dim ? (*(const u32x4 *)(row + d) & a.keep) ^ a.flip : u32x4{0u, 0u, 0u, 0u};
       }
     }
     float m = -INFINITY, l = 0.0f;
@@ -224,87 +227,113 @@ __global__ __launch_bounds__(kThreads, DIM == 256 ? 1 : 2) void attend_tile_kern
       }
     };
 
-    __syncthreads();   // the last part's tiles have been read
-    Pages pages = pages_at(k_begin);
-    fetch(k_begin, pages.own, 0);
-    uint32_t holes = pages.holes;
-    pages = pages_at(k_begin + kKeyTile);   // a tile ahead of the fetch that wants it
-    place(0);
-    tile_barrier();
-    int stage = 0;
-    for (int k = k_begin; k < k_end; k += kKeyTile, stage ^= 1) {
-      const bool more = k + kKeyTile < k_end;
-      if (more) fetch(k + kKeyTile, pages.own, stage ^ 1);
-      const uint32_t next_holes = pages.holes;
-      pages = pages_at(k + 2 * kKeyTile);
-      const uint8_t *kt = tiles[stage][0], *vt = tiles[stage][1];
-      const bool clear = k >= clear_begin && k + kKeyTile <= clear_end && k + kKeyTile <= k_end && !holes;
-      u32x4 w[4];   // the weights of 16 keys each, as the second product's operand
-      if (busy) {
-        f32x16 s[2];
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[b][i] = 0.0f;
-#pragma unroll
-          for (int c = 0; c < kSteps; ++c)
-            s[b] = mfma32(*(const u32x4 *)&kt[32 * b * T::kRowBytes + (key_at ^ (32 * c))], q[c], s[b]);
-        }
-        float top = -INFINITY;
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            f32x4 by{a.scale, a.scale, a.scale, a.scale};
-            if constexpr (kCodes) by *= scales[stage][0][8 * b + 2 * j + h];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              float t = s[b][4 * j + i] * by[i];
-              if (!clear) {
-                const int key = k + 32 * b + 8 * j + 4 * (int)h + i;
-                t = key >= low && key < high && !(holes >> (2 * b + j / 2) & 1) ? t : -INFINITY;
-              }
-              s[b][4 * j + i] = t;
-              top = fmaxf(top, t);
-            }
-          }
-        if (__any(top > m + kRaise)) {
-          const float next = fmaxf(m, other_max(top));
-          const float shrink = exp2_fast(m - finite_max(next));
-          m = next;
-          l *= shrink;
-#pragma unroll
-          for (int b = 0; b < kBlocks; ++b) o[b] *= shrink;
-        }
-        const float from = finite_max(m);
+    // The scores of the tile to weights, the second product's operands: 16 keys each in w.
+    u32x4 w[4];
+    const auto weigh = [&](f32x16 (&s)[2], int k, uint32_t holes, int stage, bool clear) __attribute__((always_inline)) {
+      // In a clear tile every row sees every key; in the others a key is compared with the row's, and with the holes.
+      const auto hide = [&](float value) __attribute__((always_inline)) {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
-            s[b][i] = exp2_fast(s[b][i] - from);
-            l += s[b][i];
+            const int key = k + 32 * b + 8 * (i / 4) + 4 * (int)h + i % 4;
+            const bool sees = key >= low && key < high && !(holes >> (2 * b + i / 8) & 1);
+            s[b][i] = sees ? s[b][i] : value;
           }
-        if constexpr (kCodes) {
+      };
+      if constexpr (kCodes) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const f32x4 by = scales[stage][0][8 * b + 2 * j + h];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[b][4 * j + i] *= by[i];
+          }
+      }
+      if (!clear) hide(-INFINITY);
+      float top = -INFINITY;
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
+      top *= a.scale;   // not negative (the queries carry its sign), and not zero
+      if (__any(top > m + kRaise)) {
+        const float next = fmaxf(m, other_max(top));
+        const float shrink = exp2_fast(m - finite_max(next));
+        m = next;
+        l *= shrink;
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) o[b] *= shrink;
+      }
+      const float from = -finite_max(m);
+      float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          s[b][i] = exp2_fast(fmaf(s[b][i], a.scale, from));
+          sum[b] += s[b][i];
+        }
+      l += sum[0] + sum[1];
+      if constexpr (kCodes) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const f32x4 by = scales[stage][1][8 * b + 2 * j + h];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[b][4 * j + i] *= by[i];
+          }
+        if (!clear) hide(0.0f);   // the scale of a key that the row does not see may be a NaN
+      }
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const int b = t / 2, i = 8 * (t % 2);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[t][e] = bf16_pair(s[b][i + 2 * e], s[b][i + 2 * e + 1]);
+      }
+    };
+
+    __syncthreads();   // the last part's tiles have been read
+    // Copies run a tile ahead of the products; codes, which wait in registers for the tile before theirs, two tiles; and
+    // the page table's entries one more.
+    Pages pages = pages_at(k_begin);
+    fetch(k_begin, pages.own, 0);
+    uint32_t holes = pages.holes;
+    pages = pages_at(k_begin + kKeyTile);
+    uint32_t next_holes = pages.holes;
+    if constexpr (kCodes) {
+      place(0);
+      if (k_begin + kKeyTile < k_end) fetch(k_begin + kKeyTile, pages.own, 1);
+      pages = pages_at(k_begin + 2 * kKeyTile);
+    }
+    tile_barrier<kCodes>();
+    int stage = 0;
+    for (int k = k_begin; k < k_end; k += kKeyTile, stage ^= 1) {
+      if constexpr (kCodes) {
+        if (k + kKeyTile < k_end) place(stage ^ 1);
+        if (k + 2 * kKeyTile < k_end) fetch(k + 2 * kKeyTile, pages.own, stage);
+      } else {
+        if (k + kKeyTile < k_end) fetch(k + kKeyTile, pages.own, stage ^ 1);
+      }
+      const uint32_t holes_after = kCodes ? next_holes : pages.holes;
+      next_holes = pages.holes;
+      pages = pages_at(k + (kCodes ? 3 : 2) * kKeyTile);
+      const uint8_t *kt = tiles[stage][0], *vt = tiles[stage][1];
+      const bool clear = k >= clear_begin && k + kKeyTile <= clear_end && k + kKeyTile <= k_end && !holes;
+      if (busy) {
+        f32x16 s[2];
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) s[b][i] = 0.0f;
+#pragma unroll
+        for (int c = 0; c < kSteps; ++c)
 #pragma unroll
           for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const f32x4 by = scales[stage][1][8 * b + 2 * j + h];
-#pragma unroll
-              for (int i = 0; i < 4; ++i) {
-                const int key = k + 32 * b + 8 * j + 4 * (int)h + i;
-                // The scale of a key that the row does not see may be a NaN.
-                const bool sees = clear || (key >= low && key < high && !(holes >> (2 * b + j / 2) & 1));
-                s[b][4 * j + i] = sees ? s[b][4 * j + i] * by[i] : 0.0f;
-              }
-            }
-        }
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          const int b = t / 2, i = 8 * (t % 2);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) w[t][e] = bf16_pair(s[b][i + 2 * e], s[b][i + 2 * e + 1]);
-        }
+            s[b] = mfma32(*(const u32x4 *)&kt[32 * b * T::kRowBytes + (key_at ^ (32 * c))], q[c], s[b]);
+        weigh(s, k, holes, stage, clear);
       }
       if constexpr (!kCodes) {
         if (!clear) {
@@ -372,9 +401,8 @@ __global__ __launch_bounds__(kThreads, DIM == 256 ? 1 : 2) void attend_tile_kern
             o[b] = mfma32(u32x4{v0[0], v0[1], v1[0], v1[1]}, w[t], o[b]);
           }
       }
-      if (more) place(stage ^ 1);
-      tile_barrier();
-      holes = next_holes;
+      tile_barrier<kCodes>();
+      holes = holes_after;
     }
     l = other_sum(l);
 

@@ -247,7 +247,10 @@ struct AttendArgs {
   uint16_t *output;
   uint32_t query_stride, output_stride, group;
   uint32_t causal, window;
+  // The scale's magnitude times log2 e; its sign is the queries', flip 0x80008000 for a negative one, and so is a zero,
+  // keep 0 (and else all ones) with a scale of 1: kernels scale -inf, the score of a key that is not seen.
   float scale;
+  uint32_t keep, flip;
   float *partials;   // the workspace: parts, then notes
   void *notes;
   uint32_t workgroups;
@@ -274,8 +277,8 @@ inline uint32_t attend_resident(uint32_t tile_rows, uint32_t waves, uint32_t hea
 hipError_t launch_attend_rows(uint32_t tile_rows, uint32_t waves, const AttendArgs &args, hipStream_t stream);
 // Tiles of kAttendWideRows rows.
 hipError_t launch_attend_tile(const AttendArgs &args, hipStream_t stream);
-// The join of the parts that either left, after it.
-hipError_t launch_attend_join(uint32_t tile_rows, const AttendArgs &args, hipStream_t stream);
+// The join of the parts that either left, after it. units: the most there are (attend.hpp).
+hipError_t launch_attend_join(uint32_t tile_rows, uint32_t units, const AttendArgs &args, hipStream_t stream);
 // The length (attend.hpp) up to which a batch of few units is never cut (launch_attend_rows).
 constexpr uint32_t kAttendLeast = 1024;
 
