@@ -18,6 +18,8 @@
 #include "attend.hpp"
 #include "device.hpp"
 
+#include <utility>
+
 namespace sq::kern {
 namespace {
 
@@ -74,6 +76,16 @@ __device__ __forceinline__ void tile_barrier() {
   asm volatile("" ::: "memory");
 }
 
+// f of 0 .. N - 1, each a constant.
+template <int N, typename F, int... I>
+__device__ __forceinline__ void static_for(F &&f, std::integer_sequence<int, I...>) {
+  (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F>
+__device__ __forceinline__ void static_for(F &&f) {
+  static_for<N>(f, std::make_integer_sequence<int, N>{});
+}
+
 // A head row in LDS: DIM bf16 values, CHUNKS 16-byte chunks. Where chunk c of key k lies.
 template <int DIM>
 struct Tile {
@@ -93,8 +105,8 @@ __global__ __launch_bounds__(kThreads, DIM == 256 ? 1 : 2) void attend_tile_kern
   constexpr int kBlockFloats = 32 * (DIM + 2);   // of a part in the workspace
   // A wave fetches 16 keys of the tile, kLoads vectors a lane of K and of V.
   constexpr int kLoads = 16 * DIM * kBytes / 1024, kRowLanes = DIM * kBytes / 16, kLoadRows = 64 / kRowLanes;
-  __shared__ __attribute__((aligned(1024))) uint8_t tiles[2][2][T::kBytes];   // [stage][K, V]
-  __shared__ f32x4 scales[kCodes ? 2 : 1][2][kKeyTile / 4];
+  __shared__ __attribute__((aligned(1024))) uint8_t tiles[2][2][T::kBytes];   // [tile % 2][K, V]
+  __shared__ f32x4 scales[kCodes ? 4 : 1][2][kKeyTile / 4];   // [tile % 4][K, V]
   __shared__ LineShared<kThreads> shared;
   const uint32_t lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
   const uint32_t wave = uniform(threadIdx.x >> 6);
@@ -161,97 +173,104 @@ __global__ __launch_bounds__(kThreads, DIM == 256 ? 1 : 2) void attend_tile_kern
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[b][i] = 0.0f;
 
-    // The tile at k: the page of this wave's 16 keys (~0u for none), and which of the four 16 keys have none. A page of 64
-    // rows or more holds the whole tile.
+    // The page table's entries of the tile at k, lanes 0..3 those of its four 16 keys (~0u past the part's keys); and what
+    // they say: the page of this wave's 16 keys (~0u for none), and which of the four have none.
     struct Pages {
       uint32_t own, holes;
     };
-    const auto pages_at = [&](int k) __attribute__((always_inline)) {
-      Pages out{~0u, 0u};
-      if (k >= k_end) return out;
-      if (a.kv.page_shift >= 6) {
-        const uint32_t page = uniform(page_of(a.kv, part.sequence, k));
-        out = {k + 16 * (int)wave < k_end ? page : ~0u, page == ~0u ? 15u : 0u};
-      } else {
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          const uint32_t page = k + 16 * g < k_end ? uniform(page_of(a.kv, part.sequence, k + 16 * g)) : ~0u;
-          if (page == ~0u) out.holes |= 1u << g;
-          if (g == (int)wave) out.own = page;
-        }
-      }
-      return out;
+    const auto entries_at = [&](int k) __attribute__((always_inline)) {
+      const int from = k + 16 * (int)min(lane, 3u);
+      return from < k_end ? a.kv.page_table[(size_t)part.sequence * a.kv.pages_per_sequence +
+                                            ((uint32_t)from >> a.kv.page_shift)]
+                          : ~0u;
     };
+    const auto pages_of = [&](uint32_t entries) __attribute__((always_inline)) {
+      const uint32_t own = from_lane(entries, wave);
+      return Pages{own < a.kv.pages ? own : ~0u, (uint32_t)__ballot(entries >= a.kv.pages) & 15u};
+    };
+    // Copies of the tile at k into stage `to`, K or V: bf16 straight into LDS, codes into registers until place() converts
+    // them.
     u32x4 code_k[kCodes ? kLoads : 1], code_v[kCodes ? kLoads : 1];
-    float code_scale = 0.0f;
-    const auto fetch = [&](int k, uint32_t page, int stage) __attribute__((always_inline)) {
+    float code_scale[2] = {0.0f, 0.0f};
+    const auto fetch = [&](int k, uint32_t page, int to, auto of_values) __attribute__((always_inline)) {
+      constexpr bool kValues = decltype(of_values)::value;
       const int from = k + 16 * (int)wave, n = page == ~0u ? 0 : min(16, k_end - from);
       const size_t base = ((((size_t)(page == ~0u ? 0 : page) * a.kv.kv_heads + part.head) << a.kv.page_shift) +
                            ((uint32_t)from & ((1u << a.kv.page_shift) - 1)));
-      const __amdgpu_buffer_rsrc_t keys = buffer_rsrc(a.kv.keys + base * row_bytes, (uint32_t)n * row_bytes),
-                                   values = buffer_rsrc(a.kv.values + base * row_bytes, (uint32_t)n * row_bytes);
+      const __amdgpu_buffer_rsrc_t rows =
+          buffer_rsrc((kValues ? a.kv.values : a.kv.keys) + base * row_bytes, (uint32_t)n * row_bytes);
       if constexpr (kCodes) {
 #pragma unroll
-        for (int j = 0; j < kLoads; ++j) {
-          code_k[j] = buffer_b128<0>(keys, key_from[j], 0);
-          code_v[j] = buffer_b128<0>(values, value_from[j], 0);
-        }
-        // Lanes 0..15 the keys' scales, 16..31 the values'.
-        const float *from_scales = lane < 16 ? a.kv.key_scales : a.kv.value_scales;
-        code_scale = lane < 32 && (int)(lane & 15) < n ? from_scales[base + (lane & 15)] : 0.0f;
+        for (int j = 0; j < kLoads; ++j)
+          (kValues ? code_v : code_k)[j] = buffer_b128<0>(rows, (kValues ? value_from : key_from)[j], 0);
+        const __amdgpu_buffer_rsrc_t by =
+            buffer_rsrc((kValues ? a.kv.value_scales : a.kv.key_scales) + base, (uint32_t)n * 4);
+        code_scale[kValues] = __uint_as_float(buffer_b32<0>(by, 4 * (lane & 15), 0));
       } else {
-        uint8_t *to_k = &tiles[stage][0][16 * wave * T::kRowBytes], *to_v = &tiles[stage][1][16 * wave * T::kRowBytes];
+        uint8_t *lds = &tiles[to][kValues][16 * wave * T::kRowBytes];
 #pragma unroll
-        for (int j = 0; j < kLoads; ++j) {
-          copy_to_lds(keys, to_k + 1024 * j, key_from[j]);
-          copy_to_lds(values, to_v + 1024 * j, value_from[j]);
-        }
+        for (int j = 0; j < kLoads; ++j) copy_to_lds(rows, lds + 1024 * j, (kValues ? value_from : key_from)[j]);
       }
     };
-    // The fetched codes into LDS as bf16.
-    const auto place = [&](int stage) __attribute__((always_inline)) {
+    const auto place = [&](int tile, auto of_values) __attribute__((always_inline)) {
+      constexpr bool kValues = decltype(of_values)::value;
       if constexpr (kCodes) {
 #pragma unroll
         for (int j = 0; j < kLoads; ++j) {
           const uint32_t k = kLoadRows * j + lane / kRowLanes, c = 2 * (lane % kRowLanes);
+          const u32x4 w = (kValues ? code_v : code_k)[j];
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
-            const u32x2 k0 = code_pairs4<FMT>(code_k[j][2 * i]), k1 = code_pairs4<FMT>(code_k[j][2 * i + 1]);
-            const u32x2 v0 = code_pairs4<FMT>(code_v[j][2 * i]), v1 = code_pairs4<FMT>(code_v[j][2 * i + 1]);
-            *(u32x4 *)&tiles[stage][0][code_to[j] + 16 * ((c + i) ^ T::key_swap(k))] = u32x4{k0[0], k0[1], k1[0], k1[1]};
-            *(u32x4 *)&tiles[stage][1][code_to[j] + 16 * ((c + i) ^ T::value_swap(k))] =
-                u32x4{v0[0], v0[1], v1[0], v1[1]};
+            const u32x2 lo = code_pairs4<FMT>(w[2 * i]), hi = code_pairs4<FMT>(w[2 * i + 1]);
+            *(u32x4 *)&tiles[tile % 2][kValues][code_to[j] + 16 * ((c + i) ^ (kValues ? T::value_swap(k) : T::key_swap(k)))] =
+                u32x4{lo[0], lo[1], hi[0], hi[1]};
           }
         }
-        if (lane < 32) ((float *)&scales[stage][lane / 16][4 * wave])[lane & 15] = code_scale;
+        if (lane < 16) ((float *)&scales[tile % 4][kValues][4 * wave])[lane] = code_scale[kValues];
       }
     };
+    constexpr std::false_type kOfKeys{};
+    constexpr std::true_type kOfValues{};
 
-    // The scores of the tile to weights, the second product's operands: 16 keys each in w.
-    u32x4 w[4];
-    const auto weigh = [&](f32x16 (&s)[2], int k, uint32_t holes, int stage, bool clear) __attribute__((always_inline)) {
-      // In a clear tile every row sees every key; in the others a key is compared with the row's, and with the holes.
-      const auto hide = [&](float value) __attribute__((always_inline)) {
+    f32x16 s[2];   // the products of the tile at hand
+    const auto zero = [](f32x16 (&s)[2]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s[b][i] = 0.0f;
+    };
+    const auto key_operand = [&](int tile, int c, int b) __attribute__((always_inline)) {
+      return *(const u32x4 *)&tiles[tile % 2][0][32 * b * T::kRowBytes + (key_at ^ (32 * c))];
+    };
+    const auto value_operand = [&](int tile, int t, int b) __attribute__((always_inline)) {
+      const uint8_t *from = &tiles[tile % 2][1][16 * t * T::kRowBytes + (value_at ^ (64 * b))];
+      const u32x2 v0 = read_transposed(from), v1 = read_transposed(from + 8 * T::kRowBytes);
+      return u32x4{v0[0], v0[1], v1[0], v1[1]};
+    };
+
+    // A tile's scores to their final form but for the exponential: scaled (codes), hidden where the row does not see the
+    // key, the running maximum above all of them but kRaise.
+    const auto settle = [&](int tile, int k, uint32_t holes, bool clear) __attribute__((always_inline)) {
+      if constexpr (kCodes) {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const f32x4 by = scales[tile % 4][0][8 * b + 2 * j + h];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[b][4 * j + i] *= by[i];
+          }
+      }
+      if (!clear) {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
           for (int i = 0; i < 16; ++i) {
             const int key = k + 32 * b + 8 * (i / 4) + 4 * (int)h + i % 4;
             const bool sees = key >= low && key < high && !(holes >> (2 * b + i / 8) & 1);
-            s[b][i] = sees ? s[b][i] : value;
-          }
-      };
-      if constexpr (kCodes) {
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const f32x4 by = scales[stage][0][8 * b + 2 * j + h];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[b][4 * j + i] *= by[i];
+            s[b][i] = sees ? s[b][i] : -INFINITY;
           }
       }
-      if (!clear) hide(-INFINITY);
       float top = -INFINITY;
 #pragma unroll
       for (int b = 0; b < 2; ++b)
@@ -266,143 +285,200 @@ __global__ __launch_bounds__(kThreads, DIM == 256 ? 1 : 2) void attend_tile_kern
 #pragma unroll
         for (int b = 0; b < kBlocks; ++b) o[b] *= shrink;
       }
-      const float from = -finite_max(m);
-      float sum[2] = {0.0f, 0.0f};
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          s[b][i] = exp2_fast(fmaf(s[b][i], a.scale, from));
-          sum[b] += s[b][i];
-        }
-      l += sum[0] + sum[1];
-      if constexpr (kCodes) {
-#pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const f32x4 by = scales[stage][1][8 * b + 2 * j + h];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) s[b][4 * j + i] *= by[i];
-          }
-        if (!clear) hide(0.0f);   // the scale of a key that the row does not see may be a NaN
-      }
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        const int b = t / 2, i = 8 * (t % 2);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) w[t][e] = bf16_pair(s[b][i + 2 * e], s[b][i + 2 * e + 1]);
-      }
     };
 
-    __syncthreads();   // the last part's tiles have been read
-    // Copies run a tile ahead of the products; codes, which wait in registers for the tile before theirs, two tiles; and
-    // the page table's entries one more.
-    Pages pages = pages_at(k_begin);
-    fetch(k_begin, pages.own, 0);
-    uint32_t holes = pages.holes;
-    pages = pages_at(k_begin + kKeyTile);
-    uint32_t next_holes = pages.holes;
-    if constexpr (kCodes) {
-      place(0);
-      if (k_begin + kKeyTile < k_end) fetch(k_begin + kKeyTile, pages.own, 1);
-      pages = pages_at(k_begin + 2 * kKeyTile);
-    }
-    tile_barrier<kCodes>();
-    int stage = 0;
-    for (int k = k_begin; k < k_end; k += kKeyTile, stage ^= 1) {
+    // Infinities and NaNs among a tile's values (bf16) must not reach rows that do not see them through 0 * inf: the rows
+    // that do see them add their products one by one, and they leave the tile. Only tiles that are not clear can have
+    // such rows.
+    const auto set_apart = [&](int tile, int k, uint32_t holes) __attribute__((always_inline)) {
       if constexpr (kCodes) {
-        if (k + kKeyTile < k_end) place(stage ^ 1);
-        if (k + 2 * kKeyTile < k_end) fetch(k + 2 * kKeyTile, pages.own, stage);
-      } else {
-        if (k + kKeyTile < k_end) fetch(k + kKeyTile, pages.own, stage ^ 1);
-      }
-      const uint32_t holes_after = kCodes ? next_holes : pages.holes;
-      next_holes = pages.holes;
-      pages = pages_at(k + (kCodes ? 3 : 2) * kKeyTile);
-      const uint8_t *kt = tiles[stage][0], *vt = tiles[stage][1];
-      const bool clear = k >= clear_begin && k + kKeyTile <= clear_end && k + kKeyTile <= k_end && !holes;
-      if (busy) {
-        f32x16 s[2];
+        // Codes are finite; the scale of a head row that was not is a NaN, and all of it is.
+        float *by = (float *)scales[tile % 4][1];
+        const bool bad = !(fabsf(by[lane]) < INFINITY);
+        uint64_t rows_bad = __ballot(bad);
+        if (!rows_bad) return;
+        while (busy && rows_bad) {
+          const int key = __ffsll((unsigned long long)rows_bad) - 1, j = k + key;
+          rows_bad &= rows_bad - 1;
+          if (on && j >= low && j < high && !(holes >> (key / 16) & 1)) {
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
-#pragma unroll
-          for (int i = 0; i < 16; ++i) s[b][i] = 0.0f;
-#pragma unroll
-        for (int c = 0; c < kSteps; ++c)
-#pragma unroll
-          for (int b = 0; b < 2; ++b)
-            s[b] = mfma32(*(const u32x4 *)&kt[32 * b * T::kRowBytes + (key_at ^ (32 * c))], q[c], s[b]);
-        weigh(s, k, holes, stage, clear);
-      }
-      if constexpr (!kCodes) {
-        if (!clear) {
-          // Infinities and NaNs among the tile's values must not reach rows that do not see them through 0 * inf: the
-          // rows that do see them add their products one by one, and they leave the tile.
-          constexpr int kMine = T::kBytes / 16 / kThreads;
-          uint32_t any = 0;
-#pragma unroll
-          for (int i = 0; i < kMine; ++i) {
-            const u32x4 v = *(const u32x4 *)&vt[16 * (threadIdx.x + kThreads * i)];
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              any |= (uint32_t)((v[e] & 0x7F80u) == 0x7F80u) | (uint32_t)((v[e] & 0x7F800000u) == 0x7F800000u);
-          }
-          if (__syncthreads_or((int)any)) {
-            if (busy) {
-#pragma unroll
-              for (int t = 0; t < 4; ++t)
-#pragma unroll 1
-                for (uint32_t key = 0; key < 16; ++key) {
-                  // Key `key` of 16 is weight 4 (key / 8) + key % 4 of the lanes with h = key / 4 % 2.
-                  const uint32_t first = key & 8 ? w[t][2] : w[t][0], second = key & 8 ? w[t][3] : w[t][1];
-                  const uint32_t word = (uint32_t)__shfl((int)(key & 2 ? second : first), (int)(r + 32 * (key / 4 % 2)));
-                  const float weight = __uint_as_float(key & 1 ? word & 0xFFFF0000u : word << 16);
-                  const int j = k + 16 * t + (int)key;
-                  const bool sees = on && j >= low && j < high && !(holes >> t & 1);
-                  const uint32_t row = 16 * t + key;
-#pragma unroll
-                  for (int b = 0; b < kBlocks; ++b)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                      const uint32_t chunk = (4 * b + i) ^ T::value_swap(row);
-                      const u32x2 v = *(const u32x2 *)&vt[row * T::kRowBytes + 16 * chunk + 8 * h];
-#pragma unroll
-                      for (int e = 0; e < 4; ++e) {
-                        const uint32_t bits = e & 1 ? v[e / 2] >> 16 : v[e / 2] & 0xFFFFu;
-                        if (sees && (bits & 0x7F80u) == 0x7F80u) o[b][4 * i + e] += weight * bf16_to_f32(bits);
-                      }
-                    }
-                }
-            }
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < kMine; ++i) {
-              u32x4 *v = (u32x4 *)&tiles[stage][1][16 * (threadIdx.x + kThreads * i)];
-              u32x4 clean = *v;
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                if ((clean[e] & 0x7F80u) == 0x7F80u) clean[e] &= 0xFFFF0000u;
-                if ((clean[e] & 0x7F800000u) == 0x7F800000u) clean[e] &= 0x0000FFFFu;
-              }
-              *v = clean;
-            }
-            __syncthreads();
+            for (int b = 0; b < kBlocks; ++b) o[b] += __uint_as_float(0x7FC00000u);
           }
         }
+        __syncthreads();
+        if (bad && wave == 0) by[lane] = 0.0f;
+        __syncthreads();
+        return;
       }
+      constexpr int kMine = T::kBytes / 16 / kThreads;
+      uint8_t *vt = tiles[tile % 2][1];
+      uint32_t any = 0;
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        const u32x4 v = *(const u32x4 *)&vt[16 * (threadIdx.x + kThreads * i)];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          any |= (uint32_t)((v[e] & 0x7F80u) == 0x7F80u) | (uint32_t)((v[e] & 0x7F800000u) == 0x7F800000u);
+      }
+      if (!__syncthreads_or((int)any)) return;
       if (busy) {
+#pragma unroll 1
+        for (uint32_t key = 0; key < kKeyTile; ++key) {
+          // Key `key` is score 4 (key % 32 / 8) + key % 4 of block key / 32 in the lanes with h = key / 4 % 2.
+          const uint32_t i = 4 * (key % 32 / 8) + key % 4;
+          const float score = key & 32 ? s[1][i] : s[0][i];
+          const float mine = bf16_to_f32(f32_to_bf16(exp2_fast(fmaf(score, a.scale, -finite_max(m)))));
+          const float weight = __shfl(mine, (int)(r + 32 * (key / 4 % 2)));
+          const int j = k + (int)key;
+          const bool sees = on && j >= low && j < high && !(holes >> (key / 16) & 1);
 #pragma unroll
-        for (int t = 0; t < 4; ++t)
+          for (int b = 0; b < kBlocks; ++b)
 #pragma unroll
-          for (int b = 0; b < kBlocks; ++b) {
-            const uint8_t *from = &vt[16 * t * T::kRowBytes + (value_at ^ (64 * b))];
-            const u32x2 v0 = read_transposed(from), v1 = read_transposed(from + 8 * T::kRowBytes);
-            o[b] = mfma32(u32x4{v0[0], v0[1], v1[0], v1[1]}, w[t], o[b]);
-          }
+            for (int c = 0; c < 4; ++c) {
+              const uint32_t chunk = (4 * b + c) ^ T::value_swap(key);
+              const u32x2 v = *(const u32x2 *)&vt[key * T::kRowBytes + 16 * chunk + 8 * h];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const uint32_t bits = e & 1 ? v[e / 2] >> 16 : v[e / 2] & 0xFFFFu;
+                if (sees && (bits & 0x7F80u) == 0x7F80u) o[b][4 * c + e] += weight * bf16_to_f32(bits);
+              }
+            }
+        }
       }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < kMine; ++i) {
+        u32x4 *v = (u32x4 *)&vt[16 * (threadIdx.x + kThreads * i)];
+        u32x4 clean = *v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if ((clean[e] & 0x7F80u) == 0x7F80u) clean[e] &= 0xFFFF0000u;
+          if ((clean[e] & 0x7F800000u) == 0x7F800000u) clean[e] &= 0x0000FFFFu;
+        }
+        *v = clean;
+      }
+      __syncthreads();
+    };
+
+    // The rest of a tile, and the next one's first product beside it, so that the matrix unit has work while the
+    // exponentials run. The products go out in slots, each with its share of the arithmetic, its operand read from LDS
+    // kAhead slots before; a barrier to the compiler's scheduling keeps them so (left to itself it gathers the products,
+    // each behind a wait for its operand: 2048 rows at 16384 keys 653 us, and with the slots ...):
+    //  - kSteps slots: half of the next scores; the weights of the tile's first 32 keys.
+    //  - 2 kSteps: the other half in turn with those keys' values; the weights of the other 32 keys.
+    //  - kSteps: the other keys' values.
+    const auto finish = [&](int tile) __attribute__((always_inline)) {
+      constexpr int kSlots = 4 * kSteps, kAhead = 4;
+      // Slot i's product: a score (step c of block b of 32 keys), or values (16 keys t into block b of 32 values).
+      struct Slot {
+        bool score;
+        int major, minor;
+      };
+      constexpr auto slot = [](int i) {
+        if (i < kSteps) return Slot{true, i / 2, i % 2};
+        if (i < 3 * kSteps) {
+          const int j = (i - kSteps) / 2;
+          return (i - kSteps) % 2 == 0 ? Slot{true, kSteps / 2 + j / 2, j % 2} : Slot{false, j / kBlocks, j % kBlocks};
+        }
+        const int j = i - 3 * kSteps;
+        return Slot{false, 2 + j / kBlocks, j % kBlocks};
+      };
+      f32x16 next[2];
+      zero(next);
+      u32x4 w[4];   // the weights of 16 keys each
+      u32x4 operand[kSlots];
+      const float from = -finite_max(m);
+      float sum[2] = {0.0f, 0.0f};
+      f32x4 by{1.0f, 1.0f, 1.0f, 1.0f};
+      const auto read = [&](auto index) __attribute__((always_inline)) {
+        constexpr Slot at = slot(decltype(index)::value);
+        operand[index] = at.score ? key_operand(tile + 1, at.major, at.minor) : value_operand(tile, at.major, at.minor);
+      };
+      // The weight of score i of block b.
+      const auto weigh = [&](int b, int i) __attribute__((always_inline)) {
+        if constexpr (kCodes)
+          if (i % 4 == 0) by = scales[tile % 4][1][8 * b + 2 * (i / 4) + h];
+        s[b][i] = exp2_fast(fmaf(s[b][i], a.scale, from));
+        sum[i % 2] += s[b][i];
+        if constexpr (kCodes) s[b][i] *= by[i % 4];
+        if (i % 2) w[2 * b + i / 8][i % 8 / 2] = bf16_pair(s[b][i - 1], s[b][i]);
+      };
+      static_for<kAhead>([&](auto i) __attribute__((always_inline)) { read(i); });
+      static_for<kSlots>([&](auto index) __attribute__((always_inline)) {
+        constexpr int i = decltype(index)::value;
+        if constexpr (i + kAhead < kSlots) read(std::integral_constant<int, i + kAhead>{});
+        constexpr Slot at = slot(i);
+        if constexpr (at.score) next[at.minor] = mfma32(operand[i], q[at.major], next[at.minor]);
+        else o[at.minor] = mfma32(operand[i], w[at.major], o[at.minor]);
+        constexpr int j = i - kSteps;
+        if constexpr (i < kSteps)
+          for (int e = 16 * i / kSteps; e < 16 * (i + 1) / kSteps; ++e) weigh(0, e);
+        else if constexpr (j < 2 * kSteps)
+          for (int e = 8 * j / kSteps; e < 8 * (j + 1) / kSteps; ++e) weigh(1, e);
+        __builtin_amdgcn_sched_barrier(0);
+      });
+      l += sum[0] + sum[1];
+#pragma unroll
+      for (int b = 0; b < 2; ++b) s[b] = next[b];
+    };
+
+    // K runs a tile ahead of V: while a tile is finished and the next one's scores are made, the copies of K two tiles on
+    // and V one tile on are under way, into the stages that the last tile has left. Codes wait in registers one tile
+    // more, and the page table's entries are fetched a tile before the copies that want them.
+    const int tiles_n = max(part.t1 - part.t0, 0);
+    const auto at_tile = [&](int i) __attribute__((always_inline)) { return k_begin + kKeyTile * i; };
+    __syncthreads();   // the last part's tiles have been read
+    Pages pages[4];    // of the tiles from the one at hand on
+    uint32_t entries[3];
+#pragma unroll
+    for (int i = 0; i < 3; ++i) entries[i] = entries_at(at_tile(i));
+#pragma unroll
+    for (int i = 0; i < 3; ++i) pages[i] = pages_of(entries[i]);
+    uint32_t later = entries_at(at_tile(3));
+    fetch(at_tile(0), pages[0].own, 0, kOfKeys);
+    fetch(at_tile(0), pages[0].own, 0, kOfValues);
+    place(0, kOfKeys);
+    place(0, kOfValues);
+    fetch(at_tile(1), pages[1].own, 1, kOfKeys);
+    if constexpr (kCodes) {
+      place(1, kOfKeys);
+      fetch(at_tile(2), pages[2].own, 0, kOfKeys);
+      fetch(at_tile(1), pages[1].own, 1, kOfValues);
+    }
+    tile_barrier<kCodes>();
+    if (busy) {
+      zero(s);
+#pragma unroll
+      for (int c = 0; c < kSteps; ++c)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) s[b] = mfma32(key_operand(0, c, b), q[c], s[b]);
+    }
+    tile_barrier<kCodes>();   // K's first stage has been read
+    for (int tile = 0; tile < tiles_n; ++tile) {
+      const int k = at_tile(tile);
+      pages[3] = pages_of(later);
+      later = entries_at(at_tile(tile + 4));
+      if constexpr (kCodes) {
+        if (tile + 1 < tiles_n) {
+          place(tile + 2, kOfKeys);
+          place(tile + 1, kOfValues);
+        }
+        if (tile + 2 < tiles_n) {
+          fetch(at_tile(tile + 3), pages[3].own, 0, kOfKeys);
+          fetch(at_tile(tile + 2), pages[2].own, 0, kOfValues);
+        }
+      } else {
+        if (tile + 2 < tiles_n) fetch(at_tile(tile + 2), pages[2].own, tile % 2, kOfKeys);
+        if (tile + 1 < tiles_n) fetch(at_tile(tile + 1), pages[1].own, (tile + 1) % 2, kOfValues);
+      }
+      const uint32_t holes = pages[0].holes;
+      const bool clear = k >= clear_begin && k + kKeyTile <= clear_end && k + kKeyTile <= k_end && !holes;
+      if (busy) settle(tile, k, holes, clear);
+      if (!clear) set_apart(tile, k, holes);
+      if (busy) finish(tile);
       tile_barrier<kCodes>();
-      holes = holes_after;
+#pragma unroll
+      for (int i = 0; i < 3; ++i) pages[i] = pages[i + 1];
     }
     l = other_sum(l);
 
