@@ -232,13 +232,8 @@ __global__ __launch_bounds__(kThreads, DIM == 256 ? 1 : 2) void attend_tile_kern
     constexpr std::false_type kOfKeys{};
     constexpr std::true_type kOfValues{};
 
-    f32x16 s[2];   // the products of the tile at hand
-    const auto zero = [](f32x16 (&s)[2]) __attribute__((always_inline)) {
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) s[b][i] = 0.0f;
-    };
+    f32x16 s[2];   // the scores of the tile at hand
+    constexpr f32x16 kZero{};
     const auto key_operand = [&](int tile, int c, int b) __attribute__((always_inline)) {
       return *(const u32x4 *)&tiles[tile % 2][0][32 * b * T::kRowBytes + (key_at ^ (32 * c))];
     };
@@ -360,36 +355,27 @@ __global__ __launch_bounds__(kThreads, DIM == 256 ? 1 : 2) void attend_tile_kern
       __syncthreads();
     };
 
-    // The rest of a tile, and the next one's first product beside it, so that the matrix unit has work while the
-    // exponentials run. The products go out in slots, each with its share of the arithmetic, its operand read from LDS
-    // kAhead slots before; a barrier to the compiler's scheduling keeps them so (left to itself it gathers the products,
-    // each behind a wait for its operand: 2048 rows at 16384 keys 653 us, and with the slots ...):
-    //  - kSteps slots: half of the next scores; the weights of the tile's first 32 keys.
-    //  - 2 kSteps: the other half in turn with those keys' values; the weights of the other 32 keys.
-    //  - kSteps: the other keys' values.
+    // The rest of a tile, and the next one's first product: each block of 32 scores gives its registers to the next tile's
+    // as it becomes weights. The products go out in slots, scores and values in turn, operands read from LDS kAhead slots
+    // before, the second block's exponentials between the first ones' products; a barrier to the compiler's scheduling
+    // keeps them so (left to itself it gathers the products, each behind a wait for its operand).
     const auto finish = [&](int tile) __attribute__((always_inline)) {
       constexpr int kSlots = 4 * kSteps, kAhead = 4;
-      // Slot i's product: a score (step c of block b of 32 keys), or values (16 keys t into block b of 32 values).
+      // Slot i's product: a score (step of a block of 32 keys), or values (16 keys into a block of 32 values).
       struct Slot {
         bool score;
         int major, minor;
       };
       constexpr auto slot = [](int i) {
-        if (i < kSteps) return Slot{true, i / 2, i % 2};
-        if (i < 3 * kSteps) {
-          const int j = (i - kSteps) / 2;
-          return (i - kSteps) % 2 == 0 ? Slot{true, kSteps / 2 + j / 2, j % 2} : Slot{false, j / kBlocks, j % kBlocks};
-        }
-        const int j = i - 3 * kSteps;
-        return Slot{false, 2 + j / kBlocks, j % kBlocks};
+        const int half = i / (2 * kSteps), j = i % (2 * kSteps) / 2;
+        return i % 2 == 0 ? Slot{true, j, half} : Slot{false, 2 * half + j / kBlocks, j % kBlocks};
       };
-      f32x16 next[2];
-      zero(next);
       u32x4 w[4];   // the weights of 16 keys each
       u32x4 operand[kSlots];
       const float from = -finite_max(m);
       float sum[2] = {0.0f, 0.0f};
       f32x4 by{1.0f, 1.0f, 1.0f, 1.0f};
+      float even = 0.0f;
       const auto read = [&](auto index) __attribute__((always_inline)) {
         constexpr Slot at = slot(decltype(index)::value);
         operand[index] = at.score ? key_operand(tile + 1, at.major, at.minor) : value_operand(tile, at.major, at.minor);
@@ -398,28 +384,26 @@ __global__ __launch_bounds__(kThreads, DIM == 256 ? 1 : 2) void attend_tile_kern
       const auto weigh = [&](int b, int i) __attribute__((always_inline)) {
         if constexpr (kCodes)
           if (i % 4 == 0) by = scales[tile % 4][1][8 * b + 2 * (i / 4) + h];
-        s[b][i] = exp2_fast(fmaf(s[b][i], a.scale, from));
-        sum[i % 2] += s[b][i];
-        if constexpr (kCodes) s[b][i] *= by[i % 4];
-        if (i % 2) w[2 * b + i / 8][i % 8 / 2] = bf16_pair(s[b][i - 1], s[b][i]);
+        float v = exp2_fast(fmaf(s[b][i], a.scale, from));
+        sum[i % 2] += v;
+        if constexpr (kCodes) v *= by[i % 4];
+        if (i % 2) w[2 * b + i / 8][i % 8 / 2] = bf16_pair(even, v);
+        else even = v;
       };
       static_for<kAhead>([&](auto i) __attribute__((always_inline)) { read(i); });
+#pragma unroll
+      for (int i = 0; i < 16; ++i) weigh(0, i);
       static_for<kSlots>([&](auto index) __attribute__((always_inline)) {
         constexpr int i = decltype(index)::value;
         if constexpr (i + kAhead < kSlots) read(std::integral_constant<int, i + kAhead>{});
         constexpr Slot at = slot(i);
-        if constexpr (at.score) next[at.minor] = mfma32(operand[i], q[at.major], next[at.minor]);
+        if constexpr (at.score) s[at.minor] = mfma32(operand[i], q[at.major], at.major ? s[at.minor] : kZero);
         else o[at.minor] = mfma32(operand[i], w[at.major], o[at.minor]);
-        constexpr int j = i - kSteps;
-        if constexpr (i < kSteps)
-          for (int e = 16 * i / kSteps; e < 16 * (i + 1) / kSteps; ++e) weigh(0, e);
-        else if constexpr (j < 2 * kSteps)
-          for (int e = 8 * j / kSteps; e < 8 * (j + 1) / kSteps; ++e) weigh(1, e);
+        if constexpr (i < 2 * kSteps)
+          for (int e = 8 * i / kSteps; e < 8 * (i + 1) / kSteps; ++e) weigh(1, e);
         __builtin_amdgcn_sched_barrier(0);
       });
       l += sum[0] + sum[1];
-#pragma unroll
-      for (int b = 0; b < 2; ++b) s[b] = next[b];
     };
 
     // K runs a tile ahead of V: while a tile is finished and the next one's scores are made, the copies of K two tiles on
@@ -447,15 +431,18 @@ __global__ __launch_bounds__(kThreads, DIM == 256 ? 1 : 2) void attend_tile_kern
     }
     tile_barrier<kCodes>();
     if (busy) {
-      zero(s);
 #pragma unroll
       for (int c = 0; c < kSteps; ++c)
 #pragma unroll
-        for (int b = 0; b < 2; ++b) s[b] = mfma32(key_operand(0, c, b), q[c], s[b]);
+        for (int b = 0; b < 2; ++b) s[b] = mfma32(key_operand(0, c, b), q[c], c ? s[b] : kZero);
     }
     tile_barrier<kCodes>();   // K's first stage has been read
     for (int tile = 0; tile < tiles_n; ++tile) {
       const int k = at_tile(tile);
+      // Of two workgroups' waves on a SIMD the older goes first, and finishes long before the other: they take turns
+      // instead (2048 rows at 16384 keys: 372 and 468 us without the turns, 408 and 417 with them).
+      if (tile & 1) __builtin_amdgcn_s_setprio(1);
+      else __builtin_amdgcn_s_setprio(0);
       pages[3] = pages_of(later);
       later = entries_at(at_tile(tile + 4));
       if constexpr (kCodes) {
