@@ -305,7 +305,7 @@ void Attention::add(hipStream_t graph, const HeadRowsView &query, const HeadRows
   // A batch of few units, none longer than a workgroup takes at least, is cut nowhere (attend.hpp), and leaves no parts.
   const uint64_t units = (batch.rows / (plan.tileRows / shape.group()) + batch.sequences) * uint64_t{shape.kv.kvHeads};
   const bool whole = plan.tileRows != kern::kAttendWideRows && batch.sequences <= 64 && units * 4 <= plan.workgroups &&
-                     uint64_t{batch.pagesPerSequence} * cache.shape.pageRows + 128 <= kern::kAttendLeast;
+                     uint64_t{batch.pagesPerSequence} * cache.shape.pageRows + 384 <= kern::kAttendLeast;
   const OnStreamDevice on(graph);
   launched(plan.tileRows == kern::kAttendWideRows ? kern::launch_attend_tile(args, graph)
                                                   : kern::launch_attend_rows(plan.tileRows, plan.waves, args, graph),

@@ -3,8 +3,8 @@
 //
 // A unit is `fit` consecutive rows of one sequence (tile_rows / group of them, with the query heads of one key head)
 // against every key that they see, in tiles of 64 keys. Unit m of a sequence ends at key e_m = position of its last row +
-// 1 (or the sequence's end), starts at key s_m (its first row's window), and is e_m - s_m + 126 long: at least 64 for
-// each of its tiles, ceil(e_m / 64) - floor(s_m / 64) of them, and a little for its fixed cost. Lengths live on the
+// 1 (or the sequence's end), starts at key s_m (its first row's window), and is e_m - s_m + slack long, slack at least
+// 126: 64 or more for each of its tiles, ceil(e_m / 64) - floor(s_m / 64) of them, and what a unit costs besides. Lengths live on the
 // device and differ by orders of magnitude within a batch, so no grid over (sequence, head, split) is even. Two ways of
 // sharing the units out:
 //
@@ -25,6 +25,8 @@
 namespace sq::kern {
 
 constexpr int kKeyTile = 64;
+// The least that a unit is longer than its keys, which makes it 64 for each of its tiles; a tile adds what a unit costs
+// it besides keys.
 constexpr int kUnitSlack = 2 * (kKeyTile - 1);
 constexpr uint32_t kMaxSequences = SQ_KV_MAX_SEQUENCES;
 
@@ -55,7 +57,7 @@ __device__ __forceinline__ int64_t quotient_up(int64_t a, int64_t b) { return qu
 
 // One sequence's units.
 struct Units {
-  int rows, keys, base, fit, count, window;   // base: the first row's position; window 0: none
+  int rows, keys, base, fit, slack, count, window;   // base: the first row's position; window 0: none
   bool causal;
   __device__ __forceinline__ int end(int m) const {
     return causal ? max(1, base + min(rows, fit * (m + 1))) : max(1, keys);
@@ -65,19 +67,24 @@ struct Units {
   }
   __device__ __forceinline__ int first_tile(int m) const { return start(m) / kKeyTile; }
   __device__ __forceinline__ int tiles(int m) const { return (end(m) + kKeyTile - 1) / kKeyTile - first_tile(m); }
-  __device__ __forceinline__ int length(int m) const { return end(m) - start(m) + kUnitSlack; }
+  __device__ __forceinline__ int length(int m) const { return end(m) - start(m) + slack; }
   // The length of units 0 .. m - 1, m < count (the last unit may have fewer rows).
   __device__ __forceinline__ int64_t before(int m) const {
     if (!causal) return (int64_t)m * length(0);
     const int64_t starts = window ? clamped_sum(0, base - window + 1, fit, m) : 0;
-    return clamped_sum(1, base + fit, fit, m) - starts + (int64_t)kUnitSlack * m;
+    return clamped_sum(1, base + fit, fit, m) - starts + (int64_t)slack * m;
   }
   __device__ __forceinline__ int64_t total() const { return count ? before(count - 1) + length(count - 1) : 0; }
 };
-__device__ __forceinline__ Units units_of(const AttendArgs &a, const Sequence &q, int fit) {
+// How a tile cuts: the rows of a unit, the shortest piece or part worth a workgroup (four tiles at least), a unit's slack.
+struct Cut {
+  int fit, least, slack;
+};
+__device__ __forceinline__ Units units_of(const AttendArgs &a, const Sequence &q, const Cut &cut) {
   // A window as long as the keys hides none of them; clamped, it keeps the sums in range.
   const int window = a.window && a.window < (uint32_t)q.keys ? (int)a.window : 0;
-  return {(int)q.rows, q.keys, q.keys - (int)q.rows, fit, ((int)q.rows + fit - 1) / fit, window, a.causal != 0};
+  return {(int)q.rows, q.keys, q.keys - (int)q.rows, cut.fit, cut.slack, ((int)q.rows + cut.fit - 1) / cut.fit, window,
+          a.causal != 0};
 }
 
 // A unit's part that one workgroup runs: tiles [t0, t1) of the unit's, `parts` parts in all of which this is `part`.
@@ -150,17 +157,16 @@ struct LineShared {
 
 // A workgroup's work: one even part (even), or the piece [x, end) of the line.
 struct Work {
-  bool even, pending;
+  bool even, pending, entered;   // pending: the even part is still to run; entered: `only` is the last part of the line
   uint32_t piece;
+  uint32_t active;   // workgroups with work
   Part only;
   const int64_t *prefix;
   const Sequence *cached;
   int64_t share, x, end;
 
-  uint32_t active;   // workgroups with work
-
   // The next part, or false.
-  __device__ __forceinline__ bool next(const AttendArgs &a, int fit, Part &p) {
+  __device__ __forceinline__ bool next(const AttendArgs &a, const Cut &cut, Part &p) {
     if (even) {
       p = only;
       const bool more = pending;
@@ -169,8 +175,10 @@ struct Work {
     }
     do {
       if (x >= end) return false;
-      step(a, fit, p);
-    } while (p.t1 <= p.t0);
+      if (!entered) enter(a, cut);
+      else advance(a, cut);
+    } while (only.t1 <= only.t0);
+    p = only;
     return true;
   }
   // The notes that the join reads, once all of the workgroup's parts are stored: of the unit it began (began.parts 0:
@@ -181,72 +189,94 @@ struct Work {
     if (blockIdx.x == 0) unit_notes(a)[a.workgroups].parts = active;
   }
   // p in scalar registers, whichever way it came.
-  static __device__ __forceinline__ Part settled(const AttendArgs &a, int fit, const Part &p) {
+  static __device__ __forceinline__ Part settled(const AttendArgs &a, const Cut &cut, const Part &p) {
     const Sequence q{uniform(p.first_row), (uint32_t)uniform(p.units.rows), uniform(p.units.keys)};
-    return {units_of(a, q, fit),   uniform(p.sequence), uniform(p.head),  q.first, uniform(p.m), uniform(p.t0), uniform(p.t1),
-            uniform(p.part), uniform(p.parts),    uniform(p.first_piece)};
+    return {units_of(a, q, cut), uniform(p.sequence), uniform(p.head), q.first, uniform(p.m), uniform(p.t0), uniform(p.t1),
+            uniform(p.part), uniform(p.parts), uniform(p.first_piece)};
   }
-  // The part of the line at x, and x moved past it.
-  __device__ __forceinline__ void step(const AttendArgs &a, int fit, Part &p) {
+  __device__ __forceinline__ void take(const AttendArgs &a, const Cut &cut, uint32_t sequence) {
+    const Sequence q = sequence < kCached ? cached[sequence] : sequence_of(a.kv, sequence);
+    const Sequence s{uniform(q.first), uniform(q.rows), uniform(q.keys)};
+    only.sequence = sequence;
+    only.units = units_of(a, s, cut);
+    only.first_row = s.first;
+  }
+  // The tiles from offset `from` of unit only.m on, up to its end or the piece's, and x moved past them. The parts of a
+  // unit are those that start at or before its last tile: a piece is at least a tile long, so each of them has one.
+  __device__ __forceinline__ void cut_at(int64_t from) {
+    const int64_t length = only.units.length(only.m);
+    const int64_t to = length < from + (end - x) ? length : from + (end - x);
+    const int tiles = only.units.tiles(only.m);
+    const auto tile_at = [&](int64_t o) {
+      const int64_t t = (o + kKeyTile - 1) / kKeyTile;
+      return t < tiles ? (int)t : tiles;
+    };
+    only.t0 = tile_at(from);
+    only.t1 = tile_at(to);
+    const int64_t unit = x - from;
+    only.first_piece = from ? (uint32_t)uniform(quotient(unit, share)) : piece;
+    only.parts = from == 0 && to == length
+                     ? 1
+                     : (uint32_t)uniform(quotient(unit + (int64_t)kKeyTile * (tiles - 1), share)) - only.first_piece + 1;
+    only.part = piece - only.first_piece;
+    x += to - from;
+  }
+  // The first part: where the line is at x.
+  __device__ __forceinline__ void enter(const AttendArgs &a, const Cut &cut) {
     uint32_t lo = 0, hi = a.kv.sequences;   // the last sequence that starts at or before x
     while (hi - lo > 1) {
       const uint32_t mid = (lo + hi) / 2;
       if (uniform(prefix[mid]) <= x) lo = mid;
       else hi = mid;
     }
-    p.sequence = lo;
-    Sequence q = lo < kCached ? cached[lo] : sequence_of(a.kv, lo);
-    q = {uniform(q.first), uniform(q.rows), uniform(q.keys)};
-    p.units = units_of(a, q, fit);
-    p.first_row = q.first;
-    const int64_t one = p.units.total();
+    take(a, cut, lo);
+    const Units &u = only.units;
+    const int64_t one = u.total();
     int64_t rest = x - uniform(prefix[lo]);
-    p.head = (uint32_t)uniform(quotient(rest, one));
-    rest -= one * p.head;
-    int mlo = 0, mhi = p.units.count;
+    only.head = (uint32_t)uniform(quotient(rest, one));
+    rest -= one * only.head;
+    int mlo = 0, mhi = u.count;
     while (mhi - mlo > 1) {
       const int mid = (mlo + mhi) / 2;
-      if (p.units.before(mid) <= rest) mlo = mid;
+      if (u.before(mid) <= rest) mlo = mid;
       else mhi = mid;
     }
-    p.m = mlo;
-    const int64_t from = rest - p.units.before(mlo), length = p.units.length(mlo);
-    const int64_t to = length < from + (end - x) ? length : from + (end - x);
-    const int tiles = p.units.tiles(mlo);
-    const auto tile_at = [&](int64_t o) {
-      const int64_t t = (o + kKeyTile - 1) / kKeyTile;
-      return t < tiles ? (int)t : tiles;
-    };
-    p.t0 = tile_at(from);
-    p.t1 = tile_at(to);
-    // The parts of a unit are those that start at or before its last tile: a piece is at least a tile long, so each of
-    // them has one.
-    const int64_t unit = x - from;
-    p.first_piece = (uint32_t)uniform(quotient(unit, share));
-    p.parts = (uint32_t)uniform(quotient(unit + (int64_t)kKeyTile * (tiles - 1), share)) - p.first_piece + 1;
-    p.part = piece - p.first_piece;
-    x += to - from;
+    only.m = mlo;
+    entered = true;
+    cut_at(rest - u.before(mlo));
+  }
+  // The part after the last one: the next unit, from its start.
+  __device__ __forceinline__ void advance(const AttendArgs &a, const Cut &cut) {
+    if (++only.m >= only.units.count) {
+      only.m = 0;
+      if (++only.head >= a.kv.kv_heads) {
+        only.head = 0;
+        do take(a, cut, only.sequence + 1);   // there is one with units: x lies before the line's end
+        while (!only.units.count);
+      }
+    }
+    cut_at(0);
   }
 };
 
-// Every thread of the workgroup takes part. least: the shortest piece or part worth a workgroup (four tiles at least).
+// Every thread of the workgroup takes part.
 template <int THREADS>
-__device__ __forceinline__ Work make_work(const AttendArgs &a, int fit, int least, LineShared<THREADS> &shared) {
+__device__ __forceinline__ Work make_work(const AttendArgs &a, const Cut &cut, LineShared<THREADS> &shared) {
   constexpr int kWaves = THREADS / 64;
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, count = a.kv.sequences;
   Work w{};
   if (count <= 64) {
     // Each wave for itself, a sequence a lane, in registers.
     const Sequence q = lane < count ? sequence_of(a.kv, lane) : Sequence{0u, 0u, 0};
-    const Units u = units_of(a, q, fit);
+    const Units u = units_of(a, q, cut);
     const float heads = (float)a.kv.kv_heads, units = (float)u.count, last = u.count ? (float)u.length(u.count - 1) : 0.0f,
                 first = u.count ? (float)u.length(0) : 0.0f;
     const float number = uniform(heads * wave_sum(units)), most = uniform(heads * wave_sum(units * last)),
                 work = uniform(heads * wave_sum(units * 0.5f * (first + last)));
-    if (number * 4 <= (float)a.workgroups && (most <= work * 1.25f || most <= number * (float)least)) {
+    if (number * 4 <= (float)a.workgroups && (most <= work * 1.25f || most <= number * (float)cut.least)) {
       // The share that leaves every unit's last part room: units ceil(length / share) <= workgroups. The sums are off by
       // 2^-18 at most, the share made larger by as much.
-      const int share = max(least, (int)(most * (1 + 0x1p-18f) / ((float)a.workgroups - number)) + 1);
+      const int share = max(cut.least, (int)(most * (1 + 0x1p-18f) / ((float)a.workgroups - number)) + 1);
       const uint32_t parts = u.count ? (uint32_t)(u.length(u.count - 1) + share - 1) / (uint32_t)share : 0u;
       const uint32_t mine = parts * (uint32_t)u.count * a.kv.kv_heads;
       uint32_t upto = mine;
@@ -265,7 +295,7 @@ __device__ __forceinline__ Work make_work(const AttendArgs &a, int fit, int leas
       const uint32_t s = (uint32_t)__popcll(__ballot(before <= w.piece)) - 1;
       Part &p = w.only;
       p.sequence = s;
-      p.units = units_of(a, Sequence{from_lane(q.first, s), from_lane(q.rows, s), from_lane(q.keys, s)}, fit);
+      p.units = units_of(a, Sequence{from_lane(q.first, s), from_lane(q.rows, s), from_lane(q.keys, s)}, cut);
       p.first_row = from_lane(q.first, s);
       p.parts = from_lane(parts, s);
       const uint32_t rest = w.piece - from_lane(before, s), unit = rest / p.parts;
@@ -288,7 +318,7 @@ __device__ __forceinline__ Work make_work(const AttendArgs &a, int fit, int leas
     if (s < count) {
       const Sequence q = sequence_of(a.kv, s);
       if (s < kCached) shared.sequence[s] = q;
-      v = units_of(a, q, fit).total() * a.kv.kv_heads;
+      v = units_of(a, q, cut).total() * a.kv.kv_heads;
     }
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
@@ -312,7 +342,7 @@ __device__ __forceinline__ Work make_work(const AttendArgs &a, int fit, int leas
   const int64_t total = uniform(carry), even_share = uniform(quotient_up(total, a.workgroups));
   w.prefix = shared.prefix;
   w.cached = shared.sequence;
-  w.share = even_share > least ? even_share : least;
+  w.share = even_share > cut.least ? even_share : cut.least;
   w.active = (uint32_t)uniform(quotient_up(total, w.share));
   w.piece = piece_of(w.active, blockIdx.x);
   w.x = w.share * w.piece;

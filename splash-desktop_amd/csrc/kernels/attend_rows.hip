@@ -226,16 +226,16 @@ attend_rows_kernel(AttendArgs a) {
   __shared__ Shared<MB, WAVES> shared;
   const uint32_t lane = threadIdx.x & 63, r = lane & 15, kq = lane >> 4;
   const uint32_t wave = uniform(threadIdx.x >> 6);
-  const int fit = 16 * MB / (int)a.group;
+  const Cut cut{16 * MB / (int)a.group, (int)kAttendLeast, kUnitSlack + 256};
   const float by_group = 1.0f / (float)a.group;
   const uint32_t dim = a.kv.head_dim, row_bytes = dim * R::kBytes;
-  Work work = make_work<kThreads>(a, fit, (int)kAttendLeast, shared.line);
+  Work work = make_work<kThreads>(a, cut, shared.line);
   UnitNote began{};
   Part next;
-  while (work.next(a, fit, next)) {
-    const Part part = Work::settled(a, fit, next);
+  while (work.next(a, cut, next)) {
+    const Part part = Work::settled(a, cut, next);
     const Units &u = part.units;
-    const int row0 = fit * part.m, rows = min(fit, u.rows - row0), live = rows * (int)a.group;
+    const int row0 = cut.fit * part.m, rows = min(cut.fit, u.rows - row0), live = rows * (int)a.group;
     const int unit_end = u.causal ? min(u.keys, u.base + row0 + rows) : u.keys;   // keys that any row sees
     const int tile0 = u.first_tile(part.m);
     const int k_begin = kKeyTile * (tile0 + part.t0), k_end = min(unit_end, kKeyTile * (tile0 + part.t1));

@@ -110,10 +110,10 @@ __global__ __launch_bounds__(kThreads, DIM == 256 ? 1 : 2) void attend_tile_kern
   __shared__ LineShared<kThreads> shared;
   const uint32_t lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
   const uint32_t wave = uniform(threadIdx.x >> 6);
-  const int fit = kRows / (int)a.group;
+  const Cut cut{kRows / (int)a.group, 4 * kKeyTile, kUnitSlack + 192};
   const float by_group = 1.0f / (float)a.group;
   const uint32_t dim = a.kv.head_dim, row_bytes = dim * kBytes;
-  Work work = make_work<kThreads>(a, fit, 4 * kKeyTile, shared);
+  Work work = make_work<kThreads>(a, cut, shared);
   UnitNote began{};
 
   // Where this lane's vectors lie in 16 keys of a page, and (codes) in the LDS tile.
@@ -139,10 +139,10 @@ __global__ __launch_bounds__(kThreads, DIM == 256 ? 1 : 2) void attend_tile_kern
   const uint32_t value_at = vk * T::kRowBytes + 8 * (vi % 2) + 16 * ((2 * (lane / 16 % 2) + vi % 4 / 2) ^ T::value_swap(vk));
 
   Part next;
-  while (work.next(a, fit, next)) {
-    const Part part = Work::settled(a, fit, next);
+  while (work.next(a, cut, next)) {
+    const Part part = Work::settled(a, cut, next);
     const Units &u = part.units;
-    const int row0 = fit * part.m, rows = min(fit, u.rows - row0), live = rows * (int)a.group;
+    const int row0 = cut.fit * part.m, rows = min(cut.fit, u.rows - row0), live = rows * (int)a.group;
     const int unit_end = u.causal ? min(u.keys, u.base + row0 + rows) : u.keys;   // keys that any row sees
     const int tile0 = u.first_tile(part.m);
     const int k_begin = kKeyTile * (tile0 + part.t0), k_end = min(unit_end, kKeyTile * (tile0 + part.t1));

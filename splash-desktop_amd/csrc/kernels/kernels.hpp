@@ -280,6 +280,6 @@ hipError_t launch_attend_tile(const AttendArgs &args, hipStream_t stream);
 // The join of the parts that either left, after it. units: the most there are (attend.hpp).
 hipError_t launch_attend_join(uint32_t tile_rows, uint32_t units, const AttendArgs &args, hipStream_t stream);
 // The length (attend.hpp) up to which a batch of few units is never cut (launch_attend_rows).
-constexpr uint32_t kAttendLeast = 1024;
+constexpr uint32_t kAttendLeast = 1280;
 
 }  // namespace sq::kern
