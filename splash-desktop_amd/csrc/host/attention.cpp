@@ -310,7 +310,7 @@ void Attention::add(hipStream_t graph, const HeadRowsView &query, const HeadRows
   launched(plan.tileRows == kern::kAttendWideRows ? kern::launch_attend_tile(args, graph)
                                                   : kern::launch_attend_rows(plan.tileRows, plan.waves, args, graph),
            "attention");
-  if (!whole) launched(kern::launch_attend_join(plan.tileRows, uint32_t(std::min<uint64_t>(units, ~0u)), args, graph), "attention join");
+  if (!whole) launched(kern::launch_attend_join(plan.tileRows, units * 4 <= plan.workgroups, args, graph), "attention join");
 }
 
 }  // namespace sq::ops

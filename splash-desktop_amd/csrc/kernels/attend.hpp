@@ -95,6 +95,13 @@ struct Part {
   uint32_t part, parts, first_piece;    // first_piece: the workgroup's number that holds part 0
 };
 
+// p in scalar registers, whichever way it came.
+__device__ __forceinline__ Part settled(const AttendArgs &a, const Cut &cut, const Part &p) {
+  const Sequence q{uniform(p.first_row), (uint32_t)uniform(p.units.rows), uniform(p.units.keys)};
+  return {units_of(a, q, cut), uniform(p.sequence), uniform(p.head), q.first, uniform(p.m), uniform(p.t0), uniform(p.t1),
+          uniform(p.part), uniform(p.parts), uniform(p.first_piece)};
+}
+
 // A part's place in the workspace. A piece holds at most two parts of shared units: one that an earlier piece began, and
 // one that it begins itself, of which there can be one only. (An even part may be empty, where a unit has fewer tiles
 // than parts: it is stored all the same.) A part is its blocks of 16 rows (32 in the wide tile) one after the other: the
@@ -148,37 +155,53 @@ __device__ __forceinline__ uint32_t piece_of(uint32_t active, uint32_t block) {
 
 // LDS for the line.
 constexpr uint32_t kCached = 256;   // sequences whose rows and keys stay in LDS
+// Where a workgroup stands in its piece of the line between one part and the next.
+struct Place {
+  int64_t x;
+  uint32_t sequence, head;
+  int m;
+};
 template <int THREADS>
 struct LineShared {
   int64_t prefix[kMaxSequences + 1];   // where each sequence starts
   int64_t waves[THREADS / 64];
   Sequence sequence[kCached];
+  int64_t share;
+  Place place[2];
 };
 
-// A workgroup's work: one even part (even), or the piece [x, end) of the line.
+// A workgroup's work: one even part, or the piece of the line whose state lies in LDS between its parts (a place that every
+// wave reads and one thread writes into the other of two, so that the scalar registers are the tiles').
+template <int THREADS>
 struct Work {
-  bool even, pending, entered;   // pending: the even part is still to run; entered: `only` is the last part of the line
+  bool even;
+  uint32_t turn;     // even: 0 until the part is run; else of the place to read, + 2 before the first part
   uint32_t piece;
   uint32_t active;   // workgroups with work
-  Part only;
-  const int64_t *prefix;
-  const Sequence *cached;
-  int64_t share, x, end;
 
-  // The next part, or false.
-  __device__ __forceinline__ bool next(const AttendArgs &a, const Cut &cut, Part &p) {
-    if (even) {
-      p = only;
-      const bool more = pending;
-      pending = false;
-      return more;
+  // The next part of the line, or false; an even part comes from make_work. A barrier of the workgroup's lies between one
+  // call and the next.
+  __device__ __forceinline__ bool next(const AttendArgs &a, const Cut &cut, LineShared<THREADS> &shared, Part &p) {
+    if (even) return turn++ == 0;
+    const int64_t share = uniform(shared.share), total = uniform(shared.prefix[a.kv.sequences]);
+    const int64_t begin = share * piece, end = begin + share < total ? begin + share : total;
+    Place at{};
+    if (turn >= 2) {
+      at.x = begin;
+    } else {
+      const Place &last = shared.place[turn];
+      at = {uniform(last.x), uniform(last.sequence), uniform(last.head), uniform(last.m)};
     }
     do {
-      if (x >= end) return false;
-      if (!entered) enter(a, cut);
-      else advance(a, cut);
-    } while (only.t1 <= only.t0);
-    p = only;
+      if (at.x >= end) return false;
+      int64_t from = 0;
+      if (turn >= 2) from = enter(a, cut, shared, at, p);
+      else advance(a, cut, shared, at, p);
+      turn &= 1;
+      cut_at(from, share, end, at, p);
+    } while (p.t1 <= p.t0);
+    turn ^= 1;
+    if (threadIdx.x == 0) shared.place[turn] = at;
     return true;
   }
   // The notes that the join reads, once all of the workgroup's parts are stored: of the unit it began (began.parts 0:
@@ -188,83 +211,85 @@ struct Work {
     if (piece < active) unit_notes(a)[piece] = began;
     if (blockIdx.x == 0) unit_notes(a)[a.workgroups].parts = active;
   }
-  // p in scalar registers, whichever way it came.
-  static __device__ __forceinline__ Part settled(const AttendArgs &a, const Cut &cut, const Part &p) {
-    const Sequence q{uniform(p.first_row), (uint32_t)uniform(p.units.rows), uniform(p.units.keys)};
-    return {units_of(a, q, cut), uniform(p.sequence), uniform(p.head), q.first, uniform(p.m), uniform(p.t0), uniform(p.t1),
-            uniform(p.part), uniform(p.parts), uniform(p.first_piece)};
-  }
-  __device__ __forceinline__ void take(const AttendArgs &a, const Cut &cut, uint32_t sequence) {
-    const Sequence q = sequence < kCached ? cached[sequence] : sequence_of(a.kv, sequence);
+
+ private:
+  static __device__ __forceinline__ void take(const AttendArgs &a, const Cut &cut, const LineShared<THREADS> &shared,
+                                              const Place &at, Part &p) {
+    const Sequence q = at.sequence < kCached ? shared.sequence[at.sequence] : sequence_of(a.kv, at.sequence);
     const Sequence s{uniform(q.first), uniform(q.rows), uniform(q.keys)};
-    only.sequence = sequence;
-    only.units = units_of(a, s, cut);
-    only.first_row = s.first;
+    p.units = units_of(a, s, cut);
+    p.first_row = s.first;
+    p.sequence = at.sequence;
   }
-  // The tiles from offset `from` of unit only.m on, up to its end or the piece's, and x moved past them. The parts of a
+  // The tiles from offset `from` of unit at.m on, up to its end or the piece's, and at.x moved past them. The parts of a
   // unit are those that start at or before its last tile: a piece is at least a tile long, so each of them has one.
-  __device__ __forceinline__ void cut_at(int64_t from) {
-    const int64_t length = only.units.length(only.m);
-    const int64_t to = length < from + (end - x) ? length : from + (end - x);
-    const int tiles = only.units.tiles(only.m);
+  __device__ __forceinline__ void cut_at(int64_t from, int64_t share, int64_t end, Place &at, Part &p) const {
+    const int64_t length = p.units.length(at.m);
+    const int64_t to = length < from + (end - at.x) ? length : from + (end - at.x);
+    const int tiles = p.units.tiles(at.m);
     const auto tile_at = [&](int64_t o) {
       const int64_t t = (o + kKeyTile - 1) / kKeyTile;
       return t < tiles ? (int)t : tiles;
     };
-    only.t0 = tile_at(from);
-    only.t1 = tile_at(to);
-    const int64_t unit = x - from;
-    only.first_piece = from ? (uint32_t)uniform(quotient(unit, share)) : piece;
-    only.parts = from == 0 && to == length
-                     ? 1
-                     : (uint32_t)uniform(quotient(unit + (int64_t)kKeyTile * (tiles - 1), share)) - only.first_piece + 1;
-    only.part = piece - only.first_piece;
-    x += to - from;
+    p.head = at.head;
+    p.m = at.m;
+    p.t0 = tile_at(from);
+    p.t1 = tile_at(to);
+    const int64_t unit = at.x - from;
+    p.first_piece = from ? (uint32_t)uniform(quotient(unit, share)) : piece;
+    p.parts = from == 0 && to == length
+                  ? 1
+                  : (uint32_t)uniform(quotient(unit + (int64_t)kKeyTile * (tiles - 1), share)) - p.first_piece + 1;
+    p.part = piece - p.first_piece;
+    at.x += to - from;
   }
-  // The first part: where the line is at x.
-  __device__ __forceinline__ void enter(const AttendArgs &a, const Cut &cut) {
+  // The first part: the unit at at.x on the line, and the offset in it.
+  static __device__ __forceinline__ int64_t enter(const AttendArgs &a, const Cut &cut, const LineShared<THREADS> &shared,
+                                                  Place &at, Part &p) {
     uint32_t lo = 0, hi = a.kv.sequences;   // the last sequence that starts at or before x
     while (hi - lo > 1) {
       const uint32_t mid = (lo + hi) / 2;
-      if (uniform(prefix[mid]) <= x) lo = mid;
+      if (uniform(shared.prefix[mid]) <= at.x) lo = mid;
       else hi = mid;
     }
-    take(a, cut, lo);
-    const Units &u = only.units;
+    at.sequence = lo;
+    take(a, cut, shared, at, p);
+    const Units &u = p.units;
     const int64_t one = u.total();
-    int64_t rest = x - uniform(prefix[lo]);
-    only.head = (uint32_t)uniform(quotient(rest, one));
-    rest -= one * only.head;
+    int64_t rest = at.x - uniform(shared.prefix[lo]);
+    at.head = (uint32_t)uniform(quotient(rest, one));
+    rest -= one * at.head;
     int mlo = 0, mhi = u.count;
     while (mhi - mlo > 1) {
       const int mid = (mlo + mhi) / 2;
       if (u.before(mid) <= rest) mlo = mid;
       else mhi = mid;
     }
-    only.m = mlo;
-    entered = true;
-    cut_at(rest - u.before(mlo));
+    at.m = mlo;
+    return rest - u.before(mlo);
   }
   // The part after the last one: the next unit, from its start.
-  __device__ __forceinline__ void advance(const AttendArgs &a, const Cut &cut) {
-    if (++only.m >= only.units.count) {
-      only.m = 0;
-      if (++only.head >= a.kv.kv_heads) {
-        only.head = 0;
-        do take(a, cut, only.sequence + 1);   // there is one with units: x lies before the line's end
-        while (!only.units.count);
-      }
-    }
-    cut_at(0);
+  static __device__ __forceinline__ void advance(const AttendArgs &a, const Cut &cut, const LineShared<THREADS> &shared,
+                                                 Place &at, Part &p) {
+    take(a, cut, shared, at, p);
+    if (++at.m < p.units.count) return;
+    at.m = 0;
+    if (++at.head < a.kv.kv_heads) return;
+    at.head = 0;
+    do {   // there is one with units: x lies before the line's end
+      ++at.sequence;
+      take(a, cut, shared, at, p);
+    } while (!p.units.count);
   }
 };
 
 // Every thread of the workgroup takes part.
 template <int THREADS>
-__device__ __forceinline__ Work make_work(const AttendArgs &a, const Cut &cut, LineShared<THREADS> &shared) {
+__device__ __forceinline__ Work<THREADS> make_work(const AttendArgs &a, const Cut &cut, LineShared<THREADS> &shared,
+                                                   Part &p) {
   constexpr int kWaves = THREADS / 64;
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, count = a.kv.sequences;
-  Work w{};
+  Work<THREADS> w{};
   if (count <= 64) {
     // Each wave for itself, a sequence a lane, in registers.
     const Sequence q = lane < count ? sequence_of(a.kv, lane) : Sequence{0u, 0u, 0};
@@ -288,12 +313,13 @@ __device__ __forceinline__ Work make_work(const AttendArgs &a, const Cut &cut, L
       w.even = true;
       w.active = from_lane(upto, 63);
       w.piece = piece_of(w.active, blockIdx.x);
-      w.pending = w.piece < w.active;
-      if (!w.pending) return w;
+      if (w.piece >= w.active) {
+        w.turn = 1;
+        return w;
+      }
       // The last sequence that starts at or before the piece: one with units, as the next starts past it.
       const uint32_t before = upto - mine;
       const uint32_t s = (uint32_t)__popcll(__ballot(before <= w.piece)) - 1;
-      Part &p = w.only;
       p.sequence = s;
       p.units = units_of(a, Sequence{from_lane(q.first, s), from_lane(q.rows, s), from_lane(q.keys, s)}, cut);
       p.first_row = from_lane(q.first, s);
@@ -338,15 +364,13 @@ __device__ __forceinline__ Work make_work(const AttendArgs &a, const Cut &cut, L
     carry += all;
   }
   if (threadIdx.x == 0) shared.prefix[0] = 0;
-  __syncthreads();
   const int64_t total = uniform(carry), even_share = uniform(quotient_up(total, a.workgroups));
-  w.prefix = shared.prefix;
-  w.cached = shared.sequence;
-  w.share = even_share > cut.least ? even_share : cut.least;
-  w.active = (uint32_t)uniform(quotient_up(total, w.share));
+  const int64_t share = even_share > cut.least ? even_share : cut.least;
+  if (threadIdx.x == 0) shared.share = share;
+  w.active = (uint32_t)uniform(quotient_up(total, share));
   w.piece = piece_of(w.active, blockIdx.x);
-  w.x = w.share * w.piece;
-  w.end = w.x + w.share < total ? w.x + w.share : total;
+  w.turn = 2;
+  __syncthreads();
   return w;
 }
 

@@ -2,7 +2,7 @@
 // unit's parts in key order, m their largest maximum. A launch of its own after the attention's: a workgroup of that one
 // would find out that it is the last of its unit's only after its stores and an atomic have gone past the XCDs' caches
 // (3 us a part), and then join all of the unit's rows alone (one token over 131072 int8 keys, 31 parts a unit: 8 us in
-// all), where here every vector of every unit has a wave, and all parts' loads are in flight at once.
+// all), where here the vectors of every unit go over all waves, with many parts' loads in flight.
 #include "attend.hpp"
 
 namespace sq::kern {
@@ -10,7 +10,7 @@ namespace {
 
 // VECTORS of a unit's vectors (attend.hpp: the layout of a part) by a wave, AT_ONCE parts' loads in flight.
 template <bool WIDE, int VECTORS, int AT_ONCE>
-__device__ __forceinline__ void join(const AttendArgs &a, const UnitNote &note, uint32_t dim_computed,
+__device__ __forceinline__ void join(const AttendArgs &a, const UnitNote &note, uint32_t piece, uint32_t dim_computed,
                                      uint32_t tile_rows, uint32_t block, uint32_t first) {
   const uint32_t rows = WIDE ? 32 : 16, lane = threadIdx.x & 63;
   const uint32_t p = block * rows + lane % rows;
@@ -25,7 +25,7 @@ __device__ __forceinline__ void join(const AttendArgs &a, const UnitNote &note, 
     for (int d = 0; d < AT_ONCE; ++d) {
       // Past the last part the resource is empty: zeros, and nothing read.
       const bool there = j + d < note.parts;
-      const float *from = a.partials + (size_t)part_slot(blockIdx.x, there ? j + d : 0) * part_floats +
+      const float *from = a.partials + (size_t)part_slot(piece, there ? j + d : 0) * part_floats +
                           (size_t)block * block_floats;
       const __amdgpu_buffer_rsrc_t r = buffer_rsrc(from, there ? block_floats * 4 : 0);
       const u32x2 two = buffer_b64<0>(r, on ? (rows * dim_computed + 2 * (lane % rows)) * 4 : kNowhere, 0);
@@ -64,25 +64,49 @@ __device__ __forceinline__ void join(const AttendArgs &a, const UnitNote &note, 
   }
 }
 
-// blockIdx.x's unit (the one that piece began), its vectors over the waves of the blockIdx.y's. Units of two parts, which
-// a line's mostly are, eight vectors at a time; others two. DIM is the head's values as computed.
+// The blocks and vectors of a unit, from item `next` on every `stride`-th; next becomes that of the unit after. dim is the
+// head's values as computed.
+template <bool WIDE, int VECTORS, int AT_ONCE>
+__device__ __forceinline__ void join_items(const AttendArgs &a, const UnitNote &note, uint32_t piece, uint32_t dim,
+                                           uint32_t tile_rows, uint32_t &next, uint32_t stride) {
+  const uint32_t rows = WIDE ? 32 : 16, each = dim / (WIDE ? 8 : 16) / VECTORS;
+  const uint32_t items = min(tile_rows / rows, (note.live + rows - 1) / rows) * each;
+  for (; next < items; next += stride)
+    join<WIDE, VECTORS, AT_ONCE>(a, note, piece, dim, tile_rows, next / each, VECTORS * (next % each));
+  next -= items;
+}
+
+// Many units: a workgroup a piece, for the shared unit that it began if any. Those of a line mostly have two parts, which
+// go eight vectors at a time (rows of the wide tile have as many).
 template <bool WIDE>
-__global__ __launch_bounds__(256) void attend_join_kernel(AttendArgs a, uint32_t dim_computed, uint32_t tile_rows) {
+__global__ __launch_bounds__(256) void join_many_kernel(AttendArgs a, uint32_t dim, uint32_t tile_rows) {
   const UnitNote *notes = unit_notes(a);
   const uint32_t pieces = notes[a.workgroups].parts;
-  const UnitNote note = notes[blockIdx.x];
+  const UnitNote note = notes[blockIdx.x];   // read beside the number of pieces, of which it may be past
   if (blockIdx.x >= pieces || note.parts < 2) return;
-  const uint32_t rows = WIDE ? 32 : 16, vectors = dim_computed / (WIDE ? 8 : 16);
-  const uint32_t blocks = (note.live + rows - 1) / rows, wave = uniform(blockIdx.y * 4 + (threadIdx.x >> 6));
-  const auto over = [&](auto count, auto at_once) __attribute__((always_inline)) {
-    constexpr int kVectors = decltype(count)::value;
-    const uint32_t each = vectors / kVectors;
-    for (uint32_t item = wave; item < blocks * each; item += 4 * gridDim.y)
-      join<WIDE, kVectors, decltype(at_once)::value>(a, note, dim_computed, tile_rows, item / each,
-                                                     kVectors * (item % each));
-  };
-  if (WIDE && note.parts == 2) over(std::integral_constant<int, 8>{}, std::integral_constant<int, 2>{});
-  else over(std::integral_constant<int, 2>{}, std::integral_constant<int, 16>{});
+  uint32_t next = uniform(threadIdx.x >> 6);
+  if (WIDE && note.parts == 2) join_items<WIDE, 8, 2>(a, note, blockIdx.x, dim, tile_rows, next, 4);
+  else join_items<WIDE, 2, 16>(a, note, blockIdx.x, dim, tile_rows, next, 4);
+}
+
+// Few units, of many parts each: every wave looks through the notes, one a lane, and the waves of all workgroups take the
+// units' blocks and vectors in turn.
+constexpr uint32_t kFewGroups = 256;
+template <bool WIDE>
+__global__ __launch_bounds__(256) void join_few_kernel(AttendArgs a, uint32_t dim, uint32_t tile_rows) {
+  const UnitNote *notes = unit_notes(a);
+  const uint32_t lane = threadIdx.x & 63, pieces = min(notes[a.workgroups].parts, a.workgroups);
+  uint32_t next = uniform(4 * blockIdx.x + (threadIdx.x >> 6));
+  for (uint32_t first = 0; first < pieces; first += 64) {
+    const UnitNote mine = first + lane < pieces ? notes[first + lane] : UnitNote{};
+    for (uint64_t shared = __ballot(mine.parts >= 2); shared; shared &= shared - 1) {
+      const uint32_t from = (uint32_t)__ffsll((unsigned long long)shared) - 1;
+      join_items<WIDE, 1, 32>(a,
+                              {from_lane(mine.parts, from), from_lane(mine.live, from), from_lane(mine.row, from),
+                               from_lane(mine.head, from)},
+                              first + from, dim, tile_rows, next, 4 * kFewGroups);
+    }
+  }
 }
 
 uint32_t computed(uint32_t head_dim) { return head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
@@ -95,15 +119,16 @@ uint64_t attend_partials(uint32_t tile_rows, uint32_t head_dim, uint32_t workgro
          (uint64_t{workgroups} + 1) * sizeof(UnitNote);
 }
 
-hipError_t launch_attend_join(uint32_t tile_rows, uint32_t units, const AttendArgs &a, hipStream_t stream) {
-  const bool wide = tile_rows == kAttendWideRows;
+hipError_t launch_attend_join(uint32_t tile_rows, bool few, const AttendArgs &a, hipStream_t stream) {
   const uint32_t dim = computed(a.kv.head_dim);
-  // Few units have many parts each, and want more waves on each; of many, launching the workgroups would take longer than
-  // their work (34 us for 4096 of them with 32 MiB of parts).
-  const uint32_t items = tile_rows / (wide ? 32 : 16) * (dim / (wide ? 8 : 16)) / 2;
-  const dim3 grid(a.workgroups, uint64_t{units} * 4 <= a.workgroups ? min((items + 3) / 4, 8u) : 1);
-  if (wide) hipLaunchKernelGGL((attend_join_kernel<true>), grid, dim3(256), 0, stream, a, dim, tile_rows);
-  else hipLaunchKernelGGL((attend_join_kernel<false>), grid, dim3(256), 0, stream, a, dim, tile_rows);
+  const bool wide = tile_rows == kAttendWideRows;
+  const auto launch = [&](auto kernel, uint32_t groups) {
+    hipLaunchKernelGGL(kernel, dim3(groups), dim3(256), 0, stream, a, dim, tile_rows);
+  };
+  if (few && wide) launch(join_few_kernel<true>, kFewGroups);
+  else if (few) launch(join_few_kernel<false>, kFewGroups);
+  else if (wide) launch(join_many_kernel<true>, a.workgroups);
+  else launch(join_many_kernel<false>, a.workgroups);
   return hipGetLastError();
 }
 

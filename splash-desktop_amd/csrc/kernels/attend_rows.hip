@@ -229,11 +229,11 @@ attend_rows_kernel(AttendArgs a) {
   const Cut cut{16 * MB / (int)a.group, (int)kAttendLeast, kUnitSlack + 256};
   const float by_group = 1.0f / (float)a.group;
   const uint32_t dim = a.kv.head_dim, row_bytes = dim * R::kBytes;
-  Work work = make_work<kThreads>(a, cut, shared.line);
-  UnitNote began{};
   Part next;
-  while (work.next(a, cut, next)) {
-    const Part part = Work::settled(a, cut, next);
+  Work<kThreads> work = make_work<kThreads>(a, cut, shared.line, next);
+  UnitNote began{};
+  while (work.next(a, cut, shared.line, next)) {
+    const Part part = settled(a, cut, next);
     const Units &u = part.units;
     const int row0 = cut.fit * part.m, rows = min(cut.fit, u.rows - row0), live = rows * (int)a.group;
     const int unit_end = u.causal ? min(u.keys, u.base + row0 + rows) : u.keys;   // keys that any row sees

@@ -98,7 +98,7 @@ struct Tile {
 };
 
 template <uint32_t FMT, int DIM>
-__global__ __launch_bounds__(kThreads, DIM == 256 ? 1 : 2) void attend_tile_kernel(AttendArgs a) {
+__global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void attend_tile_kernel(AttendArgs a) {
   using T = Tile<DIM>;
   constexpr bool kCodes = FMT != SQ_KV_BF16;
   constexpr int kSteps = DIM / 16, kBlocks = DIM / 32, kBytes = kCodes ? 1 : 2;
@@ -113,7 +113,8 @@ __global__ __launch_bounds__(kThreads, DIM == 256 ? 1 : 2) void attend_tile_kern
   const Cut cut{kRows / (int)a.group, 4 * kKeyTile, kUnitSlack + 192};
   const float by_group = 1.0f / (float)a.group;
   const uint32_t dim = a.kv.head_dim, row_bytes = dim * kBytes;
-  Work work = make_work<kThreads>(a, cut, shared);
+  Part next;
+  Work<kThreads> work = make_work<kThreads>(a, cut, shared, next);
   UnitNote began{};
 
   // Where this lane's vectors lie in 16 keys of a page, and (codes) in the LDS tile.
@@ -138,9 +139,8 @@ __global__ __launch_bounds__(kThreads, DIM == 256 ? 1 : 2) void attend_tile_kern
   const uint32_t vi = lane & 15, vk = 4 * h + vi / 4;
   const uint32_t value_at = vk * T::kRowBytes + 8 * (vi % 2) + 16 * ((2 * (lane / 16 % 2) + vi % 4 / 2) ^ T::value_swap(vk));
 
-  Part next;
-  while (work.next(a, cut, next)) {
-    const Part part = Work::settled(a, cut, next);
+  while (work.next(a, cut, shared, next)) {
+    const Part part = settled(a, cut, next);
     const Units &u = part.units;
     const int row0 = cut.fit * part.m, rows = min(cut.fit, u.rows - row0), live = rows * (int)a.group;
     const int unit_end = u.causal ? min(u.keys, u.base + row0 + rows) : u.keys;   // keys that any row sees
@@ -156,6 +156,26 @@ __global__ __launch_bounds__(kThreads, DIM == 256 ? 1 : 2) void attend_tile_kern
     const int low = u.window ? at - u.window + 1 : 0;
     const int high = u.causal ? min(at + 1, u.keys) : u.keys;
     const bool busy = 32 * (int)wave < live;   // waves past the unit's rows only fetch
+    // The page table's entries of the tile at k, lanes 0..3 those of its four 16 keys (~0u past the part's keys); and what
+    // they say: the page of this wave's 16 keys (~0u for none), and which of the four have none.
+    struct Pages {
+      uint32_t own, holes;
+    };
+    const auto entries_at = [&](int k) __attribute__((always_inline)) {
+      const int from = k + 16 * (int)min(lane, 3u);
+      return from < k_end ? a.kv.page_table[(size_t)part.sequence * a.kv.pages_per_sequence +
+                                            ((uint32_t)from >> a.kv.page_shift)]
+                          : ~0u;
+    };
+    const auto pages_of = [&](uint32_t entries) __attribute__((always_inline)) {
+      const uint32_t own = from_lane(entries, wave);
+      return Pages{own < a.kv.pages ? own : ~0u, (uint32_t)__ballot(entries >= a.kv.pages) & 15u};
+    };
+    const int tiles_n = max(part.t1 - part.t0, 0);
+    const auto at_tile = [&](int i) __attribute__((always_inline)) { return k_begin + kKeyTile * i; };
+    uint32_t entries[3];   // on their way before the queries, which nothing wants before the first keys
+#pragma unroll
+    for (int i = 0; i < 3; ++i) entries[i] = entries_at(at_tile(i));
     u32x4 q[kSteps];
     {
       const uint16_t *row = a.query + (size_t)(part.first_row + row0 + (on ? pi : 0)) * a.query_stride +
@@ -173,21 +193,6 @@ __global__ __launch_bounds__(kThreads, DIM == 256 ? 1 : 2) void attend_tile_kern
 #pragma unroll
       for (int i = 0; i < 16; ++i) o[b][i] = 0.0f;
 
-    // The page table's entries of the tile at k, lanes 0..3 those of its four 16 keys (~0u past the part's keys); and what
-    // they say: the page of this wave's 16 keys (~0u for none), and which of the four have none.
-    struct Pages {
-      uint32_t own, holes;
-    };
-    const auto entries_at = [&](int k) __attribute__((always_inline)) {
-      const int from = k + 16 * (int)min(lane, 3u);
-      return from < k_end ? a.kv.page_table[(size_t)part.sequence * a.kv.pages_per_sequence +
-                                            ((uint32_t)from >> a.kv.page_shift)]
-                          : ~0u;
-    };
-    const auto pages_of = [&](uint32_t entries) __attribute__((always_inline)) {
-      const uint32_t own = from_lane(entries, wave);
-      return Pages{own < a.kv.pages ? own : ~0u, (uint32_t)__ballot(entries >= a.kv.pages) & 15u};
-    };
     // Copies of the tile at k into stage `to`, K or V: bf16 straight into LDS, codes into registers until place() converts
     // them.
     u32x4 code_k[kCodes ? kLoads : 1], code_v[kCodes ? kLoads : 1];
@@ -409,13 +414,8 @@ __global__ __launch_bounds__(kThreads, DIM == 256 ? 1 : 2) void attend_tile_kern
     // K runs a tile ahead of V: while a tile is finished and the next one's scores are made, the copies of K two tiles on
     // and V one tile on are under way, into the stages that the last tile has left. Codes wait in registers one tile
     // more, and the page table's entries are fetched a tile before the copies that want them.
-    const int tiles_n = max(part.t1 - part.t0, 0);
-    const auto at_tile = [&](int i) __attribute__((always_inline)) { return k_begin + kKeyTile * i; };
     __syncthreads();   // the last part's tiles have been read
     Pages pages[4];    // of the tiles from the one at hand on
-    uint32_t entries[3];
-#pragma unroll
-    for (int i = 0; i < 3; ++i) entries[i] = entries_at(at_tile(i));
 #pragma unroll
     for (int i = 0; i < 3; ++i) pages[i] = pages_of(entries[i]);
     uint32_t later = entries_at(at_tile(3));

@@ -269,16 +269,20 @@ constexpr uint32_t attend_rows_resident(uint32_t tile_rows, uint32_t head_dim, u
   const uint32_t state = (head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256) * tile_rows / 16;
   return (state <= 128 ? 2 : state <= 256 ? 1 : 0) + (format != SQ_KV_BF16 && state <= 256 ? 1 : state > 256 ? 1 : 0);
 }
+// The same of the wide tile: by its registers, and (heads of more than 128 values) its LDS.
+constexpr uint32_t attend_tile_resident(uint32_t head_dim, uint32_t format) {
+  return head_dim > 128 ? 1 : head_dim <= 64 && format == SQ_KV_BF16 ? 3 : 2;
+}
 // The workgroups of a compute unit under a plan of tiles of tile_rows rows and workgroups of `waves` waves.
 inline uint32_t attend_resident(uint32_t tile_rows, uint32_t waves, uint32_t head_dim, uint32_t format) {
-  if (tile_rows == kAttendWideRows) return head_dim <= 128 ? 2 : 1;
+  if (tile_rows == kAttendWideRows) return attend_tile_resident(head_dim, format);
   return waves == 8 ? 1 : attend_rows_resident(tile_rows, head_dim, format);
 }
 hipError_t launch_attend_rows(uint32_t tile_rows, uint32_t waves, const AttendArgs &args, hipStream_t stream);
 // Tiles of kAttendWideRows rows.
 hipError_t launch_attend_tile(const AttendArgs &args, hipStream_t stream);
-// The join of the parts that either left, after it. units: the most there are (attend.hpp).
-hipError_t launch_attend_join(uint32_t tile_rows, uint32_t units, const AttendArgs &args, hipStream_t stream);
+// The join of the parts that either left, after it. few: the batch has no more units than a quarter of the workgroups.
+hipError_t launch_attend_join(uint32_t tile_rows, bool few, const AttendArgs &args, hipStream_t stream);
 // The length (attend.hpp) up to which a batch of few units is never cut (launch_attend_rows).
 constexpr uint32_t kAttendLeast = 1280;
 
