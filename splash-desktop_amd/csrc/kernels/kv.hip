@@ -1,7 +1,8 @@
 // Rotary positions and the paged key/value cache: rows rotated, rows written into their pages in 16 or 8 bits, and read
-// back. All three are bound by the bytes they move (a value in, a value out); a workgroup takes one row of the batch,
-// a head row (head_dim values) a group of 8, 16 or 32 lanes of 8 values, so that a head row's largest magnitude is a
-// few lane exchanges away and each lane's access is one 16-byte vector (8 bytes of codes).
+// back. All three are bound by the bytes they move (a value in, a value out). A head row (head_dim values) is a group of
+// 8, 16 or 32 lanes of 8 values, so that its largest magnitude is a few lane exchanges away and each lane's access is one
+// 16-byte vector (8 bytes of codes). Of few rows each has a workgroup, of many a wave, four heads' loads in flight: a
+// workgroup a row of a 30000-key prefix takes 63 us, most of it launches, a wave a row 43 us; up to 2048 rows the workgroups are as fast or faster (2048 rotated rows 15.5 and 17.9 us).
 //
 // The angles: p f / 2 pi turns in fp64, the whole turns dropped there (p f reaches 10^6 radians, where fp32 has a 16th
 // of a radian left), then sine and cosine of the fraction in fp32. A row's pairs are worked out once, by as many
@@ -18,15 +19,30 @@ struct CosSin {
   float c, s;
 };
 
-// cs[i] of every pair for a position, by the workgroup's first threads; a barrier follows.
-__device__ __forceinline__ void angles(CosSin *cs, const RopeArgs &rope, double position) {
-  for (uint32_t i = threadIdx.x; i < rope.pairs; i += blockDim.x) {
+// The threads of a row: its workgroup's, or its wave's. t: this one's number among them.
+template <int THREADS>
+__device__ __forceinline__ void row_barrier() {
+  if constexpr (THREADS == 256) {
+    __syncthreads();
+  } else {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+  }
+}
+// The most rows that have a workgroup each (above).
+constexpr uint32_t kFewRows = 2048;
+
+// cs[i] of every pair for a position, by the row's threads.
+template <int THREADS>
+__device__ __forceinline__ void angles(CosSin *cs, const RopeArgs &rope, double position, uint32_t t) {
+  for (uint32_t i = t; i < rope.pairs; i += THREADS) {
     const double turns = position * rope.frequencies[i] * 0.15915494309189533577;
     float s, c;
     sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
     cs[i] = {c * rope.magnitude, s * rope.magnitude};
   }
-  __syncthreads();
+  row_barrier<THREADS>();
 }
 
 __device__ __forceinline__ void widen8(u32x4 w, float (&x)[8]) {
@@ -91,7 +107,7 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs rope, const uint32_t
                                                    HeadRows input, HeadRows output) {
   __shared__ CosSin cs[kMaxPairs];
   const uint32_t row = blockIdx.x, d = 8 * (threadIdx.x % LPH);
-  angles(cs, rope, (double)positions[row]);
+  angles<256>(cs, rope, (double)positions[row], threadIdx.x);
   if (d >= head_dim) return;
   const uint16_t *in = input.rows + (size_t)row * input.stride;
   uint16_t *out = output.rows + (size_t)row * output.stride;
@@ -136,82 +152,118 @@ __device__ __forceinline__ Codes codes8(u32x4 w) {
   return out;
 }
 
-template <uint32_t FMT, int LPH>
+// Heads whose loads a thread has in flight.
+constexpr int kAtOnce = 4;
+
+template <uint32_t FMT, int LPH, int THREADS>
 __global__ __launch_bounds__(256) void kv_write_kernel(KvArgs kv, HeadRows keys, HeadRows values, RopeArgs rope,
                                                        HeadRows queries, HeadRows rotated) {
-  __shared__ CosSin cs[kMaxPairs];
-  const uint32_t row = blockIdx.x, d = 8 * (threadIdx.x % LPH), dim = kv.head_dim;
+  constexpr uint32_t kHeads = THREADS / LPH;   // head rows of the row's threads at a time
+  __shared__ CosSin all[256 / THREADS][kMaxPairs];
+  CosSin *cs = all[threadIdx.x / THREADS];
+  const uint32_t t = threadIdx.x % THREADS, d = 8 * (t % LPH), dim = kv.head_dim;
+  const uint32_t row = blockIdx.x * (256 / THREADS) + threadIdx.x / THREADS;
+  if (row >= kv.rows) return;
   const RowPlace place = place_of(kv, row);
   if (place.sequence == ~0u) return;
-  if (rope.pairs) angles(cs, rope, (double)place.position);
   const uint32_t page = place.position >= 0 ? page_of(kv, place.sequence, place.position) : ~0u;
   const uint32_t slot = (uint32_t)place.position & ((1u << kv.page_shift) - 1);
   const bool live = d < dim;
-  const uint32_t heads = 2 * kv.kv_heads + (queries.rows ? queries.heads : 0);
-  for (uint32_t u = threadIdx.x / LPH; u < heads; u += 256 / LPH) {
-    if (u >= 2 * kv.kv_heads) {
-      const uint32_t h = u - 2 * kv.kv_heads;
-      if (live)
-        *(u32x4 *)(rotated.rows + (size_t)row * rotated.stride + h * dim + d) =
-            rotated8(queries.rows + (size_t)row * queries.stride + h * dim, d, cs, rope);
-      continue;
+  if (rope.pairs) angles<THREADS>(cs, rope, (double)place.position, t);
+  for (uint32_t first = t / LPH; first < 2 * kv.kv_heads; first += kAtOnce * kHeads) {
+    u32x4 w[kAtOnce];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const uint32_t u = first + i * kHeads;
+      const bool key = u < kv.kv_heads;
+      const uint32_t h = key ? u : u - kv.kv_heads;
+      const HeadRows &from = key ? keys : values;
+      w[i] = u32x4{0u, 0u, 0u, 0u};
+      if (!live || u >= 2 * kv.kv_heads) continue;
+      const uint16_t *head = from.rows + (size_t)row * from.stride + h * dim;
+      w[i] = key && rope.pairs ? rotated8(head, d, cs, rope) : *(const u32x4 *)(head + d);
     }
-    const bool key = u < kv.kv_heads;
-    const uint32_t h = key ? u : u - kv.kv_heads;
-    const HeadRows &from = key ? keys : values;
-    const uint16_t *head = from.rows + (size_t)row * from.stride + h * dim;
-    u32x4 w{0u, 0u, 0u, 0u};
-    if (live) w = key && rope.pairs ? rotated8(head, d, cs, rope) : *(const u32x4 *)(head + d);
-    const size_t at = ((((size_t)page * kv.kv_heads + h) << kv.page_shift) + slot);
-    if constexpr (FMT == SQ_KV_BF16) {
-      if (page != ~0u && live) *(u32x4 *)((key ? kv.keys : kv.values) + (at * dim + d) * 2) = w;
-    } else {
-      const Codes c = codes8<FMT, LPH>(w);
-      if (page == ~0u) continue;
-      if (live) *(u32x2 *)((key ? kv.keys : kv.values) + at * dim + d) = c.words;
-      if (d == 0) (key ? kv.key_scales : kv.value_scales)[at] = c.scale;
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const uint32_t u = first + i * kHeads;
+      if (u >= 2 * kv.kv_heads) continue;
+      const bool key = u < kv.kv_heads;
+      const uint32_t h = key ? u : u - kv.kv_heads;
+      const size_t at = ((((size_t)page * kv.kv_heads + h) << kv.page_shift) + slot);
+      if constexpr (FMT == SQ_KV_BF16) {
+        if (page != ~0u && live) *(u32x4 *)((key ? kv.keys : kv.values) + (at * dim + d) * 2) = w[i];
+      } else {
+        const Codes c = codes8<FMT, LPH>(w[i]);
+        if (page == ~0u) continue;
+        if (live) *(u32x2 *)((key ? kv.keys : kv.values) + at * dim + d) = c.words;
+        if (d == 0) (key ? kv.key_scales : kv.value_scales)[at] = c.scale;
+      }
     }
   }
+  if (!queries.rows || !live) return;
+  for (uint32_t h = t / LPH; h < queries.heads; h += kHeads)
+    *(u32x4 *)(rotated.rows + (size_t)row * rotated.stride + h * dim + d) =
+        rotated8(queries.rows + (size_t)row * queries.stride + h * dim, d, cs, rope);
 }
 
-template <uint32_t FMT, int LPH>
+template <uint32_t FMT, int LPH, int THREADS>
 __global__ __launch_bounds__(256) void kv_read_kernel(KvArgs kv, HeadRows keys, HeadRows values) {
-  const uint32_t row = blockIdx.x, d = 8 * (threadIdx.x % LPH), dim = kv.head_dim;
+  constexpr uint32_t kHeads = THREADS / LPH;
+  const uint32_t t = threadIdx.x % THREADS, d = 8 * (t % LPH), dim = kv.head_dim;
+  const uint32_t row = blockIdx.x * (256 / THREADS) + threadIdx.x / THREADS;
+  if (row >= kv.rows) return;
   const RowPlace place = place_of(kv, row);
   if (place.sequence == ~0u || d >= dim) return;
   const uint32_t page = place.position >= 0 ? page_of(kv, place.sequence, place.position) : ~0u;
   const uint32_t slot = (uint32_t)place.position & ((1u << kv.page_shift) - 1);
-  for (uint32_t u = threadIdx.x / LPH; u < 2 * kv.kv_heads; u += 256 / LPH) {
-    const bool key = u < kv.kv_heads;
-    const uint32_t h = key ? u : u - kv.kv_heads;
-    const HeadRows &to = key ? keys : values;
-    if (!to.rows) continue;
-    u32x4 w{0u, 0u, 0u, 0u};
-    if (page != ~0u) {
+  for (uint32_t first = t / LPH; first < 2 * kv.kv_heads; first += kAtOnce * kHeads) {
+    u32x4 w[kAtOnce];
+    float scale[kAtOnce];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const uint32_t u = first + i * kHeads;
+      const bool key = u < kv.kv_heads;
+      const uint32_t h = key ? u : u - kv.kv_heads;
+      w[i] = u32x4{0u, 0u, 0u, 0u};
+      scale[i] = 0.0f;
+      if (u >= 2 * kv.kv_heads || page == ~0u || !(key ? keys : values).rows) continue;
       const size_t at = ((((size_t)page * kv.kv_heads + h) << kv.page_shift) + slot);
       const uint8_t *from = key ? kv.keys : kv.values;
       if constexpr (FMT == SQ_KV_BF16) {
-        w = *(const u32x4 *)(from + (at * dim + d) * 2);
+        w[i] = *(const u32x4 *)(from + (at * dim + d) * 2);
       } else {
-        const float scale = (key ? kv.key_scales : kv.value_scales)[at];
         const u32x2 c = *(const u32x2 *)(from + at * dim + d);
-        float x[8];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if constexpr (FMT == SQ_KV_INT8) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[4 * i + e] = (float)(int8_t)(c[i] >> (8 * e)) * scale;
-          } else {
-            x[4 * i] = __builtin_amdgcn_cvt_f32_fp8((int)c[i], 0) * scale;
-            x[4 * i + 1] = __builtin_amdgcn_cvt_f32_fp8((int)c[i], 1) * scale;
-            x[4 * i + 2] = __builtin_amdgcn_cvt_f32_fp8((int)c[i], 2) * scale;
-            x[4 * i + 3] = __builtin_amdgcn_cvt_f32_fp8((int)c[i], 3) * scale;
-          }
-        }
-        w = narrow8(x);
+        w[i][0] = c[0];
+        w[i][1] = c[1];
+        scale[i] = (key ? kv.key_scales : kv.value_scales)[at];
       }
     }
-    *(u32x4 *)(to.rows + (size_t)row * to.stride + h * dim + d) = w;
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const uint32_t u = first + i * kHeads;
+      const bool key = u < kv.kv_heads;
+      const uint32_t h = key ? u : u - kv.kv_heads;
+      const HeadRows &to = key ? keys : values;
+      if (u >= 2 * kv.kv_heads || !to.rows) continue;
+      if constexpr (FMT != SQ_KV_BF16) {
+        float x[8];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const uint32_t c = w[i][j];
+          if constexpr (FMT == SQ_KV_INT8) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[4 * j + e] = (float)(int8_t)(c >> (8 * e)) * scale[i];
+          } else {
+            x[4 * j] = __builtin_amdgcn_cvt_f32_fp8((int)c, 0) * scale[i];
+            x[4 * j + 1] = __builtin_amdgcn_cvt_f32_fp8((int)c, 1) * scale[i];
+            x[4 * j + 2] = __builtin_amdgcn_cvt_f32_fp8((int)c, 2) * scale[i];
+            x[4 * j + 3] = __builtin_amdgcn_cvt_f32_fp8((int)c, 3) * scale[i];
+          }
+        }
+        w[i] = narrow8(x);
+      }
+      *(u32x4 *)(to.rows + (size_t)row * to.stride + h * dim + d) = w[i];
+    }
   }
 }
 
@@ -243,8 +295,12 @@ hipError_t launch_kv_write(const KvArgs &kv, const HeadRows &keys, const HeadRow
                            const HeadRows &queries, const HeadRows &rotated, hipStream_t stream) {
   with_kv_format(kv.format, [&](auto format) {
     with_lanes(kv.head_dim, [&](auto lanes) {
-      hipLaunchKernelGGL((kv_write_kernel<format.value, lanes.value>), dim3(kv.rows), dim3(256), 0, stream, kv, keys,
-                         values, rope, queries, rotated);
+      if (kv.rows <= kFewRows)
+        hipLaunchKernelGGL((kv_write_kernel<format.value, lanes.value, 256>), dim3(kv.rows), dim3(256), 0, stream, kv,
+                           keys, values, rope, queries, rotated);
+      else
+        hipLaunchKernelGGL((kv_write_kernel<format.value, lanes.value, 64>), dim3((kv.rows + 3) / 4), dim3(256), 0,
+                           stream, kv, keys, values, rope, queries, rotated);
     });
   });
   return hipGetLastError();
@@ -253,8 +309,12 @@ hipError_t launch_kv_write(const KvArgs &kv, const HeadRows &keys, const HeadRow
 hipError_t launch_kv_read(const KvArgs &kv, const HeadRows &keys, const HeadRows &values, hipStream_t stream) {
   with_kv_format(kv.format, [&](auto format) {
     with_lanes(kv.head_dim, [&](auto lanes) {
-      hipLaunchKernelGGL((kv_read_kernel<format.value, lanes.value>), dim3(kv.rows), dim3(256), 0, stream, kv, keys,
-                         values);
+      if (kv.rows <= kFewRows)
+        hipLaunchKernelGGL((kv_read_kernel<format.value, lanes.value, 256>), dim3(kv.rows), dim3(256), 0, stream, kv,
+                           keys, values);
+      else
+        hipLaunchKernelGGL((kv_read_kernel<format.value, lanes.value, 64>), dim3((kv.rows + 3) / 4), dim3(256), 0,
+                           stream, kv, keys, values);
     });
   });
   return hipGetLastError();

@@ -423,13 +423,15 @@ def stream_read(src, sink, workgroups: int, threads: int, nbytes: int | None = N
 
 def head_rows(tensor, head_dim: int) -> HeadRows:
     """A bf16 tensor's rows of heads: [rows, heads * head_dim] (a column slice of a fused projection's output too)."""
-    width = tensor.shape[-1]
-    if tensor.dim() != 2 or width % head_dim or (tensor.numel() and tensor.stride(1) != 1) or \
-            tensor.element_size() != 2:
+    if tensor.dim() != 2:
+        raise ValueError("head rows are a [rows, heads * head_dim] tensor")
+    (rows, width), (stride, step) = tensor.shape, tensor.stride()
+    if width % head_dim or step != 1 or tensor.element_size() != 2:
         raise ValueError("head rows are a 2-byte [rows, heads * head_dim] tensor with adjacent columns")
-    rows, stride = tensor.shape[0], tensor.stride(0) if tensor.shape[0] > 1 else max(width, tensor.stride(0))
-    nbytes = 2 * ((rows - 1) * stride + width) if rows else 0
-    return HeadRows(Buffer(tensor.data_ptr(), nbytes), width // head_dim, stride)
+    if rows <= 1:
+        stride = width
+    return HeadRows(Buffer(tensor.data_ptr(), 2 * ((rows - 1) * stride + width) if rows else 0), width // head_dim,
+                    stride)
 
 
 def rope_frequencies(config: RopeConfig) -> tuple[list[float], float]:
