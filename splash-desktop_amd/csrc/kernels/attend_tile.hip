@@ -253,13 +253,14 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
     const auto settle = [&](int tile, int k, uint32_t holes, bool clear) __attribute__((always_inline)) {
       if constexpr (kCodes) {
 #pragma unroll
-        for (int b = 0; b < 2; ++b)
+        for (int b = 0; b < 2; ++b) {
+          f32x4 by[4];   // together, so that one wait serves the four
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const f32x4 by = scales[tile % 4][0][8 * b + 2 * j + h];
+          for (int j = 0; j < 4; ++j) by[j] = scales[tile % 4][0][8 * b + 2 * j + h];
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) s[b][4 * j + i] *= by[i];
-          }
+          for (int i = 0; i < 16; ++i) s[b][i] *= by[i / 4][i % 4];
+        }
       }
       if (!clear) {
 #pragma unroll
@@ -379,7 +380,8 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
       u32x4 operand[kSlots];
       const float from = -finite_max(m);
       float sum[2] = {0.0f, 0.0f};
-      f32x4 by{1.0f, 1.0f, 1.0f, 1.0f};
+      f32x4 by{}, by_next{};   // four weights' scales of values, read four weights before
+      if constexpr (kCodes) by_next = scales[tile % 4][1][h];
       float even = 0.0f;
       const auto read = [&](auto index) __attribute__((always_inline)) {
         constexpr Slot at = slot(decltype(index)::value);
@@ -388,7 +390,11 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
       // The weight of score i of block b.
       const auto weigh = [&](int b, int i) __attribute__((always_inline)) {
         if constexpr (kCodes)
-          if (i % 4 == 0) by = scales[tile % 4][1][8 * b + 2 * (i / 4) + h];
+          if (i % 4 == 0) {
+            by = by_next;
+            const int group = 4 * b + i / 4 + 1;
+            if (group < 8) by_next = scales[tile % 4][1][2 * group + h];
+          }
         float v = exp2_fast(fmaf(s[b][i], a.scale, from));
         sum[i % 2] += v;
         if constexpr (kCodes) v *= by[i % 4];
