@@ -530,8 +530,8 @@ typedef struct sq_attention_shape {
 } sq_attention_shape;
 /* A plan for batches of at most `sequences` sequences and `rows` rows; chunk_rows, the most new rows that one sequence
  * usually has, picks the tile (any batch is computed right whatever it is). tile_rows: the rows times query heads of one
- * key head that a tile holds (16, 32, 64 or 128); waves: of a workgroup. partials: the bytes of workspace, which may hold anything before a call;
- * one workspace serves one stream at a time. */
+ * key head that a tile holds (16, 32 or 128); waves: of a workgroup. partials: the bytes of workspace, which may hold
+ * anything before a call; one workspace serves one stream at a time. */
 typedef struct sq_attention_plan {
   sq_attention_shape shape;
   uint32_t sequences, rows, chunk_rows, tile_rows, waves, workgroups;

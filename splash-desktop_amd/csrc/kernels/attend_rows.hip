@@ -1,4 +1,4 @@
-// Attention of few rows a key head (tiles of 16, 32 or 64 rows times query heads): single tokens and verify lanes,
+// Attention of few rows a key head (tiles of 16 or 32 rows times query heads): single tokens and verify lanes,
 // bound by reading the cache once.
 //
 // No shared memory lies between the cache and the matrix units. A wave takes 32 keys a step, 16 of them (A) and the next
@@ -495,9 +495,9 @@ hipError_t launch_one(uint32_t waves, const AttendArgs &a, hipStream_t stream) {
 template <uint32_t FMT, int DIM>
 hipError_t launch_blocks(uint32_t tile_rows, uint32_t waves, const AttendArgs &a, hipStream_t stream) {
   if (tile_rows == 16) return launch_one<FMT, DIM, 1>(waves, a, stream);
-  if (tile_rows == 32) return launch_one<FMT, DIM, 2>(waves, a, stream);
-  if constexpr (DIM <= 128) return launch_one<FMT, DIM, 4>(waves, a, stream);
-  else return hipErrorInvalidValue;
+  if constexpr (attend_few_rows(DIM) >= 32)
+    if (tile_rows == 32) return launch_one<FMT, DIM, 2>(waves, a, stream);
+  return hipErrorInvalidValue;
 }
 template <uint32_t FMT>
 hipError_t launch_dim(uint32_t tile_rows, uint32_t waves, const AttendArgs &a, hipStream_t stream) {

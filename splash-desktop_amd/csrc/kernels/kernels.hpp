@@ -260,14 +260,20 @@ constexpr uint32_t kAttendMaxGroup = 64;
 // workgroup and as many once more, are the last of it.
 constexpr uint32_t kAttendNoteBytes = 16;
 uint64_t attend_partials(uint32_t tile_rows, uint32_t head_dim, uint32_t workgroups);
-// Tiles of few rows: 16, 32, or (heads of at most 128 values) 64; and the wide tile.
+// Tiles of few rows, 16 or 32, and the wide tile. The few rows' work grows with each 16 of them (their queries and
+// accumulators crowd the loads out of the registers), the wide tile costs what 128 rows cost, and the largest tile of
+// few rows that beats it is, by what both took (four sequences of 20000 keys, us with the join, few / wide):
+//   heads of 128, bf16:  32 rows 60 / 72, 64 rows 100 / 72; int8: 32 rows 47 / 73, 64 rows 84 / 73
+//   heads of 64, bf16:   32 rows 38 / 45, 64 rows 61 / 45;  int8: 32 rows 37 / 52, 64 rows 51 / 52
+//   heads of 256, int8:  16 rows 39 / 45, 32 rows 50 / 45;  bf16: 16 rows 65 / 45, but 77 / 90 for a token each of 256
+//   sequences of 300 to 600 keys, and 18 / 26 for 8 sequences of 200 to 400: the commoner calls
 constexpr uint32_t kAttendWideRows = 128;
-inline uint32_t attend_few_rows(uint32_t head_dim) { return head_dim <= 128 ? 64 : 32; }
+constexpr uint32_t attend_few_rows(uint32_t head_dim) { return head_dim <= 128 ? 32 : 16; }
 // The workgroups (of four waves) that a compute unit holds of a tile of few rows at once: by the registers of a wave's
 // keys, values and accumulators.
 constexpr uint32_t attend_rows_resident(uint32_t tile_rows, uint32_t head_dim, uint32_t format) {
   const uint32_t state = (head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256) * tile_rows / 16;
-  return (state <= 128 ? 2 : state <= 256 ? 1 : 0) + (format != SQ_KV_BF16 && state <= 256 ? 1 : state > 256 ? 1 : 0);
+  return (state <= 128 ? 2 : 1) + (format != SQ_KV_BF16 ? 1 : 0);
 }
 // The same of the wide tile: by its registers, and (heads of more than 128 values) its LDS.
 constexpr uint32_t attend_tile_resident(uint32_t head_dim, uint32_t format) {

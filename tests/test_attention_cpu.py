@@ -208,13 +208,15 @@ def attention_plan(shape=None, sequences=3, rows=5, chunk=1, dev=None):
 
 
 def test_attention_plans():
-    for heads, kv_heads, chunk in ((32, 8, 1), (32, 8, 4), (40, 8, 8), (64, 1, 1), (8, 8, 100)):
-        shape = attention_shape(heads=heads, kv_heads=kv_heads, head_dim=128)
-        plan = sq.attention_plan(shape, 4, 400, chunk)
-        group = heads // kv_heads
-        assert plan.tile_rows >= group
-        assert plan.tile_rows == 16 or plan.tile_rows // 2 < chunk * group
-        assert plan.workgroups % 8 == 0 and plan.partials > 16 * plan.workgroups
+    few = {(128, sq.KV_BF16): 32, (128, sq.KV_INT8): 32, (64, sq.KV_E4M3): 32, (256, sq.KV_BF16): 16, (256, sq.KV_INT8): 16}
+    for heads, kv_heads, chunk in ((32, 8, 1), (32, 8, 4), (40, 8, 8), (34, 2, 1), (64, 1, 1), (33, 1, 1), (8, 8, 100)):
+        for (dim, format), most in few.items():
+            shape = attention_shape(heads=heads, kv_heads=kv_heads, head_dim=dim, format=format)
+            plan = sq.attention_plan(shape, 4, 400, chunk)
+            packed = heads // kv_heads * chunk
+            # The smallest tile that holds a sequence's new rows with their query heads.
+            assert plan.tile_rows == next((t for t in (16, 32) if packed <= t <= most), 128)
+            assert plan.workgroups % 8 == 0 and plan.partials > 16 * plan.workgroups
     small = attention_plan(dev=sq.Device(10))
     assert small.workgroups % 8 == 0 and 10 <= small.workgroups < 32
 
