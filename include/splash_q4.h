@@ -474,7 +474,7 @@ int sq_rope_add(void *graph, const sq_rope *rope, sq_buffer positions, uint32_t 
  * and one fp32 scale a token and head ([pages][kv_heads][page_rows], keys and values apart); a code stands for code *
  * scale. INT8: scale = m / 127, code = x 127 / m rounded to the nearest even, m the head row's largest magnitude. E4M3:
  * scale = m / 448, code = x 448 / m rounded to the nearest value of that type. A head row of zeros has scale 0; one with
- * an infinity or NaN has a NaN scale and zero codes, so all of it reads back as NaN. BF16 pages hold the rows as they
+ * an infinity or NaN has a NaN scale and zero codes, so all of it reads back as NaN; no code is E4M3's NaN. BF16 pages hold the rows as they
  * are, and have no scales. */
 #define SQ_KV_BF16 0u
 #define SQ_KV_INT8 1u
@@ -546,7 +546,8 @@ int sq_attention_plan_for(const sq_device *device, const sq_attention_shape *sha
 /* The work (tiles of 64 keys over every sequence, key head and tile of rows) is split evenly over the workgroups
  * whatever the lengths are; a second launch joins the tiles of rows whose keys several workgroups shared, in key order,
  * so a batch repeats its bits from run to run. How the work falls depends on the whole batch, so a row's output
- * bits may differ between batches. */
+ * bits may differ between batches. A call's sequences, rows, keys (pages_per_sequence * page_rows) and key heads multiply
+ * to less than 2^52. */
 int sq_attention_add(void *graph, const sq_attention_buffers *buffers, const sq_kv_cache *cache,
                      const sq_kv_batch *batch, const sq_attention_plan *plan);
 

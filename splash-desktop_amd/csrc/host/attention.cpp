@@ -10,7 +10,7 @@ namespace {
 
 // The most rows of a batch and the most keys a sequence's pages hold: sums of lengths over every unit of a batch stay
 // far inside 64 bits, and a position inside 32.
-constexpr uint32_t kMaxRows = 1u << 20, kMaxKeys = 1u << 30, kMaxHeads = 1024;
+constexpr uint32_t kMaxRows = 1u << 20, kMaxKeys = 1u << 30, kMaxHeads = 1024, kMaxUnits = 65536;
 
 void launched(hipError_t e, const char *what) {
   if (e != hipSuccess) throw std::runtime_error(std::string(what) + ": " + hipGetErrorString(e));
@@ -255,6 +255,7 @@ AttentionPlan Attention::plan(const DeviceCapabilities &device, const AttentionS
     throw std::invalid_argument("a batch has 1 to 1024 sequences");
   if (!rows || rows > kMaxRows) throw std::invalid_argument("an attention plan takes 1 to 2^20 rows");
   if (!chunkRows || chunkRows > rows) throw std::invalid_argument("a sequence's new rows are 1 to the plan's rows");
+  if (device.computeUnits > kMaxUnits) throw std::invalid_argument("an attention plan takes at most 65536 compute units");
   AttentionPlan out{shape, sequences, rows, chunkRows};
   // The smallest tile of few rows that holds a sequence's new rows with their query heads, so that their keys are read
   // once; past the largest of those, the wide tile.
@@ -280,6 +281,10 @@ void Attention::add(hipStream_t graph, const HeadRowsView &query, const HeadRows
   if (!(cache.shape == shape.kv)) throw std::invalid_argument("the attention plan is another cache's");
   if (batch.sequences > plan.sequences || batch.rows > plan.rows)
     throw std::invalid_argument("the batch is larger than its attention plan");
+  // The lengths of every sequence's units end to end (attend.hpp), row starts that overlap included, are counted in 52 bits.
+  const uint64_t keys = uint64_t{batch.pagesPerSequence} * cache.shape.pageRows;
+  if (double(batch.sequences) * (batch.rows + 1.0) * (double(keys) + 4096) * shape.kv.kvHeads > 0x1p52)
+    throw std::invalid_argument("an attention batch's sequences, rows, keys and key heads multiply to less than 2^52");
   if (!batch.rows) return;
   if (query.heads != shape.heads || output.heads != shape.heads)
     throw std::invalid_argument("query and output rows have the attention's heads");
@@ -305,7 +310,7 @@ void Attention::add(hipStream_t graph, const HeadRowsView &query, const HeadRows
   // A batch of few units, none longer than a workgroup takes at least, is cut nowhere (attend.hpp), and leaves no parts.
   const uint64_t units = (batch.rows / (plan.tileRows / shape.group()) + batch.sequences) * uint64_t{shape.kv.kvHeads};
   const bool whole = plan.tileRows != kern::kAttendWideRows && batch.sequences <= 64 && units * 4 <= plan.workgroups &&
-                     uint64_t{batch.pagesPerSequence} * cache.shape.pageRows + 384 <= kern::kAttendLeast;
+                     keys + 384 <= kern::kAttendLeast;
   const OnStreamDevice on(graph);
   launched(plan.tileRows == kern::kAttendWideRows ? kern::launch_attend_tile(args, graph)
                                                   : kern::launch_attend_rows(plan.tileRows, plan.waves, args, graph),

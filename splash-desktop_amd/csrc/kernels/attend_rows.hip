@@ -47,6 +47,12 @@ __device__ __forceinline__ u32x2 code_pairs4(uint32_t w) {
   }
 }
 
+// Four e4m3 codes, NaNs (all seven bits below the sign's set) as zeros.
+__device__ __forceinline__ uint32_t finite_codes(uint32_t w) {
+  const uint32_t nan = ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+  return w & ~(nan | (nan - (nan >> 7)));
+}
+
 // The maximum over the four lanes that hold one row's keys.
 __device__ __forceinline__ float row_max(float v) {
   auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -364,6 +370,16 @@ attend_rows_kernel(AttendArgs a) {
             w[i] = clear || (seen[b] >> i & 1) ? w[i] * value_scale[i / 4][i % 4] : 0.0f;
         }
         p[b] = u32x4{bf16_pair(w[0], w[1]), bf16_pair(w[2], w[3]), bf16_pair(w[4], w[5]), bf16_pair(w[6], w[7])};
+      }
+      if constexpr (FMT == SQ_KV_E4M3) {
+        // Keys before a window may never have been written: no NaN of their codes meets the zero weights.
+        if (k < clear_begin)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+              for (int i = 0; i < R::kValueWords; ++i) vt.w[h][e][i] = finite_codes(vt.w[h][e][i]);
       }
       if constexpr (!kCodes) {
         // Where some rows see a key and others do not, its values must not reach the others through 0 * inf: infinities

@@ -288,28 +288,29 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
       }
     };
 
-    // Infinities and NaNs among a tile's values (bf16) must not reach rows that do not see them through 0 * inf: the rows
-    // that do see them add their products one by one, and they leave the tile. Only tiles that are not clear can have
-    // such rows.
+    // Infinities and NaNs among a tile's values must not reach rows that do not see them through 0 * inf: the rows that do
+    // see them add their products one by one, and they leave the tile. Only tiles that are not clear can have such rows.
     const auto set_apart = [&](int tile, int k, uint32_t holes) __attribute__((always_inline)) {
       if constexpr (kCodes) {
-        // Codes are finite; the scale of a head row that was not is a NaN, and all of it is.
+        // The scale of a head row that was not finite is a NaN, and all of it is.
         float *by = (float *)scales[tile % 4][1];
         const bool bad = !(fabsf(by[lane]) < INFINITY);
         uint64_t rows_bad = __ballot(bad);
-        if (!rows_bad) return;
-        while (busy && rows_bad) {
-          const int key = __ffsll((unsigned long long)rows_bad) - 1, j = k + key;
-          rows_bad &= rows_bad - 1;
-          if (on && j >= low && j < high && !(holes >> (key / 16) & 1)) {
+        if (rows_bad) {
+          while (busy && rows_bad) {
+            const int key = __ffsll((unsigned long long)rows_bad) - 1, j = k + key;
+            rows_bad &= rows_bad - 1;
+            if (on && j >= low && j < high && !(holes >> (key / 16) & 1)) {
 #pragma unroll
-            for (int b = 0; b < kBlocks; ++b) o[b] += __uint_as_float(0x7FC00000u);
+              for (int b = 0; b < kBlocks; ++b) o[b] += __uint_as_float(0x7FC00000u);
+            }
           }
+          __syncthreads();
+          if (bad && wave == 0) by[lane] = 0.0f;
+          __syncthreads();
         }
-        __syncthreads();
-        if (bad && wave == 0) by[lane] = 0.0f;
-        __syncthreads();
-        return;
+        // Codes written are finite, but keys before a window may never have been.
+        if (FMT == SQ_KV_INT8 || k >= clear_begin) return;
       }
       constexpr int kMine = T::kBytes / 16 / kThreads;
       uint8_t *vt = tiles[tile % 2][1];
@@ -322,7 +323,7 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
           any |= (uint32_t)((v[e] & 0x7F80u) == 0x7F80u) | (uint32_t)((v[e] & 0x7F800000u) == 0x7F800000u);
       }
       if (!__syncthreads_or((int)any)) return;
-      if (busy) {
+      if (!kCodes && busy) {
 #pragma unroll 1
         for (uint32_t key = 0; key < kKeyTile; ++key) {
           // Key `key` is score 4 (key % 32 / 8) + key % 4 of block key / 32 in the lanes with h = key / 4 % 2.

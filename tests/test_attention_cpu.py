@@ -219,6 +219,15 @@ def test_attention_plans():
             assert plan.workgroups % 8 == 0 and plan.partials > 16 * plan.workgroups
     small = attention_plan(dev=sq.Device(10))
     assert small.workgroups % 8 == 0 and 10 <= small.workgroups < 32
+    with pytest.raises(sq.InvalidArgument, match="65536 compute units"):
+        attention_plan(dev=sq.Device(65537))
+    # The work of a call is counted in 52 bits, row starts that overlap included.
+    kv, huge, by = kv_shape(kv_heads=1024, head_dim=16, page_rows=1024, format=sq.KV_BF16), buffer(1 << 62), ctypes.byref
+    plan = sq.attention_plan(sq.AttentionShape(1024, kv, 1, 0, 0.25), 1024, 1 << 14, 1)
+    rows = sq.HeadRows(huge, 1024, 1024 * 16)
+    refused("sq_attention_add", "less than 2", by(sq.AttentionBuffers(rows, rows, huge)),
+            by(sq.KvCache(kv, 1 << 20, huge, huge, sq.Buffer(0, 0), sq.Buffer(0, 0))),
+            by(sq.KvBatch(1024, 1 << 14, 1 << 9, huge, huge, huge)), by(plan))
 
 
 @pytest.mark.parametrize("shape,sizes,message", [

@@ -254,6 +254,27 @@ def test_unseen_keys_touch_nothing(fmt, sizes, chunk):
 
 
 @pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("kv_heads,dim", [(2, 64), (1, 128), (1, 256)])
+def test_windows_over_unwritten_keys(fmt, kv_heads, dim):
+    """Keys before every row's window that were never written: NaNs (also among the codes) and NaN scales."""
+    t = torch()
+    rng = np.random.default_rng(dim)
+    window, sizes = 75, [(1, 700), (45, 900), (3, 80), (150, 333)]
+    c = Cache(rng, sizes, kv_heads, dim, 32, fmt).fill()
+    q = queries(rng, c.rows, 4, dim)
+    want, bound = attention_f64(q, c, 0.1, True, window)
+    for s, (n, keys) in enumerate(sizes):
+        for position in range(max(0, keys - n - window + 1)):
+            page, slot = c.slot(s, position)
+            for x in (c.keys, c.values):
+                x.view(t.uint8)[int(page), :, slot] = 0xFF
+            for x in (c.key_scales, c.value_scales):
+                x[int(page), :, slot] = math.nan
+    for chunk in (1, c.rows):
+        check_attention(run_attention(c, q, 0.1, True, window, chunk=chunk), want, bound, f"{fmt} chunk {chunk}")
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
 @pytest.mark.parametrize("rows", [1, 70])
 def test_holes(fmt, rows):
     """Page table entries that name no page: their keys are not seen, write nothing and read back as zeros."""
@@ -393,6 +414,33 @@ def test_graph_replays_with_other_lengths():
         t.cuda.synchronize()
         for got, want in zip((turned, out, back), e):   # bits: keys that no step has written are NaN
             assert t.equal(got.view(t.int16), want.view(t.int16))
+
+
+def test_graphs_that_share_a_workspace():
+    """Two captured calls, of single tokens and of a chunk, over one workspace and in one stream, replayed in any order."""
+    t = torch()
+    rng = np.random.default_rng(15)
+    parts = []
+    for seed, sizes in ((1, [(1, 9000), (1, 77)]), (2, [(90, 4000), (1, 12)])):
+        c = Cache(np.random.default_rng(seed), sizes, 2, 128, 64, "bf16").fill()
+        q = queries(rng, c.rows, 8, 128)
+        plan = sq.attention_plan(sq.AttentionShape(8, c.shape, 1, 0, 0.09), 2, c.rows, sizes[0][0])
+        parts.append((c, plan, to_bf16(q.reshape(c.rows, -1)), run_attention(c, q, 0.09, plan=plan)))
+    scratch = sq.AttentionScratch(max((plan for _, plan, *_ in parts), key=lambda plan: plan.partials))
+    outs, graphs = [t.zeros_like(x) for _, _, x, _ in parts], []
+    for (c, plan, x, _), out in zip(parts, outs):
+        graphs.append(t.cuda.CUDAGraph())
+        with t.cuda.graph(graphs[-1]):
+            sq.attention_add(plan, c.struct(), c.batch(), x, out, scratch)
+    for order in ((0, 1), (1, 0), (1, 1, 0), (0, 0, 1)):
+        for out in outs:
+            out.zero_()
+        scratch.partials.fill_(-1)
+        for i in order:
+            graphs[i].replay()
+        t.cuda.synchronize()
+        for (*_, want), out in zip(parts, outs):
+            assert np.array_equal(from_bf16(out).reshape(want.shape), want)
 
 
 def test_two_streams_at_once():
