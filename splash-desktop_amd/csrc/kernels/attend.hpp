@@ -104,10 +104,11 @@ __device__ __forceinline__ Part settled(const AttendArgs &a, const Cut &cut, con
 
 // A part's place in the workspace. A piece holds at most two parts of shared units: one that an earlier piece began, and
 // one that it begins itself, of which there can be one only. (An even part may be empty, where a unit has fewer tiles
-// than parts: it is stored all the same.) A part is its blocks of 16 rows (32 in the wide tile) one after the other: the
-// accumulators as vectors of four, [vector][lane], then each row's maximum and sum.
-__device__ __forceinline__ uint32_t part_slot(uint32_t first_piece, uint32_t part) {
-  return 2 * (first_piece + part) + (part == 0 ? 1 : 0);
+// than parts: it is stored all the same.) A part's blocks of 16 rows (32 in the wide tile) are each the accumulators as
+// vectors of four, [vector][lane], then each row's maximum and sum; the same block of consecutive parts lies side by
+// side, so that a join's loads of a unit of few rows stay within few pages of memory. The block's number in the workspace:
+__device__ __forceinline__ size_t part_block(const AttendArgs &a, uint32_t first_piece, uint32_t part, uint32_t block) {
+  return (size_t)(2 * block + (part == 0 ? 1 : 0)) * a.workgroups + first_piece + part;
 }
 // The first of the four values that a lane's accumulators of vector v are: in a block of 16 rows, where lane (kq, r) holds
 // accumulator t = run j + d as value d of run 4 kq + j; and in one of 32 rows, where lane (h, r) holds 4 j + i of block b

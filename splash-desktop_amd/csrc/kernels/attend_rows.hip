@@ -438,7 +438,6 @@ attend_rows_kernel(AttendArgs a) {
                       (part.head * a.group + g) * dim + value;
       *(u32x2 *)out = u32x2{bf16_pair(sum[0] * by, sum[1] * by), bf16_pair(sum[2] * by, sum[3] * by)};
     };
-    float *mine = a.partials + (size_t)part_slot(part.first_piece, part.part) * (MB * kBlockFloats);
     if (part.parts > 1 && part.part == 0) began = {part.parts, (uint32_t)live, part.first_row + (uint32_t)row0, part.head};
     __syncthreads();   // the last join has been read
     if (lane < 16) {
@@ -451,6 +450,7 @@ attend_rows_kernel(AttendArgs a) {
 #pragma unroll
     for (int b = 0; b < MB; ++b) {
       float top = -INFINITY, total = 0.0f, by[kWaves];
+      float *mine = a.partials + part_block(a, part.first_piece, part.part, b) * kBlockFloats;
 #pragma unroll
       for (int c = 0; c < kChunks; ++c) {
         if (b || c) __syncthreads();
@@ -483,11 +483,11 @@ attend_rows_kernel(AttendArgs a) {
         if (part.parts == 1) {
           write(b, c, sum, total);
         } else if (16 * b + (int)r < live) {
-          *(f32x4 *)(mine + b * kBlockFloats + ((c * kVectors + wave) * 64 + lane) * 4) = sum;
+          *(f32x4 *)(mine + ((c * kVectors + wave) * 64 + lane) * 4) = sum;
         }
       }
       if (part.parts > 1 && wave == 0 && lane < 16) {
-        float *row = mine + b * kBlockFloats + 16 * DIM + 2 * lane;
+        float *row = mine + 16 * DIM + 2 * lane;
         row[0] = top;
         row[1] = total;
       }

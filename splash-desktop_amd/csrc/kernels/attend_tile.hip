@@ -479,7 +479,7 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
     if (part.parts > 1) {
       if (part.part == 0) began = {part.parts, (uint32_t)live, part.first_row + (uint32_t)row0, part.head};
       if (busy) {
-        float *mine = a.partials + ((size_t)part_slot(part.first_piece, part.part) * kWaves + wave) * kBlockFloats;
+        float *mine = a.partials + part_block(a, part.first_piece, part.part, wave) * kBlockFloats;
         if (on) {
 #pragma unroll
           for (int b = 0; b < kBlocks; ++b)
