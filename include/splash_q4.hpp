@@ -28,6 +28,14 @@ using MoeWeights = sq_moe_weights;
 using MoeBuffers = sq_moe_buffers;
 using PreparedInput = sq_prepared_input;
 using NormWeights = sq_norm_weights;
+using HeadRows = sq_head_rows;
+using RopeConfig = sq_rope_config;
+using KvShape = sq_kv_shape;
+using KvSize = sq_kv_size;
+using KvBatch = sq_kv_batch;
+using AttentionShape = sq_attention_shape;
+using AttentionPlan = sq_attention_plan;
+using AttentionBuffers = sq_attention_buffers;
 using QuantizedSegment = sq_segment;
 using Graph = void *;   // a hipStream_t; nullptr is the default stream
 
@@ -221,6 +229,70 @@ class MoE final {
   [[nodiscard]] static uint32_t expertLoadGroups(const sq_moe_expert_load_params &params) {
     return sq_moe_expert_load_groups(&params);
   }
+};
+
+// Rotary positions: frequencies() on the host, once; then a rope that holds them on the device.
+class Rope final {
+ public:
+  // Fills frequencies[0 .. config.rotary_dim / 2) in host memory and returns the rope's magnitude.
+  static float frequencies(const RopeConfig &config, double *frequencies) {
+    float magnitude = 0;
+    check(sq_rope_frequencies(&config, frequencies, &magnitude));
+    return magnitude;
+  }
+  Rope(uint32_t rotaryDim, uint32_t layout, float magnitude, Buffer frequencies) noexcept
+      : rope_{rotaryDim, layout, magnitude, frequencies} {}
+  void add(Graph graph, Buffer positions, uint32_t rows, uint32_t headDim, const HeadRows &input,
+           const HeadRows &output) const {
+    check(sq_rope_add(graph, &rope_, positions, rows, headDim, &input, &output));
+  }
+  [[nodiscard]] const sq_rope &get() const noexcept { return rope_; }
+
+ private:
+  sq_rope rope_;
+};
+
+// The paged key/value cache over the caller's buffers (zeroed scales for SQ_KV_BF16).
+class KvCache final {
+ public:
+  [[nodiscard]] static KvSize size(const KvShape &shape, uint32_t pages) {
+    KvSize out{};
+    check(sq_kv_cache_size(&shape, pages, &out));
+    return out;
+  }
+  KvCache(KvShape shape, uint32_t pages, Buffer keys, Buffer values, Buffer keyScales = {}, Buffer valueScales = {}) noexcept
+      : cache_{shape, pages, keys, values, keyScales, valueScales} {}
+  // With a rope the keys are rotated on their way, and the queries beside them when there are any.
+  void addWrite(Graph graph, const KvBatch &batch, const HeadRows &keys, const HeadRows &values,
+                const Rope *rope = nullptr, const HeadRows *queries = nullptr, const HeadRows *rotated = nullptr) const {
+    check(sq_kv_add_write(graph, &cache_, &batch, &keys, &values, rope ? &rope->get() : nullptr, queries, rotated));
+  }
+  void addRead(Graph graph, const KvBatch &batch, const HeadRows *keys, const HeadRows *values) const {
+    check(sq_kv_add_read(graph, &cache_, &batch, keys, values));
+  }
+  [[nodiscard]] const sq_kv_cache &get() const noexcept { return cache_; }
+
+ private:
+  sq_kv_cache cache_;
+};
+
+// Attention of a batch's new rows over the cache.
+class Attention final {
+ public:
+  explicit Attention(sq_device device = {0}) noexcept : device_(device) {}
+  [[nodiscard]] AttentionPlan plan(const AttentionShape &shape, uint32_t sequences, uint32_t rows,
+                                   uint32_t chunkRows) const {
+    AttentionPlan out{};
+    check(sq_attention_plan_for(&device_, &shape, sequences, rows, chunkRows, &out));
+    return out;
+  }
+  static void add(Graph graph, const AttentionBuffers &buffers, const KvCache &cache, const KvBatch &batch,
+                  const AttentionPlan &plan) {
+    check(sq_attention_add(graph, &buffers, &cache.get(), &batch, &plan));
+  }
+
+ private:
+  sq_device device_;
 };
 
 // Load-time weight preparation (gguf_repack.metal:232-238; GgufPreparation.cpp:141-193).

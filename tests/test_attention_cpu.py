@@ -278,3 +278,19 @@ def test_head_rows_of_tensors():
     for bad in (fused.t(), fused[:, :100], fused.float(), fused[:, ::2]):
         with pytest.raises(ValueError, match="head rows"):
             sq.head_rows(bad, 64)
+
+
+def test_cxx_face(tmp_path):
+    """The C++ header compiles against the library; its sizes are the C ABI's, its refusals exceptions."""
+    import pathlib
+    import shutil
+    import subprocess
+    if shutil.which("g++") is None:
+        pytest.skip("no g++")
+    exe, libs = tmp_path / "attention_check", sq.LIBRARY.parent
+    subprocess.run(["g++", "-std=c++17", "-O1", "-I", str(sq.HEADER.parent),
+                    str(pathlib.Path(__file__).parent / "cxx_attention_check.cpp"), "-L", str(libs), "-lsplash_q4",
+                    f"-Wl,-rpath,{libs}", "-o", str(exe)], check=True)
+    out = subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout
+    assert "magnitude 1 first 1; keys 20480 scales 1280; tile 16 waves 8 workgroups 256" in out
+    assert out.count("invalid_argument:") == 4
