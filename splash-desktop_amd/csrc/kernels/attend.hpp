@@ -4,14 +4,14 @@
 // A unit is `fit` consecutive rows of one sequence (tile_rows / group of them, with the query heads of one key head)
 // against every key that they see, in tiles of 64 keys. Unit m of a sequence ends at key e_m = position of its last row +
 // 1 (or the sequence's end), starts at key s_m (its first row's window), and is e_m - s_m + slack long, slack at least
-// 126: 64 or more for each of its tiles, ceil(e_m / 64) - floor(s_m / 64) of them, and what a unit costs besides. Lengths live on the
-// device and differ by orders of magnitude within a batch, so no grid over (sequence, head, split) is even. Two ways of
-// sharing the units out:
+// 126: 64 or more for each of its tiles, ceil(e_m / 64) - floor(s_m / 64) of them, and what a unit costs besides.
+// Lengths live on the device and differ by orders of magnitude within a batch, so no grid over (sequence, head, split) is
+// even. Two ways of sharing the units out:
 //
-//  - Few units (a quarter of the workgroups or fewer, all of a sequence's about as long, or short): each is cut into equal parts,
-//    as many as give no part more than the share, and a workgroup takes one part. The share is the work over the
-//    workgroups that cutting leaves whole, so there are enough of them. One token over 700 keys of 8 key heads: 10 us,
-//    where a line (below) cuts units at odd places and gives most workgroups two parts, one after the other: 16 us.
+//  - Few units (a quarter of the workgroups or fewer, all of them about as long, or short): each is cut into equal
+//    parts, as many as give no part more than the share, and a workgroup takes one part. The share is the work over the
+//    workgroups that cutting leaves whole, so there are enough of them. One token over 700 keys of 8 key heads: 14 us,
+//    where a line (below) cuts units at odd places and gives most workgroups two parts, one after the other: 22 us.
 //  - Otherwise the units lie end to end on a line, and workgroup w takes the w-th of equal pieces of it. A piece may end
 //    inside a unit, which then has parts. The lengths are linear in m up to the clamps at both ends, so their prefix sums
 //    have a closed form, and a workgroup finds its place by a search over the sequences' sums (in LDS) and one over m.
@@ -374,6 +374,30 @@ __device__ __forceinline__ Work<THREADS> make_work(const AttendArgs &a, const Cu
   __syncthreads();
   return w;
 }
+
+// Two of a key's values for each of two keys, regrouped: two keys of each of two values.
+__device__ __forceinline__ uint32_t low_halves(uint32_t k0, uint32_t k1) {
+  return __builtin_amdgcn_perm(k1, k0, 0x05040100u);
+}
+__device__ __forceinline__ uint32_t high_halves(uint32_t k0, uint32_t k1) {
+  return __builtin_amdgcn_perm(k1, k0, 0x07060302u);
+}
+// Four codes as bf16, in their order.
+template <uint32_t FMT>
+__device__ __forceinline__ u32x2 code_pairs4(uint32_t w) {
+  if constexpr (FMT == SQ_KV_E4M3) {
+    return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false)),
+                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true))};
+  } else {
+    uint32_t f[4];   // whole numbers of at most 8 bits: their fp32 words' high halves are their bf16
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = __float_as_uint((float)(int8_t)(w >> (8 * e)));
+    return u32x2{high_halves(f[0], f[1]), high_halves(f[2], f[3])};
+  }
+}
+
+// A running maximum is raised when a score exceeds it by more than this.
+constexpr float kRaise = 8.0f;
 
 // p / group for a packed row p < 128 and a group of at most 64: the fp32 quotient of p + 1/2 is a 128th or more from a
 // whole number, its error far less.

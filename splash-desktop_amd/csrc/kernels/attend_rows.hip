@@ -14,6 +14,15 @@
 // Loads go through buffer resources of 16 keys of one page (pages are whole multiples of 16 tokens): a key past the
 // sequence, a page that is a hole and a value past head_dim all read zero, with no instruction spent on them.
 //
+// The matrix units take the weights in bf16, half a step of which is 2^-9 to 2^-8 of a weight, as much as the output's own
+// rounding: where a few weights outweigh the rest, all of it shows. They go in as two, the rounded weight and the rest
+// (2^-16 of it is lost). Reading the cache hides the second products: a token over 131072 int8 keys takes 54 us either way,
+// and is 0.0017 from 64 bits (its own rounding) for 0.0027.
+//
+// What it reaches: a token of 40 heads over 131072 int8 keys of 8 heads of 128 (277 MB) in 54 us, 5.1 TB/s (a large copy
+// reaches 4.9); a token each of 64 sequences of 200 to 8000 e4m3 keys (291 MB) in 63 us, 4.6 TB/s; one over 700 bf16 keys,
+// which is a chain of round trips (lengths, page table, keys, the waves' join), in 14 us.
+//
 // Softmax: each wave keeps its own running maximum, lane sums and accumulators, and raises the maximum (which costs
 // lane exchanges and a pass over the accumulators) only when a score exceeds it by 8 (a factor of 256, which fp32 sums
 // and bf16's exponent hold without loss); the waves of a workgroup join at the end of a part, through LDS.
@@ -24,28 +33,6 @@ namespace sq::kern {
 namespace {
 
 constexpr int kStep = 32;      // keys a wave takes a step
-constexpr float kRaise = 8.0f;
-
-// Two of a key's values for each of two keys, regrouped: two keys of each of two values.
-__device__ __forceinline__ uint32_t low_halves(uint32_t k0, uint32_t k1) {
-  return __builtin_amdgcn_perm(k1, k0, 0x05040100u);
-}
-__device__ __forceinline__ uint32_t high_halves(uint32_t k0, uint32_t k1) {
-  return __builtin_amdgcn_perm(k1, k0, 0x07060302u);
-}
-// Four codes as bf16, in their order.
-template <uint32_t FMT>
-__device__ __forceinline__ u32x2 code_pairs4(uint32_t w) {
-  if constexpr (FMT == SQ_KV_E4M3) {
-    return u32x2{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false)),
-                 __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true))};
-  } else {
-    uint32_t f[4];   // whole numbers of at most 8 bits: their fp32 words' high halves are their bf16
-#pragma unroll
-    for (int e = 0; e < 4; ++e) f[e] = __float_as_uint((float)(int8_t)(w >> (8 * e)));
-    return u32x2{high_halves(f[0], f[1]), high_halves(f[2], f[3])};
-  }
-}
 
 // Four e4m3 codes, NaNs (all seven bits below the sign's set) as zeros.
 __device__ __forceinline__ uint32_t finite_codes(uint32_t w) {
@@ -173,8 +160,9 @@ struct Rows {
     }
   }
 
-  // Adds the weights' product with 32 keys' values. Two values of a run at a time.
-  __device__ __forceinline__ void accumulate(const ValueTile &t, const u32x4 (&p)[MB]) {
+  // Adds the weights' product with 32 keys' values. Two values of a run at a time. rest: what the weights lost to their
+  // rounding.
+  __device__ __forceinline__ void accumulate(const ValueTile &t, const u32x4 (&p)[MB], const u32x4 (&rest)[MB]) {
 #pragma unroll
     for (int j = 0; j < kRun / 2; ++j) {
       uint32_t w[2][4];   // values 2 j and 2 j + 1 of each key as bf16
@@ -193,6 +181,11 @@ struct Rows {
       for (int b = 0; b < MB; ++b) {
         o[b][2 * j] = mfma_bf16(even, p[b], o[b][2 * j]);
         o[b][2 * j + 1] = mfma_bf16(odd, p[b], o[b][2 * j + 1]);
+      }
+#pragma unroll
+      for (int b = 0; b < MB; ++b) {
+        o[b][2 * j] = mfma_bf16(even, rest[b], o[b][2 * j]);
+        o[b][2 * j + 1] = mfma_bf16(odd, rest[b], o[b][2 * j + 1]);
       }
     }
   }
@@ -336,7 +329,7 @@ attend_rows_kernel(AttendArgs a) {
             }
         }
       }
-      u32x4 p[MB];
+      u32x4 p[MB], rest[MB];
 #pragma unroll
       for (int b = 0; b < MB; ++b) {
         float v[8], top = -INFINITY;
@@ -369,7 +362,12 @@ attend_rows_kernel(AttendArgs a) {
           for (int i = 0; i < 8; ++i)
             w[i] = clear || (seen[b] >> i & 1) ? w[i] * value_scale[i / 4][i % 4] : 0.0f;
         }
-        p[b] = u32x4{bf16_pair(w[0], w[1]), bf16_pair(w[2], w[3]), bf16_pair(w[4], w[5]), bf16_pair(w[6], w[7])};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          p[b][i] = bf16_pair(w[2 * i], w[2 * i + 1]);
+          rest[b][i] = bf16_pair(w[2 * i] - __uint_as_float(p[b][i] << 16),
+                                 w[2 * i + 1] - __uint_as_float(p[b][i] & 0xFFFF0000u));
+        }
       }
       if constexpr (FMT == SQ_KV_E4M3) {
         // Keys before a window may never have been written: no NaN of their codes meets the zero weights.
@@ -420,7 +418,7 @@ attend_rows_kernel(AttendArgs a) {
               }
         }
       }
-      state.accumulate(vt, p);
+      state.accumulate(vt, p, rest);
       if (more) fetch_values(na, nb);
       ka = na;
       kb = nb;

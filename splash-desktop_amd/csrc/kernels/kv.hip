@@ -2,7 +2,9 @@
 // back. All three are bound by the bytes they move (a value in, a value out). A head row (head_dim values) is a group of
 // 8, 16 or 32 lanes of 8 values, so that its largest magnitude is a few lane exchanges away and each lane's access is one
 // 16-byte vector (8 bytes of codes). Of few rows each has a workgroup, of many a wave, four heads' loads in flight: a
-// workgroup a row of a 30000-key prefix takes 63 us, most of it launches, a wave a row 43 us; up to 2048 rows the workgroups are as fast or faster (2048 rotated rows 15.5 and 17.9 us).
+// workgroup a row of a 30000-key int8 prefix reads back in 63 us, most of it launches, a wave a row in 43 us (4.4 of the
+// 4.9 TB/s that a large copy reaches); up to 2048 rows the workgroups are as fast or faster (2048 rotated rows written in
+// 15.5 and 17.9 us). One launch of a few rows takes 3 to 6 us, its loads' round trips.
 //
 // The angles: p f / 2 pi turns in fp64, the whole turns dropped there (p f reaches 10^6 radians, where fp32 has a 16th
 // of a radian left), then sine and cosine of the fraction in fp32. A row's pairs are worked out once, by as many
