@@ -7,6 +7,7 @@ library is missing: there is no fallback path.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import pathlib
 from ctypes import POINTER, Structure, byref, c_char_p, c_double, c_float, c_int, c_uint32, c_uint64, c_void_p
@@ -421,17 +422,36 @@ def stream_read(src, sink, workgroups: int, threads: int, nbytes: int | None = N
 
 # ---------------------------------------------------------------- rotary positions, paged cache, attention
 
+@functools.cache
+def _row_types():
+    import torch
+    return torch.bfloat16, torch.int16, torch.uint16   # the last two: bf16's bits
+
+
+def _whole(tensor, what: str, element: int | None = None) -> Buffer:
+    """A view of a whole device tensor with adjacent elements (of `element` bytes)."""
+    if not tensor.is_cuda or not tensor.is_contiguous() or (element and tensor.element_size() != element):
+        raise ValueError(f"{what}: a contiguous device tensor" + (f" of {8 * element}-bit elements" if element else ""))
+    return view(tensor)
+
+
 def head_rows(tensor, head_dim: int) -> HeadRows:
     """A bf16 tensor's rows of heads: [rows, heads * head_dim] (a column slice of a fused projection's output too)."""
     if tensor.dim() != 2:
         raise ValueError("head rows are a [rows, heads * head_dim] tensor")
     (rows, width), (stride, step) = tensor.shape, tensor.stride()
-    if width % head_dim or step != 1 or tensor.element_size() != 2:
-        raise ValueError("head rows are a 2-byte [rows, heads * head_dim] tensor with adjacent columns")
+    if width % head_dim or step != 1 or tensor.dtype not in _row_types():
+        raise ValueError("head rows are a bf16 [rows, heads * head_dim] tensor with adjacent columns")
     if rows <= 1:
         stride = width
     return HeadRows(Buffer(tensor.data_ptr(), 2 * ((rows - 1) * stride + width) if rows else 0), width // head_dim,
                     stride)
+
+
+def _rows(tensor, head_dim: int) -> HeadRows:
+    if not tensor.is_cuda:
+        raise ValueError("head rows lie on the device")
+    return head_rows(tensor, head_dim)
 
 
 def rope_frequencies(config: RopeConfig) -> tuple[list[float], float]:
@@ -452,9 +472,9 @@ class RotaryPositions:
 
 
 def rope_add(rope: RotaryPositions, positions, input, output, head_dim: int, stream=None) -> None:
-    x, y = head_rows(input, head_dim), head_rows(output, head_dim)
-    call("sq_rope_add", stream if stream is not None else stream_handle(), byref(rope.struct), view(positions),
-         input.shape[0], head_dim, byref(x), byref(y))
+    x, y = _rows(input, head_dim), _rows(output, head_dim)
+    call("sq_rope_add", stream if stream is not None else stream_handle(), byref(rope.struct),
+         _whole(positions, "positions", 4), input.shape[0], head_dim, byref(x), byref(y))
 
 
 def kv_cache_size(shape: KvShape, pages: int) -> KvSize:
@@ -464,26 +484,28 @@ def kv_cache_size(shape: KvShape, pages: int) -> KvSize:
 
 
 def kv_cache(shape: KvShape, pages: int, keys, values, key_scales=None, value_scales=None) -> KvCache:
-    return KvCache(shape, pages, view(keys), view(values), view(key_scales), view(value_scales))
+    return KvCache(shape, pages, *(_whole(t, name) if t is not None else Buffer(None, 0) for name, t in
+                                   zip(_KV_BUFFERS, (keys, values, key_scales, value_scales))))
 
 
 def kv_batch(row_starts, lengths, page_table, rows: int) -> KvBatch:
     """row_starts [sequences + 1], lengths [sequences] and page_table [sequences, pages] are 32-bit tensors."""
-    return KvBatch(lengths.shape[0], rows, page_table.shape[1], view(row_starts), view(lengths), view(page_table))
+    return KvBatch(lengths.shape[0], rows, page_table.shape[1], _whole(row_starts, "row starts", 4),
+                   _whole(lengths, "lengths", 4), _whole(page_table, "page table", 4))
 
 
 def kv_write(cache: KvCache, batch: KvBatch, keys, values, rope: RotaryPositions | None = None, queries=None,
              rotated=None, stream=None) -> None:
     d = cache.shape.head_dim
-    k, v = head_rows(keys, d), head_rows(values, d)
-    q, r = (byref(head_rows(t, d)) if t is not None else None for t in (queries, rotated))
+    k, v = _rows(keys, d), _rows(values, d)
+    q, r = (byref(_rows(t, d)) if t is not None else None for t in (queries, rotated))
     call("sq_kv_add_write", stream if stream is not None else stream_handle(), byref(cache), byref(batch), byref(k),
          byref(v), byref(rope.struct) if rope is not None else None, q, r)
 
 
 def kv_read(cache: KvCache, batch: KvBatch, keys=None, values=None, stream=None) -> None:
     d = cache.shape.head_dim
-    k, v = (byref(head_rows(t, d)) if t is not None else None for t in (keys, values))
+    k, v = (byref(_rows(t, d)) if t is not None else None for t in (keys, values))
     call("sq_kv_add_read", stream if stream is not None else stream_handle(), byref(cache), byref(batch), k, v)
 
 
@@ -505,6 +527,6 @@ class AttentionScratch:
 def attention_add(plan: AttentionPlan, cache: KvCache, batch: KvBatch, query, output, scratch: AttentionScratch,
                   stream=None) -> None:
     d = cache.shape.head_dim
-    buffers = AttentionBuffers(head_rows(query, d), head_rows(output, d), view(scratch.partials))
+    buffers = AttentionBuffers(_rows(query, d), _rows(output, d), view(scratch.partials))
     call("sq_attention_add", stream if stream is not None else stream_handle(), byref(buffers), byref(cache),
          byref(batch), byref(plan))

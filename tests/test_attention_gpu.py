@@ -443,6 +443,26 @@ def test_graphs_that_share_a_workspace():
             assert np.array_equal(from_bf16(out).reshape(want.shape), want)
 
 
+def test_binding_refuses_what_it_would_misread():
+    t = torch()
+    make = lambda *shape, dtype=t.int32: t.zeros(shape, dtype=dtype, device="cuda")  # noqa: E731
+    starts, lengths, table = make(2), make(1), make(1, 4)
+    sq.kv_batch(starts, lengths, table, 1)
+    for bad in ((make(2, dtype=t.int64), lengths, table), (starts, make(1, 2)[:, :1].expand(1, 2), make(2, 8)[:, :4]),
+                (starts, lengths, make(4, 4).t()), (starts.cpu(), lengths, table)):
+        with pytest.raises(ValueError):
+            sq.kv_batch(*bad, 1)
+    for bad in (make(2, 64, dtype=t.float16), make(64, 2, dtype=t.bfloat16).t(), make(2, 60, dtype=t.bfloat16),
+                make(2, 64, dtype=t.float32), make(64, dtype=t.bfloat16)):
+        with pytest.raises(ValueError):
+            sq.head_rows(bad, 64)
+    cache = Cache(np.random.default_rng(1), [(1, 5)], 2, 64, 16, "int8")
+    with pytest.raises(ValueError):
+        sq.kv_cache(cache.shape, cache.pages, cache.keys.transpose(1, 2), cache.values)
+    with pytest.raises(ValueError):
+        sq.kv_read(cache.struct(), cache.batch(), t.zeros((1, 128), dtype=t.bfloat16))
+
+
 def test_two_streams_at_once():
     """Two batches on two streams, each with a workspace of its own."""
     t = torch()
