@@ -314,8 +314,10 @@ def view(tensor=None, nbytes: int | None = None) -> Buffer:
 
 
 def stream_handle():
+    """The current device's current stream. (By its raw handle: torch.cuda.current_stream() makes a stream object of it,
+    2.7 us of the 8.8 that a small call takes on the host.)"""
     import torch
-    return c_void_p(torch.cuda.current_stream().cuda_stream)
+    return c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
 
 
 def plane_bytes(fmt: int, n: int, k: int) -> tuple[int, int]:
