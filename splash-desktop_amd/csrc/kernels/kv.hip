@@ -118,9 +118,12 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs rope, const uint32_t
 }
 
 // A head row's eight values (of this lane; lanes past head_dim pass zeros) as codes, with the row's scale. The code is
-// x top / m rounded once to fp32 and then to the format: x top is exact (8 bits times 3 or 7), and the quotient of two
-// such numbers lies on a tie of the format or so far from it (over 2^-18 of it) that fp32 keeps the side, so the codes
-// are those of the exact quotient. Rows past 2^100 divide by 2^30 first, both sides, so that x top stays finite.
+// x top / m in fp32, rounded to the format: x top is exact (8 bits times 3 or 7), and the quotient of two such numbers
+// lies on a tie of the format or further from it (2^-18 of it) than the fp32 quotient is off. That is q + r / m of a first
+// quotient q = (x top) (1 / m), off by 2^-23, and its remainder r = x top - q m, which one fma gives exactly: off by 2^-46
+// before its rounding, so a tie, which has few bits, comes out exact. The codes are those of the exact quotient, for three
+// instructions a value where a division takes ten. Both sides go by 2^-30 in rows past 2^100, where x top would be
+// infinite, and by 2^60 below 2^-60, where 1 / m and the remainder would leave the normal range.
 struct Codes {
   u32x2 words;
   float scale;
@@ -135,11 +138,15 @@ __device__ __forceinline__ Codes codes8(u32x4 w) {
   if (largest >= 0x7F80u) return {{0u, 0u}, __uint_as_float(0x7FC00000u)};
   if (!largest) return {{0u, 0u}, 0.0f};
   constexpr float kTop = FMT == SQ_KV_INT8 ? 127.0f : 448.0f;
-  const float m = bf16_to_f32(largest), down = m > 0x1p100f ? 0x1p-30f : 1.0f, by = m * down;
+  const float m = bf16_to_f32(largest), shift = m > 0x1p100f ? 0x1p-30f : m < 0x1p-60f ? 0x1p60f : 1.0f;
+  const float by = m * shift, over = 1.0f / by;
   float x[8], q[8];
   widen8(w, x);
 #pragma unroll
-  for (int e = 0; e < 8; ++e) q[e] = x[e] * (kTop * down) / by;
+  for (int e = 0; e < 8; ++e) {
+    const float top = x[e] * (kTop * shift), first = top * over;
+    q[e] = fmaf(fmaf(-first, by, top), over, first);
+  }
   Codes out{{0u, 0u}, m / kTop};
   if constexpr (FMT == SQ_KV_INT8) {
 #pragma unroll
@@ -166,14 +173,9 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvArgs kv, HeadRows keys,
   const uint32_t t = threadIdx.x % THREADS, d = 8 * (t % LPH), dim = kv.head_dim;
   const uint32_t row = blockIdx.x * (256 / THREADS) + threadIdx.x / THREADS;
   if (row >= kv.rows) return;
-  const RowPlace place = place_of(kv, row);
-  if (place.sequence == ~0u) return;
-  const uint32_t page = place.position >= 0 ? page_of(kv, place.sequence, place.position) : ~0u;
-  const uint32_t slot = (uint32_t)place.position & ((1u << kv.page_shift) - 1);
   const bool live = d < dim;
-  if (rope.pairs) angles<THREADS>(cs, rope, (double)place.position, t);
-  for (uint32_t first = t / LPH; first < 2 * kv.kv_heads; first += kAtOnce * kHeads) {
-    u32x4 w[kAtOnce];
+  u32x4 w[kAtOnce];
+  const auto load = [&](uint32_t first) {
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) {
       const uint32_t u = first + i * kHeads;
@@ -185,6 +187,16 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvArgs kv, HeadRows keys,
       const uint16_t *head = from.rows + (size_t)row * from.stride + h * dim;
       w[i] = key && rope.pairs ? rotated8(head, d, cs, rope) : *(const u32x4 *)(head + d);
     }
+  };
+  // Without a rope the first loads are on their way before the row's place is known.
+  if (!rope.pairs) load(t / LPH);
+  const RowPlace place = place_of(kv, row);
+  if (place.sequence == ~0u) return;
+  const uint32_t page = place.position >= 0 ? page_of(kv, place.sequence, place.position) : ~0u;
+  const uint32_t slot = (uint32_t)place.position & ((1u << kv.page_shift) - 1);
+  if (rope.pairs) angles<THREADS>(cs, rope, (double)place.position, t);
+  for (uint32_t first = t / LPH; first < 2 * kv.kv_heads; first += kAtOnce * kHeads) {
+    if (rope.pairs || first != t / LPH) load(first);
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) {
       const uint32_t u = first + i * kHeads;

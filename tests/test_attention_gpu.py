@@ -103,6 +103,31 @@ def test_write_and_read(fmt, kv_heads, dim, page):
 
 
 @pytest.mark.parametrize("fmt", ["int8", "e4m3"])
+def test_codes_are_those_of_the_exact_quotients(fmt):
+    """Every mantissa of a row's largest value, at magnitudes from the smallest to the largest of bf16, under values of
+    every mantissa: the ties among them (x 127 / m halfway between two codes) go to the even code."""
+    rng = np.random.default_rng(16)
+    exponents = [-133, -127, -120, -61, -60, -59, 0, 99, 100, 101, 120]
+    rows = []
+    for e in exponents:
+        for mantissa in range(128, 256):
+            x = np.ldexp(rng.integers(128, 256, 256).astype(np.float64), e - rng.integers(0, 12, 256))
+            x = np.where(x <= mantissa * 2.0 ** e, x, 0) * rng.choice([-1, 1], 256)
+            x[:3] = mantissa * 2.0 ** e, -mantissa * 2.0 ** (e - 1), mantissa * 2.0 ** (e - 2)
+            rows.append(x)
+    x = bf16(np.array(rows))
+    c = Cache(rng, [(len(x), len(x))], 1, 256, 64, fmt)
+    sq.kv_write(c.struct(), c.batch(), to_bf16(x), to_bf16(x))
+    codes, scales = quantised(x[:, None], fmt)
+    at = np.arange(len(x))
+    for name in ("key", "value"):
+        stored, by = getattr(c, name + "s").float().cpu().numpy(), getattr(c, name + "_scales").cpu().numpy()
+        pages, slots = c.table[0, at // 64], at % 64
+        assert np.array_equal(by[pages, :, slots], scales)
+        assert np.array_equal(stored[pages, :, slots], codes)
+
+
+@pytest.mark.parametrize("fmt", ["int8", "e4m3"])
 def test_write_of_unbounded_rows(fmt):
     t = torch()
     rng = np.random.default_rng(5)
