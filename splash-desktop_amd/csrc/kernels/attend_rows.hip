@@ -15,9 +15,10 @@
 // sequence, a page that is a hole and a value past head_dim all read zero, with no instruction spent on them.
 //
 // The matrix units take the weights in bf16, half a step of which is 2^-9 to 2^-8 of a weight, as much as the output's own
-// rounding: where a few weights outweigh the rest, all of it shows. They go in as two, the rounded weight and the rest
+// rounding: where a few weights outweigh the rest, all of it shows. They go in as two, the weight rounded down and the rest
 // (2^-16 of it is lost). Reading the cache hides the second products: a token over 131072 int8 keys takes 54 us either way,
-// and is 0.0017 from 64 bits (its own rounding) for 0.0027.
+// and is 0.0017 from 64 bits (its own rounding) for 0.0027. An infinite value meets both, so neither may be zero or
+// negative where the weight is not (0 inf and inf - inf are NaN): hence down, and hence kMore.
 //
 // What it reaches: a token of 40 heads over 131072 int8 keys of 8 heads of 128 (277 MB) in 54 us, 5.1 TB/s (a large copy
 // reaches 4.9); a token each of 64 sequences of 200 to 8000 e4m3 keys (291 MB) in 63 us, 4.6 TB/s; one over 700 bf16 keys,
@@ -33,6 +34,10 @@ namespace sq::kern {
 namespace {
 
 constexpr int kStep = 32;      // keys a wave takes a step
+// What all weights are multiplied by on their way into the second product, so that the rest of one that bf16 holds exactly
+// is 2^-18 of it and not zero. The outputs grow by as much, a 2^-10 of their own rounding. (The rest of a weight below
+// 2^-108 leaves bf16's normal range: an infinite value under it may give NaN, as it does in fp32 where e^x has become 0.)
+constexpr float kMore = 1 + 0x1p-18f;
 
 // Four e4m3 codes, NaNs (all seven bits below the sign's set) as zeros.
 __device__ __forceinline__ uint32_t finite_codes(uint32_t w) {
@@ -364,9 +369,9 @@ attend_rows_kernel(AttendArgs a) {
         }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          p[b][i] = bf16_pair(w[2 * i], w[2 * i + 1]);
-          rest[b][i] = bf16_pair(w[2 * i] - __uint_as_float(p[b][i] << 16),
-                                 w[2 * i + 1] - __uint_as_float(p[b][i] & 0xFFFF0000u));
+          p[b][i] = high_halves(__float_as_uint(w[2 * i]), __float_as_uint(w[2 * i + 1]));
+          rest[b][i] = bf16_pair(fmaf(w[2 * i], kMore, -__uint_as_float(p[b][i] << 16)),
+                                 fmaf(w[2 * i + 1], kMore, -__uint_as_float(p[b][i] & 0xFFFF0000u)));
         }
       }
       if constexpr (FMT == SQ_KV_E4M3) {
