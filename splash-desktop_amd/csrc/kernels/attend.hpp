@@ -396,6 +396,9 @@ __device__ __forceinline__ u32x2 code_pairs4(uint32_t w) {
   }
 }
 
+// The sign bits of a word's e4m3 codes that are NaN (all seven bits below the sign's set), in their places.
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
+
 // A running maximum is raised when a score exceeds it by more than this.
 constexpr float kRaise = 8.0f;
 

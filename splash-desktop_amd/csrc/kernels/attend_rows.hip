@@ -39,12 +39,11 @@ constexpr int kStep = 32;      // keys a wave takes a step
 // 2^-108 leaves bf16's normal range: an infinite value under it may give NaN, as it does in fp32 where e^x has become 0.)
 constexpr float kMore = 1 + 0x1p-18f;
 
-// Four e4m3 codes, NaNs (all seven bits below the sign's set) as zeros.
+// Four e4m3 codes, NaNs as zeros.
 __device__ __forceinline__ uint32_t finite_codes(uint32_t w) {
-  const uint32_t nan = ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+  const uint32_t nan = nan_codes(w);
   return w & ~(nan | (nan - (nan >> 7)));
 }
-
 // The maximum over the four lanes that hold one row's keys.
 __device__ __forceinline__ float row_max(float v) {
   auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -165,12 +164,20 @@ struct Rows {
     }
   }
 
+  // The operands of values 2 j and 2 j + 1 of a run, from each key's word of them as bf16.
+  static __device__ __forceinline__ void value_operands(const uint32_t (&w)[2][4], u32x4 &even, u32x4 &odd) {
+    even = u32x4{low_halves(w[0][0], w[0][1]), low_halves(w[0][2], w[0][3]), low_halves(w[1][0], w[1][1]),
+                 low_halves(w[1][2], w[1][3])};
+    odd = u32x4{high_halves(w[0][0], w[0][1]), high_halves(w[0][2], w[0][3]), high_halves(w[1][0], w[1][1]),
+                high_halves(w[1][2], w[1][3])};
+  }
+
   // Adds the weights' product with 32 keys' values. Two values of a run at a time. rest: what the weights lost to their
   // rounding.
   __device__ __forceinline__ void accumulate(const ValueTile &t, const u32x4 (&p)[MB], const u32x4 (&rest)[MB]) {
 #pragma unroll
     for (int j = 0; j < kRun / 2; ++j) {
-      uint32_t w[2][4];   // values 2 j and 2 j + 1 of each key as bf16
+      uint32_t w[2][4];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -178,10 +185,8 @@ struct Rows {
           if constexpr (!kCodes) w[h][e] = t.w[h][e][j];
           else w[h][e] = code_pairs4<FMT>(t.w[h][e][j / 2])[j % 2];
         }
-      const u32x4 even{low_halves(w[0][0], w[0][1]), low_halves(w[0][2], w[0][3]), low_halves(w[1][0], w[1][1]),
-                       low_halves(w[1][2], w[1][3])};
-      const u32x4 odd{high_halves(w[0][0], w[0][1]), high_halves(w[0][2], w[0][3]), high_halves(w[1][0], w[1][1]),
-                      high_halves(w[1][2], w[1][3])};
+      u32x4 even, odd;
+      value_operands(w, even, odd);
 #pragma unroll
       for (int b = 0; b < MB; ++b) {
         o[b][2 * j] = mfma_bf16(even, p[b], o[b][2 * j]);
@@ -194,10 +199,56 @@ struct Rows {
       }
     }
   }
+
+  // e4m3's NaN codes leave the tile, and the accumulators of the rows that see them become NaN: products of large values in
+  // the places of such codes and of keys seen, which overflow, once to infinity and once below it, leave NaNs, and add zeros
+  // to all other accumulators. (Bit 4 h + i of seen: key 16 h + 4 kq + i.) A word of each key at a time: this hardly ever
+  // runs, and takes no more registers than the kernel has.
+  __device__ __forceinline__ void take_nans(ValueTile &t, const uint32_t (&seen)[MB]) {
+    constexpr uint32_t kLarge = 0x7Eu, kHuge = 0x7F00u;   // e4m3's 448, bf16's 2^127
+#pragma unroll
+    for (int i = 0; i < kValueWords; ++i) {
+      uint32_t at[2][4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          uint32_t &word = t.w[h][e][i];
+          asm volatile("" : "+v"(word));   // or the terms of the check before would wait in registers for their use here
+          at[h][e] = (nan_codes(word) >> 7) * kLarge;
+          word = finite_codes(word);
+        }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        uint32_t w[2][4];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) w[h][e] = code_pairs4<FMT>(at[h][e])[j];
+        u32x4 even, odd;
+        value_operands(w, even, odd);
+#pragma unroll
+        for (int b = 0; b < MB; ++b) {
+          uint32_t bits = seen[b];
+          asm volatile("" : "+v"(bits));
+          u32x4 sees;
+#pragma unroll
+          for (int n = 0; n < 4; ++n) sees[n] = (bits >> (2 * n) & 1) * kHuge | (bits >> (2 * n + 1) & 1) * (kHuge << 16);
+          f32x4 &first = o[b][4 * i + 2 * j], &second = o[b][4 * i + 2 * j + 1];
+          first = mfma_bf16(even, sees, first);
+          second = mfma_bf16(odd, sees, second);
+          sees ^= 0x80008000u;
+          first = mfma_bf16(even, sees, first);
+          second = mfma_bf16(odd, sees, second);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+  }
 };
 
-// Whether any value of a bf16 tile is an infinity or NaN.
-template <int N>
+// Whether any value of a tile is an infinity or NaN (e4m3's: its NaN code).
+template <uint32_t FMT, int N>
 __device__ __forceinline__ bool unbounded(const uint32_t (&w)[2][4][N]) {
   uint32_t any = 0;
 #pragma unroll
@@ -205,8 +256,10 @@ __device__ __forceinline__ bool unbounded(const uint32_t (&w)[2][4][N]) {
 #pragma unroll
     for (int e = 0; e < 4; ++e)
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        any |= (uint32_t)((w[h][e][i] & 0x7F80u) == 0x7F80u) | (uint32_t)((w[h][e][i] & 0x7F800000u) == 0x7F800000u);
+      for (int i = 0; i < N; ++i) {
+        if constexpr (FMT == SQ_KV_E4M3) any |= nan_codes(w[h][e][i]);
+        else any |= (uint32_t)((w[h][e][i] & 0x7F80u) == 0x7F80u) | (uint32_t)((w[h][e][i] & 0x7F800000u) == 0x7F800000u);
+      }
   return any != 0;
 }
 
@@ -374,20 +427,10 @@ attend_rows_kernel(AttendArgs a) {
                                  fmaf(w[2 * i + 1], kMore, -__uint_as_float(p[b][i] & 0xFFFF0000u)));
         }
       }
-      if constexpr (FMT == SQ_KV_E4M3) {
-        // Keys before a window may never have been written: no NaN of their codes meets the zero weights.
-        if (k < clear_begin)
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-              for (int i = 0; i < R::kValueWords; ++i) vt.w[h][e][i] = finite_codes(vt.w[h][e][i]);
-      }
       if constexpr (!kCodes) {
         // Where some rows see a key and others do not, its values must not reach the others through 0 * inf: infinities
         // and NaNs leave the tile, and the rows that see them add their products one by one.
-        if (!clear && __any(unbounded(vt.w))) {
+        if (!clear && __any(unbounded<FMT>(vt.w))) {
 #pragma unroll
           for (int b = 0; b < MB; ++b)
             for (int key = 0; key < kStep; ++key) {
@@ -422,6 +465,10 @@ attend_rows_kernel(AttendArgs a) {
                 if ((word & 0x7F800000u) == 0x7F800000u) word &= 0x0000FFFFu;
               }
         }
+      }
+      if constexpr (FMT == SQ_KV_E4M3) {
+        // The same of NaN codes. (No write makes one, but pages may hold them that have not been written yet, or by another.)
+        if (!clear && __any(unbounded<FMT>(vt.w))) state.take_nans(vt, seen);
       }
       state.accumulate(vt, p, rest);
       if (more) fetch_values(na, nb);

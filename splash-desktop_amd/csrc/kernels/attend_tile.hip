@@ -97,6 +97,7 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
   constexpr int kLoads = 16 * DIM * kBytes / 1024, kRowLanes = DIM * kBytes / 16, kLoadRows = 64 / kRowLanes;
   __shared__ __attribute__((aligned(1024))) uint8_t tiles[2][2][T::kBytes];   // [tile % 2][K, V]
   __shared__ f32x4 scales[kCodes ? 4 : 1][2][kKeyTile / 4];   // [tile % 4][K, V]
+  __shared__ u32x4 nans[FMT == SQ_KV_E4M3 ? 4 : 1];   // [tile % 4][wave]: whether its 16 keys' values hold a NaN code
   __shared__ LineShared<kThreads> shared;
   const uint32_t lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
   const uint32_t wave = uniform(threadIdx.x >> 6);
@@ -207,8 +208,25 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
         for (int j = 0; j < kLoads; ++j) copy_to_lds(rows, lds + 1024 * j, (kValues ? value_from : key_from)[j]);
       }
     };
+    // Whether rows of the unit see other keys than others among the 64 from k on (not for their holes or the sequence's end).
+    const auto differs = [&](int k) __attribute__((always_inline)) {
+      return k < clear_begin || k + kKeyTile > clear_end;
+    };
     const auto place = [&](int tile, auto of_values) __attribute__((always_inline)) {
       constexpr bool kValues = decltype(of_values)::value;
+      if constexpr (FMT == SQ_KV_E4M3 && kValues) {
+        // Looked at here, where the codes are at hand, for 2 to 4% of a chunk; a pass over the tile in LDS and its barrier took
+        // 1 to 8 (most where a window begins in the middle of every unit).
+        if (differs(at_tile(tile))) {
+          uint32_t any = 0;
+#pragma unroll
+          for (int j = 0; j < kLoads; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) any |= nan_codes(code_v[j][i]);
+          const bool some = __any(any != 0);
+          if (lane == 0) ((uint32_t *)&nans[tile % 4])[wave] = some;
+        }
+      }
       if constexpr (kCodes) {
 #pragma unroll
         for (int j = 0; j < kLoads; ++j) {
@@ -299,21 +317,52 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
           if (bad && wave == 0) by[lane] = 0.0f;
           __syncthreads();
         }
-        // Codes written are finite, but keys before a window may never have been.
-        if (FMT == SQ_KV_INT8 || k >= clear_begin) return;
+        // int8 codes are finite, and so are e4m3's that a write has made; pages may hold its NaN that have not been written
+        // yet, or by another.
+        if constexpr (FMT == SQ_KV_INT8) return;
+        if (!differs(k)) return;
+        const u32x4 any = nans[tile % 4];
+        if (!uniform(any[0] | any[1] | any[2] | any[3])) return;
       }
       constexpr int kMine = T::kBytes / 16 / kThreads;
       uint8_t *vt = tiles[tile % 2][1];
-      uint32_t any = 0;
+      if constexpr (!kCodes) {
+        uint32_t any = 0;
 #pragma unroll
-      for (int i = 0; i < kMine; ++i) {
-        const u32x4 v = *(const u32x4 *)&vt[16 * (threadIdx.x + kThreads * i)];
+        for (int i = 0; i < kMine; ++i) {
+          const u32x4 v = *(const u32x4 *)&vt[16 * (threadIdx.x + kThreads * i)];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          any |= (uint32_t)((v[e] & 0x7F80u) == 0x7F80u) | (uint32_t)((v[e] & 0x7F800000u) == 0x7F800000u);
+          for (int e = 0; e < 4; ++e)
+            any |= (uint32_t)((v[e] & 0x7F80u) == 0x7F80u) | (uint32_t)((v[e] & 0x7F800000u) == 0x7F800000u);
+        }
+        if (!__syncthreads_or((int)any)) return;
       }
-      if (!__syncthreads_or((int)any)) return;
-      if (!kCodes && busy) {
+      if constexpr (kCodes) {
+        // All of them are NaNs, whatever the weights. Products of kHuge in their places and in those of keys seen, which
+        // overflow, once to infinity and once below it, leave NaNs, and add zeros to all other accumulators.
+        constexpr uint32_t kHuge = 0x7F00u;   // bf16's 2^127
+        if (busy) {
+#pragma unroll 1
+          for (int t = 0; t < 4; ++t) {
+            u32x4 sees;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int j = k + 16 * t + 8 * (i / 2) + 4 * (int)h + 2 * (i % 2);   // and the next key
+              sees[i] = (on && j >= low && j < high ? kHuge : 0u) | (on && j + 1 >= low && j + 1 < high ? kHuge << 16 : 0u);
+            }
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) {
+              u32x4 at = value_operand(tile, t, b);
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                at[i] = ((at[i] & 0x7F80u) == 0x7F80u ? kHuge : 0u) | ((at[i] & 0x7F800000u) == 0x7F800000u ? kHuge << 16 : 0u);
+              o[b] = mfma32(at, sees, o[b]);
+              o[b] = mfma32(at ^ 0x80008000u, sees, o[b]);
+              __builtin_amdgcn_sched_barrier(0);
+            }
+          }
+        }
+      } else if (busy) {
 #pragma unroll 1
         for (uint32_t key = 0; key < kKeyTile; ++key) {
           // Key `key` is score 4 (key % 32 / 8) + key % 4 of block key / 32 in the lanes with h = key / 4 % 2.

@@ -54,3 +54,40 @@ def test_seen_infinities(heads, kv_heads, dim, sizes, tile):
         got = b[:n, heads - group:, column]
         assert np.array_equal(got, np.full_like(got, value), equal_nan=True), (column, value, got)
     check_bits(b, a, changed, tile)
+
+
+@pytest.mark.parametrize("window", [0, 40])
+@pytest.mark.parametrize("heads,kv_heads,dim,sizes,tile", TILES)
+def test_nan_codes(heads, kv_heads, dim, sizes, tile, window):
+    """E4M3's NaN codes under finite scales (no write makes them, but pages may be filled by others, or not yet): the rows
+    that see such a value have NaN in its column, the rows before it or past whose window it lies keep their bits."""
+    t = torch()
+    rng = np.random.default_rng(dim + heads)
+    clean, bad = (Cache(np.random.default_rng(7), sizes, kv_heads, dim, 16, "e4m3").fill() for _ in range(2))
+    plan = sq.attention_plan(sq.AttentionShape(heads, clean.shape, 1, window, 0.1), len(sizes), clean.rows,
+                             max(r for r, _ in sizes))
+    assert plan.tile_rows == tile
+    n, keys = sizes[0]
+    first, group = keys - n, heads // kv_heads
+    position = np.arange(first, keys)
+    nan = np.zeros((clean.rows, heads, dim), bool)
+
+    def put(tensor, head, key, column, code):
+        page, slot = bad.slot(0, key)
+        tensor.view(t.uint8)[int(page), head, slot, column] = code
+        sees = (key <= position) & (key > position - (window or keys))
+        columns = [column] if tensor is bad.values else range(dim)
+        for r in np.flatnonzero(sees):
+            nan[r, head * group:(head + 1) * group, columns] = True
+
+    put(bad.values, kv_heads - 1, keys - 2, 3, 0x7F)
+    put(bad.values, kv_heads - 1, keys - 1, dim - 1, 0xFF)
+    put(bad.values, kv_heads - 1, first, 8, 0x7F)
+    put(bad.values, kv_heads - 1, 3, 7, 0xFF)
+    put(bad.values, kv_heads - 1, max(0, first - 36), 5, 0xFF)     # with the window: the first four rows see it
+    if kv_heads > 1:
+        put(bad.keys, 0, keys - 1, 2, 0x7F)
+    q = queries(rng, clean, heads, dim)
+    a, b = (run_attention(c, q, 0.1, window=window, plan=plan) for c in (clean, bad))
+    assert np.isnan(b[nan]).all(), f"{np.sum(~np.isnan(b[nan]))} of {nan.sum()} that see a NaN have none"
+    check_bits(b, a, nan, tile)
