@@ -425,15 +425,22 @@ def stream_read(src, sink, workgroups: int, threads: int, nbytes: int | None = N
 # ---------------------------------------------------------------- rotary positions, paged cache, attention
 
 @functools.cache
-def _row_types():
+def _types(kind):
+    """The tensor types that hold `kind`: rows of heads, 32-bit words, a cache format's values or its scales. (int16, uint16:
+    bf16's bits. uint8: a cache's buffers as bytes, which is how kv_cache_size counts them.)"""
     import torch
-    return torch.bfloat16, torch.int16, torch.uint16   # the last two: bf16's bits
+    rows = (torch.bfloat16, torch.int16, torch.uint16)
+    return {"rows": rows, "words": (torch.int32, torch.uint32), "scales": (torch.float32, torch.uint8),
+            KV_BF16: (*rows, torch.uint8), KV_INT8: (torch.int8, torch.uint8),
+            KV_E4M3: (torch.float8_e4m3fn, torch.int8, torch.uint8)}[kind]
 
 
-def _whole(tensor, what: str, element: int | None = None) -> Buffer:
-    """A view of a whole device tensor with adjacent elements (of `element` bytes)."""
-    if not tensor.is_cuda or not tensor.is_contiguous() or (element and tensor.element_size() != element):
-        raise ValueError(f"{what}: a contiguous device tensor" + (f" of {8 * element}-bit elements" if element else ""))
+def _whole(tensor, what: str, kind, dims: int | None = None) -> Buffer:
+    """A view of a whole device tensor with adjacent elements of the kind's types."""
+    if (not tensor.is_cuda or not tensor.is_contiguous() or tensor.dtype not in _types(kind)
+            or dims is not None and tensor.dim() != dims):
+        raise ValueError(f"{what}: a contiguous device tensor of " + " or ".join(map(str, _types(kind))) +
+                         (f", of {dims} dimension{'s' * (dims > 1)}" if dims is not None else ""))
     return view(tensor)
 
 
@@ -442,7 +449,7 @@ def head_rows(tensor, head_dim: int) -> HeadRows:
     if tensor.dim() != 2:
         raise ValueError("head rows are a [rows, heads * head_dim] tensor")
     (rows, width), (stride, step) = tensor.shape, tensor.stride()
-    if width % head_dim or step != 1 or tensor.dtype not in _row_types():
+    if width % head_dim or step != 1 or tensor.dtype not in _types("rows"):
         raise ValueError("head rows are a bf16 [rows, heads * head_dim] tensor with adjacent columns")
     if rows <= 1:
         stride = width
@@ -476,7 +483,7 @@ class RotaryPositions:
 def rope_add(rope: RotaryPositions, positions, input, output, head_dim: int, stream=None) -> None:
     x, y = _rows(input, head_dim), _rows(output, head_dim)
     call("sq_rope_add", stream if stream is not None else stream_handle(), byref(rope.struct),
-         _whole(positions, "positions", 4), input.shape[0], head_dim, byref(x), byref(y))
+         _whole(positions, "positions", "words"), input.shape[0], head_dim, byref(x), byref(y))
 
 
 def kv_cache_size(shape: KvShape, pages: int) -> KvSize:
@@ -486,14 +493,18 @@ def kv_cache_size(shape: KvShape, pages: int) -> KvSize:
 
 
 def kv_cache(shape: KvShape, pages: int, keys, values, key_scales=None, value_scales=None) -> KvCache:
-    return KvCache(shape, pages, *(_whole(t, name) if t is not None else Buffer(None, 0) for name, t in
-                                   zip(_KV_BUFFERS, (keys, values, key_scales, value_scales))))
+    if shape.format not in (KV_BF16, KV_INT8, KV_E4M3):
+        raise ValueError("unknown cache format")
+    kinds = (shape.format, shape.format, "scales", "scales")
+    return KvCache(shape, pages, *(_whole(t, name, kind) if t is not None else Buffer(None, 0) for name, kind, t in
+                                   zip(_KV_BUFFERS, kinds, (keys, values, key_scales, value_scales))))
 
 
 def kv_batch(row_starts, lengths, page_table, rows: int) -> KvBatch:
-    """row_starts [sequences + 1], lengths [sequences] and page_table [sequences, pages] are 32-bit tensors."""
-    return KvBatch(lengths.shape[0], rows, page_table.shape[1], _whole(row_starts, "row starts", 4),
-                   _whole(lengths, "lengths", 4), _whole(page_table, "page table", 4))
+    """row_starts [sequences + 1], lengths [sequences] and page_table [sequences, pages] are 32-bit whole numbers."""
+    starts, lengths_, table = (_whole(t, name, "words", dims) for t, name, dims in (
+        (row_starts, "row starts", 1), (lengths, "lengths", 1), (page_table, "page table", 2)))
+    return KvBatch(lengths.shape[0], rows, page_table.shape[1], starts, lengths_, table)
 
 
 def kv_write(cache: KvCache, batch: KvBatch, keys, values, rope: RotaryPositions | None = None, queries=None,

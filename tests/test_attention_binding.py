@@ -1,0 +1,107 @@
+"""The Python binding of rope, cache and attention refuses tensors that its views would misread, before the library is
+called: checked on stand-ins for device tensors, which are never looked into."""
+import pytest
+
+import splash_q4 as sq
+
+torch = pytest.importorskip("torch")
+
+
+class Device:
+    """A device tensor's outside: `like` says its shape, strides and type."""
+
+    is_cuda = True
+
+    def __init__(self, like, at=1 << 20, device=0):
+        self.like, self.at, self.device = like, at, device
+        self.dtype, self.shape = like.dtype, like.shape
+
+    def data_ptr(self):
+        return self.at
+
+    def get_device(self):
+        return self.device
+
+    def __getattr__(self, name):
+        return getattr(self.like, name)
+
+
+def device(*shape, dtype=torch.int32):
+    return Device(torch.empty(shape, dtype=dtype))
+
+
+ROW, WORD = torch.bfloat16, torch.int32
+STORED = {sq.KV_BF16: (torch.bfloat16, torch.int16), sq.KV_INT8: (torch.int8,), sq.KV_E4M3: (torch.float8_e4m3fn, torch.int8)}
+
+
+@pytest.mark.parametrize("format", STORED)
+@pytest.mark.parametrize("stored", [torch.bfloat16, torch.int16, torch.float16, torch.int8, torch.float8_e4m3fn,
+                                    torch.float8_e4m3fnuz, torch.float8_e5m2, torch.float32, torch.int32])
+def test_pools_of_another_type(format, stored):
+    shape = sq.KvShape(2, 64, 16, format)
+    pool, good = device(4, 2, 16, 64, dtype=stored), device(4, 2, 16, 64, dtype=STORED[format][0])
+    scales = [device(4, 2, 16, dtype=torch.float32) for _ in range(2)]
+    fits = stored in STORED[format]
+    for keys, values in ((pool, good), (good, pool)):
+        if fits:
+            assert sq.kv_cache(shape, 4, keys, values, *scales).keys.bytes == 4 * 2 * 16 * 64 * stored.itemsize
+        else:
+            with pytest.raises(ValueError, match="keys|values"):
+                sq.kv_cache(shape, 4, keys, values, *scales)
+
+
+@pytest.mark.parametrize("format", STORED)
+def test_buffers_as_bytes(format):
+    """What kv_cache_size counts, allocated as that many bytes."""
+    shape = sq.KvShape(2, 64, 16, format)
+    size = sq.kv_cache_size(shape, 4)
+    buffers = [device(n, dtype=torch.uint8) for n in (size.keys, size.values, size.key_scales, size.value_scales)]
+    cache = sq.kv_cache(shape, 4, *buffers)
+    assert [getattr(cache, n).bytes for n in ("keys", "value_scales")] == [size.keys, size.value_scales]
+
+
+@pytest.mark.parametrize("wrong", [torch.float64, torch.bfloat16, torch.int32])
+def test_scales_of_another_type(wrong):
+    shape, pool = sq.KvShape(2, 64, 16, sq.KV_INT8), device(4, 2, 16, 64, dtype=torch.int8)
+    good, bad = device(4, 2, 16, dtype=torch.float32), device(4, 2, 16, dtype=wrong)
+    sq.kv_cache(shape, 4, pool, pool, good, good)
+    for scales in ((bad, good), (good, bad)):
+        with pytest.raises(ValueError, match="scales"):
+            sq.kv_cache(shape, 4, pool, pool, *scales)
+
+
+def test_an_unknown_format():
+    with pytest.raises(ValueError, match="format"):
+        sq.kv_cache(sq.KvShape(2, 64, 16, 3), 4, device(8, dtype=torch.int8), device(8, dtype=torch.int8))
+
+
+@pytest.mark.parametrize("wrong", [torch.float32, torch.int64, torch.bool, torch.int16])
+def test_batches_of_another_type(wrong):
+    starts, lengths, table = device(3), device(2), device(2, 5)
+    batch = sq.kv_batch(starts, lengths, table, 4)
+    assert (batch.sequences, batch.rows, batch.pages_per_sequence) == (2, 4, 5)
+    sq.kv_batch(device(3, dtype=torch.uint32), lengths, table, 4)
+    for at, name in enumerate(("row starts", "lengths", "page table")):
+        parts = [starts, lengths, table]
+        parts[at] = device(*parts[at].shape, dtype=wrong)
+        with pytest.raises(ValueError, match=name):
+            sq.kv_batch(*parts, 4)
+
+
+def test_batches_of_other_dimensions():
+    starts, lengths, table = device(3), device(2), device(2, 5)
+    for parts, name in (((device(1, 3), lengths, table), "row starts"), ((starts, device(1, 2), table), "lengths"),
+                        ((starts, lengths, device(10)), "page table"), ((starts, lengths, device(1, 2, 5)), "page table")):
+        with pytest.raises(ValueError, match=name):
+            sq.kv_batch(*parts, 4)
+
+
+class Rope:
+    struct = sq.Rope(64, sq.ROPE_HALF, 1.0, sq.Buffer(1 << 20, 256))
+
+
+@pytest.mark.parametrize("wrong", [torch.float32, torch.int64])
+def test_positions_of_another_type(wrong):
+    x = device(3, 128, dtype=ROW)
+    with pytest.raises(ValueError, match="positions"):
+        sq.rope_add(Rope, device(3, dtype=wrong), x, x, 64, stream=0)
