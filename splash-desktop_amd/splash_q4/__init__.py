@@ -315,9 +315,11 @@ def view(tensor=None, nbytes: int | None = None) -> Buffer:
 
 def stream_handle():
     """The current device's current stream. (By its raw handle: torch.cuda.current_stream() makes a stream object of it,
-    2.7 us of the 8.8 that a small call takes on the host.)"""
+    2.7 us of the 8.8 that a small call takes on the host. The handle's function is torch's own and not promised, so a
+    torch without it goes the long way.)"""
     import torch
-    return c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return c_void_p(raw(torch.cuda.current_device()) if raw else torch.cuda.current_stream().cuda_stream)
 
 
 def plane_bytes(fmt: int, n: int, k: int) -> tuple[int, int]:

@@ -30,7 +30,7 @@ def device(*shape, dtype=torch.int32):
     return Device(torch.empty(shape, dtype=dtype))
 
 
-ROW, WORD = torch.bfloat16, torch.int32
+ROW = torch.bfloat16
 STORED = {sq.KV_BF16: (torch.bfloat16, torch.int16), sq.KV_INT8: (torch.int8,), sq.KV_E4M3: (torch.float8_e4m3fn, torch.int8)}
 
 
@@ -105,3 +105,17 @@ def test_positions_of_another_type(wrong):
     x = device(3, 128, dtype=ROW)
     with pytest.raises(ValueError, match="positions"):
         sq.rope_add(Rope, device(3, dtype=wrong), x, x, 64, stream=0)
+
+
+@pytest.mark.parametrize("raw", [True, False])
+def test_the_current_stream_with_and_without_its_raw_handle(monkeypatch, raw):
+    class Stream:
+        cuda_stream = 0x5000
+
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 3)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: Stream)
+    if raw:
+        monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda device: 0x4000 + device, raising=False)
+    else:
+        monkeypatch.delattr(torch._C, "_cuda_getCurrentRawStream", raising=False)
+    assert sq.stream_handle().value == (0x4003 if raw else 0x5000)
