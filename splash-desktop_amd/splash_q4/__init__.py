@@ -313,13 +313,18 @@ def view(tensor=None, nbytes: int | None = None) -> Buffer:
     return Buffer(tensor.data_ptr(), total if nbytes is None else nbytes)
 
 
+def _stream_of(device: int):
+    import torch
+    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+    return c_void_p(raw(device) if raw else torch.cuda.current_stream(device).cuda_stream)
+
+
 def stream_handle():
     """The current device's current stream. (By its raw handle: torch.cuda.current_stream() makes a stream object of it,
     2.7 us of the 8.8 that a small call takes on the host. The handle's function is torch's own and not promised, so a
     torch without it goes the long way.)"""
     import torch
-    raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
-    return c_void_p(raw(torch.cuda.current_device()) if raw else torch.cuda.current_stream().cuda_stream)
+    return _stream_of(torch.cuda.current_device())
 
 
 def plane_bytes(fmt: int, n: int, k: int) -> tuple[int, int]:
@@ -465,6 +470,20 @@ def _rows(tensor, head_dim: int) -> HeadRows:
     return head_rows(tensor, head_dim)
 
 
+def _launch_stream(stream, *tensors):
+    """The stream given, or the current one of the tensors' device, which has to be the current device: a call on another's
+    tensors would run on the wrong GPU."""
+    if stream is not None:
+        return stream
+    import torch
+    device = torch.cuda.current_device()
+    for tensor in tensors:
+        if tensor is not None and tensor.get_device() != device:
+            raise ValueError("the tensors lie on another device than the current one: make theirs current, or pass a stream "
+                             "of it")
+    return _stream_of(device)
+
+
 def rope_frequencies(config: RopeConfig) -> tuple[list[float], float]:
     """The pairs' radians a position, and the magnitude."""
     values, magnitude = (c_double * max(config.rotary_dim // 2, 1))(), c_float()
@@ -484,7 +503,7 @@ class RotaryPositions:
 
 def rope_add(rope: RotaryPositions, positions, input, output, head_dim: int, stream=None) -> None:
     x, y = _rows(input, head_dim), _rows(output, head_dim)
-    call("sq_rope_add", stream if stream is not None else stream_handle(), byref(rope.struct),
+    call("sq_rope_add", _launch_stream(stream, input, output, positions), byref(rope.struct),
          _whole(positions, "positions", "words"), input.shape[0], head_dim, byref(x), byref(y))
 
 
@@ -514,14 +533,14 @@ def kv_write(cache: KvCache, batch: KvBatch, keys, values, rope: RotaryPositions
     d = cache.shape.head_dim
     k, v = _rows(keys, d), _rows(values, d)
     q, r = (byref(_rows(t, d)) if t is not None else None for t in (queries, rotated))
-    call("sq_kv_add_write", stream if stream is not None else stream_handle(), byref(cache), byref(batch), byref(k),
+    call("sq_kv_add_write", _launch_stream(stream, keys, values, queries, rotated), byref(cache), byref(batch), byref(k),
          byref(v), byref(rope.struct) if rope is not None else None, q, r)
 
 
 def kv_read(cache: KvCache, batch: KvBatch, keys=None, values=None, stream=None) -> None:
     d = cache.shape.head_dim
     k, v = (byref(_rows(t, d)) if t is not None else None for t in (keys, values))
-    call("sq_kv_add_read", stream if stream is not None else stream_handle(), byref(cache), byref(batch), k, v)
+    call("sq_kv_add_read", _launch_stream(stream, keys, values), byref(cache), byref(batch), k, v)
 
 
 def attention_plan(shape: AttentionShape, sequences: int, rows: int, chunk_rows: int,
@@ -543,5 +562,5 @@ def attention_add(plan: AttentionPlan, cache: KvCache, batch: KvBatch, query, ou
                   stream=None) -> None:
     d = cache.shape.head_dim
     buffers = AttentionBuffers(_rows(query, d), _rows(output, d), view(scratch.partials))
-    call("sq_attention_add", stream if stream is not None else stream_handle(), byref(buffers), byref(cache),
+    call("sq_attention_add", _launch_stream(stream, query, output, scratch.partials), byref(buffers), byref(cache),
          byref(batch), byref(plan))

@@ -119,3 +119,38 @@ def test_the_current_stream_with_and_without_its_raw_handle(monkeypatch, raw):
     else:
         monkeypatch.delattr(torch._C, "_cuda_getCurrentRawStream", raising=False)
     assert sq.stream_handle().value == (0x4003 if raw else 0x5000)
+
+
+def test_tensors_of_another_device(monkeypatch):
+    """Without a stream of its own a call goes to the current device: tensors of another are refused, whichever they are.
+    With one they are taken (and no rows mean no launch)."""
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(sq, "_stream_of", lambda device: 0)
+    shape = sq.KvShape(2, 64, 16, sq.KV_BF16)
+    pool = device(4, 2, 16, 64, dtype=ROW)
+    cache, batch = sq.kv_cache(shape, 4, pool, pool), sq.kv_batch(device(3), device(2), device(2, 5), 0)
+    plan = sq.attention_plan(sq.AttentionShape(2, shape, 1, 0, 0.125), 2, 3, 1)
+
+    class Scratch:
+        partials = device(plan.partials, dtype=torch.uint8)
+
+    class FarScratch:
+        partials = Device(Scratch.partials.like, device=1)
+
+    here, far = (Device(torch.empty(3, 128, dtype=ROW), device=n) for n in (0, 1))
+    words = device(3)
+    calls = [lambda x, y, **kw: sq.kv_write(cache, batch, x, y, **kw),
+             lambda x, y, **kw: sq.kv_read(cache, batch, x, y, **kw),
+             lambda x, y, **kw: sq.kv_write(cache, batch, here, here, rope=Rope, queries=x, rotated=y, **kw),
+             lambda x, y, **kw: sq.attention_add(plan, cache, batch, x, y, Scratch, **kw)]
+    for run in calls:
+        run(here, here)                       # no rows: checked, and nothing launched
+        run(far, far, stream=0)
+        for x, y in ((far, here), (here, far)):
+            with pytest.raises(ValueError, match="another device"):
+                run(x, y)
+    for x, y, p in ((far, here, words), (here, far, words), (here, here, Device(words.like, device=1))):
+        with pytest.raises(ValueError, match="another device"):
+            sq.rope_add(Rope, p, x, y, 64)
+    with pytest.raises(ValueError, match="another device"):
+        sq.attention_add(plan, cache, batch, here, here, FarScratch)
