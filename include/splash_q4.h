@@ -519,8 +519,9 @@ int sq_kv_add_read(void *graph, const sq_kv_cache *cache, const sq_kv_batch *bat
  *   output = sum_j e^(scale q.k_j - max) v_j / sum_j e^(scale q.k_j - max)
  * with key/value head h / (heads / kv_heads). causal: a row sees the keys up to its own position, and with a window
  * (0: none) only the last `window` of them, its own among them; not causal: every key of its sequence. A row that sees
- * no key gets zeros. Keys that a row does not see do not touch its output, whatever they hold. heads is a multiple of
- * kv_heads, at most 64 times as many. Scores, maxima, sums and the output's accumulators are fp32; the weights e^...
+ * no key gets zeros, and so does one all of whose scores are minus infinity. Keys that a row does not see do not touch its
+ * output, whatever they hold. scale is finite, and its product with log2 e is. heads is a multiple of kv_heads, at most 64
+ * times as many. Scores, maxima, sums and the output's accumulators are fp32; the weights e^...
  * enter the matrix units as two bf16 each in tiles of 16 or 32 rows, rounded to one in those of 128, 8-bit codes exactly. */
 typedef struct sq_attention_shape {
   uint32_t heads;

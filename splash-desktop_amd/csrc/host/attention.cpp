@@ -240,12 +240,15 @@ void KvCache::addRead(hipStream_t graph, const KvCache &cache, const KvBatch &ba
   launched(kern::launch_kv_read(args, k, v, graph), "cache read");
 }
 
+float AttentionShape::exponentScale() const { return float(std::fabs(double(scale)) * std::numbers::log2e); }
+
 void AttentionShape::require() const {
   kv.require();
   if (!heads || heads % kv.kvHeads || heads / kv.kvHeads > kern::kAttendMaxGroup)
     throw std::invalid_argument("attention heads are a multiple of the key heads, at most 64 times as many");
   if (window && !causal) throw std::invalid_argument("a window takes causal attention");
   if (!std::isfinite(scale)) throw std::invalid_argument("an attention scale is finite");
+  if (!std::isfinite(exponentScale())) throw std::invalid_argument("an attention scale is finite times log2 e too");
 }
 
 AttentionPlan Attention::plan(const DeviceCapabilities &device, const AttentionShape &shape, uint32_t sequences,
@@ -301,7 +304,7 @@ void Attention::add(hipStream_t graph, const HeadRowsView &query, const HeadRows
                               shape.group(),
                               shape.causal,
                               shape.window,
-                              shape.scale == 0 ? 1.0f : float(std::fabs(double(shape.scale)) * std::numbers::log2e),
+                              shape.scale == 0 ? 1.0f : shape.exponentScale(),
                               shape.scale == 0 ? 0u : ~0u,
                               shape.scale < 0 ? 0x80008000u : 0u,
                               partials.as<float>(),

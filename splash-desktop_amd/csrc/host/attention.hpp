@@ -73,6 +73,7 @@ struct AttentionShape {
   float scale = 1;
   void require() const;
   [[nodiscard]] uint32_t group() const noexcept { return heads / kv.kvHeads; }
+  [[nodiscard]] float exponentScale() const;   // the scale's magnitude as the kernels' powers of two take it
 };
 struct AttentionPlan {
   AttentionShape shape;

@@ -78,3 +78,15 @@ def test_weights_of_few_rows(fmt, heads, kv_heads, dim, sizes, tile):
             assert np.all(err <= bound), (sizes[s], h, np.max(err / bound))
             missed += np.sum(np.abs(bf16(attend(x, k[h], v[h], 1 / math.sqrt(dim), one)[0]) - want) > bound)
     assert missed or sizes == [20001], "one rounding a weight would have kept the bound here"
+
+
+@pytest.mark.parametrize("scale,fits", [(2.3e38, True), (-2.3e38, True), (2.4e38, False), (-3.4e38, False), (1e-45, True)])
+def test_scales_whose_product_overflows(scale, fits):
+    """The exponentials are of two, their arguments scale log2 e times the products: past fp32's range that is infinite, and
+    a key that is not seen, or a product of zero, would come out as NaN."""
+    shape = sq.AttentionShape(8, sq.KvShape(2, 64, 16, sq.KV_BF16), 1, 0, scale)
+    if fits:
+        sq.attention_plan(shape, 1, 1, 1)
+    else:
+        with pytest.raises(sq.InvalidArgument, match="scale"):
+            sq.attention_plan(shape, 1, 1, 1)
