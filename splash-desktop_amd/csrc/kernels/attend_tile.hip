@@ -13,11 +13,19 @@
 // straight into LDS (the exchange is in the addresses that the lanes read from); codes pass through registers and become
 // bf16 once for all four waves, exactly. Scales multiply the scores, and the weights before they are rounded.
 //
+// The weights enter the second product as one bf16 each, half a step of which is as much as the output's own rounding: 0.0022
+// to 0.0024 from 64 bits, where two (attend_rows.hip) give 0.0017. Two make half as many products again, which nothing hides here: a chunk at 16384
+// keys takes 708 us for 518 (int8 794 for 648), prompts of 500 to 900 keys 7% more, 8 rows of heads of 256 6%.
+//
 // What it reaches: 2048 bf16 rows of 32 heads of 128 at 16384 keys of 8 in 520 us, 0.99 PFLOP/s where a large matrix product
-// of the library reaches 1.34: the matrix units are busy 54% of the cycles and the VALU (mostly the exponentials' 32 a lane
-// and tile) 50%, at clocks that the power limit holds near 1.75 GHz. The same with 8-bit pages takes 710 to 770 us (the
-// scales' and codes' VALU). Narrow heads are bound by the VALU: heads of 64 have half the products for the same
-// exponentials, 380 VALU instructions a wave and tile, issued 58% of the time (24 GFLOP of int8 prompts in 81 us).
+// of the library reaches 1.34: the matrix units are busy 53% of the cycles and the VALU (mostly the exponentials' 32 a lane
+// and tile) 48%, at clocks that the power limit holds near 1.75 GHz. The same with 8-bit pages takes 620 to 660 us (the
+// scales' and codes' VALU). Narrow heads have half the products for the same exponentials, 380 VALU instructions a wave and
+// tile, and keep neither pipe busy: 24 GFLOP of int8 prompts take 81 us, of whose cycles the VALU issues 44% and the matrix
+// units work 14%; the rest goes to the barriers and to the start of units of 17 tiles, a chain of loads that nothing covers.
+//
+// The registers are full: bf16 heads of 256 spill 13 of them (40 bytes a lane), int8 ones of 128 and 256 4 and 12 (12 and 0
+// bytes: accumulation registers hold the others), e4m3 ones 13 and 20 (40 and 24). Heads of 64 and bf16 ones of 128 none.
 //
 // Keys past the sequence's end and holes read as zeros (buffer resources end there). Only tiles that some row does not
 // see whole compare positions.
@@ -297,7 +305,7 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
     };
 
     // Infinities and NaNs among a tile's values must not reach rows that do not see them through 0 * inf: the rows that do
-    // see them add their products one by one, and they leave the tile. Only tiles that are not clear can have such rows.
+    // see them take their products apart, and they leave the tile. Only tiles that are not clear can have such rows.
     const auto set_apart = [&](int tile, int k, uint32_t holes) __attribute__((always_inline)) {
       if constexpr (kCodes) {
         // The scale of a head row that was not finite is a NaN, and all of it is.

@@ -261,16 +261,20 @@ constexpr uint32_t kAttendMaxGroup = 64;
 constexpr uint32_t kAttendNoteBytes = 16;
 uint64_t attend_partials(uint32_t tile_rows, uint32_t head_dim, uint32_t workgroups);
 // Tiles of few rows, 16 or 32, and the wide tile. The few rows' work grows with each 16 of them (their queries and
-// accumulators crowd the loads out of the registers), the wide tile costs what 128 rows cost, and the largest tile of
-// few rows that beats it is, by what both took (four sequences of 20000 keys, us with the join, few / wide):
-//   heads of 128, bf16:  32 rows 60 / 72, 64 rows 100 / 72; int8: 32 rows 47 / 73, 64 rows 84 / 73
-//   heads of 64, bf16:   32 rows 38 / 45, 64 rows 61 / 45;  int8: 32 rows 37 / 52, 64 rows 51 / 52
-//   heads of 256, int8:  16 rows 39 / 45, 32 rows 50 / 45;  bf16: 16 rows 65 / 45, but 77 / 90 for a token each of 256
-//   sequences of 300 to 600 keys, and 18 / 26 for 8 sequences of 200 to 400: the commoner calls
+// accumulators crowd the loads out of the registers), the wide tile costs what 128 rows cost. The largest tile of few rows
+// is the one that beats it in most calls, by what both take (us with the join, few / wide) over 4 sequences of 20000 keys,
+// 16 of 2000 to 8000, 64 of 300 to 600 and 8 of 200 to 400:
+//   32 rows, heads of 128:  bf16 75/77 72/76 56/39 19/27   int8 61/66 62/71 56/43 19/28   e4m3 54/67 59/71 55/44 18/28
+//   32 rows, heads of 64:   bf16 45/47 46/54 42/30 16/20   int8 43/48 44/50 41/33 15/21   e4m3 41/49 43/52 40/35 15/21
+//   16 rows, heads of 256:  bf16 69/55 68/60 62/48 26/25   int8 40/55 42/61 45/50 19/28   e4m3 39/54 41/60 43/49 17/27
+//   and a token each of 256 sequences of 300 to 600 keys:  bf16 78/91                     int8 61/94      e4m3 59/92
+// So it loses in batches of many short sequences, and with bf16 heads of 256 wherever those batches are not the largest;
+// there the most common call, a token of each of many sequences, decides. Its outputs are also the more exact ones.
 constexpr uint32_t kAttendWideRows = 128;
 constexpr uint32_t attend_few_rows(uint32_t head_dim) { return head_dim <= 128 ? 32 : 16; }
-// The workgroups (of four waves) that a compute unit holds of a tile of few rows at once: by the registers of a wave's
-// keys, values and accumulators.
+// The workgroups (of four waves) of a tile of few rows that a plan gives a compute unit. Its registers hold them: those of a
+// wave's keys, values and accumulators. (They would hold four of 16 rows at heads of 64, 127 registers a wave. Twice the
+// workgroups there take 35 us for 39 over 100000 int8 keys, and as long in bf16 and over short sequences.)
 constexpr uint32_t attend_rows_resident(uint32_t tile_rows, uint32_t head_dim, uint32_t format) {
   const uint32_t state = (head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256) * tile_rows / 16;
   return (state <= 128 ? 2 : 1) + (format != SQ_KV_BF16 ? 1 : 0);

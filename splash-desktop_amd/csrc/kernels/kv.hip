@@ -2,9 +2,18 @@
 // back. All three are bound by the bytes they move (a value in, a value out). A head row (head_dim values) is a group of
 // 8, 16 or 32 lanes of 8 values, so that its largest magnitude is a few lane exchanges away and each lane's access is one
 // 16-byte vector (8 bytes of codes). Of few rows each has a workgroup, of many a wave, four heads' loads in flight: a
-// workgroup a row of a 30000-key int8 prefix reads back in 63 us, most of it launches, a wave a row in 43 us (4.4 of the
-// 4.9 TB/s that a large copy reaches); up to 2048 rows the workgroups are as fast or faster (2048 rotated rows written in
-// 15.5 and 17.9 us). One launch of a few rows takes 3 to 6 us, its loads' round trips.
+// workgroup a row of a 30000-key int8 prefix reads back in 68 us, most of it launches, a wave a row in 45 us (4.1 of the
+// 4.9 TB/s that a large copy reaches). Both are level at some 1500 rows without a rope and 3500 with one, whatever the
+// format (written and read back, 8 heads of 128, us, workgroups / waves):
+//   rows              256        1024       2048       3000       4096       8192        30000
+//   int8              7.0/9.4    9.1/10.3   13.7/12.9  18.1/16.1  21.8/19.5  36.9/28.7   118/86
+//   bf16              6.1/7.3    8.3/8.5    12.2/11.6  15.7/14.7  18.7/17.7  32.1/27.0   126/96
+//   int8 with a rope  9.5/16.5   14.5/20.6  22.1/24.5  29.1/30.1  36.4/34.4  74.3/68.0   260/206
+// One launch of a few rows takes 3 to 6 us, its loads' round trips.
+//
+// A rope on the way rounds the keys to bf16 before they are quantised, as sq_rope_add and a write of its output would: the
+// cache then holds the same bits whichever way they came, a half step of bf16 (2^-8) against the codes' own (2^-8 of the
+// row's largest for int8, 2^-4 of the value for e4m3).
 //
 // The angles: p f / 2 pi turns in fp64, the whole turns dropped there (p f reaches 10^6 radians, where fp32 has a 16th
 // of a radian left), then sine and cosine of the fraction in fp32. A row's pairs are worked out once, by as many
