@@ -479,6 +479,14 @@ int sq_rope_add(void *graph, const sq_rope *rope, sq_buffer positions, uint32_t 
 #define SQ_KV_BF16 0u
 #define SQ_KV_INT8 1u
 #define SQ_KV_E4M3 2u
+/* Four bits (no format has the id 3): e2m1 codes, magnitudes 0, 0.5, 1, 1.5, 2, 3, 4 and 6 under a sign, two a byte, the first
+ * in its low half, so keys and values are each [pages][kv_heads][page_rows][head_dim / 2] bytes; head_dim is a multiple of 32.
+ * A group of 32 values has a scale byte b for 2^(b - 127): the least (2 to 252) under which the group's largest magnitude is
+ * at most 7. The code is that of x / scale rounded to the nearest, ties to the even code, 6 above it; a value is code * scale,
+ * exactly a bf16. A group with an infinity or NaN has byte 255 and zero codes, so all of it reads back as NaN. No write makes
+ * bytes 253 and 254, under which values past bf16's range are infinite. Scales: [pages][kv_heads][page_rows] times 2, 4 or 8
+ * bytes (head_dim up to 64, 128, 256) in the order of the groups; bytes past head_dim / 32 are 2 as written and not read. */
+#define SQ_KV_E2M1 4u
 #define SQ_KV_MAX_SEQUENCES 1024u
 typedef struct sq_kv_shape {
   uint32_t kv_heads, head_dim, page_rows, format;

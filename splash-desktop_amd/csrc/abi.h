@@ -223,4 +223,5 @@ static_assert(sizeof(SqMoeExpertLoadParams) == 192, "MoeExpertLoadParams is 192 
 #define SQ_KV_BF16 0u
 #define SQ_KV_INT8 1u
 #define SQ_KV_E4M3 2u
+#define SQ_KV_E2M1 4u
 #define SQ_KV_MAX_SEQUENCES 1024u

@@ -171,8 +171,10 @@ void KvShape::require() const {
   if (!kvHeads || kvHeads > kMaxHeads) throw std::invalid_argument("a cache has 1 to 1024 key heads");
   if (pageRows < 16 || pageRows > 1024 || (pageRows & (pageRows - 1)))
     throw std::invalid_argument("a cache's pages have a power of two of rows, 16 to 1024");
-  if (format != KvFormat::BFloat16 && format != KvFormat::Int8 && format != KvFormat::E4m3)
+  if (format != KvFormat::BFloat16 && format != KvFormat::Int8 && format != KvFormat::E4m3 && format != KvFormat::E2m1)
     throw std::invalid_argument("unknown cache format");
+  if (format == KvFormat::E2m1 && headDim % 32)
+    throw std::invalid_argument("heads of a 4-bit cache have a multiple of 32 values");
 }
 
 KvSize KvShape::bytes(uint32_t pages) const {
@@ -180,6 +182,10 @@ KvSize KvShape::bytes(uint32_t pages) const {
   if (!pages || pages == ~0u) throw std::invalid_argument("a cache has pages");
   const uint64_t rows = uint64_t{pages} * kvHeads * pageRows;
   if (format == KvFormat::BFloat16) return {rows * headDim * 2, rows * headDim * 2, 0, 0};
+  if (format == KvFormat::E2m1) {
+    const uint64_t scales = rows * (headDim <= 64 ? 2 : headDim <= 128 ? 4 : 8);
+    return {rows * headDim / 2, rows * headDim / 2, scales, scales};
+  }
   return {rows * headDim, rows * headDim, rows * 4, rows * 4};
 }
 

@@ -38,7 +38,7 @@ struct Rope {
                   const HeadRowsView &input, const HeadRowsView &output);
 };
 
-enum class KvFormat : uint32_t { BFloat16 = SQ_KV_BF16, Int8 = SQ_KV_INT8, E4m3 = SQ_KV_E4M3 };
+enum class KvFormat : uint32_t { BFloat16 = SQ_KV_BF16, Int8 = SQ_KV_INT8, E4m3 = SQ_KV_E4M3, E2m1 = SQ_KV_E2M1 };
 struct KvSize {
   uint64_t keys = 0, values = 0, keyScales = 0, valueScales = 0;
 };

@@ -69,18 +69,26 @@ struct Keys16 {
 // DIM: the head's values as computed (64, 128 or 256; values past head_dim are zero). MB: blocks of 16 rows.
 template <uint32_t FMT, int DIM, int MB>
 struct Rows {
-  static constexpr bool kCodes = FMT != SQ_KV_BF16;
-  static constexpr int kBytes = kCodes ? 1 : 2, kRun = DIM / 16, kChains = DIM / 32;
-  // Vectors a lane loads for its share of 16 keys: K 16 bytes each, V kRun values a key.
-  static constexpr int kKeyLoads = DIM * kBytes / 64, kValueWords = kRun * kBytes / 4;
+  static constexpr bool kFour = FMT == SQ_KV_E2M1;
+  static constexpr bool kScaled = FMT == SQ_KV_INT8 || FMT == SQ_KV_E4M3;   // a scale a token
+  static constexpr int kBits = kFour ? 4 : kScaled ? 8 : 16, kRun = DIM / 16, kChains = DIM / 32;
+  // Vectors a lane loads for its share of 16 keys: K 16 bytes each (heads of 64 in 4 bits: 8 of them), V kRun values a key
+  // (the same: 2 bytes).
+  static constexpr int kKeyLoads = DIM * kBits < 512 ? 1 : DIM * kBits / 512;
+  static constexpr int kValueWords = kRun * kBits < 32 ? 1 : kRun * kBits / 32;
+  static constexpr uint32_t kGroups = DIM / 32;   // scale bytes of a head row in 4 bits
+  static constexpr int kGroupWords = DIM == 64 ? 2 : 4;
+  static __device__ __forceinline__ uint32_t bytes_of(uint32_t values) { return values * kBits / 8; }
 
   struct KeyTile {
     u32x4 w[2][kKeyLoads];
     f32x4 scale[2];
+    uint32_t group[kFour ? 2 : 1][kKeyLoads];   // each vector's scale
   };
   struct ValueTile {
     uint32_t w[2][4][kValueWords];
     f32x4 scale[2];
+    uint32_t groups[kFour ? 2 : 1][kGroupWords];   // the lane's four keys' scale bytes (two keys a word: heads of 64)
   };
 
   u32x4 q[MB][kChains];
@@ -100,22 +108,42 @@ struct Rows {
   static __device__ __forceinline__ void load_keys(KeyTile &t, const KvArgs &kv, const Keys16 &k, int half,
                                                    uint32_t row_bytes, uint32_t lane) {
     const __amdgpu_buffer_rsrc_t r = buffer_rsrc(kv.keys + k.at * row_bytes, k.count * row_bytes);
+    if constexpr (kFour) {
+      // A vector is one group's (half of one's, heads of 64).
+      const __amdgpu_buffer_rsrc_t by =
+          buffer_rsrc((const uint8_t *)kv.key_scales + k.at * kGroups, k.count * kGroups);
+#pragma unroll
+      for (int j = 0; j < kKeyLoads; ++j) {
+        const uint32_t at = DIM == 64 ? 8 * (lane >> 4) : 64 * j + 16 * (lane >> 4);
+        const uint32_t from = at < row_bytes ? (lane & 15) * row_bytes + at : kNowhere;
+        if constexpr (DIM == 64) {
+          const u32x2 v = buffer_b64(r, from, 0);
+          t.w[half][j] = u32x4{v[0], v[1], 0u, 0u};
+        } else {
+          t.w[half][j] = buffer_b128(r, from, 0);
+        }
+        t.group[half][j] = buffer_b8(by, at < row_bytes ? (lane & 15) * kGroups + at / 16 : kNowhere, 0);
+      }
+      return;
+    }
 #pragma unroll
     for (int j = 0; j < kKeyLoads; ++j) {
       const uint32_t at = 64 * j + 16 * (lane >> 4);
       t.w[half][j] = buffer_b128(r, at < row_bytes ? (lane & 15) * row_bytes + at : kNowhere, 0);
     }
-    if constexpr (kCodes)
+    if constexpr (kScaled)
       t.scale[half] = __builtin_bit_cast(f32x4, buffer_b128(buffer_rsrc(kv.key_scales + k.at, k.count ? 64 : 0), 16 * (lane >> 4), 0));
   }
   static __device__ __forceinline__ void load_values(ValueTile &t, const KvArgs &kv, const Keys16 &k, int half,
                                                      uint32_t row_bytes, uint32_t lane) {
     const __amdgpu_buffer_rsrc_t r = buffer_rsrc(kv.values + k.at * row_bytes, k.count * row_bytes);
-    const uint32_t at = (lane & 15) * kRun * kBytes;
+    const uint32_t at = (lane & 15) * kRun * kBits / 8;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const uint32_t from = at < row_bytes ? (4 * (lane >> 4) + e) * row_bytes + at : kNowhere;
-      if constexpr (kValueWords == 1) {
+      if constexpr (kRun * kBits == 16) {
+        t.w[half][e][0] = buffer_b16(r, from, 0);
+      } else if constexpr (kValueWords == 1) {
         t.w[half][e][0] = buffer_b32(r, from, 0);
       } else if constexpr (kValueWords == 2) {
         const u32x2 v = buffer_b64(r, from, 0);
@@ -130,19 +158,51 @@ struct Rows {
         }
       }
     }
-    if constexpr (kCodes)
+    if constexpr (kFour) {
+      // All 16 keys' bytes are there to read (a page holds whole sixteens): those of keys past the last one belong to none.
+      const __amdgpu_buffer_rsrc_t by =
+          buffer_rsrc((const uint8_t *)kv.value_scales + k.at * kGroups, k.count ? 16 * kGroups : 0);
+      const uint32_t first = at < row_bytes ? 4 * (lane >> 4) * kGroups : kNowhere;
+      if constexpr (DIM == 64) {
+        const u32x2 v = buffer_b64(by, first, 0);
+        t.groups[half][0] = v[0];
+        t.groups[half][1] = v[1];
+      } else if constexpr (DIM == 128) {
+        const u32x4 v = buffer_b128(by, first, 0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t.groups[half][e] = v[e];
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) t.groups[half][e] = buffer_b32(by, first + kGroups * e + 4 * ((lane & 15) / 8), 0);
+      }
+    }
+    if constexpr (kScaled)
       t.scale[half] =
           __builtin_bit_cast(f32x4, buffer_b128(buffer_rsrc(kv.value_scales + k.at, k.count ? 64 : 0), 16 * (lane >> 4), 0));
   }
 
+  // The scale of half h's key 4 kq + e for the lane's values (kRun of one group).
+  static __device__ __forceinline__ uint32_t value_scale(const ValueTile &t, int h, int e, uint32_t lane) {
+    const uint32_t i = lane & 15;
+    if constexpr (DIM == 64) return fp4_scale(t.groups[h][e / 2], 2 * (e % 2) + i / 8);
+    else if constexpr (DIM == 128) return fp4_scale(t.groups[h][e], i / 4);
+    else return fp4_scale(t.groups[h][e], i / 2 % 4);
+  }
+
   // The rows' values in the K operand's order: bf16 chain j takes values 32 j + 8 kq + e; of codes, whose 16-byte vector
-  // holds 16 values, chains 2 j and 2 j + 1 take values 64 j + 16 kq + e and + 8 + e.
+  // holds 16 values, chains 2 j and 2 j + 1 take values 64 j + 16 kq + e and + 8 + e; in 4 bits, of whose 32 a vector chains
+  // 4 j to 4 j + 3 take 8 each, values 128 j + 32 kq + 8 (chain - 4 j) + e.
   static __device__ __forceinline__ uint32_t query_at(int chain, uint32_t lane) {
-    return kCodes ? 64 * (chain / 2) + 16 * (lane >> 4) + 8 * (chain % 2) : 32 * chain + 8 * (lane >> 4);
+    if constexpr (kFour)
+      return DIM == 64 ? 16 * (lane >> 4) + 8 * chain : 128 * (chain / 4) + 32 * (lane >> 4) + 8 * (chain % 4);
+    return kScaled ? 64 * (chain / 2) + 16 * (lane >> 4) + 8 * (chain % 2) : 32 * chain + 8 * (lane >> 4);
   }
 
   static __device__ __forceinline__ u32x4 key_operand(const KeyTile &t, int half, int chain) {
-    if constexpr (!kCodes) {
+    if constexpr (kFour) {
+      const uint32_t w = t.w[half][chain / 4][chain % 4], by = t.group[half][chain / 4] << 23;
+      return u32x4{fp4_pair(w, by, 0), fp4_pair(w, by, 1), fp4_pair(w, by, 2), fp4_pair(w, by, 3)};
+    } else if constexpr (!kScaled) {
       return t.w[half][chain];
     } else {
       const u32x4 w = t.w[half][chain / 2];
@@ -176,7 +236,13 @@ struct Rows {
 
   // Adds the weights' product with 32 keys' values. Two values of a run at a time. rest: what the weights lost to their
   // rounding.
-  __device__ __forceinline__ void accumulate(const ValueTile &t, const u32x4 (&p)[MB], const u32x4 (&rest)[MB]) {
+  __device__ __forceinline__ void accumulate(const ValueTile &t, const u32x4 (&p)[MB], const u32x4 (&rest)[MB], uint32_t lane) {
+    uint32_t by[2][4];
+    if constexpr (kFour)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) by[h][e] = value_scale(t, h, e, lane);
 #pragma unroll
     for (int j = 0; j < kRun / 2; ++j) {
       uint32_t w[2][4];
@@ -184,7 +250,8 @@ struct Rows {
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          if constexpr (!kCodes) w[h][e] = t.w[h][e][j];
+          if constexpr (kFour) w[h][e] = fp4_pair(t.w[h][e][j / 4], by[h][e], j % 4);
+          else if constexpr (!kScaled) w[h][e] = t.w[h][e][j];
           else w[h][e] = code_pairs4<FMT>(t.w[h][e][j / 2])[j % 2];
         }
       u32x4 even, odd;
@@ -265,6 +332,17 @@ __device__ __forceinline__ bool unbounded(const uint32_t (&w)[2][4][N]) {
   return any != 0;
 }
 
+// The same of a tile in 4 bits, by its keys' scales: whether a value may be one.
+template <typename R>
+__device__ __forceinline__ bool unbounded4(const typename R::ValueTile &t, uint32_t lane) {
+  bool any = false;
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) any |= fp4_unbounded(R::value_scale(t, h, e, lane));
+  return any;
+}
+
 template <int MB, int WAVES>
 struct Shared {
   LineShared<64 * WAVES> line;
@@ -277,7 +355,7 @@ __global__ __launch_bounds__(64 * WAVES, (WAVES == 8 ? 2 : attend_rows_resident(
 attend_rows_kernel(AttendArgs a) {
   using R = Rows<FMT, DIM, MB>;
   constexpr int kWaves = WAVES, kThreads = 64 * WAVES, kJoin = 4 * WAVES;
-  constexpr bool kCodes = R::kCodes;
+  constexpr bool kScaled = R::kScaled;
   // Accumulator t = kRun j + d of a block is value d of run j.
   constexpr int kRun = R::kRun, kRegs = 4 * kRun, kChunks = (kRegs + kJoin - 1) / kJoin;
   constexpr int kVectors = kRegs < kJoin ? kRegs / 4 : kJoin / 4;   // of four accumulators, in a chunk
@@ -287,7 +365,7 @@ attend_rows_kernel(AttendArgs a) {
   const uint32_t wave = uniform(threadIdx.x >> 6);
   const Cut cut{16 * MB / (int)a.group, (int)kAttendLeast, kUnitSlack + 256};
   const float by_group = 1.0f / (float)a.group;
-  const uint32_t dim = a.kv.head_dim, row_bytes = dim * R::kBytes;
+  const uint32_t dim = a.kv.head_dim, row_bytes = R::bytes_of(dim);
   Part next;
   Work<kThreads> work = make_work<kThreads>(a, cut, shared.line, next);
   UnitNote began{};
@@ -365,7 +443,7 @@ attend_rows_kernel(AttendArgs a) {
       f32x4 s[MB][2];
       state.scores(kt, s);
       f32x4 key_scale[2], value_scale[2];
-      if constexpr (kCodes) {
+      if constexpr (kScaled) {
         key_scale[0] = kt.scale[0] * a.scale;
         key_scale[1] = kt.scale[1] * a.scale;
         value_scale[0] = vt.scale[0];
@@ -397,7 +475,7 @@ attend_rows_kernel(AttendArgs a) {
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const float t = kCodes ? s[b][h][i] * key_scale[h][i] : s[b][h][i] * a.scale;
+            const float t = kScaled ? s[b][h][i] * key_scale[h][i] : s[b][h][i] * a.scale;
             v[4 * h + i] = clear || (seen[b] >> (4 * h + i) & 1) ? t : -INFINITY;
             top = fmaxf(top, v[4 * h + i]);
           }
@@ -416,7 +494,7 @@ attend_rows_kernel(AttendArgs a) {
           w[i] = exp2_fast(v[i] - from);
           state.l[b] += w[i];
         }
-        if constexpr (kCodes) {
+        if constexpr (kScaled) {
           // A scale past the row's keys may be anything (a NaN of its own row among it): no product with it there.
 #pragma unroll
           for (int i = 0; i < 8; ++i)
@@ -429,10 +507,15 @@ attend_rows_kernel(AttendArgs a) {
                                  fmaf(w[2 * i + 1], kMore, -__uint_as_float(p[b][i] & 0xFFFF0000u)));
         }
       }
-      if constexpr (!kCodes) {
+      if constexpr (!kScaled) {
         // Where some rows see a key and others do not, its values must not reach the others through 0 * inf: infinities
         // and NaNs leave the tile, and the rows that see them add their products one by one.
-        if (!clear && __any(unbounded<FMT>(vt.w))) {
+        bool some = false;
+        if (!clear) {
+          if constexpr (R::kFour) some = unbounded4<R>(vt, lane);
+          else some = unbounded<FMT>(vt.w);
+        }
+        if (!clear && __any(some)) {
 #pragma unroll
           for (int b = 0; b < MB; ++b)
             for (int key = 0; key < kStep; ++key) {
@@ -445,11 +528,24 @@ attend_rows_kernel(AttendArgs a) {
               const Keys16 &from = h ? kb : ka;
               const __amdgpu_buffer_rsrc_t values =
                   buffer_rsrc(a.kv.values + from.at * row_bytes, from.count * row_bytes);
+              const __amdgpu_buffer_rsrc_t groups = buffer_rsrc(
+                  (const uint8_t *)a.kv.value_scales + from.at * R::kGroups, R::kFour ? from.count * R::kGroups : 0);
 #pragma unroll
               for (int j = 0; j < 4; ++j)
 #pragma unroll
                 for (int d = 0; d < kRun; d += 2) {
                   const uint32_t at = kRun * (4 * kq + j) + d;
+                  if constexpr (R::kFour) {
+                    // All of a group under a byte above 252, of 253 and 254 the finite ones too.
+                    const uint32_t by =
+                        at < dim ? buffer_b8(groups, (key % 16) * R::kGroups + at / 32, 0) << 23 : 0u;
+                    if (sees && fp4_unbounded(by)) {
+                      const uint32_t two = fp4_pair(buffer_b8(values, (key % 16) * row_bytes + at / 2, 0), by, 0);
+                      state.o[b][d][j] += weight * bf16_to_f32(two & 0xFFFFu);
+                      state.o[b][d + 1][j] += weight * __uint_as_float(two & 0xFFFF0000u);
+                    }
+                    continue;
+                  }
                   const uint32_t two = at < dim ? buffer_b32(values, (key % 16) * row_bytes + 2 * at, 0) : 0u;
                   if (sees && (two & 0x7F80u) == 0x7F80u) state.o[b][d][j] += weight * bf16_to_f32(two & 0xFFFFu);
                   if (sees && (two & 0x7F800000u) == 0x7F800000u)
@@ -463,16 +559,32 @@ attend_rows_kernel(AttendArgs a) {
 #pragma unroll
               for (int i = 0; i < R::kValueWords; ++i) {
                 uint32_t &word = vt.w[h][e][i];
-                if ((word & 0x7F80u) == 0x7F80u) word &= 0xFFFF0000u;
-                if ((word & 0x7F800000u) == 0x7F800000u) word &= 0x0000FFFFu;
+                if constexpr (R::kFour) {
+                  if (fp4_unbounded(R::value_scale(vt, h, e, lane))) word = 0;
+                } else {
+                  if ((word & 0x7F80u) == 0x7F80u) word &= 0xFFFF0000u;
+                  if ((word & 0x7F800000u) == 0x7F800000u) word &= 0x0000FFFFu;
+                }
               }
+          if constexpr (R::kFour) {
+            // Their scales too, whichever lane's they are: a byte of zero.
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+              for (int e = 0; e < R::kGroupWords; ++e) {
+                uint32_t &word = vt.groups[h][e];
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                  if (fp4_unbounded(fp4_scale(word, g))) word &= ~(0xFFu << (8 * g));
+              }
+          }
         }
       }
       if constexpr (FMT == SQ_KV_E4M3) {
         // The same of NaN codes. (No write makes one, but pages may hold them that have not been written yet, or by another.)
         if (!clear && __any(unbounded<FMT>(vt.w))) state.take_nans(vt, seen);
       }
-      state.accumulate(vt, p, rest);
+      state.accumulate(vt, p, rest, lane);
       if (more) fetch_values(na, nb);
       ka = na;
       kb = nb;
@@ -579,6 +691,7 @@ hipError_t launch_dim(uint32_t tile_rows, uint32_t waves, const AttendArgs &a, h
 hipError_t launch_attend_rows(uint32_t tile_rows, uint32_t waves, const AttendArgs &a, hipStream_t stream) {
   if (a.kv.format == SQ_KV_BF16) return launch_dim<SQ_KV_BF16>(tile_rows, waves, a, stream);
   if (a.kv.format == SQ_KV_INT8) return launch_dim<SQ_KV_INT8>(tile_rows, waves, a, stream);
+  if (a.kv.format == SQ_KV_E2M1) return launch_dim<SQ_KV_E2M1>(tile_rows, waves, a, stream);
   return launch_dim<SQ_KV_E4M3>(tile_rows, waves, a, stream);
 }
 

@@ -98,30 +98,40 @@ struct Tile {
 template <uint32_t FMT, int DIM>
 __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void attend_tile_kernel(AttendArgs a) {
   using T = Tile<DIM>;
-  constexpr bool kCodes = FMT != SQ_KV_BF16;
-  constexpr int kSteps = DIM / 16, kBlocks = DIM / 32, kBytes = kCodes ? 1 : 2;
+  constexpr bool kFour = FMT == SQ_KV_E2M1;
+  constexpr bool kCodes = FMT != SQ_KV_BF16;   // they pass through registers
+  constexpr bool kScaled = kCodes && !kFour;   // and have a scale a token, which the tile keeps
+  constexpr int kSteps = DIM / 16, kBlocks = DIM / 32, kBits = kFour ? 4 : kCodes ? 8 : 16;
   constexpr int kBlockFloats = 32 * (DIM + 2);   // of a part in the workspace
-  // A wave fetches 16 keys of the tile, kLoads vectors a lane of K and of V.
-  constexpr int kLoads = 16 * DIM * kBytes / 1024, kRowLanes = DIM * kBytes / 16, kLoadRows = 64 / kRowLanes;
+  // A wave fetches 16 keys of the tile, kLoads vectors a lane of K and of V (of 16 bytes; of 8, heads of 64 in 4 bits).
+  constexpr int kVector = DIM * kBits < 512 ? 8 : 16, kLoads = 2 * DIM * kBits / 64 / kVector;
+  constexpr int kRowLanes = DIM * kBits / 8 / kVector, kLoadRows = 64 / kRowLanes;
+  constexpr uint32_t kGroups = DIM / 32;   // scale bytes of a head row in 4 bits
   __shared__ __attribute__((aligned(1024))) uint8_t tiles[2][2][T::kBytes];   // [tile % 2][K, V]
-  __shared__ f32x4 scales[kCodes ? 4 : 1][2][kKeyTile / 4];   // [tile % 4][K, V]
-  __shared__ u32x4 nans[FMT == SQ_KV_E4M3 ? 4 : 1];   // [tile % 4][wave]: whether its 16 keys' values hold a NaN code
+  __shared__ f32x4 scales[kScaled ? 4 : 1][2][kKeyTile / 4];   // [tile % 4][K, V]
+  // [tile % 4][wave]: whether its 16 keys' values hold a NaN code (4 bits: a scale byte above 252)
+  __shared__ u32x4 nans[FMT == SQ_KV_E4M3 || kFour ? 4 : 1];
   __shared__ LineShared<kThreads> shared;
   const uint32_t lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
   const uint32_t wave = uniform(threadIdx.x >> 6);
   const Cut cut{kRows / (int)a.group, 4 * kKeyTile, kUnitSlack + 192};
   const float by_group = 1.0f / (float)a.group;
-  const uint32_t dim = a.kv.head_dim, row_bytes = dim * kBytes;
+  const uint32_t dim = a.kv.head_dim, row_bytes = dim * kBits / 8;
   Part next;
   Work<kThreads> work = make_work<kThreads>(a, cut, shared, next);
   UnitNote began{};
 
   // Where this lane's vectors lie in 16 keys of a page, and (codes) in the LDS tile.
-  uint32_t key_from[kLoads], value_from[kLoads], code_to[kLoads];
+  uint32_t key_from[kLoads], value_from[kLoads], code_to[kLoads], group_from[kFour ? kLoads : 1];
 #pragma unroll
   for (int j = 0; j < kLoads; ++j) {
     const uint32_t k = kLoadRows * j + lane / kRowLanes, c = lane % kRowLanes;
-    if constexpr (kCodes) {
+    if constexpr (kFour) {
+      // A vector of 32 codes is a group, and four chunks of LDS, 4 c and the next (one of 16 half a group, and two of them).
+      key_from[j] = value_from[j] = kVector * c < row_bytes ? k * row_bytes + kVector * c : kNowhere;
+      group_from[j] = kVector * c < row_bytes ? k * kGroups + kVector * c / 16 : kNowhere;
+      code_to[j] = (16 * wave + k) * T::kRowBytes;
+    } else if constexpr (kCodes) {
       // A vector of 16 codes is two chunks of LDS, 2 c and 2 c + 1.
       key_from[j] = value_from[j] = 16 * c < dim ? k * row_bytes + 16 * c : kNowhere;
       code_to[j] = (16 * wave + k) * T::kRowBytes;
@@ -196,6 +206,7 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
     // them.
     u32x4 code_k[kCodes ? kLoads : 1], code_v[kCodes ? kLoads : 1];
     float code_scale[2] = {0.0f, 0.0f};
+    uint32_t group_k[kFour ? kLoads : 1], group_v[kFour ? kLoads : 1];   // the vectors' scale bytes
     const auto fetch = [&](int k, uint32_t page, int to, auto of_values) __attribute__((always_inline)) {
       constexpr bool kValues = decltype(of_values)::value;
       const int from = k + 16 * (int)wave, n = page == ~0u ? 0 : min(16, k_end - from);
@@ -203,7 +214,21 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
                            ((uint32_t)from & ((1u << a.kv.page_shift) - 1)));
       const __amdgpu_buffer_rsrc_t rows =
           buffer_rsrc((kValues ? a.kv.values : a.kv.keys) + base * row_bytes, (uint32_t)n * row_bytes);
-      if constexpr (kCodes) {
+      if constexpr (kFour) {
+        const __amdgpu_buffer_rsrc_t by = buffer_rsrc(
+            (const uint8_t *)(kValues ? a.kv.value_scales : a.kv.key_scales) + base * kGroups, (uint32_t)n * kGroups);
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+          u32x4 &v = (kValues ? code_v : code_k)[j];
+          if constexpr (kVector == 8) {
+            const u32x2 two = buffer_b64<0>(rows, key_from[j], 0);
+            v = u32x4{two[0], two[1], 0u, 0u};
+          } else {
+            v = buffer_b128<0>(rows, key_from[j], 0);
+          }
+          (kValues ? group_v : group_k)[j] = buffer_b8<0>(by, group_from[j], 0);
+        }
+      } else if constexpr (kCodes) {
 #pragma unroll
         for (int j = 0; j < kLoads; ++j)
           (kValues ? code_v : code_k)[j] = buffer_b128<0>(rows, (kValues ? value_from : key_from)[j], 0);
@@ -235,7 +260,26 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
           if (lane == 0) ((uint32_t *)&nans[tile % 4])[wave] = some;
         }
       }
-      if constexpr (kCodes) {
+      if constexpr (kFour) {
+        if constexpr (kValues)
+          if (differs(at_tile(tile))) {
+            bool any = false;
+#pragma unroll
+            for (int j = 0; j < kLoads; ++j) any |= group_v[j] > 252u;
+            const bool some = __any(any);
+            if (lane == 0) ((uint32_t *)&nans[tile % 4])[wave] = some;
+          }
+#pragma unroll
+        for (int j = 0; j < kLoads; ++j) {
+          const uint32_t k = kLoadRows * j + lane / kRowLanes, c = kVector / 4 * (lane % kRowLanes);
+          const u32x4 w = (kValues ? code_v : code_k)[j];
+          const uint32_t by = (kValues ? group_v : group_k)[j] << 23;
+#pragma unroll
+          for (int i = 0; i < kVector / 4; ++i)
+            *(u32x4 *)&tiles[tile % 2][kValues][code_to[j] + 16 * ((c + i) ^ (kValues ? T::value_swap(k) : T::key_swap(k)))] =
+                u32x4{fp4_pair(w[i], by, 0), fp4_pair(w[i], by, 1), fp4_pair(w[i], by, 2), fp4_pair(w[i], by, 3)};
+        }
+      } else if constexpr (kCodes) {
 #pragma unroll
         for (int j = 0; j < kLoads; ++j) {
           const uint32_t k = kLoadRows * j + lane / kRowLanes, c = 2 * (lane % kRowLanes);
@@ -267,7 +311,7 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
     // A tile's scores to their final form but for the exponential: scaled (codes), hidden where the row does not see the
     // key, the running maximum above all of them but kRaise.
     const auto settle = [&](int tile, int k, uint32_t holes, bool clear) __attribute__((always_inline)) {
-      if constexpr (kCodes) {
+      if constexpr (kScaled) {
 #pragma unroll
         for (int b = 0; b < 2; ++b) {
           f32x4 by[4];   // together, so that one wait serves the four
@@ -307,7 +351,12 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
     // Infinities and NaNs among a tile's values must not reach rows that do not see them through 0 * inf: the rows that do
     // see them take their products apart, and they leave the tile. Only tiles that are not clear can have such rows.
     const auto set_apart = [&](int tile, int k, uint32_t holes) __attribute__((always_inline)) {
-      if constexpr (kCodes) {
+      if constexpr (kFour) {
+        if (!differs(k)) return;
+        const u32x4 any = nans[tile % 4];
+        if (!uniform(any[0] | any[1] | any[2] | any[3])) return;
+      }
+      if constexpr (kScaled) {
         // The scale of a head row that was not finite is a NaN, and all of it is.
         float *by = (float *)scales[tile % 4][1];
         const bool bad = !(fabsf(by[lane]) < INFINITY);
@@ -345,7 +394,7 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
         }
         if (!__syncthreads_or((int)any)) return;
       }
-      if constexpr (kCodes) {
+      if constexpr (kScaled) {
         // All of them are NaNs, whatever the weights. Products of kHuge in their places and in those of keys seen, which
         // overflow, once to infinity and once below it, leave NaNs, and add zeros to all other accumulators.
         constexpr uint32_t kHuge = 0x7F00u;   // bf16's 2^127
@@ -429,7 +478,7 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
       const float from = -finite_max(m);
       float sum[2] = {0.0f, 0.0f};
       f32x4 by{}, by_next{};   // four weights' scales of values, read four weights before
-      if constexpr (kCodes) by_next = scales[tile % 4][1][h];
+      if constexpr (kScaled) by_next = scales[tile % 4][1][h];
       float even = 0.0f;
       const auto read = [&](auto index) __attribute__((always_inline)) {
         constexpr Slot at = slot(decltype(index)::value);
@@ -437,7 +486,7 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
       };
       // The weight of score i of block b.
       const auto weigh = [&](int b, int i) __attribute__((always_inline)) {
-        if constexpr (kCodes)
+        if constexpr (kScaled)
           if (i % 4 == 0) {
             by = by_next;
             const int group = 4 * b + i / 4 + 1;
@@ -445,7 +494,7 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
           }
         float v = exp2_fast(fmaf(s[b][i], a.scale, from));
         sum[i % 2] += v;
-        if constexpr (kCodes) v *= by[i % 4];
+        if constexpr (kScaled) v *= by[i % 4];
         if (i % 2) w[2 * b + i / 8][i % 8 / 2] = bf16_pair(even, v);
         else even = v;
       };
@@ -573,6 +622,7 @@ hipError_t launch_dim(const AttendArgs &a, hipStream_t stream) {
 hipError_t launch_attend_tile(const AttendArgs &a, hipStream_t stream) {
   if (a.kv.format == SQ_KV_BF16) return launch_dim<SQ_KV_BF16>(a, stream);
   if (a.kv.format == SQ_KV_INT8) return launch_dim<SQ_KV_INT8>(a, stream);
+  if (a.kv.format == SQ_KV_E2M1) return launch_dim<SQ_KV_E2M1>(a, stream);
   return launch_dim<SQ_KV_E4M3>(a, stream);
 }
 

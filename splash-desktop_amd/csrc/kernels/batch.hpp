@@ -41,4 +41,21 @@ __device__ __forceinline__ uint32_t page_of(const KvArgs &kv, uint32_t sequence,
   return page < kv.pages ? page : ~0u;
 }
 
+// Pages of 4 bits: byte `pair` (0..3) of w holds two e2m1 codes, the first in its low half; as two bf16 under a scale whose
+// exponent alone counts (the byte b of a group shifted to a float's exponent, b << 23: 2^(b - 127), and NaN for 255).
+// Exact: a code has one bit behind its first, and a product past bf16's range is infinite.
+__device__ __forceinline__ uint32_t fp4_pair(uint32_t w, uint32_t scale, int pair) {
+  const float s = __uint_as_float(scale);
+  switch (pair) {
+    case 0: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 0));
+    case 1: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 1));
+    case 2: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 2));
+    default: return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, s, 3));
+  }
+}
+// Group g's scale of a word of them.
+__device__ __forceinline__ uint32_t fp4_scale(uint32_t word, uint32_t g) { return (word >> (8 * g) & 0xFFu) << 23; }
+// Scales of bytes above 252, under which values are not finite, or may not be.
+__device__ __forceinline__ bool fp4_unbounded(uint32_t scale) { return scale > (252u << 23); }
+
 }  // namespace sq::kern

@@ -229,7 +229,7 @@ hipError_t launch_rope(const RopeArgs &rope, const uint32_t *positions, uint32_t
 // the kernels check what the row starts, lengths and page table hold.
 struct KvArgs {
   uint8_t *keys, *values;
-  float *key_scales, *value_scales;
+  float *key_scales, *value_scales;   // SQ_KV_E2M1: bytes
   const uint32_t *row_starts, *lengths, *page_table;
   uint32_t sequences, rows, pages_per_sequence, pages, page_shift, kv_heads, head_dim, format;
 };

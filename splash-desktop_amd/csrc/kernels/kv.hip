@@ -11,6 +11,10 @@
 //   int8 with a rope  9.5/16.5   14.5/20.6  22.1/24.5  29.1/30.1  36.4/34.4  74.3/68.0   260/206
 // One launch of a few rows takes 3 to 6 us, its loads' round trips.
 //
+// 4-bit pages: a group of 32 values is four lanes' and has a power of two for its scale, so that codes and values are
+// exact products, no quotients: the group's largest magnitude is two lane exchanges away, its scale an integer sum of its
+// exponent, and the conversions' own rounding (to the nearest, ties to the even code) is the format's.
+//
 // A rope on the way rounds the keys to bf16 before they are quantised, as sq_rope_add and a write of its output would: the
 // cache then holds the same bits whichever way they came, a half step of bf16 (2^-8) against the codes' own (2^-8 of the
 // row's largest for int8, 2^-4 of the value for e4m3).
@@ -170,6 +174,33 @@ __device__ __forceinline__ Codes codes8(u32x4 w) {
   return out;
 }
 
+// The same as e2m1 codes, with the scale byte of the lane's group of 32 values (four lanes). The scale is the least power of
+// two under which the group's largest value is at most 7: the largest code is 6 and the step below it 2, so no value is off
+// by more than 1 of it. Byte 252 is the largest, under which 6 is still within bf16's range, 2 the least, under which the
+// smallest code is in the normal range.
+struct Codes4 {
+  uint32_t word, scale;
+};
+__device__ __forceinline__ Codes4 codes4(u32x4 w) {
+  uint32_t largest = 0;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) largest = max(largest, max(w[e] & 0x7FFFu, (w[e] >> 16) & 0x7FFFu));
+#pragma unroll
+  for (int m = 1; m < 4; m <<= 1) largest = max(largest, (uint32_t)__shfl_xor((int)largest, m));
+  if (largest >= 0x7F80u) return {0u, 255u};
+  const int exponent = (int)(largest >> 7) - 2 + ((largest & 0x7Fu) > 0x60u ? 1 : 0);   // past 1.75 of a power of two
+  const uint32_t scale = (uint32_t)min(max(exponent, 2), 252);
+  const float by = __uint_as_float((254u - scale) << 23);
+  float x[8];
+  widen8(w, x);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] *= by;
+  uint32_t v = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(0u, x[0], x[1], 1.0f, 0);
+  v = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(v, x[2], x[3], 1.0f, 1);
+  v = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(v, x[4], x[5], 1.0f, 2);
+  return {__builtin_amdgcn_cvt_scalef32_pk_fp4_f32(v, x[6], x[7], 1.0f, 3), scale};
+}
+
 // Heads whose loads a thread has in flight.
 constexpr int kAtOnce = 4;
 
@@ -215,6 +246,11 @@ __global__ __launch_bounds__(256) void kv_write_kernel(KvArgs kv, HeadRows keys,
       const size_t at = ((((size_t)page * kv.kv_heads + h) << kv.page_shift) + slot);
       if constexpr (FMT == SQ_KV_BF16) {
         if (page != ~0u && live) *(u32x4 *)((key ? kv.keys : kv.values) + (at * dim + d) * 2) = w[i];
+      } else if constexpr (FMT == SQ_KV_E2M1) {
+        const Codes4 c = codes4(w[i]);
+        if (page == ~0u) continue;
+        if (live) *(uint32_t *)((key ? kv.keys : kv.values) + (at * dim + d) / 2) = c.word;
+        if (d % 32 == 0) ((uint8_t *)(key ? kv.key_scales : kv.value_scales))[at * (LPH / 4) + d / 32] = (uint8_t)c.scale;
       } else {
         const Codes c = codes8<FMT, LPH>(w[i]);
         if (page == ~0u) continue;
@@ -254,6 +290,9 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvArgs kv, HeadRows keys, 
       const uint8_t *from = key ? kv.keys : kv.values;
       if constexpr (FMT == SQ_KV_BF16) {
         w[i] = *(const u32x4 *)(from + (at * dim + d) * 2);
+      } else if constexpr (FMT == SQ_KV_E2M1) {
+        w[i][0] = *(const uint32_t *)(from + (at * dim + d) / 2);
+        w[i][1] = ((const uint8_t *)(key ? kv.key_scales : kv.value_scales))[at * (LPH / 4) + d / 32];
       } else {
         const u32x2 c = *(const u32x2 *)(from + at * dim + d);
         w[i][0] = c[0];
@@ -268,7 +307,10 @@ __global__ __launch_bounds__(256) void kv_read_kernel(KvArgs kv, HeadRows keys, 
       const uint32_t h = key ? u : u - kv.kv_heads;
       const HeadRows &to = key ? keys : values;
       if (u >= 2 * kv.kv_heads || !to.rows) continue;
-      if constexpr (FMT != SQ_KV_BF16) {
+      if constexpr (FMT == SQ_KV_E2M1) {
+        const uint32_t c = w[i][0], by = w[i][1] << 23;
+        w[i] = u32x4{fp4_pair(c, by, 0), fp4_pair(c, by, 1), fp4_pair(c, by, 2), fp4_pair(c, by, 3)};
+      } else if constexpr (FMT != SQ_KV_BF16) {
         float x[8];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -300,6 +342,7 @@ template <typename F>
 void with_kv_format(uint32_t format, F &&f) {
   if (format == SQ_KV_BF16) f(std::integral_constant<uint32_t, SQ_KV_BF16>{});
   else if (format == SQ_KV_INT8) f(std::integral_constant<uint32_t, SQ_KV_INT8>{});
+  else if (format == SQ_KV_E2M1) f(std::integral_constant<uint32_t, SQ_KV_E2M1>{});
   else f(std::integral_constant<uint32_t, SQ_KV_E4M3>{});
 }
 

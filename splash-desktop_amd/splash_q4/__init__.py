@@ -149,7 +149,7 @@ class MoeBuffers(Structure):
 
 ROPE_HALF, ROPE_INTERLEAVED = 0, 1
 ROPE_SCALING_NONE, ROPE_SCALING_LINEAR, ROPE_SCALING_NTK, ROPE_SCALING_YARN, ROPE_SCALING_WAVELENGTH = range(5)
-KV_BF16, KV_INT8, KV_E4M3 = 0, 1, 2
+KV_BF16, KV_INT8, KV_E4M3, KV_E2M1 = 0, 1, 2, 4
 KV_MAX_SEQUENCES = 1024
 
 
@@ -438,8 +438,10 @@ def _types(kind):
     import torch
     rows = (torch.bfloat16, torch.int16, torch.uint16)
     return {"rows": rows, "words": (torch.int32, torch.uint32), "scales": (torch.float32, torch.uint8),
+            "scale bytes": tuple(getattr(torch, n) for n in ("uint8", "float8_e8m0fnu") if hasattr(torch, n)),
             KV_BF16: (*rows, torch.uint8), KV_INT8: (torch.int8, torch.uint8),
-            KV_E4M3: (torch.float8_e4m3fn, torch.int8, torch.uint8)}[kind]
+            KV_E4M3: (torch.float8_e4m3fn, torch.int8, torch.uint8),
+            KV_E2M1: tuple(getattr(torch, n) for n in ("uint8", "int8", "float4_e2m1fn_x2") if hasattr(torch, n))}[kind]
 
 
 def _whole(tensor, what: str, kind, dims: int | None = None) -> Buffer:
@@ -514,9 +516,10 @@ def kv_cache_size(shape: KvShape, pages: int) -> KvSize:
 
 
 def kv_cache(shape: KvShape, pages: int, keys, values, key_scales=None, value_scales=None) -> KvCache:
-    if shape.format not in (KV_BF16, KV_INT8, KV_E4M3):
+    if shape.format not in (KV_BF16, KV_INT8, KV_E4M3, KV_E2M1):
         raise ValueError("unknown cache format")
-    kinds = (shape.format, shape.format, "scales", "scales")
+    scales = "scale bytes" if shape.format == KV_E2M1 else "scales"
+    kinds = (shape.format, shape.format, scales, scales)
     return KvCache(shape, pages, *(_whole(t, name, kind) if t is not None else Buffer(None, 0) for name, kind, t in
                                    zip(_KV_BUFFERS, kinds, (keys, values, key_scales, value_scales))))
 
