@@ -562,6 +562,65 @@ int sq_attention_plan_for(const sq_device *device, const sq_attention_shape *sha
  * to less than 2^52. */
 int sq_attention_add(void *graph, const sq_attention_buffers *buffers, const sq_kv_cache *cache,
                      const sq_kv_batch *batch, const sq_attention_plan *plan);
+/* What sq_attention_add_scored does to the scores t = scale q.k of a row at position p and a key at j, and to which keys the
+ * row sees; each part may be absent (cap 0, views NULL), and all of it (scores NULL: sq_attention_add).
+ *  cap       t becomes cap tanh(t / cap), off by 2^-21 of the cap (of a cap up to 128), or 2^-20 of t (of a larger one).
+ *            Finite, 2^-100 or more; the cap and |scale| / cap, each times log2 e, are finite too.
+ *  slopes    then t - slopes[h] |p - j|, fp32 [heads] on the device, 4-byte aligned.
+ *  begins    uint32 [sequences], 4-byte aligned: rows of sequence s see no key before begins[s]. Packed documents, each for
+ *            itself, are sequences of a batch that share a page table row: a document that ends at position e of them has
+ *            length e, and begins at its first key.
+ *  prefixes  uint32 [sequences], 4-byte aligned: rows of sequence s see its keys before prefixes[s] too, where they lie behind
+ *            the row. Causal attention only.
+ * A window hides what it hides of the keys seen by these. The plan is sq_attention_plan_for's. */
+typedef struct sq_attention_scores {
+  float cap;
+  sq_buffer slopes, begins, prefixes;
+} sq_attention_scores;
+int sq_attention_add_scored(void *graph, const sq_attention_buffers *buffers, const sq_kv_cache *cache,
+                            const sq_kv_batch *batch, const sq_attention_plan *plan, const sq_attention_scores *scores);
+
+/* ---- the pages of a cache ---- */
+
+/* The books of a cache's pages, on the device: how many entries of the page table name each page (references, uint32 [pages];
+ * 0: the page is free), the table (uint32 [sequences][pages_per_sequence]; a kv batch's own, or the rows that batches are made
+ * of), and the keys of each sequence (lengths, uint32 [sequences]). A call of the four below takes them from one consistent
+ * state to the next, in stream order and with no word from the host; a captured one does so at each replay. New pages are
+ * always the free ones of lowest number, in the order of the requests and of their entries, so that results repeat.
+ * An empty pool has zero references and lengths and a table of ~0u. Entries of a sequence past its keys are ~0u; an entry that
+ * names no page is a hole, shares and releases nothing.
+ * report (uint32 [4]) tells what the last call did: [0] requests not carried out, [1] pages copied, [2] (compact alone writes
+ * it) pages in use. Requests are uint32 arrays on the device, at most SQ_KV_MAX_SEQUENCES of them a call. One that names no
+ * sequence, or one that an earlier request of the call names, is not carried out; nor is one that needs new pages where too
+ * few are free for it and the requests before it. All views are 4-byte aligned; workspace (16-byte aligned, of
+ * sq_kv_pool_workspace's bytes) may hold anything before a call and serves one stream at a time. Nothing here reads or writes
+ * past the views, whatever they hold. */
+typedef struct sq_kv_pool {
+  sq_kv_cache cache;
+  uint32_t sequences, pages_per_sequence; /* sequences at most 2^20, sequences * pages_per_sequence at most 2^28 */
+  sq_buffer references, page_table, lengths, report;
+} sq_kv_pool;
+int sq_kv_pool_workspace(const sq_kv_pool *pool, uint64_t *bytes);
+/* Cuts sequence rows[i] back to keeps[i] keys (0: frees it; as many as it has or more: leaves it): entries past the kept keys'
+ * pages become holes, and a page that no entry names any more is free. A sequence may be named twice: the shorter counts. */
+int sq_kv_pool_add_release(void *graph, const sq_kv_pool *pool, sq_buffer rows, sq_buffer keeps, uint32_t requests);
+/* Makes sequence rows[i] hold more[i] keys more, which a write then fills: entries for them name new pages, and its length
+ * grows. If its last page holds keys and other entries name it too, the sequence gets a copy of it (of the rows with keys) in a
+ * new page before. A sequence that would outgrow its table row is not grown. */
+int sq_kv_pool_add_grow(void *graph, const sq_kv_pool *pool, sq_buffer rows, sq_buffer more, uint32_t requests,
+                        sq_buffer workspace);
+/* Makes sequence children[i] a fork of sequence parents[i]: the same keys, whole pages shared with it, the last page (if it
+ * is not full) a copy, of the rows with keys, in a new page that the child goes on writing. What the child's entries named
+ * before is not released. A child that is a parent of the call is not forked. */
+int sq_kv_pool_add_fork(void *graph, const sq_kv_pool *pool, sq_buffer parents, sq_buffer children, uint32_t requests,
+                        sq_buffer workspace);
+/* Moves the pages in use to the front: of n of them, the last one goes to the first free place, the one before it to the second,
+ * until all lie in places 0 to n - 1. References and table entries follow; the places left are free and keep their bits. */
+int sq_kv_pool_add_compact(void *graph, const sq_kv_pool *pool, sq_buffer workspace);
+/* Copies page pairs[2 i] of `from` to page pairs[2 i + 1] of `to` (uint32 [pairs][2] on the device, 8-byte aligned), keys,
+ * values and scales. Both caches have one shape, and may be one cache. No page is written twice, or read and written, by one
+ * call; a pair that names a page that its cache has not copies nothing. */
+int sq_kv_add_copy(void *graph, const sq_kv_cache *from, const sq_kv_cache *to, sq_buffer pairs, uint32_t count);
 
 #ifdef __cplusplus
 }

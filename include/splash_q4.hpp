@@ -36,6 +36,7 @@ using KvBatch = sq_kv_batch;
 using AttentionShape = sq_attention_shape;
 using AttentionPlan = sq_attention_plan;
 using AttentionBuffers = sq_attention_buffers;
+using AttentionScores = sq_attention_scores;
 using QuantizedSegment = sq_segment;
 using Graph = void *;   // a hipStream_t; nullptr is the default stream
 
@@ -276,6 +277,36 @@ class KvCache final {
   sq_kv_cache cache_;
 };
 
+// The books of a cache's pages, over the caller's buffers.
+class KvPool final {
+ public:
+  KvPool(const KvCache &cache, uint32_t sequences, uint32_t pagesPerSequence, Buffer references, Buffer pageTable,
+         Buffer lengths, Buffer report) noexcept
+      : pool_{cache.get(), sequences, pagesPerSequence, references, pageTable, lengths, report} {}
+  [[nodiscard]] uint64_t workspace() const {
+    uint64_t bytes = 0;
+    check(sq_kv_pool_workspace(&pool_, &bytes));
+    return bytes;
+  }
+  void addRelease(Graph graph, Buffer rows, Buffer keeps, uint32_t requests) const {
+    check(sq_kv_pool_add_release(graph, &pool_, rows, keeps, requests));
+  }
+  void addGrow(Graph graph, Buffer rows, Buffer more, uint32_t requests, Buffer workspace) const {
+    check(sq_kv_pool_add_grow(graph, &pool_, rows, more, requests, workspace));
+  }
+  void addFork(Graph graph, Buffer parents, Buffer children, uint32_t requests, Buffer workspace) const {
+    check(sq_kv_pool_add_fork(graph, &pool_, parents, children, requests, workspace));
+  }
+  void addCompact(Graph graph, Buffer workspace) const { check(sq_kv_pool_add_compact(graph, &pool_, workspace)); }
+  // Pages from[pairs[2 i]] to to[pairs[2 i + 1]].
+  static void addCopy(Graph graph, const KvCache &from, const KvCache &to, Buffer pairs, uint32_t count) {
+    check(sq_kv_add_copy(graph, &from.get(), &to.get(), pairs, count));
+  }
+
+ private:
+  sq_kv_pool pool_;
+};
+
 // Attention of a batch's new rows over the cache.
 class Attention final {
  public:
@@ -289,6 +320,11 @@ class Attention final {
   static void add(Graph graph, const AttentionBuffers &buffers, const KvCache &cache, const KvBatch &batch,
                   const AttentionPlan &plan) {
     check(sq_attention_add(graph, &buffers, &cache.get(), &batch, &plan));
+  }
+  // With capped or biased scores, or keys hidden or shown by more than causality and window.
+  static void add(Graph graph, const AttentionBuffers &buffers, const KvCache &cache, const KvBatch &batch,
+                  const AttentionPlan &plan, const AttentionScores &scores) {
+    check(sq_attention_add_scored(graph, &buffers, &cache.get(), &batch, &plan, &scores));
   }
 
  private:

@@ -4,6 +4,7 @@
 #include <numbers>
 
 #include "../kernels/kernels.hpp"
+#include "stream.hpp"
 
 namespace sq::ops {
 namespace {
@@ -11,35 +12,6 @@ namespace {
 // The most rows of a batch and the most keys a sequence's pages hold: sums of lengths over every unit of a batch stay
 // far inside 64 bits, and a position inside 32.
 constexpr uint32_t kMaxRows = 1u << 20, kMaxKeys = 1u << 30, kMaxHeads = 1024, kMaxUnits = 65536;
-
-void launched(hipError_t e, const char *what) {
-  if (e != hipSuccess) throw std::runtime_error(std::string(what) + ": " + hipGetErrorString(e));
-}
-
-// Launches go to the stream's device, whichever is current; the current one is put back.
-class OnStreamDevice {
- public:
-  explicit OnStreamDevice(hipStream_t stream) {
-    hipDevice_t device = 0;
-    int current = 0;
-    if (!stream) return;
-    launched(hipStreamGetDevice(stream, &device), "stream device");
-    launched(hipGetDevice(&current), "current device");
-    if (current == device) return;
-    launched(hipSetDevice(device), "stream device");
-    before_ = current;
-  }
-  ~OnStreamDevice() {
-    if (before_ >= 0) (void)hipSetDevice(before_);
-  }
-  OnStreamDevice(const OnStreamDevice &) = delete;
-  OnStreamDevice &operator=(const OnStreamDevice &) = delete;
-
- private:
-  int before_ = -1;
-};
-
-bool aligned(const Buffer &b, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(b.ptr) % bytes == 0; }
 
 void requireHeadDim(uint32_t dim) {
   if (!dim || dim > 256 || dim % 16)
@@ -189,7 +161,7 @@ KvSize KvShape::bytes(uint32_t pages) const {
   return {rows * headDim, rows * headDim, rows * 4, rows * 4};
 }
 
-void KvCache::require(const KvBatch &batch) const {
+void KvCache::require() const {
   const KvSize size = shape.bytes(pages);
   requireBytes(keys, size.keys, "cache keys");
   requireBytes(values, size.values, "cache values");
@@ -197,6 +169,10 @@ void KvCache::require(const KvBatch &batch) const {
   requireBytes(valueScales, size.valueScales, "cache value scales");
   if (!aligned(keys, 16) || !aligned(values, 16) || !aligned(keyScales, 16) || !aligned(valueScales, 16))
     throw std::invalid_argument("a cache's buffers are 16-byte aligned");
+}
+
+void KvCache::require(const KvBatch &batch) const {
+  require();
   if (!batch.sequences || batch.sequences > SQ_KV_MAX_SEQUENCES)
     throw std::invalid_argument("a batch has 1 to 1024 sequences");
   if (batch.rows > kMaxRows) throw std::invalid_argument("a batch has at most 2^20 rows");
@@ -284,7 +260,7 @@ AttentionPlan Attention::plan(const DeviceCapabilities &device, const AttentionS
 }
 
 void Attention::add(hipStream_t graph, const HeadRowsView &query, const HeadRowsView &output, Buffer partials,
-                    const KvCache &cache, const KvBatch &batch, const AttentionPlan &plan) {
+                    const KvCache &cache, const KvBatch &batch, const AttentionPlan &plan, const AttentionScores &scores) {
   const kern::KvArgs kv = kvArgs(cache, batch);
   const AttentionShape &shape = plan.shape;
   if (!(cache.shape == shape.kv)) throw std::invalid_argument("the attention plan is another cache's");
@@ -302,6 +278,21 @@ void Attention::add(hipStream_t graph, const HeadRowsView &query, const HeadRows
   requireInPlace(query, output, "attention");
   requireBytes(partials, plan.partials, "attention partials");
   if (!aligned(partials, 16)) throw std::invalid_argument("attention partials are 16-byte aligned");
+  if (!std::isfinite(scores.cap) || scores.cap < 0) throw std::invalid_argument("a score cap is finite, and not negative");
+  const float exponent = shape.scale == 0 ? 1.0f : shape.exponentScale();
+  const double log2e = std::numbers::log2e, cap = scores.cap;
+  if (scores.cap != 0 && (!std::isfinite(float(2 * exponent / cap)) || !std::isfinite(float(2 / cap)) ||
+                          !std::isfinite(float(cap * log2e)) || float(cap) < 0x1p-100f))
+    throw std::invalid_argument("an attention scale over its score cap, and the cap times log2 e, are finite");
+  const auto optional = [&](Buffer b, uint64_t words, const char *what) {
+    if (!b.ptr) return;
+    requireBytes(b, words * 4, what);
+    if (!aligned(b, 4)) throw std::invalid_argument(std::string(what) + " are 4-byte aligned");
+  };
+  optional(scores.slopes, shape.heads, "attention slopes");
+  optional(scores.begins, batch.sequences, "sequence begins");
+  optional(scores.prefixes, batch.sequences, "sequence prefixes");
+  if (scores.prefixes.ptr && !shape.causal) throw std::invalid_argument("prefixes take causal attention");
   const kern::AttendArgs args{kv,
                               q.rows,
                               o.rows,
@@ -310,7 +301,7 @@ void Attention::add(hipStream_t graph, const HeadRowsView &query, const HeadRows
                               shape.group(),
                               shape.causal,
                               shape.window,
-                              shape.scale == 0 ? 1.0f : shape.exponentScale(),
+                              exponent,
                               shape.scale == 0 ? 0u : ~0u,
                               shape.scale < 0 ? 0x80008000u : 0u,
                               partials.as<float>(),
@@ -321,9 +312,24 @@ void Attention::add(hipStream_t graph, const HeadRowsView &query, const HeadRows
   const bool whole = plan.tileRows != kern::kAttendWideRows && batch.sequences <= 64 && units * 4 <= plan.workgroups &&
                      keys + 384 <= kern::kAttendLeast;
   const OnStreamDevice on(graph);
-  launched(plan.tileRows == kern::kAttendWideRows ? kern::launch_attend_tile(args, graph)
-                                                  : kern::launch_attend_rows(plan.tileRows, plan.waves, args, graph),
-           "attention");
+  const bool wide = plan.tileRows == kern::kAttendWideRows;
+  if (scores.none()) {
+    launched(wide ? kern::launch_attend_tile(args, graph)
+                  : kern::launch_attend_rows(plan.tileRows, plan.waves, args, graph),
+             "attention");
+  } else {
+    const kern::ScoredArgs scored{args,
+                                  scores.slopes.as<const float>(),
+                                  scores.begins.as<const uint32_t>(),
+                                  scores.prefixes.as<const uint32_t>(),
+                                  float(cap * log2e),
+                                  cap != 0 ? float(2 / cap) : 0.0f,
+                                  cap != 0 ? float(1 / (cap * log2e)) : 0.0f,
+                                  cap > 128};
+    launched(wide ? kern::launch_attend_tile_scored(scored, graph)
+                  : kern::launch_attend_rows_scored(plan.tileRows, plan.waves, scored, graph),
+             "scored attention");
+  }
   if (!whole) launched(kern::launch_attend_join(plan.tileRows, units * 4 <= plan.workgroups, args, graph), "attention join");
 }
 

@@ -57,6 +57,7 @@ struct KvCache {
   KvShape shape;
   uint32_t pages = 0;
   Buffer keys, values, keyScales, valueScales;
+  void require() const;
   void require(const KvBatch &batch) const;
   static void addWrite(hipStream_t graph, const KvCache &cache, const KvBatch &batch, const HeadRowsView &keys,
                        const HeadRowsView &values, const Rope *rope, const HeadRowsView *queries,
@@ -80,11 +81,18 @@ struct AttentionPlan {
   uint32_t sequences = 0, rows = 0, chunkRows = 0, tileRows = 0, waves = 0, workgroups = 0;
   uint64_t partials = 0;   // bytes of workspace
 };
+// What a scored call does to scores, and which keys it hides or shows (splash_q4.h); none of it: absent.
+struct AttentionScores {
+  float cap = 0;
+  Buffer slopes, begins, prefixes;
+  [[nodiscard]] bool none() const noexcept { return cap == 0 && !slopes.ptr && !begins.ptr && !prefixes.ptr; }
+};
 struct Attention {
   static AttentionPlan plan(const DeviceCapabilities &device, const AttentionShape &shape, uint32_t sequences,
                             uint32_t rows, uint32_t chunkRows);
   static void add(hipStream_t graph, const HeadRowsView &query, const HeadRowsView &output, Buffer partials,
-                  const KvCache &cache, const KvBatch &batch, const AttentionPlan &plan);
+                  const KvCache &cache, const KvBatch &batch, const AttentionPlan &plan,
+                  const AttentionScores &scores = {});
 };
 
 }  // namespace sq::ops

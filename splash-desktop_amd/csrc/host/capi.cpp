@@ -9,6 +9,7 @@
 
 #include "../kernels/kernels.hpp"
 #include "attention.hpp"
+#include "pages.hpp"
 #include "moe.hpp"
 #include "ops.hpp"
 
@@ -634,6 +635,10 @@ AttentionShape attentionShape(const sq_attention_shape &s) {
   if (s.causal > 1) throw std::invalid_argument("attention is causal (1) or not (0)");
   return {s.heads, kvShape(s.kv), s.causal != 0, s.window, s.scale};
 }
+KvPool kvPool(const sq_kv_pool &p) {
+  return {kvCache(p.cache), p.sequences, p.pages_per_sequence, buf(p.references), buf(p.page_table), buf(p.lengths),
+          buf(p.report)};
+}
 sq_attention_plan cattention(const AttentionPlan &p) {
   sq_attention_plan out{};
   const AttentionShape &s = p.shape;
@@ -734,6 +739,55 @@ int sq_attention_add(void *graph, const sq_attention_buffers *b, const sq_kv_cac
     Attention::add(stream(graph), headRows(buffers.query), headRows(buffers.output), buf(buffers.partials),
                    kvCache(need(cache, "cache")), kvBatch(need(batch, "batch")),
                    attentionPlan(need(plan, "attention plan")));
+  });
+}
+
+int sq_attention_add_scored(void *graph, const sq_attention_buffers *b, const sq_kv_cache *cache, const sq_kv_batch *batch,
+                            const sq_attention_plan *plan, const sq_attention_scores *scores) {
+  return guarded([&] {
+    const sq_attention_buffers &buffers = need(b, "attention buffers");
+    AttentionScores s;
+    if (scores) s = {scores->cap, buf(scores->slopes), buf(scores->begins), buf(scores->prefixes)};
+    Attention::add(stream(graph), headRows(buffers.query), headRows(buffers.output), buf(buffers.partials),
+                   kvCache(need(cache, "cache")), kvBatch(need(batch, "batch")),
+                   attentionPlan(need(plan, "attention plan")), s);
+  });
+}
+
+int sq_kv_pool_workspace(const sq_kv_pool *pool, uint64_t *bytes) {
+  return guarded([&] {
+    const KvPool p = kvPool(need(pool, "pool"));
+    p.require();
+    *need(bytes, "workspace bytes") = p.workspaceBytes();
+  });
+}
+
+int sq_kv_pool_add_release(void *graph, const sq_kv_pool *pool, sq_buffer rows, sq_buffer keeps, uint32_t requests) {
+  return guarded([&] { KvPool::addRelease(stream(graph), kvPool(need(pool, "pool")), buf(rows), buf(keeps), requests); });
+}
+
+int sq_kv_pool_add_grow(void *graph, const sq_kv_pool *pool, sq_buffer rows, sq_buffer more, uint32_t requests,
+                        sq_buffer workspace) {
+  return guarded([&] {
+    KvPool::addGrow(stream(graph), kvPool(need(pool, "pool")), buf(rows), buf(more), requests, buf(workspace));
+  });
+}
+
+int sq_kv_pool_add_fork(void *graph, const sq_kv_pool *pool, sq_buffer parents, sq_buffer children, uint32_t requests,
+                        sq_buffer workspace) {
+  return guarded([&] {
+    KvPool::addFork(stream(graph), kvPool(need(pool, "pool")), buf(parents), buf(children), requests, buf(workspace));
+  });
+}
+
+int sq_kv_pool_add_compact(void *graph, const sq_kv_pool *pool, sq_buffer workspace) {
+  return guarded([&] { KvPool::addCompact(stream(graph), kvPool(need(pool, "pool")), buf(workspace)); });
+}
+
+int sq_kv_add_copy(void *graph, const sq_kv_cache *from, const sq_kv_cache *to, sq_buffer pairs, uint32_t count) {
+  return guarded([&] {
+    KvPool::addCopy(stream(graph), kvCache(need(from, "source cache")), kvCache(need(to, "target cache")), buf(pairs),
+                    count);
   });
 }
 

@@ -19,6 +19,8 @@
 //
 // Parts go to the workspace, and a second launch (attend_join.hip) joins them.
 #pragma once
+#include <type_traits>
+
 #include "batch.hpp"
 #include "device.hpp"
 
@@ -55,15 +57,52 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
 }
 __device__ __forceinline__ int64_t quotient_up(int64_t a, int64_t b) { return quotient(a + b - 1, b); }
 
+// Scored calls: where a sequence's keys begin for all of its rows, and the prefix that all of them see. A unit starts at the
+// begin at the earliest (or at the first row, where that comes first: no unit is empty) and ends at the prefix at the latest;
+// the kernel hides what lies before the begin itself.
+template <typename A>
+constexpr bool kScoredCall = std::is_same_v<A, ScoredArgs>;
+struct Bounds {
+  int begin, prefix;
+};
+struct NoBounds {};
+template <typename A>
+using BoundsOf = std::conditional_t<kScoredCall<A>, Bounds, NoBounds>;
+// A sequence of the batch with them.
+template <typename A>
+struct Member : Sequence {
+  [[no_unique_address]] BoundsOf<A> bounds;
+};
+template <typename A>
+__device__ __forceinline__ Member<A> member_of(const A &a, uint32_t s) {
+  Member<A> out{sequence_of(a.kv, s), {}};
+  if constexpr (kScoredCall<A>) {
+    if (a.begins) out.bounds.begin = (int)min(a.begins[s], (uint32_t)out.keys);
+    if (a.prefixes) out.bounds.prefix = (int)min(a.prefixes[s], (uint32_t)out.keys);
+  }
+  return out;
+}
+
 // One sequence's units.
+template <typename A>
 struct Units {
   int rows, keys, base, fit, slack, count, window;   // base: the first row's position; window 0: none
   bool causal;
+  [[no_unique_address]] BoundsOf<A> bounds;
+  // The least that a unit's end and start are.
+  __device__ __forceinline__ int least_end() const {
+    if constexpr (kScoredCall<A>) return max(1, bounds.prefix);
+    else return 1;
+  }
+  __device__ __forceinline__ int least_start() const {
+    if constexpr (kScoredCall<A>) return min(bounds.begin, max(base, 0));
+    else return 0;
+  }
   __device__ __forceinline__ int end(int m) const {
-    return causal ? max(1, base + min(rows, fit * (m + 1))) : max(1, keys);
+    return causal ? max(least_end(), base + min(rows, fit * (m + 1))) : max(1, keys);
   }
   __device__ __forceinline__ int start(int m) const {
-    return window ? max(0, base + fit * m - window + 1) : 0;
+    return window ? max(least_start(), base + fit * m - window + 1) : least_start();
   }
   __device__ __forceinline__ int first_tile(int m) const { return start(m) / kKeyTile; }
   __device__ __forceinline__ int tiles(int m) const { return (end(m) + kKeyTile - 1) / kKeyTile - first_tile(m); }
@@ -71,8 +110,8 @@ struct Units {
   // The length of units 0 .. m - 1, m < count (the last unit may have fewer rows).
   __device__ __forceinline__ int64_t before(int m) const {
     if (!causal) return (int64_t)m * length(0);
-    const int64_t starts = window ? clamped_sum(0, base - window + 1, fit, m) : 0;
-    return clamped_sum(1, base + fit, fit, m) - starts + (int64_t)slack * m;
+    const int64_t starts = window ? clamped_sum(least_start(), base - window + 1, fit, m) : (int64_t)least_start() * m;
+    return clamped_sum(least_end(), base + fit, fit, m) - starts + (int64_t)slack * m;
   }
   __device__ __forceinline__ int64_t total() const { return count ? before(count - 1) + length(count - 1) : 0; }
 };
@@ -80,24 +119,28 @@ struct Units {
 struct Cut {
   int fit, least, slack;
 };
-__device__ __forceinline__ Units units_of(const AttendArgs &a, const Sequence &q, const Cut &cut) {
+template <typename A>
+__device__ __forceinline__ Units<A> units_of(const A &a, const Member<A> &q, const Cut &cut) {
   // A window as long as the keys hides none of them; clamped, it keeps the sums in range.
   const int window = a.window && a.window < (uint32_t)q.keys ? (int)a.window : 0;
   return {(int)q.rows, q.keys, q.keys - (int)q.rows, cut.fit, cut.slack, ((int)q.rows + cut.fit - 1) / cut.fit, window,
-          a.causal != 0};
+          a.causal != 0, q.bounds};
 }
 
 // A unit's part that one workgroup runs: tiles [t0, t1) of the unit's, `parts` parts in all of which this is `part`.
+template <typename A>
 struct Part {
-  Units units;
+  Units<A> units;
   uint32_t sequence, head, first_row;   // first_row: of the sequence, in the batch
   int m, t0, t1;
   uint32_t part, parts, first_piece;    // first_piece: the workgroup's number that holds part 0
 };
 
 // p in scalar registers, whichever way it came.
-__device__ __forceinline__ Part settled(const AttendArgs &a, const Cut &cut, const Part &p) {
-  const Sequence q{uniform(p.first_row), (uint32_t)uniform(p.units.rows), uniform(p.units.keys)};
+template <typename A>
+__device__ __forceinline__ Part<A> settled(const A &a, const Cut &cut, const Part<A> &p) {
+  Member<A> q{{uniform(p.first_row), (uint32_t)uniform(p.units.rows), uniform(p.units.keys)}, {}};
+  if constexpr (kScoredCall<A>) q.bounds = {uniform(p.units.bounds.begin), uniform(p.units.bounds.prefix)};
   return {units_of(a, q, cut), uniform(p.sequence), uniform(p.head), q.first, uniform(p.m), uniform(p.t0), uniform(p.t1),
           uniform(p.part), uniform(p.parts), uniform(p.first_piece)};
 }
@@ -162,18 +205,18 @@ struct Place {
   uint32_t sequence, head;
   int m;
 };
-template <int THREADS>
+template <int THREADS, typename A>
 struct LineShared {
   int64_t prefix[kMaxSequences + 1];   // where each sequence starts
   int64_t waves[THREADS / 64];
-  Sequence sequence[kCached];
+  Member<A> sequence[kCached];
   int64_t share;
   Place place[2];
 };
 
 // A workgroup's work: one even part, or the piece of the line whose state lies in LDS between its parts (a place that every
 // wave reads and one thread writes into the other of two, so that the scalar registers are the tiles').
-template <int THREADS>
+template <int THREADS, typename A>
 struct Work {
   bool even;
   uint32_t turn;     // even: 0 until the part is run; else of the place to read, + 2 before the first part
@@ -182,7 +225,7 @@ struct Work {
 
   // The next part of the line, or false; an even part comes from make_work. A barrier of the workgroup's lies between one
   // call and the next.
-  __device__ __forceinline__ bool next(const AttendArgs &a, const Cut &cut, LineShared<THREADS> &shared, Part &p) {
+  __device__ __forceinline__ bool next(const A &a, const Cut &cut, LineShared<THREADS, A> &shared, Part<A> &p) {
     if (even) return turn++ == 0;
     const int64_t share = uniform(shared.share), total = uniform(shared.prefix[a.kv.sequences]);
     const int64_t begin = share * piece, end = begin + share < total ? begin + share : total;
@@ -207,24 +250,25 @@ struct Work {
   }
   // The notes that the join reads, once all of the workgroup's parts are stored: of the unit it began (began.parts 0:
   // none), and one workgroup's of how many there are.
-  __device__ __forceinline__ void leave(const AttendArgs &a, const UnitNote &began) const {
+  __device__ __forceinline__ void leave(const A &a, const UnitNote &began) const {
     if (threadIdx.x) return;
     if (piece < active) unit_notes(a)[piece] = began;
     if (blockIdx.x == 0) unit_notes(a)[a.workgroups].parts = active;
   }
 
  private:
-  static __device__ __forceinline__ void take(const AttendArgs &a, const Cut &cut, const LineShared<THREADS> &shared,
-                                              const Place &at, Part &p) {
-    const Sequence q = at.sequence < kCached ? shared.sequence[at.sequence] : sequence_of(a.kv, at.sequence);
-    const Sequence s{uniform(q.first), uniform(q.rows), uniform(q.keys)};
+  static __device__ __forceinline__ void take(const A &a, const Cut &cut, const LineShared<THREADS, A> &shared,
+                                              const Place &at, Part<A> &p) {
+    const Member<A> q = at.sequence < kCached ? shared.sequence[at.sequence] : member_of(a, at.sequence);
+    Member<A> s{{uniform(q.first), uniform(q.rows), uniform(q.keys)}, {}};
+    if constexpr (kScoredCall<A>) s.bounds = {uniform(q.bounds.begin), uniform(q.bounds.prefix)};
     p.units = units_of(a, s, cut);
     p.first_row = s.first;
     p.sequence = at.sequence;
   }
   // The tiles from offset `from` of unit at.m on, up to its end or the piece's, and at.x moved past them. The parts of a
   // unit are those that start at or before its last tile: a piece is at least a tile long, so each of them has one.
-  __device__ __forceinline__ void cut_at(int64_t from, int64_t share, int64_t end, Place &at, Part &p) const {
+  __device__ __forceinline__ void cut_at(int64_t from, int64_t share, int64_t end, Place &at, Part<A> &p) const {
     const int64_t length = p.units.length(at.m);
     const int64_t to = length < from + (end - at.x) ? length : from + (end - at.x);
     const int tiles = p.units.tiles(at.m);
@@ -245,8 +289,8 @@ struct Work {
     at.x += to - from;
   }
   // The first part: the unit at at.x on the line, and the offset in it.
-  static __device__ __forceinline__ int64_t enter(const AttendArgs &a, const Cut &cut, const LineShared<THREADS> &shared,
-                                                  Place &at, Part &p) {
+  static __device__ __forceinline__ int64_t enter(const A &a, const Cut &cut, const LineShared<THREADS, A> &shared,
+                                                  Place &at, Part<A> &p) {
     uint32_t lo = 0, hi = a.kv.sequences;   // the last sequence that starts at or before x
     while (hi - lo > 1) {
       const uint32_t mid = (lo + hi) / 2;
@@ -255,7 +299,7 @@ struct Work {
     }
     at.sequence = lo;
     take(a, cut, shared, at, p);
-    const Units &u = p.units;
+    const Units<A> &u = p.units;
     const int64_t one = u.total();
     int64_t rest = at.x - uniform(shared.prefix[lo]);
     at.head = (uint32_t)uniform(quotient(rest, one));
@@ -270,8 +314,8 @@ struct Work {
     return rest - u.before(mlo);
   }
   // The part after the last one: the next unit, from its start.
-  static __device__ __forceinline__ void advance(const AttendArgs &a, const Cut &cut, const LineShared<THREADS> &shared,
-                                                 Place &at, Part &p) {
+  static __device__ __forceinline__ void advance(const A &a, const Cut &cut, const LineShared<THREADS, A> &shared,
+                                                 Place &at, Part<A> &p) {
     take(a, cut, shared, at, p);
     if (++at.m < p.units.count) return;
     at.m = 0;
@@ -285,16 +329,16 @@ struct Work {
 };
 
 // Every thread of the workgroup takes part.
-template <int THREADS>
-__device__ __forceinline__ Work<THREADS> make_work(const AttendArgs &a, const Cut &cut, LineShared<THREADS> &shared,
-                                                   Part &p) {
+template <int THREADS, typename A>
+__device__ __forceinline__ Work<THREADS, A> make_work(const A &a, const Cut &cut, LineShared<THREADS, A> &shared,
+                                                      Part<A> &p) {
   constexpr int kWaves = THREADS / 64;
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, count = a.kv.sequences;
-  Work<THREADS> w{};
+  Work<THREADS, A> w{};
   if (count <= 64) {
     // Each wave for itself, a sequence a lane, in registers.
-    const Sequence q = lane < count ? sequence_of(a.kv, lane) : Sequence{0u, 0u, 0};
-    const Units u = units_of(a, q, cut);
+    const Member<A> q = lane < count ? member_of(a, lane) : Member<A>{};
+    const Units<A> u = units_of(a, q, cut);
     const float heads = (float)a.kv.kv_heads, units = (float)u.count, last = u.count ? (float)u.length(u.count - 1) : 0.0f,
                 first = u.count ? (float)u.length(0) : 0.0f;
     const float number = uniform(heads * wave_sum(units)), most = uniform(heads * wave_sum(units * last)),
@@ -322,7 +366,9 @@ __device__ __forceinline__ Work<THREADS> make_work(const AttendArgs &a, const Cu
       const uint32_t before = upto - mine;
       const uint32_t s = (uint32_t)__popcll(__ballot(before <= w.piece)) - 1;
       p.sequence = s;
-      p.units = units_of(a, Sequence{from_lane(q.first, s), from_lane(q.rows, s), from_lane(q.keys, s)}, cut);
+      Member<A> mine_of{{from_lane(q.first, s), from_lane(q.rows, s), from_lane(q.keys, s)}, {}};
+      if constexpr (kScoredCall<A>) mine_of.bounds = {from_lane(q.bounds.begin, s), from_lane(q.bounds.prefix, s)};
+      p.units = units_of(a, mine_of, cut);
       p.first_row = from_lane(q.first, s);
       p.parts = from_lane(parts, s);
       const uint32_t rest = w.piece - from_lane(before, s), unit = rest / p.parts;
@@ -343,7 +389,7 @@ __device__ __forceinline__ Work<THREADS> make_work(const AttendArgs &a, const Cu
     const uint32_t s = s0 + threadIdx.x;
     int64_t v = 0;
     if (s < count) {
-      const Sequence q = sequence_of(a.kv, s);
+      const Member<A> q = member_of(a, s);
       if (s < kCached) shared.sequence[s] = q;
       v = units_of(a, q, cut).total() * a.kv.kv_heads;
     }
@@ -409,6 +455,17 @@ __device__ __forceinline__ int row_of(int p, float by_group) { return (int)(((fl
 // 2^x by the hardware instruction (an ulp; results below the normal range flush to zero, far below any weight that
 // counts).
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+// Scores in powers of two (t = scale q.k log2 e) as a scored call has them: C tanh(t / C), C the cap times log2 e, from
+// tanh y = 1 - 2 / (1 + e^2y): an exponential, a reciprocal and three more instructions, right at both ends (e^2y infinite or
+// zero), off by C 2^-22. For caps past 128, where that would show in small scores, those below 0.3 C take the series of tanh
+// up to y^9 (the next term is 2^-24 of y there).
+__device__ __forceinline__ float capped(const ScoredArgs &a, float t) {
+  const float big = fmaf(-2.0f * a.cap, __builtin_amdgcn_rcpf(1.0f + exp2_fast(t * a.cap_by)), a.cap);
+  if (!a.cap_exact) return big;
+  const float y = t * a.cap_over, y2 = y * y;
+  const float series = fmaf(y2, fmaf(y2, fmaf(y2, fmaf(y2, 62.0f / 2835, -17.0f / 315), 2.0f / 15), -1.0f / 3), 1.0f);
+  return fabsf(y) < 0.3f ? t * series : big;
+}
 // The maximum to subtract: scores of -inf (nothing seen yet) must give weights of zero, not of NaN.
 __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.0f : m; }
 

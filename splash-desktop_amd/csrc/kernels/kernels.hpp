@@ -255,6 +255,13 @@ struct AttendArgs {
   void *notes;
   uint32_t workgroups;
 };
+// The same with scores that are capped or biased, or with keys hidden or shown by more than causality and window.
+struct ScoredArgs : AttendArgs {
+  const float *slopes;                 // a query head's; null: none
+  const uint32_t *begins, *prefixes;   // a sequence's; null: zeros
+  float cap, cap_by, cap_over;         // times log2 e (0: none), 2 / the cap, and 1 / cap
+  uint32_t cap_exact;                  // a cap so large that small scores need their own form
+};
 constexpr uint32_t kAttendMaxGroup = 64;
 // The bytes of workspace that `workgroups` workgroups on tiles of tile_rows rows use; its notes, kAttendNoteBytes a
 // workgroup and as many once more, are the last of it.
@@ -289,8 +296,10 @@ inline uint32_t attend_resident(uint32_t tile_rows, uint32_t waves, uint32_t hea
   return waves == 8 ? 1 : attend_rows_resident(tile_rows, head_dim, format);
 }
 hipError_t launch_attend_rows(uint32_t tile_rows, uint32_t waves, const AttendArgs &args, hipStream_t stream);
+hipError_t launch_attend_rows_scored(uint32_t tile_rows, uint32_t waves, const ScoredArgs &args, hipStream_t stream);
 // Tiles of kAttendWideRows rows.
 hipError_t launch_attend_tile(const AttendArgs &args, hipStream_t stream);
+hipError_t launch_attend_tile_scored(const ScoredArgs &args, hipStream_t stream);
 // The join of the parts that either left, after it. few: the batch has no more units than a quarter of the workgroups.
 hipError_t launch_attend_join(uint32_t tile_rows, bool few, const AttendArgs &args, hipStream_t stream);
 // The length (attend.hpp) up to which a batch of few units is never cut (launch_attend_rows).

@@ -200,6 +200,15 @@ class AttentionBuffers(Structure):
     _fields_ = [("query", HeadRows), ("output", HeadRows), ("partials", Buffer)]
 
 
+class AttentionScores(Structure):
+    _fields_ = [("cap", c_float)] + [(n, Buffer) for n in ("slopes", "begins", "prefixes")]
+
+
+class KvPool(Structure):
+    _fields_ = [("cache", KvCache), ("sequences", c_uint32), ("pages_per_sequence", c_uint32)] + \
+               [(n, Buffer) for n in ("references", "page_table", "lengths", "report")]
+
+
 class SqError(RuntimeError):
     def __init__(self, code: int, message: str):
         super().__init__(message)
@@ -273,6 +282,14 @@ _SIGNATURES = {
                               POINTER(AttentionPlan)],
     "sq_attention_add": [c_void_p, POINTER(AttentionBuffers), POINTER(KvCache), POINTER(KvBatch),
                          POINTER(AttentionPlan)],
+    "sq_attention_add_scored": [c_void_p, POINTER(AttentionBuffers), POINTER(KvCache), POINTER(KvBatch),
+                                POINTER(AttentionPlan), POINTER(AttentionScores)],
+    "sq_kv_pool_workspace": [POINTER(KvPool), POINTER(c_uint64)],
+    "sq_kv_pool_add_release": [c_void_p, POINTER(KvPool), Buffer, Buffer, c_uint32],
+    "sq_kv_pool_add_grow": [c_void_p, POINTER(KvPool), Buffer, Buffer, c_uint32, Buffer],
+    "sq_kv_pool_add_fork": [c_void_p, POINTER(KvPool), Buffer, Buffer, c_uint32, Buffer],
+    "sq_kv_pool_add_compact": [c_void_p, POINTER(KvPool), Buffer],
+    "sq_kv_add_copy": [c_void_p, POINTER(KvCache), POINTER(KvCache), Buffer, c_uint32],
 }
 
 
@@ -437,7 +454,7 @@ def _types(kind):
     bf16's bits. uint8: a cache's buffers as bytes, which is how kv_cache_size counts them.)"""
     import torch
     rows = (torch.bfloat16, torch.int16, torch.uint16)
-    return {"rows": rows, "words": (torch.int32, torch.uint32), "scales": (torch.float32, torch.uint8),
+    return {"rows": rows, "words": (torch.int32, torch.uint32), "slopes": (torch.float32,), "scales": (torch.float32, torch.uint8),
             "scale bytes": tuple(getattr(torch, n) for n in ("uint8", "float8_e8m0fnu") if hasattr(torch, n)),
             KV_BF16: (*rows, torch.uint8), KV_INT8: (torch.int8, torch.uint8),
             KV_E4M3: (torch.float8_e4m3fn, torch.int8, torch.uint8),
@@ -561,9 +578,78 @@ class AttentionScratch:
         self.partials = torch.empty(max(plan.partials, 16), dtype=torch.uint8, device=device_name)
 
 
+def attention_scores(cap: float = 0.0, slopes=None, begins=None, prefixes=None) -> AttentionScores:
+    """What attention_add does to scores: a cap, slopes [heads] (float32) times the distance, and for each sequence (32-bit
+    whole numbers) the first key that its rows see and the end of the prefix that all of them see."""
+    views = [_whole(t, name, kind, 1) if t is not None else Buffer(None, 0) for t, name, kind in (
+        (slopes, "slopes", "slopes"), (begins, "begins", "words"), (prefixes, "prefixes", "words"))]
+    return AttentionScores(cap, *views)
+
+
 def attention_add(plan: AttentionPlan, cache: KvCache, batch: KvBatch, query, output, scratch: AttentionScratch,
-                  stream=None) -> None:
+                  stream=None, scores: AttentionScores | None = None) -> None:
     d = cache.shape.head_dim
     buffers = AttentionBuffers(_rows(query, d), _rows(output, d), view(scratch.partials))
-    call("sq_attention_add", _launch_stream(stream, query, output, scratch.partials), byref(buffers), byref(cache),
-         byref(batch), byref(plan))
+    args = (_launch_stream(stream, query, output, scratch.partials), byref(buffers), byref(cache), byref(batch), byref(plan))
+    if scores is None:
+        call("sq_attention_add", *args)
+    else:
+        call("sq_attention_add_scored", *args, byref(scores))
+
+
+# ---------------------------------------------------------------- the pages of a cache
+
+def kv_pool(cache: KvCache, references, page_table, lengths, report) -> KvPool:
+    """The books of a cache's pages: references [pages], page_table [sequences, pages a sequence], lengths [sequences] and
+    report [4] are 32-bit whole numbers."""
+    views = [_whole(t, name, "words", dims) for t, name, dims in (
+        (references, "references", 1), (page_table, "page table", 2), (lengths, "lengths", 1), (report, "report", 1))]
+    if lengths.shape[0] != page_table.shape[0]:
+        raise ValueError("a pool has a length for each row of its table")
+    return KvPool(cache, *page_table.shape, *views)
+
+
+class KvPoolScratch:
+    """Device workspace for a pool's calls."""
+
+    def __init__(self, pool: KvPool, device_name: str = "cuda"):
+        import torch
+        size = c_uint64()
+        call("sq_kv_pool_workspace", byref(pool), byref(size))
+        self.workspace = torch.empty(size.value, dtype=torch.uint8, device=device_name)
+
+
+def _requests(first, second):
+    views = [_whole(t, "requests", "words", 1) for t in (first, second)]
+    if first.shape[0] != second.shape[0]:
+        raise ValueError("a request's two numbers come in two tensors of one length")
+    return *views, first.shape[0]
+
+
+def kv_release(pool: KvPool, rows, keeps, stream=None) -> None:
+    views = _requests(rows, keeps)
+    call("sq_kv_pool_add_release", _launch_stream(stream, rows, keeps), byref(pool), *views)
+
+
+def kv_grow(pool: KvPool, rows, more, scratch: KvPoolScratch, stream=None) -> None:
+    views = _requests(rows, more)
+    call("sq_kv_pool_add_grow", _launch_stream(stream, rows, more, scratch.workspace), byref(pool), *views,
+         view(scratch.workspace))
+
+
+def kv_fork(pool: KvPool, parents, children, scratch: KvPoolScratch, stream=None) -> None:
+    views = _requests(parents, children)
+    call("sq_kv_pool_add_fork", _launch_stream(stream, parents, children, scratch.workspace), byref(pool), *views,
+         view(scratch.workspace))
+
+
+def kv_compact(pool: KvPool, scratch: KvPoolScratch, stream=None) -> None:
+    call("sq_kv_pool_add_compact", _launch_stream(stream, scratch.workspace), byref(pool), view(scratch.workspace))
+
+
+def kv_copy(source: KvCache, target: KvCache, pairs, stream=None) -> None:
+    """Copies page pairs[i, 0] of `source` to page pairs[i, 1] of `target`, for every i."""
+    if pairs.dim() != 2 or pairs.shape[1] != 2:
+        raise ValueError("page pairs are a [pairs, 2] tensor")
+    call("sq_kv_add_copy", _launch_stream(stream, pairs), byref(source), byref(target), _whole(pairs, "page pairs", "words", 2),
+         pairs.shape[0])
