@@ -84,10 +84,10 @@ struct Rows {
   struct KeyTile {
     u32x4 w[2][kKeyLoads];
     f32x4 scale[2];
-    uint32_t group[kFour ? 2 : 1][kKeyLoads];   // each vector's scale
+    uint32_t group[kFour ? 2 : 1][kKeyLoads];   // the word with each vector's scale byte
   };
   struct ValueTile {
-    uint32_t w[2][4][kValueWords];
+    uint32_t w[2][4][kValueWords];   // (heads of 64 in 4 bits: the lane's half of it)
     f32x4 scale[2];
     uint32_t groups[kFour ? 2 : 1][kGroupWords];   // the lane's four keys' scale bytes (two keys a word: heads of 64)
   };
@@ -110,9 +110,10 @@ struct Rows {
                                                    uint32_t row_bytes, uint32_t lane) {
     const __amdgpu_buffer_rsrc_t r = buffer_rsrc(kv.keys + k.at * row_bytes, k.count * row_bytes);
     if constexpr (kFour) {
-      // A vector is one group's (half of one's, heads of 64).
+      // A vector is one group's (half of one's, heads of 64). Whole words, here and of the values: the compiler zero-extends
+      // what it loads of a byte or two at the loop's end, where it waits for it.
       const __amdgpu_buffer_rsrc_t by =
-          buffer_rsrc((const uint8_t *)kv.key_scales + k.at * kGroups, k.count * kGroups);
+          buffer_rsrc((const uint8_t *)kv.key_scales + k.at * kGroups, k.count ? 16 * kGroups : 0);
 #pragma unroll
       for (int j = 0; j < kKeyLoads; ++j) {
         const uint32_t at = DIM == 64 ? 8 * (lane >> 4) : 64 * j + 16 * (lane >> 4);
@@ -123,7 +124,7 @@ struct Rows {
         } else {
           t.w[half][j] = buffer_b128(r, from, 0);
         }
-        t.group[half][j] = buffer_b8(by, at < row_bytes ? (lane & 15) * kGroups + at / 16 : kNowhere, 0);
+        t.group[half][j] = buffer_b32(by, at < row_bytes ? ((lane & 15) * kGroups & ~3u) + 4 * j : kNowhere, 0);
       }
       return;
     }
@@ -141,9 +142,11 @@ struct Rows {
     const uint32_t at = (lane & 15) * kRun * kBits / 8;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const uint32_t from = at < row_bytes ? (4 * (lane >> 4) + e) * row_bytes + at : kNowhere;
+      uint32_t from = at < row_bytes ? (4 * (lane >> 4) + e) * row_bytes + at : kNowhere;
+      // One select for the four keys, or the compiler branches round each of these loads and waits for all of them.
+      if constexpr (kFour) from = (at < row_bytes ? 4 * (lane >> 4) * row_bytes + at : kNowhere) + e * row_bytes;
       if constexpr (kRun * kBits == 16) {
-        t.w[half][e][0] = buffer_b16(r, from, 0);
+        t.w[half][e][0] = buffer_b32(r, from & ~3u, 0);
       } else if constexpr (kValueWords == 1) {
         t.w[half][e][0] = buffer_b32(r, from, 0);
       } else if constexpr (kValueWords == 2) {
@@ -199,9 +202,14 @@ struct Rows {
     return kScaled ? 64 * (chain / 2) + 16 * (lane >> 4) + 8 * (chain % 2) : 32 * chain + 8 * (lane >> 4);
   }
 
-  static __device__ __forceinline__ u32x4 key_operand(const KeyTile &t, int half, int chain) {
+  // The scale of a lane's vector j of half h's keys.
+  static __device__ __forceinline__ uint32_t key_scale(const KeyTile &t, int h, int j, uint32_t lane) {
+    const uint32_t kq = lane >> 4;
+    return fp4_scale(t.group[h][j], DIM == 64 ? 2 * (lane & 1) + kq / 2 : kq);
+  }
+  static __device__ __forceinline__ u32x4 key_operand(const KeyTile &t, int half, int chain, uint32_t lane) {
     if constexpr (kFour) {
-      const uint32_t w = t.w[half][chain / 4][chain % 4], by = t.group[half][chain / 4] << 23;
+      const uint32_t w = t.w[half][chain / 4][chain % 4], by = key_scale(t, half, chain / 4, lane);
       return u32x4{fp4_pair(w, by, 0), fp4_pair(w, by, 1), fp4_pair(w, by, 2), fp4_pair(w, by, 3)};
     } else if constexpr (!kScaled) {
       return t.w[half][chain];
@@ -213,14 +221,14 @@ struct Rows {
   }
 
   // s = the raw products of 32 keys for block b's rows: half h's value i is key 16 h + 4 kq + i.
-  __device__ __forceinline__ void scores(const KeyTile &t, f32x4 (&s)[MB][2]) const {
+  __device__ __forceinline__ void scores(const KeyTile &t, f32x4 (&s)[MB][2], uint32_t lane) const {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
 #pragma unroll
       for (int b = 0; b < MB; ++b) s[b][h] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int c = 0; c < kChains; ++c) {
-        const u32x4 k = key_operand(t, h, c);
+        const u32x4 k = key_operand(t, h, c, lane);
 #pragma unroll
         for (int b = 0; b < MB; ++b) s[b][h] = mfma_bf16(k, q[b][c], s[b][h]);
       }
@@ -251,7 +259,7 @@ struct Rows {
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          if constexpr (kFour) w[h][e] = fp4_pair(t.w[h][e][j / 4], by[h][e], j % 4);
+          if constexpr (kFour) w[h][e] = fp4_pair(DIM == 64 ? t.w[h][e][0] >> (16 * (lane & 1)) : t.w[h][e][j / 4], by[h][e], j % 4);
           else if constexpr (!kScaled) w[h][e] = t.w[h][e][j];
           else w[h][e] = code_pairs4<FMT>(t.w[h][e][j / 2])[j % 2];
         }
@@ -415,48 +423,65 @@ attend_rows_kernel(A a) {
     }
 
     // The page of the 16 keys from k on as the table has it (~0u past the part's keys), and their place: none in a hole.
+    constexpr int kDepth = attend_rows_depth(16 * MB, DIM, FMT);   // steps in flight
     const auto page_at = [&](int k) __attribute__((always_inline)) {
+      // Several steps in flight: loads on every path alike (past the end the last key's entry, and no keys), so that a step
+      // waits for its own tile and not, as where paths with fewer loads meet, for all of them.
+      if constexpr (kDepth > 1)
+        return a.kv.page_table[(size_t)part.sequence * a.kv.pages_per_sequence +
+                               ((uint32_t)max(min(k, k_end - 1), 0) >> a.kv.page_shift)];
       return k < k_end ? a.kv.page_table[(size_t)part.sequence * a.kv.pages_per_sequence +
                                          ((uint32_t)k >> a.kv.page_shift)]
                        : ~0u;
     };
     const auto keys_at = [&](int k, uint32_t entry) __attribute__((always_inline)) {
       const uint32_t page = uniform(entry);
-      if (page >= a.kv.pages) return Keys16{0, 0u};
+      if (page >= a.kv.pages || (kDepth > 1 && k >= k_end)) return Keys16{0, 0u};
       return Keys16{(((size_t)page * a.kv.kv_heads + part.head) << a.kv.page_shift) +
                         ((uint32_t)k & ((1u << a.kv.page_shift) - 1)),
                     (uint32_t)min(16, k_end - k)};
     };
 
-    typename R::KeyTile kt;
-    typename R::ValueTile vt;
+    typename R::KeyTile kts[kDepth];
+    typename R::ValueTile vts[kDepth];
+    Keys16 kas[kDepth], kbs[kDepth];
     int k = k_begin + kStep * (int)wave;
-    const auto fetch_keys = [&](const Keys16 &ka, const Keys16 &kb) __attribute__((always_inline)) {
+    const auto fetch_keys = [&](typename R::KeyTile &kt, const Keys16 &ka, const Keys16 &kb) __attribute__((always_inline)) {
       R::load_keys(kt, a.kv, ka, 0, row_bytes, lane);
       R::load_keys(kt, a.kv, kb, 1, row_bytes, lane);
     };
-    const auto fetch_values = [&](const Keys16 &ka, const Keys16 &kb) __attribute__((always_inline)) {
+    const auto fetch_values = [&](typename R::ValueTile &vt, const Keys16 &ka, const Keys16 &kb) __attribute__((always_inline)) {
       R::load_values(vt, a.kv, ka, 0, row_bytes, lane);
       R::load_values(vt, a.kv, kb, 1, row_bytes, lane);
     };
-    // Fetches run a step ahead of the products, and the page table's entries a step ahead of the fetches.
+    // Nothing is pending here: a store to memory that the compiler takes for LDS's too, left from the last part, would make each
+    // step wait for every load.
+    if constexpr (kDepth > 1) __builtin_amdgcn_s_waitcnt(0);
+    // Fetches run kDepth steps ahead of the products, and the page table's entries a step ahead of the fetches.
     constexpr int kStride = kStep * kWaves;
     uint32_t entry_a = page_at(k), entry_b = page_at(k + 16);
-    Keys16 ka = keys_at(k, entry_a), kb = keys_at(k + 16, entry_b);
-    entry_a = page_at(k + kStride);
-    entry_b = page_at(k + kStride + 16);
-    if (k < k_end) {
-      fetch_keys(ka, kb);
-      fetch_values(ka, kb);
+#pragma unroll
+    for (int d = 0; d < kDepth; ++d) {
+      const int at = k + d * kStride;
+      kas[d] = keys_at(at, entry_a);
+      kbs[d] = keys_at(at + 16, entry_b);
+      entry_a = page_at(at + kStride);
+      entry_b = page_at(at + kStride + 16);
+      if constexpr (kDepth > 1) __builtin_amdgcn_sched_barrier(0);   // the order of loads that a step counts on
+      if (kDepth > 1 || at < k_end) {
+        fetch_keys(kts[d], kas[d], kbs[d]);
+        fetch_values(vts[d], kas[d], kbs[d]);
+      }
     }
-    for (; k < k_end; k += kStride) {
-      const bool more = k + kStride < k_end;
+    const auto step = [&](typename R::KeyTile &kt, typename R::ValueTile &vt, Keys16 &ka, Keys16 &kb)
+                          __attribute__((always_inline)) {
+      const bool more = kDepth > 1 || k + kStride < k_end;
       const uint32_t hole = (ka.count ? 0u : 1u) | (kb.count ? 0u : 2u);
-      const Keys16 na = keys_at(k + kStride, entry_a), nb = keys_at(k + kStride + 16, entry_b);
-      entry_a = page_at(k + 2 * kStride);
-      entry_b = page_at(k + 2 * kStride + 16);
+      const Keys16 na = keys_at(k + kDepth * kStride, entry_a), nb = keys_at(k + kDepth * kStride + 16, entry_b);
+      entry_a = page_at(k + (kDepth + 1) * kStride);
+      entry_b = page_at(k + (kDepth + 1) * kStride + 16);
       f32x4 s[MB][2];
-      state.scores(kt, s);
+      state.scores(kt, s, lane);
       f32x4 key_scale[2], value_scale[2];
       if constexpr (kScaled) {
         key_scale[0] = kt.scale[0] * a.scale;
@@ -464,7 +489,7 @@ attend_rows_kernel(A a) {
         value_scale[0] = vt.scale[0];
         value_scale[1] = vt.scale[1];
       }
-      if (more) fetch_keys(na, nb);
+      if (more) fetch_keys(kt, na, nb);
 
       const bool clear = k >= clear_begin && k + kStep <= clear_end && k + kStep <= k_end && !hole;
       uint32_t seen[MB];   // bit 4 h + i: key 16 h + 4 kq + i
@@ -620,9 +645,15 @@ attend_rows_kernel(A a) {
         if (!clear && __any(unbounded<FMT>(vt.w))) state.take_nans(vt, seen);
       }
       state.accumulate(vt, p, rest, lane);
-      if (more) fetch_values(na, nb);
+      if (more) fetch_values(vt, na, nb);
       ka = na;
       kb = nb;
+      k += kStride;
+    };
+    while (k < k_end) {
+#pragma unroll
+      for (int d = 0; d < kDepth; ++d)
+        if (d == 0 || k < k_end) step(kts[d], vts[d], kas[d], kbs[d]);
     }
 #pragma unroll
     for (int b = 0; b < MB; ++b) state.l[b] = row_sum(state.l[b]);

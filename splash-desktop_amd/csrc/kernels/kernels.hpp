@@ -279,10 +279,16 @@ uint64_t attend_partials(uint32_t tile_rows, uint32_t head_dim, uint32_t workgro
 // there the most common call, a token of each of many sequences, decides. Its outputs are also the more exact ones.
 constexpr uint32_t kAttendWideRows = 128;
 constexpr uint32_t attend_few_rows(uint32_t head_dim) { return head_dim <= 128 ? 32 : 16; }
+// The steps of keys and values that a wave of a tile of few rows has in flight. In 4 bits a step is too few bytes to cover a
+// round trip at the copy's rate, and its registers so few that two fit.
+constexpr uint32_t attend_rows_depth(uint32_t tile_rows, uint32_t head_dim, uint32_t format) {
+  return format == SQ_KV_E2M1 && head_dim <= 128 && tile_rows == 16 ? 2 : 1;
+}
 // The workgroups (of four waves) of a tile of few rows that a plan gives a compute unit. Its registers hold them: those of a
 // wave's keys, values and accumulators. (They would hold four of 16 rows at heads of 64, 127 registers a wave. Twice the
 // workgroups there take 35 us for 39 over 100000 int8 keys, and as long in bf16 and over short sequences.)
 constexpr uint32_t attend_rows_resident(uint32_t tile_rows, uint32_t head_dim, uint32_t format) {
+  if (attend_rows_depth(tile_rows, head_dim, format) > 1) return 2;
   const uint32_t state = (head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256) * tile_rows / 16;
   return (state <= 128 ? 2 : 1) + (format != SQ_KV_BF16 ? 1 : 0);
 }
