@@ -185,12 +185,16 @@ struct Rows {
           __builtin_bit_cast(f32x4, buffer_b128(buffer_rsrc(kv.value_scales + k.at, k.count ? 64 : 0), 16 * (lane >> 4), 0));
   }
 
-  // The scale of half h's key 4 kq + e for the lane's values (kRun of one group).
+  // Byte g of a word where fp4_pair reads it, the exponent's bits, among others that it does not: one instruction.
+  static __device__ __forceinline__ uint32_t turned(uint32_t word, uint32_t g) {
+    return __builtin_amdgcn_alignbit(word, word, 8 * g + 9);
+  }
+  // The scale of half h's key 4 kq + e for the lane's values (kRun of one group), in its place (turned) or alone.
+  template <bool TURNED = false>
   static __device__ __forceinline__ uint32_t value_scale(const ValueTile &t, int h, int e, uint32_t lane) {
-    const uint32_t i = lane & 15;
-    if constexpr (DIM == 64) return fp4_scale(t.groups[h][e / 2], 2 * (e % 2) + i / 8);
-    else if constexpr (DIM == 128) return fp4_scale(t.groups[h][e], i / 4);
-    else return fp4_scale(t.groups[h][e], i / 2 % 4);
+    const uint32_t i = lane & 15, word = t.groups[h][DIM == 64 ? e / 2 : e];
+    const uint32_t g = DIM == 64 ? 2 * (e % 2) + i / 8 : DIM == 128 ? i / 4 : i / 2 % 4;
+    return TURNED ? turned(word, g) : fp4_scale(word, g);
   }
 
   // The rows' values in the K operand's order: bf16 chain j takes values 32 j + 8 kq + e; of codes, whose 16-byte vector
@@ -205,7 +209,7 @@ struct Rows {
   // The scale of a lane's vector j of half h's keys.
   static __device__ __forceinline__ uint32_t key_scale(const KeyTile &t, int h, int j, uint32_t lane) {
     const uint32_t kq = lane >> 4;
-    return fp4_scale(t.group[h][j], DIM == 64 ? 2 * (lane & 1) + kq / 2 : kq);
+    return turned(t.group[h][j], DIM == 64 ? 2 * (lane & 1) + kq / 2 : kq);
   }
   static __device__ __forceinline__ u32x4 key_operand(const KeyTile &t, int half, int chain, uint32_t lane) {
     if constexpr (kFour) {
@@ -251,7 +255,7 @@ struct Rows {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) by[h][e] = value_scale(t, h, e, lane);
+        for (int e = 0; e < 4; ++e) by[h][e] = value_scale<true>(t, h, e, lane);
 #pragma unroll
     for (int j = 0; j < kRun / 2; ++j) {
       uint32_t w[2][4];
@@ -536,9 +540,16 @@ attend_rows_kernel(A a) {
             const float t = kScored   ? s[b][h][i]
                             : kScaled ? s[b][h][i] * key_scale[h][i]
                                       : s[b][h][i] * a.scale;
-            v[4 * h + i] = clear || (seen[b] >> (4 * h + i) & 1) ? t : -INFINITY;
-            top = fmaxf(top, v[4 * h + i]);
+            v[4 * h + i] = (R::kFour && kDepth > 1) || clear || (seen[b] >> (4 * h + i) & 1) ? t : -INFINITY;
+            if constexpr (!R::kFour || kDepth == 1) top = fmaxf(top, v[4 * h + i]);
           }
+        if constexpr (R::kFour && kDepth > 1) {   // in 4 bits the VALU counts: no selects where all keys are seen
+          if (!clear)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = seen[b] >> i & 1 ? v[i] : -INFINITY;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) top = fmaxf(top, v[i]);
+        }
         if (__any(top > state.m[b] + kRaise)) {
           const float next = fmaxf(state.m[b], row_max(top));
           const float shrink = exp2_fast(state.m[b] - finite_max(next));

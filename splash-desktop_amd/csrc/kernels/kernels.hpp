@@ -288,7 +288,7 @@ constexpr uint32_t attend_rows_depth(uint32_t tile_rows, uint32_t head_dim, uint
 // wave's keys, values and accumulators. (They would hold four of 16 rows at heads of 64, 127 registers a wave. Twice the
 // workgroups there take 35 us for 39 over 100000 int8 keys, and as long in bf16 and over short sequences.)
 constexpr uint32_t attend_rows_resident(uint32_t tile_rows, uint32_t head_dim, uint32_t format) {
-  if (attend_rows_depth(tile_rows, head_dim, format) > 1) return 2;
+  if (attend_rows_depth(tile_rows, head_dim, format) > 1) return head_dim <= 64 ? 3 : 2;
   const uint32_t state = (head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256) * tile_rows / 16;
   return (state <= 128 ? 2 : 1) + (format != SQ_KV_BF16 ? 1 : 0);
 }
