@@ -325,9 +325,11 @@ void Attention::add(hipStream_t graph, const HeadRowsView &query, const HeadRows
                                   float(cap * log2e),
                                   cap != 0 ? float(2 / cap) : 0.0f,
                                   cap != 0 ? float(1 / (cap * log2e)) : 0.0f,
-                                  cap > 128};
-    launched(wide ? kern::launch_attend_tile_scored(scored, graph)
-                  : kern::launch_attend_rows_scored(plan.tileRows, plan.waves, scored, graph),
+                                  cap > kern::kCapWithScores};
+    const bool capped = cap != 0 && cap <= kern::kCapWithScores && !scores.slopes.ptr;
+    launched(!wide ? kern::launch_attend_rows_scored(plan.tileRows, plan.waves, scored, graph)
+             : capped ? kern::launch_attend_tile_capped({scored}, graph)
+                      : kern::launch_attend_tile_scored(scored, graph),
              "scored attention");
   }
   if (!whole) launched(kern::launch_attend_join(plan.tileRows, units * 4 <= plan.workgroups, args, graph), "attention join");

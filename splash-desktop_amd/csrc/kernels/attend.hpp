@@ -61,7 +61,7 @@ __device__ __forceinline__ int64_t quotient_up(int64_t a, int64_t b) { return qu
 // begin at the earliest (or at the first row, where that comes first: no unit is empty) and ends at the prefix at the latest;
 // the kernel hides what lies before the begin itself.
 template <typename A>
-constexpr bool kScoredCall = std::is_same_v<A, ScoredArgs>;
+constexpr bool kScoredCall = std::is_base_of_v<ScoredArgs, A>;
 struct Bounds {
   int begin, prefix;
 };
@@ -457,14 +457,15 @@ __device__ __forceinline__ int row_of(int p, float by_group) { return (int)(((fl
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 // Scores in powers of two (t = scale q.k log2 e) as a scored call has them: C tanh(t / C), C the cap times log2 e, from
 // tanh y = 1 - 2 / (1 + e^2y): an exponential, a reciprocal and three more instructions, right at both ends (e^2y infinite or
-// zero), off by C 2^-22. For caps past 128, where that would show in small scores, those below 0.3 C take the series of tanh
-// up to y^9 (the next term is 2^-24 of y there).
+// zero), off by C 2^-22. Up to y = 0.4 it is also C y P(y^2), P the polynomial of degree 3 that is nearest to tanh y / y there
+// (off by 2^-23 of it): the wide tile takes it where all of a tile's scores are that small, and caps past 128, where C 2^-22
+// would show in small scores, take it for those.
+constexpr float kTanhSmall = 0.4f, kTanh0 = 0.99999988f, kTanh1 = -0.33331391f, kTanh2 = 0.13271436f, kTanh3 = -0.0475728f;
 __device__ __forceinline__ float capped(const ScoredArgs &a, float t) {
   const float big = fmaf(-2.0f * a.cap, __builtin_amdgcn_rcpf(1.0f + exp2_fast(t * a.cap_by)), a.cap);
   if (!a.cap_exact) return big;
-  const float y = t * a.cap_over, y2 = y * y;
-  const float series = fmaf(y2, fmaf(y2, fmaf(y2, fmaf(y2, 62.0f / 2835, -17.0f / 315), 2.0f / 15), -1.0f / 3), 1.0f);
-  return fabsf(y) < 0.3f ? t * series : big;
+  const float y = t * a.cap_over, z = y * y;
+  return fabsf(y) < kTanhSmall ? t * fmaf(z, fmaf(z, fmaf(z, kTanh3, kTanh2), kTanh1), kTanh0) : big;
 }
 // The maximum to subtract: scores of -inf (nothing seen yet) must give weights of zero, not of NaN.
 __device__ __forceinline__ float finite_max(float m) { return m == -INFINITY ? 0.0f : m; }

@@ -98,7 +98,9 @@ struct Tile {
 
 template <uint32_t FMT, int DIM, typename A>
 __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void attend_tile_kernel(A a) {
-  constexpr bool kScored = kScoredCall<A>;
+  constexpr bool kScored = kScoredCall<A>, kCapped = std::is_same_v<A, CappedArgs>;
+  // The score of a hidden key where a cap's polynomial passes over it: no weight, and no infinity among its products.
+  constexpr float kHidden = -1e15f;
   using T = Tile<DIM>;
   constexpr bool kFour = FMT == SQ_KV_E2M1;
   constexpr bool kCodes = FMT != SQ_KV_BF16;   // they pass through registers
@@ -177,6 +179,8 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
       if (at >= 0) high = max(high, u.bounds.prefix);
       if (on && a.slopes) slope = a.slopes[part.head * a.group + pg] * 1.44269504089f;
     }
+    [[maybe_unused]] float cap_scale = 0.0f;   // of a score as the product leaves it, to its share of the cap
+    if constexpr (kCapped) cap_scale = a.scale * a.cap_over;
     const float unit = kScored ? 1.0f : a.scale;   // what scores are still to be multiplied by once they are settled
     const bool busy = 32 * (int)wave < live;   // waves past the unit's rows only fetch
     // The page table's entries of the tile at k, lanes 0..3 those of its four 16 keys (~0u past the part's keys); and what
@@ -322,8 +326,20 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
       return u32x4{v0[0], v0[1], v1[0], v1[1]};
     };
 
+    // The running maximum above a tile's largest score but kRaise.
+    const auto raise = [&](float top) __attribute__((always_inline)) {
+      if (__any(top > m + kRaise)) {
+        const float next = fmaxf(m, other_max(top));
+        const float shrink = exp2_fast(m - finite_max(next));
+        m = next;
+        l *= shrink;
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) o[b] *= shrink;
+      }
+    };
     // A tile's scores to their final form but for the exponential: scaled (codes), hidden where the row does not see the
-    // key, the running maximum above all of them but kRaise.
+    // key, the running maximum above all of them but kRaise. Returns whether a cap is left for finish() to do (a cap keeps the
+    // order of scores, so the maximum is the largest one's).
     const auto settle = [&](int tile, int k, uint32_t holes, bool clear) __attribute__((always_inline)) {
       if constexpr (kScaled) {
 #pragma unroll
@@ -338,7 +354,23 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
       }
       if constexpr (kScored) {
         const float ahead = (float)(k + 4 * (int)h - at);   // of the lane's first key
-        if (a.cap != 0.0f) {
+        if constexpr (kCapped) {
+          if (clear) {
+            float top = s[0][0], bottom = s[0][0];
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+              for (int i = 0; i < 16; ++i) {
+                top = fmaxf(top, s[b][i]);
+                bottom = fminf(bottom, s[b][i]);
+              }
+            if (!__any(fmaxf(top, -bottom) * cap_scale > kTanhSmall)) {
+              raise(capped(a, top * a.scale));
+              return true;
+            }
+          }
+        }
+        if (kCapped || a.cap != 0.0f) {
 #pragma unroll
           for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -347,7 +379,7 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
           s[0] *= a.scale;
           s[1] *= a.scale;
         }
-        if (a.slopes) {
+        if (!kCapped && a.slopes) {
 #pragma unroll
           for (int b = 0; b < 2; ++b)
 #pragma unroll
@@ -362,7 +394,7 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
           for (int i = 0; i < 16; ++i) {
             const int key = k + 32 * b + 8 * (i / 4) + 4 * (int)h + i % 4;
             const bool sees = key >= low && key < high && !(holes >> (2 * b + i / 8) & 1);
-            s[b][i] = sees ? s[b][i] : -INFINITY;
+            s[b][i] = sees ? s[b][i] : kCapped ? kHidden : -INFINITY;
           }
       }
       float top = -INFINITY;
@@ -370,15 +402,10 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
       for (int b = 0; b < 2; ++b)
 #pragma unroll
         for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
+      if constexpr (kCapped) top = top == kHidden ? -INFINITY : top;
       if constexpr (!kScored) top *= a.scale;   // not negative (the queries carry its sign), and not zero
-      if (__any(top > m + kRaise)) {
-        const float next = fmaxf(m, other_max(top));
-        const float shrink = exp2_fast(m - finite_max(next));
-        m = next;
-        l *= shrink;
-#pragma unroll
-        for (int b = 0; b < kBlocks; ++b) o[b] *= shrink;
-      }
+      raise(top);
+      return false;
     };
 
     // Infinities and NaNs among a tile's values must not reach rows that do not see them through 0 * inf: the rows that do
@@ -495,7 +522,20 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
     // as it becomes weights. The products go out in slots, scores and values in turn, operands read from LDS kAhead slots
     // before, the second block's exponentials between the first ones' products; a barrier to the compiler's scheduling
     // keeps them so (left to itself it gathers the products, each behind a wait for its operand).
-    const auto finish = [&](int tile) __attribute__((always_inline)) {
+    // A cap of the whole call is a polynomial here, five instructions more a score, which the products partly hide (2048 rows of
+    // 16 heads of 256 at 16384 keys: %CAPPED%). Scores that are settled already go through the polynomial 1: one form
+    // of this code is what the registers hold.
+    const auto finish = [&](int tile, [[maybe_unused]] bool to_cap) __attribute__((always_inline)) {
+      [[maybe_unused]] float by_y = 1.0f, p0 = 1.0f, p1 = 0.0f, p2 = 0.0f, p3 = 0.0f;
+      if constexpr (kCapped) {
+        if (to_cap) {
+          by_y = cap_scale;
+          p0 = kTanh0 * a.cap;
+          p1 = kTanh1 * a.cap;
+          p2 = kTanh2 * a.cap;
+          p3 = kTanh3 * a.cap;
+        }
+      }
       constexpr int kSlots = 4 * kSteps, kAhead = 4;
       // Slot i's product: a score (step of a block of 32 keys), or values (16 keys into a block of 32 values).
       struct Slot {
@@ -525,7 +565,13 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
             const int group = 4 * b + i / 4 + 1;
             if (group < 8) by_next = scales[tile % 4][1][2 * group + h];
           }
-        float v = exp2_fast(fmaf(s[b][i], unit, from));
+        float v;
+        if constexpr (kCapped) {
+          const float y = s[b][i] * by_y, z = y * y;
+          v = exp2_fast(fmaf(y, fmaf(z, fmaf(z, fmaf(z, p3, p2), p1), p0), from));
+        } else {
+          v = exp2_fast(fmaf(s[b][i], unit, from));
+        }
         sum[i % 2] += v;
         if constexpr (kScaled) v *= by[i % 4];
         if (i % 2) w[2 * b + i / 8][i % 8 / 2] = bf16_pair(even, v);
@@ -596,9 +642,10 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
       }
       const uint32_t holes = pages[0].holes;
       const bool clear = k >= clear_begin && k + kKeyTile <= clear_end && k + kKeyTile <= k_end && !holes;
-      if (busy) settle(tile, k, holes, clear);
+      bool to_cap = false;
+      if (busy) to_cap = settle(tile, k, holes, clear);
       if (!clear) set_apart(tile, k, holes);
-      if (busy) finish(tile);
+      if (busy) finish(tile, to_cap);
       tile_barrier<kCodes>();
 #pragma unroll
       for (int i = 0; i < 3; ++i) pages[i] = pages[i + 1];

@@ -262,6 +262,9 @@ struct ScoredArgs : AttendArgs {
   float cap, cap_by, cap_over;         // times log2 e (0: none), 2 / the cap, and 1 / cap
   uint32_t cap_exact;                  // a cap so large that small scores need their own form
 };
+// The same where a cap of at most 128 is all that is done to scores (attend_tile.hpp).
+struct CappedArgs : ScoredArgs {};
+constexpr float kCapWithScores = 128.0f;
 constexpr uint32_t kAttendMaxGroup = 64;
 // The bytes of workspace that `workgroups` workgroups on tiles of tile_rows rows use; its notes, kAttendNoteBytes a
 // workgroup and as many once more, are the last of it.
@@ -306,6 +309,7 @@ hipError_t launch_attend_rows_scored(uint32_t tile_rows, uint32_t waves, const S
 // Tiles of kAttendWideRows rows.
 hipError_t launch_attend_tile(const AttendArgs &args, hipStream_t stream);
 hipError_t launch_attend_tile_scored(const ScoredArgs &args, hipStream_t stream);
+hipError_t launch_attend_tile_capped(const CappedArgs &args, hipStream_t stream);
 // The join of the parts that either left, after it. few: the batch has no more units than a quarter of the workgroups.
 hipError_t launch_attend_join(uint32_t tile_rows, bool few, const AttendArgs &args, hipStream_t stream);
 // The length (attend.hpp) up to which a batch of few units is never cut (launch_attend_rows).
