@@ -326,7 +326,9 @@ void Attention::add(hipStream_t graph, const HeadRowsView &query, const HeadRows
                                   cap != 0 ? float(2 / cap) : 0.0f,
                                   cap != 0 ? float(1 / (cap * log2e)) : 0.0f,
                                   cap > kern::kCapWithScores};
-    const bool capped = cap != 0 && cap <= kern::kCapWithScores && !scores.slopes.ptr;
+    // Powers up to the seventh of the score's share of the cap are normal numbers.
+    const double share = exponent / (cap * log2e);
+    const bool capped = cap != 0 && cap <= kern::kCapWithScores && !scores.slopes.ptr && share > 0x1p-15 && share < 0x1p15;
     launched(!wide ? kern::launch_attend_rows_scored(plan.tileRows, plan.waves, scored, graph)
              : capped ? kern::launch_attend_tile_capped({scored}, graph)
                       : kern::launch_attend_tile_scored(scored, graph),

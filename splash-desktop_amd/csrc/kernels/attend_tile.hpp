@@ -120,7 +120,7 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
   const uint32_t wave = uniform(threadIdx.x >> 6);
   const Cut cut{kRows / (int)a.group, 4 * kKeyTile, kUnitSlack + 192};
   const float by_group = 1.0f / (float)a.group;
-  const uint32_t dim = a.kv.head_dim, row_bytes = dim * kBits / 8;
+  const uint32_t dim = a.kv.head_dim, row_bytes = kFour ? dim / 2 : dim * (kBits / 8);
   Part<A> next;
   Work<kThreads, A> work = make_work<kThreads>(a, cut, shared, next);
   UnitNote began{};
@@ -181,7 +181,13 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
     }
     [[maybe_unused]] float cap_scale = 0.0f;   // of a score as the product leaves it, to its share of the cap
     if constexpr (kCapped) cap_scale = a.scale * a.cap_over;
-    const float unit = kScored ? 1.0f : a.scale;   // what scores are still to be multiplied by once they are settled
+    // What scores are still to be multiplied by once they are settled. Slopes are taken off scores as the product leaves them,
+    // unless a scale is so small that they would grow past all bounds.
+    float unit = a.scale;
+    if constexpr (kScored) {
+      if (a.cap != 0.0f || (a.slopes && a.scale < 0x1p-40f)) unit = 1.0f;
+      else slope = fminf(fmaxf(slope / a.scale, -0x1p127f), 0x1p127f);
+    }
     const bool busy = 32 * (int)wave < live;   // waves past the unit's rows only fetch
     // The page table's entries of the tile at k, lanes 0..3 those of its four 16 keys (~0u past the part's keys); and what
     // they say: the page of this wave's 16 keys (~0u for none), and which of the four have none.
@@ -375,7 +381,7 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
           for (int b = 0; b < 2; ++b)
 #pragma unroll
             for (int i = 0; i < 16; ++i) s[b][i] = capped(a, s[b][i] * a.scale);
-        } else {
+        } else if (unit != a.scale) {
           s[0] *= a.scale;
           s[1] *= a.scale;
         }
@@ -403,7 +409,7 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
 #pragma unroll
         for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
       if constexpr (kCapped) top = top == kHidden ? -INFINITY : top;
-      if constexpr (!kScored) top *= a.scale;   // not negative (the queries carry its sign), and not zero
+      if constexpr (!kCapped) top *= unit;   // not negative (the queries carry its sign), and not zero
       raise(top);
       return false;
     };
@@ -522,18 +528,18 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
     // as it becomes weights. The products go out in slots, scores and values in turn, operands read from LDS kAhead slots
     // before, the second block's exponentials between the first ones' products; a barrier to the compiler's scheduling
     // keeps them so (left to itself it gathers the products, each behind a wait for its operand).
-    // A cap of the whole call is a polynomial here, five instructions more a score, which the products partly hide (2048 rows of
+    // A cap of the whole call is a polynomial here, four instructions more a score, which the products partly hide (2048 rows of
     // 16 heads of 256 at 16384 keys: %CAPPED%). Scores that are settled already go through the polynomial 1: one form
     // of this code is what the registers hold.
     const auto finish = [&](int tile, [[maybe_unused]] bool to_cap) __attribute__((always_inline)) {
-      [[maybe_unused]] float by_y = 1.0f, p0 = 1.0f, p1 = 0.0f, p2 = 0.0f, p3 = 0.0f;
+      [[maybe_unused]] float p0 = 1.0f, p1 = 0.0f, p2 = 0.0f, p3 = 0.0f;
       if constexpr (kCapped) {
         if (to_cap) {
-          by_y = cap_scale;
-          p0 = kTanh0 * a.cap;
-          p1 = kTanh1 * a.cap;
-          p2 = kTanh2 * a.cap;
-          p3 = kTanh3 * a.cap;
+          const float two = cap_scale * cap_scale, four = two * two;
+          p0 = kTanh0 * a.scale;
+          p1 = kTanh1 * a.scale * two;
+          p2 = kTanh2 * a.scale * four;
+          p3 = kTanh3 * a.scale * (two * four);
         }
       }
       constexpr int kSlots = 4 * kSteps, kAhead = 4;
@@ -567,8 +573,8 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
           }
         float v;
         if constexpr (kCapped) {
-          const float y = s[b][i] * by_y, z = y * y;
-          v = exp2_fast(fmaf(y, fmaf(z, fmaf(z, fmaf(z, p3, p2), p1), p0), from));
+          const float z = s[b][i] * s[b][i];
+          v = exp2_fast(fmaf(s[b][i], fmaf(z, fmaf(z, fmaf(z, p3, p2), p1), p0), from));
         } else {
           v = exp2_fast(fmaf(s[b][i], unit, from));
         }
