@@ -181,13 +181,7 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
     }
     [[maybe_unused]] float cap_scale = 0.0f;   // of a score as the product leaves it, to its share of the cap
     if constexpr (kCapped) cap_scale = a.scale * a.cap_over;
-    // What scores are still to be multiplied by once they are settled. Slopes are taken off scores as the product leaves them,
-    // unless a scale is so small that they would grow past all bounds.
-    float unit = a.scale;
-    if constexpr (kScored) {
-      if (a.cap != 0.0f || (a.slopes && a.scale < 0x1p-40f)) unit = 1.0f;
-      else slope = fminf(fmaxf(slope / a.scale, -0x1p127f), 0x1p127f);
-    }
+    const float unit = kScored ? 1.0f : a.scale;   // what scores are still to be multiplied by once they are settled
     const bool busy = 32 * (int)wave < live;   // waves past the unit's rows only fetch
     // The page table's entries of the tile at k, lanes 0..3 those of its four 16 keys (~0u past the part's keys); and what
     // they say: the page of this wave's 16 keys (~0u for none), and which of the four have none.
@@ -358,60 +352,61 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
           for (int i = 0; i < 16; ++i) s[b][i] *= by[i / 4][i % 4];
         }
       }
-      if constexpr (kScored) {
-        const float ahead = (float)(k + 4 * (int)h - at);   // of the lane's first key
-        if constexpr (kCapped) {
-          if (clear) {
-            float top = s[0][0], bottom = s[0][0];
+      float top = -INFINITY;
+      [[maybe_unused]] bool small = false;   // all of them, of a call with a cap: the cap is finish()'s
+      if constexpr (kCapped) {
+        if (clear) {
+          float bottom = INFINITY;
+#pragma unroll
+          for (int b = 0; b < 2; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              top = fmaxf(top, s[b][i]);
+              bottom = fminf(bottom, s[b][i]);
+            }
+          small = !__any(fmaxf(top, -bottom) * cap_scale > kTanhSmall);
+          top = small ? capped(a, top * a.scale) : -INFINITY;
+        }
+      }
+      if (!small) {
+        if constexpr (kScored) {
+          const float ahead = (float)(k + 4 * (int)h - at);   // of the lane's first key
+          if (kCapped || a.cap != 0.0f) {
 #pragma unroll
             for (int b = 0; b < 2; ++b)
 #pragma unroll
-              for (int i = 0; i < 16; ++i) {
-                top = fmaxf(top, s[b][i]);
-                bottom = fminf(bottom, s[b][i]);
-              }
-            if (!__any(fmaxf(top, -bottom) * cap_scale > kTanhSmall)) {
-              raise(capped(a, top * a.scale));
-              return true;
-            }
+              for (int i = 0; i < 16; ++i) s[b][i] = capped(a, s[b][i] * a.scale);
+          } else {
+            s[0] *= a.scale;
+            s[1] *= a.scale;
+          }
+          if (!kCapped && a.slopes) {
+#pragma unroll
+            for (int b = 0; b < 2; ++b)
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                s[b][i] = fmaf(-slope, fabsf(ahead + (float)(32 * b + 8 * (i / 4) + i % 4)), s[b][i]);
           }
         }
-        if (kCapped || a.cap != 0.0f) {
+        if (!clear) {
 #pragma unroll
           for (int b = 0; b < 2; ++b)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s[b][i] = capped(a, s[b][i] * a.scale);
-        } else if (unit != a.scale) {
-          s[0] *= a.scale;
-          s[1] *= a.scale;
+            for (int i = 0; i < 16; ++i) {
+              const int key = k + 32 * b + 8 * (i / 4) + 4 * (int)h + i % 4;
+              const bool sees = key >= low && key < high && !(holes >> (2 * b + i / 8) & 1);
+              s[b][i] = sees ? s[b][i] : kCapped ? kHidden : -INFINITY;
+            }
         }
-        if (!kCapped && a.slopes) {
-#pragma unroll
-          for (int b = 0; b < 2; ++b)
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              s[b][i] = fmaf(-slope, fabsf(ahead + (float)(32 * b + 8 * (i / 4) + i % 4)), s[b][i]);
-        }
-      }
-      if (!clear) {
 #pragma unroll
         for (int b = 0; b < 2; ++b)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const int key = k + 32 * b + 8 * (i / 4) + 4 * (int)h + i % 4;
-            const bool sees = key >= low && key < high && !(holes >> (2 * b + i / 8) & 1);
-            s[b][i] = sees ? s[b][i] : kCapped ? kHidden : -INFINITY;
-          }
+          for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
+        if constexpr (kCapped) top = top == kHidden ? -INFINITY : top;
       }
-      float top = -INFINITY;
-#pragma unroll
-      for (int b = 0; b < 2; ++b)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) top = fmaxf(top, s[b][i]);
-      if constexpr (kCapped) top = top == kHidden ? -INFINITY : top;
-      if constexpr (!kCapped) top *= unit;   // not negative (the queries carry its sign), and not zero
+      if constexpr (!kScored) top *= a.scale;   // not negative (the queries carry its sign), and not zero
       raise(top);
-      return false;
+      return small;
     };
 
     // Infinities and NaNs among a tile's values must not reach rows that do not see them through 0 * inf: the rows that do
@@ -528,18 +523,22 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
     // as it becomes weights. The products go out in slots, scores and values in turn, operands read from LDS kAhead slots
     // before, the second block's exponentials between the first ones' products; a barrier to the compiler's scheduling
     // keeps them so (left to itself it gathers the products, each behind a wait for its operand).
-    // A cap of the whole call is a polynomial here, four instructions more a score, which the products partly hide (2048 rows of
-    // 16 heads of 256 at 16384 keys: %CAPPED%). Scores that are settled already go through the polynomial 1: one form
-    // of this code is what the registers hold.
+    // A call's cap is a polynomial here where the tile's scores are small, four instructions more a score, which the products
+    // partly hide (2048 rows at 16384 keys, 8 key heads: 16 heads of 256 805 us, 700 without a cap; 32 of 128 665, of 64 450).
+    // Scores that are settled go through the polynomial 1, as the registers hold no second form of this code. The share of the
+    // cap goes into the coefficients, or, one more instruction, is taken first: bf16 heads of 256 spill less so (805 for 859 us;
+    // int8 ones 974 for 961, heads of 128 680 for 665).
     const auto finish = [&](int tile, [[maybe_unused]] bool to_cap) __attribute__((always_inline)) {
-      [[maybe_unused]] float p0 = 1.0f, p1 = 0.0f, p2 = 0.0f, p3 = 0.0f;
+      constexpr bool kShareFirst = FMT == SQ_KV_BF16 && DIM == 256;
+      [[maybe_unused]] float by_y = 1.0f, p0 = 1.0f, p1 = 0.0f, p2 = 0.0f, p3 = 0.0f;
       if constexpr (kCapped) {
         if (to_cap) {
-          const float two = cap_scale * cap_scale, four = two * two;
-          p0 = kTanh0 * a.scale;
-          p1 = kTanh1 * a.scale * two;
-          p2 = kTanh2 * a.scale * four;
-          p3 = kTanh3 * a.scale * (two * four);
+          const float by = kShareFirst ? a.cap : a.scale, two = kShareFirst ? 1.0f : cap_scale * cap_scale;
+          if constexpr (kShareFirst) by_y = cap_scale;
+          p0 = kTanh0 * by;
+          p1 = kTanh1 * by * two;
+          p2 = kTanh2 * by * (two * two);
+          p3 = kTanh3 * by * (two * two * two);
         }
       }
       constexpr int kSlots = 4 * kSteps, kAhead = 4;
@@ -573,8 +572,8 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
           }
         float v;
         if constexpr (kCapped) {
-          const float z = s[b][i] * s[b][i];
-          v = exp2_fast(fmaf(s[b][i], fmaf(z, fmaf(z, fmaf(z, p3, p2), p1), p0), from));
+          const float y = kShareFirst ? s[b][i] * by_y : s[b][i], z = y * y;
+          v = exp2_fast(fmaf(y, fmaf(z, fmaf(z, fmaf(z, p3, p2), p1), p0), from));
         } else {
           v = exp2_fast(fmaf(s[b][i], unit, from));
         }
