@@ -222,11 +222,14 @@ struct Work {
   uint32_t turn;     // even: 0 until the part is run; else of the place to read, + 2 before the first part
   uint32_t piece;
   uint32_t active;   // workgroups with work
+  uint32_t units;    // dealt out whole: how many (0: not)
 
   // The next part of the line, or false; an even part comes from make_work. A barrier of the workgroup's lies between one
   // call and the next.
   __device__ __forceinline__ bool next(const A &a, const Cut &cut, LineShared<THREADS, A> &shared, Part<A> &p) {
     if (even) return turn++ == 0;
+    if constexpr (kScoredCall<A>)
+      if (units) return deal(a, cut, shared, p);
     const int64_t share = uniform(shared.share), total = uniform(shared.prefix[a.kv.sequences]);
     const int64_t begin = share * piece, end = begin + share < total ? begin + share : total;
     Place at{};
@@ -257,6 +260,29 @@ struct Work {
   }
 
  private:
+  // The next of the units that workgroups take whole, every active-th.
+  __device__ __forceinline__ bool deal(const A &a, const Cut &cut, const LineShared<THREADS, A> &shared, Part<A> &p) {
+    const uint32_t unit = piece + turn++ * active;
+    if (unit >= units) return false;
+    uint32_t lo = 0, hi = a.kv.sequences;   // the last sequence that starts at or before the unit: one with units
+    while (hi - lo > 1) {
+      const uint32_t mid = (lo + hi) / 2;
+      if (uniform(shared.prefix[mid]) <= (int64_t)unit) lo = mid;
+      else hi = mid;
+    }
+    Place at{};
+    at.sequence = lo;
+    take(a, cut, shared, at, p);
+    const uint32_t rest = unit - (uint32_t)uniform(shared.prefix[lo]);
+    p.head = rest / (uint32_t)p.units.count;
+    p.m = (int)(rest - p.head * (uint32_t)p.units.count);
+    p.t0 = 0;
+    p.t1 = p.units.tiles(p.m);
+    p.part = 0;
+    p.parts = 1;
+    p.first_piece = piece;
+    return true;
+  }
   static __device__ __forceinline__ void take(const A &a, const Cut &cut, const LineShared<THREADS, A> &shared,
                                               const Place &at, Part<A> &p) {
     const Member<A> q = at.sequence < kCached ? shared.sequence[at.sequence] : member_of(a, at.sequence);
@@ -327,6 +353,71 @@ struct Work {
     } while (!p.units.count);
   }
 };
+
+// How many units there are, where the workgroups take them whole (0: they do not), and then shared.prefix their numbers in the
+// place of their lengths. A piece of the line mostly holds two parts, each with what a unit costs besides its keys, and the
+// join reads the parts of nearly all units again; whole units leave workgroups idle behind the longest. So they stay whole
+// where the workgroup with the most has kWhole more than a piece, 2000 rows of eleven packed documents of up to 750 keys
+// (504 units of 32 heads of 128 on 512 workgroups): %WHOLE%.
+constexpr int kWhole = 640;
+template <int THREADS, typename A>
+__device__ __forceinline__ uint32_t whole_units(const A &a, const Cut &cut, LineShared<THREADS, A> &shared, int64_t share) {
+  constexpr int kWaves = THREADS / 64;
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, count = a.kv.sequences;
+  const auto units_at = [&](uint32_t s) __attribute__((always_inline)) {
+    return units_of(a, s < kCached ? shared.sequence[s] : member_of(a, s), cut);
+  };
+  // Their number and the longest, the first or the last of a sequence. (Sequences up to kCached are in LDS behind this barrier.)
+  __syncthreads();
+  int64_t number = 0;
+  int longest = 0;
+  for (uint32_t s = threadIdx.x; s < count; s += THREADS) {
+    const Units<A> u = units_at(s);
+    if (!u.count) continue;
+    number += (int64_t)u.count * a.kv.kv_heads;
+    longest = max(longest, max(u.length(0), u.length(u.count - 1)));
+  }
+  number = wave_sum(number);
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) longest = max(longest, __shfl_xor(longest, d));
+  if (lane == 0) shared.waves[wave] = number;
+  __syncthreads();
+  number = 0;
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) number += shared.waves[i];
+  __syncthreads();
+  if (lane == 0) shared.waves[wave] = longest;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kWaves; ++i) longest = max(longest, (int)shared.waves[i]);
+  number = uniform(number);
+  longest = uniform(longest);
+  const int64_t rounds = (number + a.workgroups - 1) / a.workgroups;
+  if (!number || number > 8 * (int64_t)a.workgroups || rounds * longest > share + kWhole) return 0;
+  int64_t carry = 0;
+  for (uint32_t s0 = 0; s0 < count; s0 += THREADS) {
+    const uint32_t s = s0 + threadIdx.x;
+    int64_t v = s < count ? (int64_t)units_at(s).count * a.kv.kv_heads : 0;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int64_t below = __shfl_up(v, d);
+      if (lane >= (uint32_t)d) v += below;
+    }
+    __syncthreads();   // the last sums have been read
+    if (lane == 63) shared.waves[wave] = v;
+    __syncthreads();
+    int64_t all = 0;
+#pragma unroll
+    for (int i = 0; i < kWaves; ++i) {
+      if ((uint32_t)i < wave) v += shared.waves[i];
+      all += shared.waves[i];
+    }
+    if (s < count) shared.prefix[s + 1] = carry + v;   // prefix[0] is 0
+    carry += all;
+  }
+  __syncthreads();
+  return (uint32_t)number;
+}
 
 // Every thread of the workgroup takes part.
 template <int THREADS, typename A>
@@ -415,6 +506,14 @@ __device__ __forceinline__ Work<THREADS, A> make_work(const A &a, const Cut &cut
   const int64_t share = even_share > cut.least ? even_share : cut.least;
   if (threadIdx.x == 0) shared.share = share;
   w.active = (uint32_t)uniform(quotient_up(total, share));
+  if constexpr (kScoredCall<A>) {
+    w.units = whole_units<THREADS>(a, cut, shared, share);
+    if (w.units) {
+      w.active = min(w.units, a.workgroups);
+      w.piece = piece_of(w.active, blockIdx.x);
+      return w;
+    }
+  }
   w.piece = piece_of(w.active, blockIdx.x);
   w.turn = 2;
   __syncthreads();
