@@ -118,6 +118,7 @@ struct Units {
 // How a tile cuts: the rows of a unit, the shortest piece or part worth a workgroup (four tiles at least), a unit's slack.
 struct Cut {
   int fit, least, slack;
+  int whole = 0;   // scored: what cutting units costs a workgroup, in keys (whole_units)
 };
 template <typename A>
 __device__ __forceinline__ Units<A> units_of(const A &a, const Member<A> &q, const Cut &cut) {
@@ -216,20 +217,21 @@ struct LineShared {
 
 // A workgroup's work: one even part, or the piece of the line whose state lies in LDS between its parts (a place that every
 // wave reads and one thread writes into the other of two, so that the scalar registers are the tiles').
+constexpr uint32_t kSnapped = ~0u;   // a Work's units
 template <int THREADS, typename A>
 struct Work {
   bool even;
   uint32_t turn;     // even: 0 until the part is run; else of the place to read, + 2 before the first part
   uint32_t piece;
   uint32_t active;   // workgroups with work
-  uint32_t units;    // dealt out whole: how many (0: not)
+  uint32_t units;    // dealt out whole: how many (0: not; kSnapped: by where they lie on the line)
 
   // The next part of the line, or false; an even part comes from make_work. A barrier of the workgroup's lies between one
   // call and the next.
   __device__ __forceinline__ bool next(const A &a, const Cut &cut, LineShared<THREADS, A> &shared, Part<A> &p) {
     if (even) return turn++ == 0;
     if constexpr (kScoredCall<A>)
-      if (units) return deal(a, cut, shared, p);
+      if (units) return units == kSnapped ? snap(a, cut, shared, p) : deal(a, cut, shared, p);
     const int64_t share = uniform(shared.share), total = uniform(shared.prefix[a.kv.sequences]);
     const int64_t begin = share * piece, end = begin + share < total ? begin + share : total;
     Place at{};
@@ -261,7 +263,7 @@ struct Work {
 
  private:
   // The next of the units that workgroups take whole, every active-th.
-  __device__ __forceinline__ bool deal(const A &a, const Cut &cut, const LineShared<THREADS, A> &shared, Part<A> &p) {
+  __device__ __forceinline__ bool deal(const A &a, const Cut &cut, LineShared<THREADS, A> &shared, Part<A> &p) {
     const uint32_t unit = piece + turn++ * active;
     if (unit >= units) return false;
     uint32_t lo = 0, hi = a.kv.sequences;   // the last sequence that starts at or before the unit: one with units
@@ -274,14 +276,48 @@ struct Work {
     at.sequence = lo;
     take(a, cut, shared, at, p);
     const uint32_t rest = unit - (uint32_t)uniform(shared.prefix[lo]);
-    p.head = rest / (uint32_t)p.units.count;
-    p.m = (int)(rest - p.head * (uint32_t)p.units.count);
+    at.head = rest / (uint32_t)p.units.count;
+    at.m = (int)(rest - at.head * (uint32_t)p.units.count);
+    whole(p, at);
+    return true;
+  }
+  // The next of the units whose middles lie in the workgroup's piece of the line.
+  __device__ __forceinline__ bool snap(const A &a, const Cut &cut, LineShared<THREADS, A> &shared, Part<A> &p) {
+    const int64_t share = uniform(shared.share), total = uniform(shared.prefix[a.kv.sequences]);
+    const int64_t begin = share * piece;
+    if (piece >= active) return false;
+    Place at{};
+    if (turn >= 2) {
+      at.x = begin;
+      at.x -= enter(a, cut, shared, at, p);
+      const int length = p.units.length(at.m);
+      if (2 * at.x + length < 2 * begin) {   // its middle lies before
+        at.x += length;
+        if (at.x >= total) return false;
+        advance(a, cut, shared, at, p);
+      }
+    } else {
+      const Place &last = shared.place[turn];
+      at = {uniform(last.x), uniform(last.sequence), uniform(last.head), uniform(last.m)};
+      if (at.x >= total) return false;
+      advance(a, cut, shared, at, p);
+    }
+    const int length = p.units.length(at.m);
+    if (2 * at.x + length >= 2 * (begin + share)) return false;
+    at.x += length;
+    whole(p, at);
+    turn = (turn & 1) ^ 1;
+    if (threadIdx.x == 0) shared.place[turn] = at;
+    return true;
+  }
+  __device__ __forceinline__ void whole(Part<A> &p, const Place &at) const {
+    p.head = at.head;
+    p.m = at.m;
     p.t0 = 0;
-    p.t1 = p.units.tiles(p.m);
+    p.t1 = p.units.tiles(at.m);
     p.part = 0;
     p.parts = 1;
     p.first_piece = piece;
-    return true;
   }
   static __device__ __forceinline__ void take(const A &a, const Cut &cut, const LineShared<THREADS, A> &shared,
                                               const Place &at, Part<A> &p) {
@@ -354,12 +390,15 @@ struct Work {
   }
 };
 
-// How many units there are, where the workgroups take them whole (0: they do not), and then shared.prefix their numbers in the
-// place of their lengths. A piece of the line mostly holds two parts, each with what a unit costs besides its keys, and the
-// join reads the parts of nearly all units again; whole units leave workgroups idle behind the longest. So they stay whole
-// where the workgroup with the most has kWhole more than a piece, 2000 rows of eleven packed documents of up to 750 keys
-// (504 units of 32 heads of 128 on 512 workgroups): %WHOLE%.
-constexpr int kWhole = 640;
+// How many units there are, where the workgroups take them whole, and then shared.prefix their numbers in the place of their
+// lengths; kSnapped, where each workgroup takes those whose middles lie in its piece; 0, where pieces cut them. A piece mostly
+// holds two parts, each with what a unit costs besides its keys, parts are written and read again, and the join has nearly all
+// units to join; whole units leave workgroups idle behind the one with the most. Dealt out in turn, that one has as many as
+// there are rounds; snapped, no more than the longest unit or than two pieces' length (of two units or more, whose middles lie
+// within a piece, the outer halves come to less than another). So they stay whole where that is cut.whole more than a piece. In
+// us, cut / whole: 2000 bf16 rows of eleven packed documents of up to 750 keys, 32 heads of 128, 73 / 57, of five 95 / 79, 16
+// heads of 256 109 / 81; 2000 rows of one prompt 104 / 83; 2048 rows at 16384 keys, 16 heads of 256 with a cap, 805 / 766; 64
+// tokens over 300 to 800 int8 keys 45 / 31. (Where they are cut all the same, finding that out takes 1 us.)
 template <int THREADS, typename A>
 __device__ __forceinline__ uint32_t whole_units(const A &a, const Cut &cut, LineShared<THREADS, A> &shared, int64_t share) {
   constexpr int kWaves = THREADS / 64;
@@ -380,20 +419,20 @@ __device__ __forceinline__ uint32_t whole_units(const A &a, const Cut &cut, Line
   number = wave_sum(number);
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) longest = max(longest, __shfl_xor(longest, d));
-  if (lane == 0) shared.waves[wave] = number;
+  // Both in a word: more units than are ever dealt out count as that many.
+  if (lane == 0) shared.waves[wave] = (number < 0x7FFFFFFF ? number : 0x7FFFFFFF) << 32 | (uint32_t)longest;
   __syncthreads();
   number = 0;
 #pragma unroll
-  for (int i = 0; i < kWaves; ++i) number += shared.waves[i];
-  __syncthreads();
-  if (lane == 0) shared.waves[wave] = longest;
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < kWaves; ++i) longest = max(longest, (int)shared.waves[i]);
+  for (int i = 0; i < kWaves; ++i) {
+    number += shared.waves[i] >> 32;
+    longest = max(longest, (int)(uint32_t)shared.waves[i]);
+  }
   number = uniform(number);
   longest = uniform(longest);
   const int64_t rounds = (number + a.workgroups - 1) / a.workgroups;
-  if (!number || number > 8 * (int64_t)a.workgroups || rounds * longest > share + kWhole) return 0;
+  if (!number || number > 8 * (int64_t)a.workgroups) return 0;
+  if (rounds * longest > share + cut.whole) return longest <= share + cut.whole && share <= cut.whole ? kSnapped : 0;
   int64_t carry = 0;
   for (uint32_t s0 = 0; s0 < count; s0 += THREADS) {
     const uint32_t s = s0 + threadIdx.x;
@@ -508,7 +547,7 @@ __device__ __forceinline__ Work<THREADS, A> make_work(const A &a, const Cut &cut
   w.active = (uint32_t)uniform(quotient_up(total, share));
   if constexpr (kScoredCall<A>) {
     w.units = whole_units<THREADS>(a, cut, shared, share);
-    if (w.units) {
+    if (w.units && w.units != kSnapped) {
       w.active = min(w.units, a.workgroups);
       w.piece = piece_of(w.active, blockIdx.x);
       return w;

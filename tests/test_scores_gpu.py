@@ -212,6 +212,34 @@ def test_many_sequences():
     check(c, queries(rng, c.rows, 4, 64), 0.125, (None, 40), begins=begins, prefixes=prefixes, slopes=slopes_of(4), cap=10.0)
 
 
+@pytest.mark.parametrize("units", [1, 3, 8, 40])
+@pytest.mark.parametrize("fmt", ["bf16", "e2m1"])
+def test_units_dealt_whole(fmt, units):
+    """Batches whose units nearly fill a small device's workgroups, alike and of many lengths, so that they are dealt out in turn,
+    snapped to pieces or cut: the same function, and the same bits each time."""
+    rng = np.random.default_rng(units)
+    t = torch()
+    for sizes, chunk in (([(1, 300 + 7 * i) for i in range(24)], 1), ([(1, int(n)) for n in rng.integers(1, 700, 70)], 1),
+                         ([(64 + 3 * i, 64 + 3 * i) for i in range(9)], 64), ([(500, 900)], 500), ([(1, 10)] * 300, 1),
+                         ([(int(n), int(n) + 30) for n in rng.integers(0, 130, 25)], 100)):
+        c = make(rng, sizes, 2, 64, 16, fmt).fill()
+        q = queries(rng, c.rows, 4, 64)
+        begins = [int(rng.integers(0, k // 2 + 1)) for _, k in sizes]
+        want, bound = scored_f64(q, c, 0.125, begins=begins, cap=20.0)
+        scores, keep = scores_of(cap=20.0, begins=begins)
+        plan = sq.attention_plan(sq.AttentionShape(4, c.shape, 1, 0, 0.125), len(sizes), c.rows, min(chunk, c.rows),
+                                 sq.Device(units))
+        outs = []
+        for _ in range(2):
+            out, scratch = t.zeros((c.rows, 256), dtype=t.bfloat16, device="cuda"), sq.AttentionScratch(plan)
+            scratch.partials.fill_(0xFF)
+            sq.attention_add(plan, c.struct(), c.batch(), to_bf16(q.reshape(c.rows, -1)), out, scratch, scores=scores)
+            outs.append(from_bf16(out).reshape(q.shape))
+        check_attention(outs[0], want, bound, f"{len(sizes)} sequences")
+        assert np.array_equal(*outs)
+        del keep
+
+
 def test_holes_under_a_prefix():
     t = torch()
     rng = np.random.default_rng(6)
