@@ -17,6 +17,9 @@
 //    have a closed form, and a workgroup finds its place by a search over the sequences' sums (in LDS) and one over m.
 //    Offset o of a unit lies before its tile ceil(o / 64), or past its last tile.
 //
+//  - Scored calls and 4-bit pages may also keep every unit whole, where the workgroups then hold no more than the line's cuts
+//    cost them (whole_units): units dealt out in rounds, or each to the piece of the line in which its middle lies.
+//
 // Parts go to the workspace, and a second launch (attend_join.hip) joins them.
 #pragma once
 #include <type_traits>
@@ -118,7 +121,7 @@ struct Units {
 // How a tile cuts: the rows of a unit, the shortest piece or part worth a workgroup (four tiles at least), a unit's slack.
 struct Cut {
   int fit, least, slack;
-  int whole = 0;   // scored: what cutting units costs a workgroup, in keys (whole_units)
+  int whole;   // what cutting units costs a workgroup, in keys (whole_units)
 };
 template <typename A>
 __device__ __forceinline__ Units<A> units_of(const A &a, const Member<A> &q, const Cut &cut) {
@@ -218,7 +221,8 @@ struct LineShared {
 // A workgroup's work: one even part, or the piece of the line whose state lies in LDS between its parts (a place that every
 // wave reads and one thread writes into the other of two, so that the scalar registers are the tiles').
 constexpr uint32_t kSnapped = ~0u;   // a Work's units
-template <int THREADS, typename A>
+// WHOLE: units may stay whole (whole_units).
+template <int THREADS, typename A, bool WHOLE>
 struct Work {
   bool even;
   uint32_t turn;     // even: 0 until the part is run; else of the place to read, + 2 before the first part
@@ -230,7 +234,7 @@ struct Work {
   // call and the next.
   __device__ __forceinline__ bool next(const A &a, const Cut &cut, LineShared<THREADS, A> &shared, Part<A> &p) {
     if (even) return turn++ == 0;
-    if constexpr (kScoredCall<A>)
+    if constexpr (WHOLE)
       if (units) return units == kSnapped ? snap(a, cut, shared, p) : deal(a, cut, shared, p);
     const int64_t share = uniform(shared.share), total = uniform(shared.prefix[a.kv.sequences]);
     const int64_t begin = share * piece, end = begin + share < total ? begin + share : total;
@@ -459,12 +463,12 @@ __device__ __forceinline__ uint32_t whole_units(const A &a, const Cut &cut, Line
 }
 
 // Every thread of the workgroup takes part.
-template <int THREADS, typename A>
-__device__ __forceinline__ Work<THREADS, A> make_work(const A &a, const Cut &cut, LineShared<THREADS, A> &shared,
-                                                      Part<A> &p) {
+template <int THREADS, bool WHOLE, typename A>
+__device__ __forceinline__ Work<THREADS, A, WHOLE> make_work(const A &a, const Cut &cut, LineShared<THREADS, A> &shared,
+                                                             Part<A> &p) {
   constexpr int kWaves = THREADS / 64;
   const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, count = a.kv.sequences;
-  Work<THREADS, A> w{};
+  Work<THREADS, A, WHOLE> w{};
   if (count <= 64) {
     // Each wave for itself, a sequence a lane, in registers.
     const Member<A> q = lane < count ? member_of(a, lane) : Member<A>{};
@@ -545,7 +549,7 @@ __device__ __forceinline__ Work<THREADS, A> make_work(const A &a, const Cut &cut
   const int64_t share = even_share > cut.least ? even_share : cut.least;
   if (threadIdx.x == 0) shared.share = share;
   w.active = (uint32_t)uniform(quotient_up(total, share));
-  if constexpr (kScoredCall<A>) {
+  if constexpr (WHOLE) {
     w.units = whole_units<THREADS>(a, cut, shared, share);
     if (w.units && w.units != kSnapped) {
       w.active = min(w.units, a.workgroups);

@@ -268,7 +268,8 @@ attend_rows_kernel(A a) {
   const float by_group = 1.0f / (float)a.group;
   const uint32_t dim = a.kv.head_dim, row_bytes = kFour ? dim / 2 : dim * (kCodes ? 1 : 2);
   Part<A> next;
-  Work<kThreads, A> work = make_work<kThreads>(a, cut, shared.line, next);
+  constexpr bool kWhole = kScored || kFour;   // (the others keep the shares, and so the bits, that they have)
+  Work<kThreads, A, kWhole> work = make_work<kThreads, kWhole>(a, cut, shared.line, next);
   UnitNote began{};
   while (work.next(a, cut, shared.line, next)) {
     const Part<A> part = settled(a, cut, next);

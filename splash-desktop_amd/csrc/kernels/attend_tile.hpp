@@ -122,7 +122,8 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
   const float by_group = 1.0f / (float)a.group;
   const uint32_t dim = a.kv.head_dim, row_bytes = kFour ? dim / 2 : dim * (kBits / 8);
   Part<A> next;
-  Work<kThreads, A> work = make_work<kThreads>(a, cut, shared, next);
+  constexpr bool kWhole = kScored || kFour;   // (the others keep the shares, and so the bits, that they have)
+  Work<kThreads, A, kWhole> work = make_work<kThreads, kWhole>(a, cut, shared, next);
   UnitNote began{};
 
   // Where this lane's vectors lie in 16 keys of a page, and (codes) in the LDS tile.

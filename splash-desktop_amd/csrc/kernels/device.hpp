@@ -187,11 +187,7 @@ template <int POLICY = kStream>
 __device__ __forceinline__ uint32_t buffer_b32(__amdgpu_buffer_rsrc_t r, uint32_t voffset, uint32_t soffset) {
   return __builtin_amdgcn_raw_buffer_load_b32(r, voffset, soffset, POLICY);
 }
-// Two bytes, or one, zero-extended.
-template <int POLICY = kStream>
-__device__ __forceinline__ uint32_t buffer_b16(__amdgpu_buffer_rsrc_t r, uint32_t voffset, uint32_t soffset) {
-  return __builtin_amdgcn_raw_buffer_load_b16(r, voffset, soffset, POLICY);
-}
+// One byte, zero-extended.
 template <int POLICY = kStream>
 __device__ __forceinline__ uint32_t buffer_b8(__amdgpu_buffer_rsrc_t r, uint32_t voffset, uint32_t soffset) {
   return __builtin_amdgcn_raw_buffer_load_b8(r, voffset, soffset, POLICY);
