@@ -121,7 +121,7 @@ struct Units {
 // How a tile cuts: the rows of a unit, the shortest piece or part worth a workgroup (four tiles at least), a unit's slack.
 struct Cut {
   int fit, least, slack;
-  int whole;   // what cutting units costs a workgroup, in keys (whole_units)
+  int whole, fall;   // what cutting units costs a workgroup, in keys, and 1 / what that falls by for each of a piece (whole_units)
 };
 template <typename A>
 __device__ __forceinline__ Units<A> units_of(const A &a, const Member<A> &q, const Cut &cut) {
@@ -235,7 +235,7 @@ struct Work {
   __device__ __forceinline__ bool next(const A &a, const Cut &cut, LineShared<THREADS, A> &shared, Part<A> &p) {
     if (even) return turn++ == 0;
     if constexpr (WHOLE)
-      if (units) return units == kSnapped ? snap(a, cut, shared, p) : deal(a, cut, shared, p);
+      if (units && units != kSnapped) return deal(a, cut, shared, p);
     const int64_t share = uniform(shared.share), total = uniform(shared.prefix[a.kv.sequences]);
     const int64_t begin = share * piece, end = begin + share < total ? begin + share : total;
     Place at{};
@@ -251,7 +251,16 @@ struct Work {
       if (turn >= 2) from = enter(a, cut, shared, at, p);
       else advance(a, cut, shared, at, p);
       turn &= 1;
-      cut_at(from, share, end, at, p);
+      if (WHOLE && units == kSnapped) {
+        const int length = p.units.length(at.m);
+        const int64_t middles = 2 * (at.x - from) + length;   // twice its middle
+        at.x += length - from;
+        if (middles >= 2 * (begin + share)) return false;
+        whole(p, at);
+        if (middles < 2 * begin) p.t1 = 0;   // the piece's before
+      } else {
+        cut_at(from, share, end, at, p);
+      }
     } while (p.t1 <= p.t0);
     turn ^= 1;
     if (threadIdx.x == 0) shared.place[turn] = at;
@@ -283,35 +292,6 @@ struct Work {
     at.head = rest / (uint32_t)p.units.count;
     at.m = (int)(rest - at.head * (uint32_t)p.units.count);
     whole(p, at);
-    return true;
-  }
-  // The next of the units whose middles lie in the workgroup's piece of the line.
-  __device__ __forceinline__ bool snap(const A &a, const Cut &cut, LineShared<THREADS, A> &shared, Part<A> &p) {
-    const int64_t share = uniform(shared.share), total = uniform(shared.prefix[a.kv.sequences]);
-    const int64_t begin = share * piece;
-    if (piece >= active) return false;
-    Place at{};
-    if (turn >= 2) {
-      at.x = begin;
-      at.x -= enter(a, cut, shared, at, p);
-      const int length = p.units.length(at.m);
-      if (2 * at.x + length < 2 * begin) {   // its middle lies before
-        at.x += length;
-        if (at.x >= total) return false;
-        advance(a, cut, shared, at, p);
-      }
-    } else {
-      const Place &last = shared.place[turn];
-      at = {uniform(last.x), uniform(last.sequence), uniform(last.head), uniform(last.m)};
-      if (at.x >= total) return false;
-      advance(a, cut, shared, at, p);
-    }
-    const int length = p.units.length(at.m);
-    if (2 * at.x + length >= 2 * (begin + share)) return false;
-    at.x += length;
-    whole(p, at);
-    turn = (turn & 1) ^ 1;
-    if (threadIdx.x == 0) shared.place[turn] = at;
     return true;
   }
   __device__ __forceinline__ void whole(Part<A> &p, const Place &at) const {
@@ -399,10 +379,13 @@ struct Work {
 // holds two parts, each with what a unit costs besides its keys, parts are written and read again, and the join has nearly all
 // units to join; whole units leave workgroups idle behind the one with the most. Dealt out in turn, that one has as many as
 // there are rounds; snapped, no more than the longest unit or than two pieces' length (of two units or more, whose middles lie
-// within a piece, the outer halves come to less than another). So they stay whole where that is cut.whole more than a piece. In
-// us, cut / whole: 2000 bf16 rows of eleven packed documents of up to 750 keys, 32 heads of 128, 73 / 57, of five 95 / 79, 16
-// heads of 256 109 / 81; 2000 rows of one prompt 104 / 83; 2048 rows at 16384 keys, 16 heads of 256 with a cap, 805 / 766; 64
-// tokens over 300 to 800 int8 keys 45 / 31. (Where they are cut all the same, finding that out takes 1 us.)
+// within a piece, the outer halves come to less than another). So they stay whole where that is at most cut.whole more than a
+// piece, cut / whole in us: 2000 bf16 rows of eleven packed documents of up to 750 keys, 32 heads of 128, 73 / 57, of five 95 /
+// 79, 2000 rows of one prompt 104 / 83; 2048 rows at 16384 keys, with a cap, 665 / 631; 64 tokens over 300 to 800 int8 keys 45
+// / 31, over as many of 4 bits 37 / 23. With heads of 256, one workgroup a CU, nothing else runs where one idles, and the
+// longer the units the less the cuts cost: 2048 rows of 16 such heads at 2048 keys 134 / 115, at 3000 183 / 160, at 5000 247 /
+// 250 (int8 294 / 317), at 8000 374 / 421, at 16384 776 / 843; the documents 113 / 84 and 141 / 108. (Where units are cut all
+// the same, finding that out takes 1 us.)
 template <int THREADS, typename A>
 __device__ __forceinline__ uint32_t whole_units(const A &a, const Cut &cut, LineShared<THREADS, A> &shared, int64_t share) {
   constexpr int kWaves = THREADS / 64;
@@ -418,7 +401,7 @@ __device__ __forceinline__ uint32_t whole_units(const A &a, const Cut &cut, Line
     const Units<A> u = units_at(s);
     if (!u.count) continue;
     number += (int64_t)u.count * a.kv.kv_heads;
-    longest = max(longest, max(u.length(0), u.length(u.count - 1)));
+    longest = max(longest, max(u.length(0), u.length(u.count - 1)));   // (those between: a unit's rows more at most)
   }
   number = wave_sum(number);
 #pragma unroll
@@ -436,7 +419,8 @@ __device__ __forceinline__ uint32_t whole_units(const A &a, const Cut &cut, Line
   longest = uniform(longest);
   const int64_t rounds = (number + a.workgroups - 1) / a.workgroups;
   if (!number || number > 8 * (int64_t)a.workgroups) return 0;
-  if (rounds * longest > share + cut.whole) return longest <= share + cut.whole && share <= cut.whole ? kSnapped : 0;
+  const int64_t most = share + cut.whole - (cut.fall ? share / cut.fall : 0);
+  if (rounds * longest > most) return longest <= most && share <= cut.whole ? kSnapped : 0;
   int64_t carry = 0;
   for (uint32_t s0 = 0; s0 < count; s0 += THREADS) {
     const uint32_t s = s0 + threadIdx.x;
