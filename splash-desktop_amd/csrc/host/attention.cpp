@@ -310,7 +310,7 @@ void Attention::add(hipStream_t graph, const HeadRowsView &query, const HeadRows
   // A batch of few units, none longer than a workgroup takes at least, is cut nowhere (attend.hpp), and leaves no parts.
   const uint64_t units = (batch.rows / (plan.tileRows / shape.group()) + batch.sequences) * uint64_t{shape.kv.kvHeads};
   const bool whole = plan.tileRows != kern::kAttendWideRows && batch.sequences <= 64 && units * 4 <= plan.workgroups &&
-                     keys + 384 <= kern::kAttendLeast;
+                     keys + 384 <= kern::attend_least(shape.kv.headDim, args.kv.format, !scores.none());
   const OnStreamDevice on(graph);
   const bool wide = plan.tileRows == kern::kAttendWideRows;
   if (scores.none()) {

@@ -264,11 +264,11 @@ attend_rows_kernel(A a) {
   __shared__ Shared<MB, WAVES, A> shared;
   const uint32_t lane = threadIdx.x & 63, r = lane & 15, kq = lane >> 4;
   const uint32_t wave = uniform(threadIdx.x >> 6);
-  const Cut cut{16 * MB / (int)a.group, (int)kAttendLeast, kUnitSlack + 256, 640, 0};
+  constexpr bool kWhole = kScored || kFour;   // (the others keep the shares, and so the bits, that they have)
+  const Cut cut{16 * MB / (int)a.group, (int)attend_least(DIM, FMT, kScored), kUnitSlack + 256, 640, 0};
   const float by_group = 1.0f / (float)a.group;
   const uint32_t dim = a.kv.head_dim, row_bytes = kFour ? dim / 2 : dim * (kCodes ? 1 : 2);
   Part<A> next;
-  constexpr bool kWhole = kScored || kFour;   // (the others keep the shares, and so the bits, that they have)
   Work<kThreads, A, kWhole> work = make_work<kThreads, kWhole>(a, cut, shared.line, next);
   UnitNote began{};
   while (work.next(a, cut, shared.line, next)) {

@@ -312,7 +312,13 @@ hipError_t launch_attend_tile_scored(const ScoredArgs &args, hipStream_t stream)
 hipError_t launch_attend_tile_capped(const CappedArgs &args, hipStream_t stream);
 // The join of the parts that either left, after it. few: the batch has no more units than a quarter of the workgroups.
 hipError_t launch_attend_join(uint32_t tile_rows, bool few, const AttendArgs &args, hipStream_t stream);
-// The length (attend.hpp) up to which a batch of few units is never cut (launch_attend_rows).
-constexpr uint32_t kAttendLeast = 1280;
+// The length (attend.hpp) up to which tiles of few rows never cut a batch of few units. The join's launch takes 5 us, and more
+// keys a workgroup than it takes are read in that time; of heads of 256 few, as a CU holds four waves with a step of 16 or 32 KB
+// each: a token with a cap over 700 bf16 keys of 8 heads of 256 in 25 us whole and 19 in parts of 256, over 1500 38 / 22, over
+// 300 17 / 17, over 700 int8 keys 21 / 18, of 4 bits 16 / 18; of heads of 128 over 700 16 / 16, over 450 13 / 14, of 64 over 700
+// 12 / 14. (Plain calls keep the parts, and so the bits, that they have.)
+constexpr uint32_t attend_least(uint32_t head_dim, uint32_t format, bool scored) {
+  return scored && head_dim > 128 && format != SQ_KV_E2M1 ? 256 : 1280;
+}
 
 }  // namespace sq::kern
