@@ -11,7 +11,8 @@
 // 8-bit codes become bf16 operands exactly (127 and e4m3's four bits both fit its eight); the scales of their tokens
 // multiply the scores, and the weights before they are rounded.
 //
-// Heads of 256 of e4m3 spill 2 or 6 registers (12 or 28 bytes a lane), no others any.
+// Heads of 256 of e4m3 spill 2 or 6 registers (12 or 28 bytes a lane; scored ones 8 or 14, 36 or 60), scored 8-bit heads of 64
+// in tiles of 32 rows 4 or 5 (20 or 24), no others any.
 //
 // Loads go through buffer resources of 16 keys of one page (pages are whole multiples of 16 tokens): a key past the
 // sequence, a page that is a hole and a value past head_dim all read zero, with no instruction spent on them.

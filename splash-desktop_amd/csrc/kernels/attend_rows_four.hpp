@@ -7,9 +7,13 @@
 // A step is half the bytes of 8-bit codes and as many instructions, so two things bind it that do not bind them. Its bytes: one
 // step ahead is too few in flight, so where registers allow a wave keeps two (a token over 131072 keys of 8 heads of 128, with
 // the join: 50 us with one, 41 with two), and every path loads alike, past the end from empty resources: where paths with fewer
-// loads meet, or after a store to memory that may be LDS's, the compiler waits for all loads at each step. Its VALU (57% of
-// a launch's cycles): 64 conversions and 32 transposes a step stay; scales come by one rotation, and no selects are made
-// where all keys are seen.
+// loads meet, or after a store to memory that may be LDS's, the compiler waits for all loads at each step. Its VALU (52% of
+// a launch's cycles, the matrix units 17%): 64 conversions and 32 transposes a step stay; scales come by one rotation, and no
+// selects are made where all keys are seen.
+//
+// What it reaches: a token of 40 heads over 131072 keys of 8 heads of 128 (143 MB) in 35 us, 4.1 TB/s, where int8 takes 54; a
+// token each of 64 sequences of 200 to 8000 keys (151 MB) in 52, 2.9 TB/s, four of a tile's 16 rows live, and a
+// start and a join of the waves for each of some 1000 parts.
 #pragma once
 #include "attend_few.hpp"
 

@@ -24,8 +24,18 @@
 // tile, and keep neither pipe busy: 24 GFLOP of int8 prompts take 81 us, of whose cycles the VALU issues 44% and the matrix
 // units work 14%; the rest goes to the barriers and to the start of units of 17 tiles, a chain of loads that nothing covers.
 //
+// 4-bit pages: a lane's eight codes and the byte of their group become eight bf16 on the way to LDS, scales and all, so no
+// scale is left for scores or weights: the chunk at 16384 keys in 522 to 545 us (VALU 45% of the cycles, matrix units 42%).
+//
+// Scored calls are their own instances, so that plain ones compile as if there were none. A cap that is all there is has one
+// more (CappedArgs): where a tile's scores are below 0.4 of the cap, cap tanh(t / cap) is an odd polynomial of the seventh
+// degree beside the second product, and no exponential or quotient. 2048 rows of 16 heads of 256 with a cap of 50 at 16384 keys
+// take 798 us so, 973 with the exponential form (a cap of 10), 660 with no cap (32 heads of 128: 626, 806).
+//
 // The registers are full: bf16 heads of 256 spill 13 of them (40 bytes a lane), int8 ones of 128 and 256 4 and 12 (12 and 0
-// bytes: accumulation registers hold the others), e4m3 ones 13 and 20 (40 and 24). Heads of 64 and bf16 ones of 128 none.
+// bytes: accumulation registers hold the others), e4m3 ones 13 and 20 (40 and 24), 4-bit ones of 256 38 (140). Scored ones of
+// 256 spill 21 to 47 (72 to 168 bytes), capped ones 24 to 48 (48 to 180) and of 128 as plain ones. Heads of 64 and bf16 and
+// 4-bit ones of 128 none.
 //
 // Keys past the sequence's end and holes read as zeros (buffer resources end there). Only tiles that some row does not
 // see whole compare positions.
