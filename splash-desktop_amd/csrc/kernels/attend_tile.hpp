@@ -128,7 +128,7 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
   __shared__ LineShared<kThreads, A> shared;
   const uint32_t lane = threadIdx.x & 63, r = lane & 31, h = lane >> 5;
   const uint32_t wave = uniform(threadIdx.x >> 6);
-  const Cut cut{kRows / (int)a.group, 4 * kKeyTile, kUnitSlack + 192, 1152, DIM <= 128 ? 0 : 16};
+  const Cut cut{kRows / (int)a.group, 4 * kKeyTile, kUnitSlack + 192, attend_tile_resident(DIM, FMT), 1152, DIM <= 128 ? 0 : 16};
   const float by_group = 1.0f / (float)a.group;
   const uint32_t dim = a.kv.head_dim, row_bytes = kFour ? dim / 2 : dim * (kBits / 8);
   Part<A> next;

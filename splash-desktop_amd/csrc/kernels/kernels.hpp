@@ -300,7 +300,7 @@ constexpr uint32_t attend_tile_resident(uint32_t head_dim, uint32_t format) {
   return head_dim > 128 ? 1 : head_dim <= 64 && format == SQ_KV_BF16 ? 3 : 2;
 }
 // The workgroups of a compute unit under a plan of tiles of tile_rows rows and workgroups of `waves` waves.
-inline uint32_t attend_resident(uint32_t tile_rows, uint32_t waves, uint32_t head_dim, uint32_t format) {
+constexpr uint32_t attend_resident(uint32_t tile_rows, uint32_t waves, uint32_t head_dim, uint32_t format) {
   if (tile_rows == kAttendWideRows) return attend_tile_resident(head_dim, format);
   return waves == 8 ? 1 : attend_rows_resident(tile_rows, head_dim, format);
 }
