@@ -18,7 +18,7 @@
 //    Offset o of a unit lies before its tile ceil(o / 64), or past its last tile.
 //
 //  - Scored calls and 4-bit pages may also keep every unit whole, where the workgroups then hold no more than the line's cuts
-//    cost them (whole_units): units dealt out in rounds, or each to the piece of the line in which its middle lies.
+//    cost them (whole_units): dealt out by their lengths, long ones first.
 //
 // Parts go to the workspace, and a second launch (attend_join.hip) joins them.
 #pragma once
@@ -34,6 +34,7 @@ constexpr int kKeyTile = 64;
 // it besides keys.
 constexpr int kUnitSlack = 2 * (kKeyTile - 1);
 constexpr uint32_t kMaxSequences = SQ_KV_MAX_SEQUENCES;
+constexpr uint32_t kMaxWhole = kMaxSequences / 2;   // sequences of a batch whose units may stay whole
 
 // sum over i < m of max(lo, a + r i).
 __device__ __forceinline__ int64_t clamped_sum(int lo, int a, int r, int m) {
@@ -201,17 +202,6 @@ __device__ __forceinline__ uint32_t piece_of(uint32_t active, uint32_t block) {
   const uint32_t each = (active + 7) / 8;
   return block / 8 < each ? block % 8 * each + block / 8 : active;
 }
-// The same for one sequence's units, dealt out whole. Workgroups fill an XCD's compute units one each, then a second each, and
-// units grow with the position, so every second turn counts backwards: a compute unit's long unit has a short one beside it.
-// 2048 rows of 2048 keys of 8 heads of 128, 84 us without and 79 with it (4-bit pages 76, 72), 2001 of 2001 83 and 79. (Of many
-// sequences it is as often the other way: five documents 80 and 77, eleven short ones 41.6 and 43.8, four prompts 39 and 41.)
-__device__ __forceinline__ uint32_t dealt_piece_of(uint32_t active, uint32_t block, uint32_t units_of_xcd) {
-  const uint32_t each = (active + 7) / 8, i = block / 8, turn = i / units_of_xcd, first = turn * units_of_xcd;
-  if (i >= each) return active;
-  const uint32_t past = min(first + units_of_xcd, each);
-  return block % 8 * each + (turn % 2 ? past - 1 - (i - first) : i);
-}
-
 // LDS for the line.
 constexpr uint32_t kCached = 256;   // sequences whose rows and keys stay in LDS
 // Where a workgroup stands in its piece of the line between one part and the next.
@@ -220,6 +210,12 @@ struct Place {
   uint32_t sequence, head;
   int m;
 };
+// A unit that a workgroup has whole.
+struct Whole {
+  uint32_t sequence, head;
+  int m;
+};
+constexpr uint32_t kMaxRounds = 8;
 template <int THREADS, typename A>
 struct LineShared {
   int64_t prefix[kMaxSequences + 1];   // where each sequence starts
@@ -231,7 +227,6 @@ struct LineShared {
 
 // A workgroup's work: one even part, or the piece of the line whose state lies in LDS between its parts (a place that every
 // wave reads and one thread writes into the other of two, so that the scalar registers are the tiles').
-constexpr uint32_t kSnapped = ~0u;   // a Work's units
 // WHOLE: units may stay whole (whole_units).
 template <int THREADS, typename A, bool WHOLE>
 struct Work {
@@ -239,14 +234,27 @@ struct Work {
   uint32_t turn;     // even: 0 until the part is run; else of the place to read, + 2 before the first part
   uint32_t piece;
   uint32_t active;   // workgroups with work
-  uint32_t units;    // dealt out whole: how many (0: not; kSnapped: by where they lie on the line)
+  uint32_t units;    // whole: its own, and one more (0: cut)
 
   // The next part of the line, or false; an even part comes from make_work. A barrier of the workgroup's lies between one
   // call and the next.
   __device__ __forceinline__ bool next(const A &a, const Cut &cut, LineShared<THREADS, A> &shared, Part<A> &p) {
     if (even) return turn++ == 0;
     if constexpr (WHOLE)
-      if (units && units != kSnapped) return deal(a, cut, shared, p);
+      if (units) {
+        if (turn + 1 >= units) return false;
+        const Whole &own = whole_of(shared)[turn++];
+        const Place at{0, uniform(own.sequence), uniform(own.head), uniform(own.m)};
+        take(a, cut, shared, at, p);
+        p.head = at.head;
+        p.m = at.m;
+        p.t0 = 0;
+        p.t1 = p.units.tiles(at.m);
+        p.part = 0;
+        p.parts = 1;
+        p.first_piece = piece;
+        return true;
+      }
     const int64_t share = uniform(shared.share), total = uniform(shared.prefix[a.kv.sequences]);
     const int64_t begin = share * piece, end = begin + share < total ? begin + share : total;
     Place at{};
@@ -262,20 +270,48 @@ struct Work {
       if (turn >= 2) from = enter(a, cut, shared, at, p);
       else advance(a, cut, shared, at, p);
       turn &= 1;
-      if (WHOLE && units == kSnapped) {
-        const int length = p.units.length(at.m);
-        const int64_t middles = 2 * (at.x - from) + length;   // twice its middle
-        at.x += length - from;
-        if (middles >= 2 * (begin + share)) return false;
-        whole(p, at);
-        if (middles < 2 * begin) p.t1 = 0;   // the piece's before
-      } else {
-        cut_at(from, share, end, at, p);
-      }
+      cut_at(from, share, end, at, p);
     } while (p.t1 <= p.t0);
     turn ^= 1;
     if (threadIdx.x == 0) shared.place[turn] = at;
     return true;
+  }
+  // Takes units whole, `number` of a key head (shared.prefix holds the sequences' numbers of all): the XCDs have them in turn,
+  // the longest first, key heads next to each other (so that an XCD holds few heads' keys), and a row of workgroups has them
+  // in turn too, every second time backwards. Workgroups fill an XCD's compute units one each, then a second each: every
+  // second of these counts backwards as well, so that short units come beside and behind long ones.
+  __device__ __forceinline__ void take_whole(const A &a, const Cut &cut, LineShared<THREADS, A> &shared, uint32_t number) {
+    const uint32_t heads = a.kv.kv_heads, all = number * heads, t = threadIdx.x;
+    int *tiles = (int *)(whole_of(shared) + kMaxRounds), mine = 0, m = 0;
+    uint32_t s = 0;
+    if (t < number) {
+      uint32_t hi = a.kv.sequences;   // the last sequence that starts at or before unit t of each head: one with units
+      while (hi - s > 1) {
+        const uint32_t mid = (s + hi) / 2;
+        if (shared.prefix[mid] <= (int64_t)(t * heads)) s = mid;
+        else hi = mid;
+      }
+      m = (int)((t * heads - (uint32_t)shared.prefix[s]) / heads);
+      tiles[t] = mine = units_of(a, s < kCached ? shared.sequence[s] : member_of(a, s), cut).tiles(m);
+    }
+    __syncthreads();
+    const uint32_t xcd = blockIdx.x % 8, i = blockIdx.x / 8, each = (all + 7 - xcd) / 8, row = min(each, a.workgroups / 8);
+    const uint32_t cus = max(a.workgroups / (8 * cut.resident), 1u), first = i / cus * cus;
+    const uint32_t at = i / cus % 2 ? min(first + cus, row) - 1 - (i - first) : i;
+    active = min(all, a.workgroups);
+    piece = i < row ? 8 * at + xcd : active;
+    uint32_t before = 0;
+    if (t < number)
+      for (uint32_t k = 0; k < number; ++k) before += tiles[k] > mine || (tiles[k] == mine && k < t);
+    units = 1;
+    for (uint32_t k = 0; i < row && k < kMaxRounds; ++k) {
+      const uint32_t rank = k % 2 ? (k + 1) * row - 1 - at : k * row + at;
+      if (rank >= each) break;
+      const uint32_t unit = 8 * rank + xcd, place = unit / heads;
+      if (t < number && before == place) whole_of(shared)[k] = {s, unit - place * heads, m};
+      ++units;
+    }
+    __syncthreads();
   }
   // The notes that the join reads, once all of the workgroup's parts are stored: of the unit it began (began.parts 0:
   // none), and one workgroup's of how many there are.
@@ -286,33 +322,8 @@ struct Work {
   }
 
  private:
-  // The next of the units that workgroups take whole, every active-th.
-  __device__ __forceinline__ bool deal(const A &a, const Cut &cut, LineShared<THREADS, A> &shared, Part<A> &p) {
-    const uint32_t unit = piece + turn++ * active;
-    if (unit >= units) return false;
-    uint32_t lo = 0, hi = a.kv.sequences;   // the last sequence that starts at or before the unit: one with units
-    while (hi - lo > 1) {
-      const uint32_t mid = (lo + hi) / 2;
-      if (uniform(shared.prefix[mid]) <= (int64_t)unit) lo = mid;
-      else hi = mid;
-    }
-    Place at{};
-    at.sequence = lo;
-    take(a, cut, shared, at, p);
-    const uint32_t rest = unit - (uint32_t)uniform(shared.prefix[lo]);
-    at.head = rest / (uint32_t)p.units.count;
-    at.m = (int)(rest - at.head * (uint32_t)p.units.count);
-    whole(p, at);
-    return true;
-  }
-  __device__ __forceinline__ void whole(Part<A> &p, const Place &at) const {
-    p.head = at.head;
-    p.m = at.m;
-    p.t0 = 0;
-    p.t1 = p.units.tiles(at.m);
-    p.part = 0;
-    p.parts = 1;
-    p.first_piece = piece;
+  static __device__ __forceinline__ Whole *whole_of(LineShared<THREADS, A> &shared) {
+    return (Whole *)(shared.prefix + kMaxWhole + 1);
   }
   static __device__ __forceinline__ void take(const A &a, const Cut &cut, const LineShared<THREADS, A> &shared,
                                               const Place &at, Part<A> &p) {
@@ -385,18 +396,17 @@ struct Work {
   }
 };
 
-// How many units there are, where the workgroups take them whole, and then shared.prefix their numbers in the place of their
-// lengths; kSnapped, where each workgroup takes those whose middles lie in its piece; 0, where pieces cut them. A piece mostly
-// holds two parts, each with what a unit costs besides its keys, parts are written and read again, and the join has nearly all
-// units to join; whole units leave workgroups idle behind the one with the most. Dealt out in turn, that one has as many as
-// there are rounds; snapped, no more than the longest unit or than two pieces' length (of two units or more, whose middles lie
-// within a piece, the outer halves come to less than another). So they stay whole where that is at most cut.whole more than a
-// piece, cut / whole in us: 2000 bf16 rows of eleven packed documents of up to 750 keys, 32 heads of 128, 73 / 57, of five 95 /
-// 79, 2000 rows of one prompt 104 / 83; 2048 rows at 16384 keys, with a cap, 665 / 631; 64 tokens over 300 to 800 int8 keys 45
-// / 31, over as many of 4 bits 37 / 23. With heads of 256, one workgroup a CU, nothing else runs where one idles, and the
-// longer the units the less the cuts cost: 2048 rows of 16 such heads at 2048 keys 134 / 115, at 3000 183 / 160, at 5000 247 /
-// 250 (int8 294 / 317), at 8000 374 / 421, at 16384 776 / 843; the documents 113 / 84 and 141 / 108. (Where units are cut all
-// the same, finding that out takes 1 us.)
+// How many units there are of a key head, where the workgroups take them whole (and then shared.prefix their numbers in the place of their
+// lengths); 0, where pieces cut them. A piece mostly holds two parts, each with what a unit costs besides its keys, parts are
+// written and read again, and the join has nearly all units to join; whole units leave workgroups idle behind the one with the
+// most. That one has as many as there are rounds, or, as long ones come first and short ones behind them, no more than the
+// longest unit or about two pieces' length. So they stay whole where that is at most cut.whole more than a
+// piece, cut / whole in us: 2000 bf16 rows of eleven packed documents of up to 750 keys, 32 heads of 128, 73 / 50, of five 95 /
+// 71, 2000 rows of one prompt 104 / 79; 2048 rows at 16384 keys, with a cap, 665 / 613; 64 tokens over 300 to 800 int8 keys 45
+// / 31, over as many of 4 bits 37 / 23. (In the line's order, with no regard to lengths, the documents take 57 and 80 whole.)
+// With heads of 256, one workgroup a CU, nothing else runs where one idles, and the longer the units the less the cuts cost:
+// 2048 rows of 16 such heads at 2048 keys 134 / 115, at 3000 183 / 160, at 5000 247 / 250 (int8 294 / 317), at 8000 374 / 421,
+// at 16384 776 / 843; the documents 113 / 70 and 141 / 108. (Where units are cut all the same, finding that out takes 1 us.)
 template <int THREADS, typename A>
 __device__ __forceinline__ uint32_t whole_units(const A &a, const Cut &cut, LineShared<THREADS, A> &shared, int64_t share) {
   constexpr int kWaves = THREADS / 64;
@@ -417,7 +427,7 @@ __device__ __forceinline__ uint32_t whole_units(const A &a, const Cut &cut, Line
   number = wave_sum(number);
 #pragma unroll
   for (int d = 1; d < 64; d <<= 1) longest = max(longest, __shfl_xor(longest, d));
-  // Both in a word: more units than are ever dealt out count as that many.
+  // Both in a word: more units than are ever kept whole count as that many.
   if (lane == 0) shared.waves[wave] = (number < 0x7FFFFFFF ? number : 0x7FFFFFFF) << 32 | (uint32_t)longest;
   __syncthreads();
   number = 0;
@@ -429,9 +439,9 @@ __device__ __forceinline__ uint32_t whole_units(const A &a, const Cut &cut, Line
   number = uniform(number);
   longest = uniform(longest);
   const int64_t rounds = (number + a.workgroups - 1) / a.workgroups;
-  if (!number || number > 8 * (int64_t)a.workgroups) return 0;
+  if (!number || number > kMaxRounds * (int64_t)a.workgroups || number > (int64_t)THREADS * a.kv.kv_heads || count > kMaxWhole) return 0;
   const int64_t most = share + cut.whole - (cut.fall ? share / cut.fall : 0);
-  if (rounds * longest > most) return longest <= most && share <= cut.whole ? kSnapped : 0;
+  if (rounds * longest > most && !(longest <= most && share <= cut.whole)) return 0;
   int64_t carry = 0;
   for (uint32_t s0 = 0; s0 < count; s0 += THREADS) {
     const uint32_t s = s0 + threadIdx.x;
@@ -454,7 +464,7 @@ __device__ __forceinline__ uint32_t whole_units(const A &a, const Cut &cut, Line
     carry += all;
   }
   __syncthreads();
-  return (uint32_t)number;
+  return (uint32_t)number / a.kv.kv_heads;
 }
 
 // Every thread of the workgroup takes part.
@@ -546,10 +556,8 @@ __device__ __forceinline__ Work<THREADS, A, WHOLE> make_work(const A &a, const C
   w.active = (uint32_t)uniform(quotient_up(total, share));
   if constexpr (WHOLE) {
     w.units = whole_units<THREADS>(a, cut, shared, share);
-    if (w.units && w.units != kSnapped) {
-      w.active = min(w.units, a.workgroups);
-      w.piece = count == 1 ? dealt_piece_of(w.active, blockIdx.x, max(a.workgroups / (8 * cut.resident), 1u))
-                           : piece_of(w.active, blockIdx.x);
+    if (w.units) {
+      w.take_whole(a, cut, shared, w.units);
       return w;
     }
   }

@@ -215,8 +215,8 @@ def test_many_sequences():
 @pytest.mark.parametrize("units", [1, 3, 8, 40])
 @pytest.mark.parametrize("fmt", ["bf16", "e2m1"])
 def test_units_dealt_whole(fmt, units):
-    """Batches whose units nearly fill a small device's workgroups, alike and of many lengths, so that they are dealt out in turn,
-    snapped to pieces or cut: the same function, and the same bits each time."""
+    """Batches whose units nearly fill a small device's workgroups, alike and of many lengths, so that they stay whole in one turn,
+    in several, or are cut: the same function, and the same bits each time."""
     rng = np.random.default_rng(units)
     t = torch()
     for sizes, chunk in (([(1, 300 + 7 * i) for i in range(24)], 1), ([(1, int(n)) for n in rng.integers(1, 700, 70)], 1),
@@ -237,6 +237,29 @@ def test_units_dealt_whole(fmt, units):
             outs.append(from_bf16(out).reshape(q.shape))
         check_attention(outs[0], want, bound, f"{len(sizes)} sequences")
         assert np.array_equal(*outs)
+        del keep
+
+
+@pytest.mark.parametrize("kv_heads", [1, 3, 5, 8])
+@pytest.mark.parametrize("window,prefix", [(0, 0), (90, 0), (0, 150), (70, 130)])
+def test_whole_units_of_uneven_heads(kv_heads, window, prefix):
+    """Units kept whole whose key heads do not divide the eight dies' workgroups, and whose lengths do not grow with the row."""
+    rng = np.random.default_rng(kv_heads + window)
+    t = torch()
+    for sizes, chunk, units in (([(1, 200 + 9 * i) for i in range(40)], 1, 16), ([(150 + 11 * i, 170 + 13 * i) for i in range(8)], 300, 24),
+                                ([(int(n), int(n) + 3) for n in rng.integers(0, 200, 30)], 200, 256)):
+        c = make(rng, sizes, kv_heads, 64, 16, "bf16").fill()
+        heads = 2 * kv_heads
+        q = queries(rng, c.rows, heads, 64)
+        prefixes = [prefix] * len(sizes)
+        want, bound = scored_f64(q, c, 0.125, window=window, prefixes=prefixes, slopes=slopes_of(heads))
+        scores, keep = scores_of(prefixes=prefixes, slopes=slopes_of(heads))
+        plan = sq.attention_plan(sq.AttentionShape(heads, c.shape, 1, window, 0.125), len(sizes), c.rows, min(chunk, c.rows),
+                                 sq.Device(units))
+        out, scratch = t.full((c.rows, heads * 64), 123.0, dtype=t.bfloat16, device="cuda"), sq.AttentionScratch(plan)
+        scratch.partials.fill_(0xFF)
+        sq.attention_add(plan, c.struct(), c.batch(), to_bf16(q.reshape(c.rows, -1)), out, scratch, scores=scores)
+        check_attention(from_bf16(out).reshape(q.shape)[:c.live_rows], want, bound, f"{len(sizes)} sequences")
         del keep
 
 
