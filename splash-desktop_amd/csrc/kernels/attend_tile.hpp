@@ -34,8 +34,8 @@
 //
 // The registers are full: bf16 heads of 256 spill 13 of them (40 bytes a lane), int8 ones of 128 and 256 4 and 12 (12 and 0
 // bytes: accumulation registers hold the others), e4m3 ones 13 and 20 (40 and 24), 4-bit ones of 256 38 (140). Scored ones of
-// 256 spill 21 to 47 (72 to 168 bytes), capped ones 24 to 48 (48 to 180) and of 128 as plain ones. Heads of 64 and bf16 and
-// 4-bit ones of 128 none.
+// 256 spill 21 to 50 (72 to 168 bytes) and of bf16 64 4 (12), capped ones of 256 24 to 48 (48 to 180) and of e4m3 128 13 (40).
+// No others any.
 //
 // Keys past the sequence's end and holes read as zeros (buffer resources end there). Only tiles that some row does not
 // see whole compare positions.
