@@ -123,7 +123,8 @@ struct Units {
 struct Cut {
   int fit, least, slack;
   uint32_t resident;   // workgroups of a compute unit
-  int whole, fall;   // what cutting units costs a workgroup, in keys, and 1 / what that falls by for each of a piece (whole_units)
+  // whole_units: what cutting units costs a workgroup, in keys, and 1 / what that falls by for each of a piece (0: nothing).
+  int whole, fall;
 };
 template <typename A>
 __device__ __forceinline__ Units<A> units_of(const A &a, const Member<A> &q, const Cut &cut) {
@@ -396,8 +397,8 @@ struct Work {
   }
 };
 
-// How many units there are of a key head, where the workgroups take them whole (and then shared.prefix their numbers in the place of their
-// lengths); 0, where pieces cut them. A piece mostly holds two parts, each with what a unit costs besides its keys, parts are
+// How many units there are of a key head, where the workgroups take them whole (and then shared.prefix their numbers in the
+// place of their lengths); 0, where pieces cut them. A piece mostly holds two parts, each with what a unit costs besides its keys, parts are
 // written and read again, and the join has nearly all units to join; whole units leave workgroups idle behind the one with the
 // most. That one has as many as there are rounds, or, as long ones come first and short ones behind them, no more than the
 // longest unit or about two pieces' length. So they stay whole where that is at most cut.whole more than a
@@ -414,7 +415,7 @@ __device__ __forceinline__ uint32_t whole_units(const A &a, const Cut &cut, Line
   const auto units_at = [&](uint32_t s) __attribute__((always_inline)) {
     return units_of(a, s < kCached ? shared.sequence[s] : member_of(a, s), cut);
   };
-  // Their number and the longest, the first or the last of a sequence. (Sequences up to kCached are in LDS behind this barrier.)
+  // Their number and the longest, the first or last of a sequence (others are a unit's rows longer at most). (Those up to kCached are in LDS behind this barrier.)
   __syncthreads();
   int64_t number = 0;
   int longest = 0;
@@ -422,7 +423,7 @@ __device__ __forceinline__ uint32_t whole_units(const A &a, const Cut &cut, Line
     const Units<A> u = units_at(s);
     if (!u.count) continue;
     number += (int64_t)u.count * a.kv.kv_heads;
-    longest = max(longest, max(u.length(0), u.length(u.count - 1)));   // (those between: a unit's rows more at most)
+    longest = max(longest, max(u.length(0), u.length(u.count - 1)));
   }
   number = wave_sum(number);
 #pragma unroll
@@ -439,7 +440,7 @@ __device__ __forceinline__ uint32_t whole_units(const A &a, const Cut &cut, Line
   number = uniform(number);
   longest = uniform(longest);
   const int64_t rounds = (number + a.workgroups - 1) / a.workgroups;
-  if (!number || number > kMaxRounds * (int64_t)a.workgroups || number > (int64_t)THREADS * a.kv.kv_heads || count > kMaxWhole) return 0;
+  if (!number || count > kMaxWhole || number > (int64_t)THREADS * a.kv.kv_heads || rounds > kMaxRounds) return 0;
   const int64_t most = share + cut.whole - (cut.fall ? share / cut.fall : 0);
   if (rounds * longest > most && !(longest <= most && share <= cut.whole)) return 0;
   int64_t carry = 0;

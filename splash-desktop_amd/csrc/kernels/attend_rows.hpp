@@ -266,7 +266,8 @@ attend_rows_kernel(A a) {
   const uint32_t lane = threadIdx.x & 63, r = lane & 15, kq = lane >> 4;
   const uint32_t wave = uniform(threadIdx.x >> 6);
   constexpr bool kWhole = kScored || kFour;   // (the others keep the shares, and so the bits, that they have)
-  const Cut cut{16 * MB / (int)a.group, (int)attend_least(DIM, FMT, kScored), kUnitSlack + 256, attend_resident(16 * MB, WAVES, DIM, FMT), 640, 0};
+  const Cut cut{16 * MB / (int)a.group, (int)attend_least(DIM, FMT, kScored), kUnitSlack + 256,
+                attend_resident(16 * MB, WAVES, DIM, FMT), 640, 0};
   const float by_group = 1.0f / (float)a.group;
   const uint32_t dim = a.kv.head_dim, row_bytes = kFour ? dim / 2 : dim * (kCodes ? 1 : 2);
   Part<A> next;
