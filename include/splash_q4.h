@@ -597,7 +597,8 @@ int sq_attention_add_scored(void *graph, const sq_attention_buffers *buffers, co
  * past the views, whatever they hold. */
 typedef struct sq_kv_pool {
   sq_kv_cache cache;
-  uint32_t sequences, pages_per_sequence; /* sequences at most 2^20, sequences * pages_per_sequence at most 2^28 */
+  /* sequences at most 2^20, sequences * pages_per_sequence at most 2^28, pages_per_sequence * page_rows at most 2^30 */
+  uint32_t sequences, pages_per_sequence;
   sq_buffer references, page_table, lengths, report;
 } sq_kv_pool;
 int sq_kv_pool_workspace(const sq_kv_pool *pool, uint64_t *bytes);

@@ -9,9 +9,8 @@
 namespace sq::ops {
 namespace {
 
-// The most rows of a batch and the most keys a sequence's pages hold: sums of lengths over every unit of a batch stay
-// far inside 64 bits, and a position inside 32.
-constexpr uint32_t kMaxRows = 1u << 20, kMaxKeys = 1u << 30, kMaxHeads = 1024, kMaxUnits = 65536;
+// The most rows of a batch: with kMaxKeys, sums of lengths over every unit of a batch stay far inside 64 bits.
+constexpr uint32_t kMaxRows = 1u << 20, kMaxHeads = 1024, kMaxUnits = 65536;
 
 void requireHeadDim(uint32_t dim) {
   if (!dim || dim > 256 || dim % 16)

@@ -38,6 +38,8 @@ struct Rope {
                   const HeadRowsView &input, const HeadRowsView &output);
 };
 
+// The most keys that a sequence's pages hold: a position, and a length that grows, stay inside 32 bits.
+constexpr uint32_t kMaxKeys = 1u << 30;
 enum class KvFormat : uint32_t { BFloat16 = SQ_KV_BF16, Int8 = SQ_KV_INT8, E4m3 = SQ_KV_E4M3, E2m1 = SQ_KV_E2M1 };
 struct KvSize {
   uint64_t keys = 0, values = 0, keyScales = 0, valueScales = 0;

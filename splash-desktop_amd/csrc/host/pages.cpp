@@ -60,6 +60,8 @@ void KvPool::require() const {
   if (!sequences || sequences > kMaxTableRows) throw std::invalid_argument("a pool has 1 to 2^20 sequences");
   if (!pagesPerSequence || uint64_t{sequences} * pagesPerSequence > kMaxEntries)
     throw std::invalid_argument("a pool's table has entries, at most 2^28");
+  if (uint64_t{pagesPerSequence} * cache.shape.pageRows > kMaxKeys)
+    throw std::invalid_argument("a pool's sequences have pages for at most 2^30 keys");
   requireWords(references, cache.pages, "page references");
   requireWords(pageTable, uint64_t{sequences} * pagesPerSequence, "page table entries");
   requireWords(lengths, sequences, "sequence lengths");

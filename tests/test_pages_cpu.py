@@ -57,6 +57,21 @@ def test_pool_refusals(message, sizes, views):
         workspace_of(p)
 
 
+@pytest.mark.parametrize("page_rows,per,fits", [(1024, 1 << 20, True), (1024, (1 << 20) + 1, False), (1024, 1 << 23, False),
+                                                (1024, 1 << 28, False), (16, 1 << 26, True), (16, (1 << 26) + 1, False)])
+def test_keys_of_a_sequence(page_rows, per, fits):
+    """A pool's sequences have at most the keys of a batch's, 2^30: with more a length could grow past its 32 bits."""
+    p, words = pool(cache=cache(page_rows=page_rows), sequences=1, per=per, page_table=buffer(4 * per)), buffer(8)
+    if fits:
+        assert workspace_of(p)
+        return
+    for name, rest in (("release", (words, words, 2)), ("grow", (words, words, 2, buffer(1 << 30))),
+                       ("fork", (words, words, 2, buffer(1 << 30))), ("compact", (buffer(1 << 30),))):
+        refused(f"sq_kv_pool_add_{name}", "2\\^30 keys", by(p), *rest)
+    with pytest.raises(sq.InvalidArgument, match="2\\^30 keys"):
+        workspace_of(p)
+
+
 def test_request_refusals():
     p, words = pool(), buffer(8)
     size = workspace_of(p)
