@@ -20,6 +20,13 @@
 namespace sq::kern {
 namespace {
 
+// Ones in the places of a word's codes whose values are finite under a scale byte above 252: none under 255, magnitudes up to
+// 1.5 (codes with no bit of 4) under 254, and up to 3 (codes without bits 4 and 2 together) under 253.
+__device__ __forceinline__ uint32_t finite_codes4(uint32_t w, uint32_t by) {
+  const uint32_t infinite = (by == 254 ? w : w & w << 1) & 0x44444444u;
+  return by == 255 ? 0u : ~((infinite >> 2) * 15);
+}
+
 template <int DIM, int MB>
 struct Rows4 {
   static constexpr int kRun = DIM / 16, kChains = DIM / 32;
@@ -180,9 +187,9 @@ struct Rows4 {
     return any;
   }
 
-  // Groups under a byte above 252 leave the tile where some rows see a key of it and others do not (they must not reach the
-  // others through 0 * inf), and the rows that see them add their products one by one, of bytes 253 and 254 the finite ones
-  // too. Bit 4 h + i of seen: key 16 h + 4 kq + i.
+  // Infinities and NaNs (under bytes above 252) leave the tile where some rows see a key of it and others do not (they must not
+  // reach the others through 0 * inf), and the rows that see them add their products one by one. Finite values under such bytes
+  // stay, for the products with both halves of a weight. Bit 4 h + i of seen: key 16 h + 4 kq + i.
   __device__ __forceinline__ void set_apart(ValueTile &t, const KvArgs &kv, const Keys16 (&at)[2], const u32x4 (&p)[MB],
                                             const uint32_t (&seen)[MB], uint32_t row_bytes, uint32_t lane) {
     const uint32_t r = lane & 15, kq = lane >> 4;
@@ -209,23 +216,25 @@ struct Rows4 {
             const uint32_t by = buffer_b8(groups, (key % 16) * kGroups + value / 32, 0) << 23;
             if (!sees || !fp4_unbounded(by)) continue;
             const uint32_t two = fp4_pair(buffer_b8(codes, (key % 16) * row_bytes + value / 2, 0), by, 0);
-            o[b][d][j] += weight * bf16_to_f32(two & 0xFFFFu);
-            o[b][d + 1][j] += weight * __uint_as_float(two & 0xFFFF0000u);
+            if ((two & 0x7F80u) == 0x7F80u) o[b][d][j] += weight * bf16_to_f32(two & 0xFFFFu);
+            if ((two & 0x7F800000u) == 0x7F800000u) o[b][d + 1][j] += weight * __uint_as_float(two & 0xFFFF0000u);
           }
       }
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (fp4_unbounded(value_scale(t, h, e, lane)))
+      for (int e = 0; e < 4; ++e) {
+        const uint32_t by = value_scale(t, h, e, lane) >> 23;
+        if (by > 252)
 #pragma unroll
-          for (int i = 0; i < kValueWords; ++i) t.w[h][e][i] = 0;
-      // Their scales too, whichever lane's they are: a byte of zero.
+          for (int i = 0; i < kValueWords; ++i) t.w[h][e][i] &= finite_codes4(t.w[h][e][i], by);
+      }
+      // The scales of NaNs too, whichever lane's they are: a byte of zero.
 #pragma unroll
       for (int e = 0; e < kGroupWords; ++e)
 #pragma unroll
         for (int g = 0; g < 4; ++g)
-          if (fp4_unbounded(fp4_scale(t.groups[h][e], g))) t.groups[h][e] &= ~(0xFFu << (8 * g));
+          if (fp4_scale(t.groups[h][e], g) >> 23 == 255) t.groups[h][e] &= ~(0xFFu << (8 * g));
     }
   }
 };

@@ -8,6 +8,7 @@ import pytest
 import splash_q4 as sq
 from attention_oracle import attention_f64, bf16, check_attention, from_bf16, run_attention, to_bf16, torch
 from cache4_oracle import Cache4, packed, quantised4, scale_bytes, values4
+from test_attention_weights import attend
 
 pytestmark = pytest.mark.gpu
 
@@ -222,6 +223,38 @@ def test_scale_bytes_of_no_write(byte, code, want, chunk):
         assert np.all(got[59, :, 40] == want) and np.isfinite(np.delete(got[59], 40, -1)).all()
     else:
         assert np.isfinite(got[59]).all()
+
+
+@pytest.mark.parametrize("byte", [253, 254])
+@pytest.mark.parametrize("heads,kv_heads,dim,tile", [(8, 1, 64, 16), (16, 2, 96, 16), (8, 1, 128, 16), (24, 1, 128, 32), (20, 1, 64, 32),
+                                                     (8, 1, 256, 16)])
+def test_finite_values_under_scale_bytes_of_no_write(byte, heads, kv_heads, dim, tile):
+    """The largest finite values that another program's bytes make, which some rows of a tile see and others do not, within the
+    bound of all weights of few rows: two bf16 each. (Weights are alike, so that none takes a sum past fp32's range.)"""
+    t = torch()
+    rng = np.random.default_rng(byte + dim)
+    sizes, scale = [(3, 60), (1, 33), (2, 700)], 0.01
+    c = Cache4(rng, sizes, kv_heads, dim, 16).fill()
+    held = [c.stored(s) for s in range(len(sizes))]
+    for s, (n, keys) in enumerate(sizes):
+        for position in range(keys - n, keys):
+            page, slot = c.slot(s, position)
+            codes = rng.choice(np.array([0, 1, 2, 9, 10] if byte == 253 else [0, 1, 9], np.uint8), (kv_heads, 32))
+            c.values[int(page), :, slot, 16:32] = t.from_numpy(packed(codes)).cuda()      # group 1
+            c.value_scales[int(page), :, slot, 1] = byte
+            held[s][1][:, position, 32:64] = np.where(codes & 8, -0.5, 0.5) * (codes & 7) * 2.0 ** (byte - 127)
+    q = queries(rng, c.rows, heads, dim)
+    plan = sq.attention_plan(sq.AttentionShape(heads, c.shape, 1, 0, scale), len(sizes), c.rows, 1)
+    assert plan.tile_rows == tile
+    got, group = run_attention(c, q, scale, plan=plan), heads // kv_heads
+    for s, (n, keys) in enumerate(sizes):
+        for i in range(n):
+            for h in range(kv_heads):
+                k, v = (x[h, :keys - n + i + 1] for x in held[s])
+                rows = slice(h * group, (h + 1) * group)
+                want, bound = attend(q[c.starts[s] + i, rows], k, v, scale)
+                err = np.abs(got[c.starts[s] + i, rows] - want)
+                assert np.all(err <= bound), (s, i, h, np.max(err / bound))
 
 
 @pytest.mark.parametrize("kv_heads,dim", [(2, 64), (1, 96), (1, 128), (1, 256)])
