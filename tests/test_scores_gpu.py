@@ -191,6 +191,77 @@ def test_infinite_scores_under_a_cap(chunk):
     assert np.isnan(got[2]).all()
 
 
+@pytest.mark.parametrize("fmt", ALL)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("cap", [30.0, 400.0])
+@pytest.mark.parametrize("chunk", [None, 1])
+def test_hidden_keys_touch_nothing_under_a_cap_alone(fmt, dim, cap, chunk):
+    """The same for calls that have a cap and no slopes (a kernel of their own where rows are many and the cap is not above 128):
+    NaN in keys, values and scales before the begins and behind the prefixes."""
+    t = torch()
+    rng = np.random.default_rng(dim)
+    sizes = [(130, 400), (1, 200), (100, 500), (64, 77)]
+    begins, prefixes = [250, 150, 130, 70], [290, 0, 450, 77]
+    c = make(rng, sizes, 2, dim, 16, fmt).fill()
+    q = queries(rng, c.rows, 4, dim)
+    what = dict(cap=cap, begins=begins, prefixes=prefixes)
+    want, bound = scored_f64(q, c, 0.1, **what)
+    clean = run_scored(c, q, 0.1, chunk=chunk, **what)
+    for s in range(len(sizes)):
+        for position in range(begins[s]):
+            page, slot = c.slot(s, position)
+            for x in (c.keys, c.values, c.key_scales, c.value_scales):
+                x.view(t.uint8)[int(page), :, slot] = 0xFF
+    got = run_scored(c, q, 0.1, chunk=chunk, **what)
+    check_attention(got, want, bound, fmt)
+    assert np.array_equal(got, clean)
+
+
+@pytest.mark.parametrize("fmt", ALL)
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("cap", [5.0, 60.0, 300.0])
+@pytest.mark.parametrize("chunk", [None, 1])
+def test_unbounded_scores_that_all_rows_see(fmt, dim, cap, chunk):
+    """Products that overflow, in a tile that all rows see: their scores are the cap, or below zero. (One key has a value where
+    the queries are large and nothing else there; the other keys' scores are far within the cap or not.) A key that is NaN makes the
+    outputs of its head NaN, whichever tile it lies in, and no others."""
+    rng = np.random.default_rng(dim + int(cap))
+    c = make(rng, [(140, 400)], 2, dim, 16, fmt)
+    for part in c.k:
+        part[:, :, 3] = 0.0
+        part[:, 70] = 0.0
+        part[:, 70, 3] = 1e30
+    q = queries(rng, c.rows, 4, dim, 0.3)
+    q[:, ::2, 3], q[:, 1::2, 3] = 1e30, -1e30
+    got = run_scored(c.fill(), bf16(q), 0.05, chunk=chunk, cap=cap)
+    # In 64 bits by products of 20 caps, of which the hyperbolic tangent is one to 2^-56.
+    for part in c.k:
+        part[:, 70, 3] = bf16(400.0 * cap)
+    q[:, ::2, 3], q[:, 1::2, 3] = 1.0, -1.0
+    want, bound = scored_f64(q, c, 0.05, cap=cap)
+    check_attention(got, want, bound, fmt)
+    c.k[0][1, 200, 5] = np.nan
+    nan = run_scored(c.fill(), q, 0.05, chunk=chunk, cap=cap)
+    assert np.isnan(nan[:, 2:]).all() and np.isfinite(nan[:, :2]).all()
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("chunk", [None, 1])
+def test_unbounded_values_under_a_cap_alone(dim, chunk):
+    """Infinite and NaN values that some rows of a tile see: those rows have them, and the others keep their bits."""
+    rng = np.random.default_rng(dim)
+    c = make(rng, [(140, 400)], 2, dim, 16, "bf16").fill()
+    q = queries(rng, c.rows, 4, dim)
+    clean = run_scored(c, q, 0.05, chunk=chunk, cap=30.0)
+    c.v[0][0, 300, 7], c.v[0][1, 390, 40] = np.inf, np.nan
+    got = run_scored(c.fill(), q, 0.05, chunk=chunk, cap=30.0)
+    at = np.arange(260, 400)
+    want = clean.copy()
+    want[at >= 300, :2, 7] = np.inf
+    want[at >= 390, 2:, 40] = np.nan
+    assert np.array_equal(got, want, equal_nan=True)
+
+
 def test_nothing_to_do_is_the_plain_call():
     """No part given: the bits of the plain call; neutral parts: its function."""
     rng = np.random.default_rng(4)
