@@ -590,11 +590,13 @@ int sq_attention_add_scored(void *graph, const sq_attention_buffers *buffers, co
  * An empty pool has zero references and lengths and a table of ~0u. Entries of a sequence past its keys are ~0u; an entry that
  * names no page is a hole, shares and releases nothing.
  * report (uint32 [4]) tells what the last call did: [0] requests not carried out, [1] pages copied, [2] (compact alone writes
- * it) pages in use. Requests are uint32 arrays on the device, at most SQ_KV_MAX_SEQUENCES of them a call. One that names no
- * sequence, or one that an earlier request of the call names, is not carried out; nor is one that needs new pages where too
- * few are free for it and the requests before it. All views are 4-byte aligned; workspace (16-byte aligned, of
- * sq_kv_pool_workspace's bytes) may hold anything before a call and serves one stream at a time. Nothing here reads or writes
- * past the views, whatever they hold. */
+ * it) pages in use. A release, grow or fork of no requests launches nothing, and leaves the report as it was. Requests are
+ * uint32 arrays on the device, at most SQ_KV_MAX_SEQUENCES of them a call. One that names no sequence, or one that an earlier
+ * request of the call names, is not carried out; nor is one that needs new pages where too few are free for it and the requests
+ * before it. All views are 4-byte aligned; workspace (16-byte aligned, of sq_kv_pool_workspace's bytes) may hold anything
+ * before a call and serves one stream at a time. Nothing here reads or writes past the views, whatever they hold.
+ * The books are of one cache, and which pages a call moved or copied is not told. A model's caches, one a layer, have books
+ * each: the same calls make the same of equal books, and their tables stay equal. */
 typedef struct sq_kv_pool {
   sq_kv_cache cache;
   /* sequences at most 2^20, sequences * pages_per_sequence at most 2^28, pages_per_sequence * page_rows at most 2^30 */

@@ -93,6 +93,17 @@ def test_request_refusals():
     refused("sq_kv_pool_workspace".replace("workspace", "add_compact"), "16-byte", by(p), buffer(size, (1 << 20) + 8))
 
 
+def test_calls_of_no_requests():
+    """Checked like all others, and nothing is launched (the views point nowhere)."""
+    p, none = pool(), sq.Buffer(None, 0)
+    work = buffer(workspace_of(p))
+    sq.call("sq_kv_pool_add_release", None, by(p), none, none, 0)
+    for call in ("sq_kv_pool_add_grow", "sq_kv_pool_add_fork"):
+        sq.call(call, None, by(p), none, none, 0, work)
+        refused(call, "workspace", by(p), none, none, 0, none)
+        refused(call, "lengths", by(pool(lengths=none)), none, none, 0, work)
+
+
 def test_copy_refusals():
     a, pairs = cache(), buffer(16)
     refused("sq_kv_add_copy", "one shape", by(a), by(cache(page_rows=64)), pairs, 2)

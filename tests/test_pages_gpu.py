@@ -146,6 +146,26 @@ def test_many_requests():
         device.release([0] * 1025, [0] * 1025)
 
 
+def test_calls_of_no_requests():
+    """They launch nothing: books, bytes and the report of the last call stay as they were."""
+    pool, device = grown([70, 64, 5], pages=12)
+    both(pool, device, "grow", [0, 2], [200, 1])                   # one does not fit
+    report = pool.report.copy()
+    assert report[0] == 1
+    for call in ("release", "grow", "fork"):
+        getattr(device, call)([], [])
+        device.check(call)
+    assert np.array_equal(device.state()["report"], report)
+    graph = torch().cuda.CUDAGraph()
+    words = device.words([])
+    with torch().cuda.graph(graph):
+        sq.kv_release(device.struct, words, words)
+        sq.kv_compact(device.struct, device.scratch)
+    graph.replay()
+    pool.compact()
+    device.check("replay")
+
+
 def test_long_tables():
     """Rows of the table longer than a workgroup takes at once."""
     rng = np.random.default_rng(4)
