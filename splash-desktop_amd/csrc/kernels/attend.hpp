@@ -12,6 +12,8 @@
 //    parts, as many as give no part more than the share, and a workgroup takes one part. The share is the work over the
 //    workgroups that cutting leaves whole, so there are enough of them. One token over 700 keys of 8 key heads: 14 us,
 //    where a line (below) cuts units at odd places and gives most workgroups two parts, one after the other: 22 us.
+//    (A sequence's last unit stands for all of its units in this, the longest of causal rows. Under a prefix and a window the
+//    first one is, and its parts are longer than the share; every tile is some part's all the same.)
 //  - Otherwise the units lie end to end on a line, and workgroup w takes the w-th of equal pieces of it. A piece may end
 //    inside a unit, which then has parts. The lengths are linear in m up to the clamps at both ends, so their prefix sums
 //    have a closed form, and a workgroup finds its place by a search over the sequences' sums (in LDS) and one over m.
@@ -408,6 +410,7 @@ struct Work {
 // With heads of 256, one workgroup a CU, nothing else runs where one idles, and the longer the units the less the cuts cost:
 // 2048 rows of 16 such heads at 2048 keys 134 / 115, at 3000 183 / 160, at 5000 247 / 250 (int8 294 / 317), at 8000 374 / 421,
 // at 16384 776 / 843; the documents 113 / 70 and 141 / 108. (Where units are cut all the same, finding that out takes 1 us.)
+// The ranking has a thread a unit of a key head: with more of them than threads units are cut, whatever that costs.
 template <int THREADS, typename A>
 __device__ __forceinline__ uint32_t whole_units(const A &a, const Cut &cut, LineShared<THREADS, A> &shared, int64_t share) {
   constexpr int kWaves = THREADS / 64;

@@ -14,6 +14,10 @@
 // What it reaches: a token of 40 heads over 131072 keys of 8 heads of 128 (143 MB) in 35 us, 4.1 TB/s, where int8 takes 54; a
 // token each of 64 sequences of 200 to 8000 keys (151 MB) in 52, 2.9 TB/s, four of a tile's 16 rows live, and a
 // start and a join of the waves for each of some 1000 parts.
+// Tiles of 32 rows and heads of 256 keep one step in flight. With the join, one / two steps: eight rows each of those 64 sequences
+// 77 / 77 us (int8 95), four rows of 64 heads over 131072 keys 53 / 53; of heads of 64, where two spill 19 registers, 54 / 60;
+// heads of 256 (37 spilled), a token over 131072 keys 64 / 78, 4.4 TB/s with one (int8 108), of each of 64 sequences 83 / 103
+// (int8 128).
 #pragma once
 #include "attend_few.hpp"
 

@@ -25,12 +25,14 @@
 // units work 14%; the rest goes to the barriers and to the start of units of 17 tiles, a chain of loads that nothing covers.
 //
 // 4-bit pages: a lane's eight codes and the byte of their group become eight bf16 on the way to LDS, scales and all, so no
-// scale is left for scores or weights: the chunk at 16384 keys in 522 to 545 us (VALU 45% of the cycles, matrix units 42%).
+// scale is left for scores or weights: the chunk at 16384 keys in 3% more than a bf16 one, heads of 256 in 47% more (their codes
+// wait in registers that are full; VALU 45% of the cycles, matrix units 42%, heads of 128).
 //
 // Scored calls are their own instances, so that plain ones compile as if there were none. A cap that is all there is has one
 // more (CappedArgs): where a tile's scores are below 0.4 of the cap, cap tanh(t / cap) is an odd polynomial of the seventh
-// degree beside the second product, and no exponential or quotient. 2048 rows of 16 heads of 256 with a cap of 50 at 16384 keys
-// take 798 us so, 973 with the exponential form (a cap of 10), 660 with no cap (32 heads of 128: 626, 806).
+// degree beside the second product, and no exponential or quotient. 2048 rows at 16384 keys of 8, in one run: 16 heads of 256
+// with a cap of 50 so 779 us, with the exponential form (a cap of 10) 965, with slopes 836, with neither 693; 32 heads of 128 638,
+// 814, 645 and 545 (slopes over int8 keys 728); 32 of 64 452 with the cap and 346 without. (Between cards and runs 5%.)
 //
 // The registers are full: bf16 heads of 256 spill 13 of them (40 bytes a lane), int8 ones of 128 and 256 4 and 12 (12 and 0
 // bytes: accumulation registers hold the others), e4m3 ones 13 and 20 (40 and 24), 4-bit ones of 256 38 (140). Scored ones of
@@ -535,10 +537,9 @@ __global__ __launch_bounds__(kThreads, attend_tile_resident(DIM, FMT)) void atte
     // before, the second block's exponentials between the first ones' products; a barrier to the compiler's scheduling
     // keeps them so (left to itself it gathers the products, each behind a wait for its operand).
     // A call's cap is a polynomial here where the tile's scores are small, four instructions more a score, which the products
-    // partly hide (2048 rows at 16384 keys, 8 key heads: 16 heads of 256 805 us, 700 without a cap; 32 of 128 665, of 64 450).
-    // Scores that are settled go through the polynomial 1, as the registers hold no second form of this code. The share of the
-    // cap goes into the coefficients, or, one more instruction, is taken first: bf16 heads of 256 spill less so (805 for 859 us;
-    // int8 ones 974 for 961, heads of 128 680 for 665).
+    // partly hide. Scores that are settled go through the polynomial 1, as the registers hold no second form of this code. The
+    // share of the cap goes into the coefficients, or, one more instruction, is taken first: bf16 heads of 256 spill less so, 6%
+    // less time (int8 ones would take 1% more, heads of 128 2%).
     const auto finish = [&](int tile, [[maybe_unused]] bool to_cap) __attribute__((always_inline)) {
       constexpr bool kShareFirst = FMT == SQ_KV_BF16 && DIM == 256;
       [[maybe_unused]] float by_y = 1.0f, p0 = 1.0f, p1 = 0.0f, p2 = 0.0f, p3 = 0.0f;

@@ -283,7 +283,8 @@ uint64_t attend_partials(uint32_t tile_rows, uint32_t head_dim, uint32_t workgro
 constexpr uint32_t kAttendWideRows = 128;
 constexpr uint32_t attend_few_rows(uint32_t head_dim) { return head_dim <= 128 ? 32 : 16; }
 // The steps of keys and values that a wave of a tile of few rows has in flight. In 4 bits a step is too few bytes to cover a
-// round trip at the copy's rate, and its registers so few that two fit.
+// round trip at the copy's rate, and its registers so few that two fit, but with heads of 256 or tiles of 32 rows, which gain
+// nothing from a second or lose by it (attend_rows_four.hpp).
 constexpr uint32_t attend_rows_depth(uint32_t tile_rows, uint32_t head_dim, uint32_t format) {
   return format == SQ_KV_E2M1 && head_dim <= 128 && tile_rows == 16 ? 2 : 1;
 }
